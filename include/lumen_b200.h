@@ -138,6 +138,60 @@ size_t lb_gemm_operands_scratch_bytes(const lb_tensor* a, const lb_tensor* b);
 int lb_gemm(const lb_tensor* a, const lb_tensor* b, const lb_gemm_out* out, const lb_gemm_cfg* cfg /* nullable */,
             void* stream);
 
+/* ---- gated feed-forward block -----------------------------------------------------------------------------------
+ * a = x Wg^T, b = x Wu^T, h = f(a) b, y = h Wd^T (+ residual), for the M rows of `x` [.., D]: `w_gate_up` [2 F, D] holds Wg's F rows, then Wu's,
+ * `w_down` is [D, F]; any strides of the operands that lb_gemm takes, results row-major. `activation`: lb_activation. `h` [.., F] and, unless null,
+ * `gate_up` [.., 2 F] = [a b] are what the backward pass reads; h is computed from the float32 sums. `residual` (nullable, 16-bit
+ * dtypes) is added to the rounded product as LB_EPILOGUE_ADD does. Backward: dh = dy Wd, [da db] = [dh b f'(a), dh f(a)] rounded to the operands' dtype,
+ * d_x = [da db] [Wg; Wu], d_w_gate_up = [da db]^T x, d_w_down = dy^T h, each with one float32 sum and one rounding. All tensors of a call
+ * share a dtype (float16, bfloat16, float32); every call repeats bit for bit. Scratch: as many bytes as the _scratch_bytes call on the same
+ * tensors says (of their `ptr` only the alignment counts), 16-byte aligned; calls that may overlap on the GPU need scratch of their own. */
+typedef enum { LB_ACTIVATION_SILU = 0, LB_ACTIVATION_GELU_TANH = 1, LB_ACTIVATION_RELU = 2 } lb_activation;
+int lb_gated_mlp_fwd_scratch_bytes(int activation, const lb_tensor* x, const lb_tensor* w_gate_up, const lb_tensor* w_down, const lb_tensor* y,
+                                   const lb_tensor* gate_up /* nullable */, const lb_tensor* h, size_t* bytes);
+int lb_gated_mlp_fwd(int activation, const lb_tensor* x, const lb_tensor* w_gate_up, const lb_tensor* w_down,
+                     const lb_tensor* residual /* nullable */, const lb_tensor* y, const lb_tensor* gate_up /* nullable */, const lb_tensor* h,
+                     void* scratch, size_t scratch_bytes, void* stream);
+int lb_gated_mlp_bwd_scratch_bytes(int activation, const lb_tensor* d_y, const lb_tensor* x, const lb_tensor* w_gate_up, const lb_tensor* w_down,
+                                   const lb_tensor* gate_up, const lb_tensor* h, const lb_tensor* d_x, const lb_tensor* d_w_gate_up,
+                                   const lb_tensor* d_w_down, size_t* bytes);
+int lb_gated_mlp_bwd(int activation, const lb_tensor* d_y, const lb_tensor* x, const lb_tensor* w_gate_up, const lb_tensor* w_down,
+                     const lb_tensor* gate_up, const lb_tensor* h, const lb_tensor* d_x, const lb_tensor* d_w_gate_up, const lb_tensor* d_w_down,
+                     void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---- norms of queries and keys with the position rotation -----------------------------------------------------------
+ * For each head's row x of `q` [B, S, N, H] and `k` [B, S, Nkv, H] (strided views, H up to 256; float16, bfloat16 or float32):
+ * z = x / sqrt(mean(x^2) + eps) * weight, then the first R = 2 * pairs elements turn in pairs, (i, i + R/2) or with `interleaved` (2i, 2i + 1):
+ * y_a = z_a cos - z_b sin, y_b = z_b cos + z_a sin, by row `position` of the float32 tables `cos` and `sin` [positions, pairs]. `positions`
+ * (int32 or int64, [S] or [B, S]; null: 0 .. S - 1) are clamped into the tables. Weights (nullable: ones) are [H] of the rows' dtype or float32.
+ * Statistics and products are float32, each result is rounded once. Results may be the operands' own memory, row for row.
+ * The backward pass reads the forward's operands and gives the gradients of both (d_q and d_k may take the place of d_q_out and d_k_out) and of
+ * the weights (one each where there is a weight, of its dtype), bit-identical from run to run. Its scratch (weights only):
+ * lb_qk_norm_rope_bwd_scratch_bytes, 16-byte aligned, not shared with a call that may overlap on the GPU. */
+typedef struct {
+    float eps;
+    int32_t interleaved;
+} lb_rope_desc;
+int lb_qk_norm_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tensor* k, const lb_tensor* cos, const lb_tensor* sin,
+                    const lb_tensor* positions /* nullable */, const lb_tensor* q_weight /* nullable */, const lb_tensor* k_weight /* nullable */,
+                    const lb_tensor* q_out, const lb_tensor* k_out, void* stream);
+size_t lb_qk_norm_rope_bwd_scratch_bytes(int head_dim);
+int lb_qk_norm_rope_bwd(const lb_rope_desc* desc, const lb_tensor* d_q_out, const lb_tensor* d_k_out, const lb_tensor* q, const lb_tensor* k,
+                        const lb_tensor* cos, const lb_tensor* sin, const lb_tensor* positions, const lb_tensor* q_weight, const lb_tensor* k_weight,
+                        const lb_tensor* d_q, const lb_tensor* d_k, const lb_tensor* d_q_weight /* nullable */, const lb_tensor* d_k_weight /* nullable */,
+                        void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---- global gradient norm and clipping -----------------------------------------------------------------------------
+ * norm = sqrt(sum of squares over all tensors), one float32 value on the device; lb_clip_grad_norm also writes outputs[k] = tensors[k] * c with
+ * c = min(1, max_norm / (norm + 1e-6)). Tensors of float16, bfloat16 and float32 in any mix, dense in any order of their dimensions; outputs of the
+ * same shape, strides and dtype, the operand itself for in place (untouched where c is 1) or memory that overlaps no tensor of the call. A tensor given
+ * twice counts twice, and is refused where it would be written twice. A norm that is infinite or NaN makes c 0 or NaN. The squares' sum is held in 64
+ * bits; the same bits every time. Scratch: lb_grad_norm_scratch_bytes, 16-byte aligned, not shared with a call that may overlap on the GPU. */
+size_t lb_grad_norm_scratch_bytes(int n_tensors);
+int lb_grad_norm(const lb_tensor* tensors, int n_tensors, const lb_tensor* norm, void* scratch, size_t scratch_bytes, void* stream);
+int lb_clip_grad_norm(const lb_tensor* tensors, const lb_tensor* outputs, int n_tensors, double max_norm, const lb_tensor* norm, void* scratch,
+                      size_t scratch_bytes, void* stream);
+
 /* ---- flash attention ----------------------------------------------------------------------------------------
  * Replaces the ATTENTION hook `fn(&Forward{operands, dtype, heads_per_kv, causal, scores, grid, heads}, tensors,
  * &Config)` (lumen/codegen/attention/cuda/mod.rs:33-62) and the Ampere FA-2 forward kernel behind it

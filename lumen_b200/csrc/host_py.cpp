@@ -19,7 +19,7 @@
 namespace {
 
 struct Names {
-    PyObject *dtype, *shape, *stride, *data_ptr, *is_cuda, *is_contiguous, *get_device;
+    PyObject *dtype, *shape, *stride, *data_ptr, *is_cuda, *is_contiguous, *get_device, *numel;
 } names;
 PyObject* code_of = nullptr;     // dict: dtype object or name -> lb_dtype code, filled as dtypes are met
 PyObject* code_miss = nullptr;   // callable(dtype) -> code, for the first meeting
@@ -193,6 +193,195 @@ PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int rc;
     Py_BEGIN_ALLOW_THREADS
     rc = lb_gemm(&ta, &tb, &out, &cfg, stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// ---- operators of a decoder layer's step ----------------------------------------------------------------------------
+// These look where a tensor lives: kernels launched on the current device do not read another one's memory.
+struct Here {
+    int device = -1;
+    bool known = false;
+    bool current(int* out) {
+        if (!known && lb_get_device(&device) != LB_OK) device = -1;  // no GPU: the call itself says so
+        known = true;
+        *out = device;
+        return device >= 0;
+    }
+};
+// 1: torch's kind of tensor, on the current GPU; 0: it does not say (the package's own); -1: a Python error
+int is_here(PyObject* t, Here& here) {
+    PyObject* g = PyObject_CallMethodNoArgs(t, names.get_device);
+    if (!g) {
+        if (!PyErr_ExceptionMatches(PyExc_AttributeError)) return -1;
+        PyErr_Clear();
+        return 0;
+    }
+    const long at = PyLong_AsLong(g);
+    Py_DECREF(g);
+    if (at == -1 && PyErr_Occurred()) return -1;
+    int device;
+    if (at < 0) PyErr_SetString(PyExc_ValueError, "expected a CUDA tensor");
+    else if (here.current(&device) && at != device) PyErr_Format(PyExc_ValueError, "a tensor is on GPU %ld, the current one is GPU %d", at, device);
+    return PyErr_Occurred() ? -1 : 1;
+}
+bool describe_here(PyObject* t, lb_tensor* out, Here& here) { return is_here(t, here) >= 0 && describe(t, out); }
+
+// A call's workspace, from `take(bytes)` where it needs any; held until the call's kernels are queued.
+struct Scratch {
+    PyObject* held = nullptr;
+    void* ptr = nullptr;
+    ~Scratch() { Py_XDECREF(held); }
+    bool get(PyObject* take, size_t bytes) {
+        if (!bytes) return true;
+        held = PyObject_CallFunction(take, "n", (Py_ssize_t)bytes);
+        return held && read_pointer(held, &ptr);
+    }
+};
+
+// qk_norm_rope(eps, interleaved, q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out, stream), None where the ABI takes a null
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 12)) return nullptr;
+    lb_rope_desc d = {(float)PyFloat_AsDouble(a[0]), (int32_t)PyLong_AsLong(a[1])};
+    lb_tensor t[9];
+    const lb_tensor* p[9];
+    Here here;
+    for (int k = 0; k < 9; k++) {
+        p[k] = a[2 + k] == Py_None ? nullptr : &t[k];
+        if (p[k] && !describe_here(a[2 + k], &t[k], here)) return nullptr;
+    }
+    void* stream = PyLong_AsVoidPtr(a[11]);
+    if (PyErr_Occurred()) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lb_qk_norm_rope(&d, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// qk_norm_rope_bwd(eps, interleaved, d_q_out, d_k_out, q, k, cos, sin, positions, q_weight, k_weight, d_q, d_k, d_q_weight, d_k_weight, take, stream)
+PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 17)) return nullptr;
+    lb_rope_desc d = {(float)PyFloat_AsDouble(a[0]), (int32_t)PyLong_AsLong(a[1])};
+    lb_tensor t[13];
+    const lb_tensor* p[13];
+    Here here;
+    for (int k = 0; k < 13; k++) {
+        p[k] = a[2 + k] == Py_None ? nullptr : &t[k];
+        if (p[k] && !describe_here(a[2 + k], &t[k], here)) return nullptr;
+    }
+    void* stream = PyLong_AsVoidPtr(a[16]);
+    if (PyErr_Occurred()) return nullptr;
+    const int64_t dim = p[2] && t[2].rank == 4 ? t[2].shape[3] : 0;
+    const size_t bytes = (p[7] || p[8]) && dim > 0 && dim <= 4096 ? lb_qk_norm_rope_bwd_scratch_bytes((int)dim) : 0;
+    Scratch scratch;
+    if (!scratch.get(a[15], bytes)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lb_qk_norm_rope_bwd(&d, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10], p[11], p[12], scratch.ptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// gated_mlp_fwd(activation, x, w_gate_up, w_down, residual, y, gate_up, h, take, stream)
+PyObject* gated_mlp_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 10)) return nullptr;
+    const int act = (int)PyLong_AsLong(a[0]);
+    lb_tensor t[7];
+    const lb_tensor* p[7];
+    Here here;
+    for (int k = 0; k < 7; k++) {
+        p[k] = a[1 + k] == Py_None ? nullptr : &t[k];
+        if (p[k] && !describe_here(a[1 + k], &t[k], here)) return nullptr;
+    }
+    void* stream = PyLong_AsVoidPtr(a[9]);
+    if (PyErr_Occurred()) return nullptr;
+    size_t bytes = 0;
+    int rc = lb_gated_mlp_fwd_scratch_bytes(act, p[0], p[1], p[2], p[4], p[5], p[6], &bytes);
+    if (rc != LB_OK) return finish(rc);
+    Scratch scratch;
+    if (!scratch.get(a[8], bytes)) return nullptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lb_gated_mlp_fwd(act, p[0], p[1], p[2], p[3], p[4], p[5], p[6], scratch.ptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// gated_mlp_bwd(activation, d_y, x, w_gate_up, w_down, gate_up, h, d_x, d_w_gate_up, d_w_down, take, stream)
+PyObject* gated_mlp_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 12)) return nullptr;
+    const int act = (int)PyLong_AsLong(a[0]);
+    lb_tensor t[9];
+    Here here;
+    for (int k = 0; k < 9; k++)
+        if (!describe_here(a[1 + k], &t[k], here)) return nullptr;
+    void* stream = PyLong_AsVoidPtr(a[11]);
+    if (PyErr_Occurred()) return nullptr;
+    size_t bytes = 0;
+    int rc = lb_gated_mlp_bwd_scratch_bytes(act, &t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8], &bytes);
+    if (rc != LB_OK) return finish(rc);
+    Scratch scratch;
+    if (!scratch.get(a[10], bytes)) return nullptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lb_gated_mlp_bwd(act, &t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], &t[8], scratch.ptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// One of many tensors, of which a contiguous one is as good as the row of its elements: half the questions of `describe`.
+bool describe_dense(PyObject* t, lb_tensor* out, Here& here) {
+    const int torch = is_here(t, here);
+    if (torch < 0) return false;
+    bool contiguous = false;
+    if (torch && !truth(PyObject_CallMethodNoArgs(t, names.is_contiguous), &contiguous)) return false;
+    if (!contiguous) return describe(t, out);
+    PyObject* count = PyObject_CallMethodNoArgs(t, names.numel);
+    if (!count) return false;
+    out->rank = 1, out->shape[0] = PyLong_AsLongLong(count), out->stride[0] = 1;
+    Py_DECREF(count);
+    return !PyErr_Occurred() && dtype_code(t, &out->dtype) && read_pointer(t, &out->ptr);
+}
+
+// clip_grad_norm(tensors, outputs or None (in place), max_norm or None (the norm alone), norm, take, stream); sequences of tensors
+PyObject* clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 6)) return nullptr;
+    const bool clips = a[2] != Py_None;
+    const double most = clips ? PyFloat_AsDouble(a[2]) : 0.0;
+    void* stream = PyLong_AsVoidPtr(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    std::vector<lb_tensor> t[2];
+    lb_tensor norm;
+    Here here;
+    for (int k = 0; k < 2; k++) {
+        if (a[k] == Py_None) continue;
+        PyObject* all = PySequence_Fast(a[k], "expected a sequence of tensors");
+        if (!all) return nullptr;
+        const Py_ssize_t count = PySequence_Fast_GET_SIZE(all);
+        bool ok = count <= INT32_MAX;
+        if (!ok) PyErr_SetString(PyExc_ValueError, "too many tensors");
+        try {
+            if (ok) t[k].resize((size_t)count);
+        } catch (const std::bad_alloc&) {
+            Py_DECREF(all);
+            return PyErr_NoMemory();
+        }
+        for (Py_ssize_t i = 0; ok && i < count; i++) ok = describe_dense(PySequence_Fast_GET_ITEM(all, i), &t[k][i], here);
+        Py_DECREF(all);
+        if (!ok) return nullptr;
+    }
+    if (a[1] != Py_None && t[0].size() != t[1].size()) {
+        PyErr_Format(PyExc_ValueError, "%zu tensors and %zu results", t[0].size(), t[1].size());
+        return nullptr;
+    }
+    if (!describe_here(a[3], &norm, here)) return nullptr;
+    const int count = (int)t[0].size();
+    const size_t bytes = lb_grad_norm_scratch_bytes(count);
+    Scratch scratch;
+    if (!scratch.get(a[4], bytes)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = clips ? lb_clip_grad_norm(t[0].data(), a[1] == Py_None ? t[0].data() : t[1].data(), count, most, &norm, scratch.ptr, bytes, stream)
+               : lb_grad_norm(t[0].data(), count, &norm, scratch.ptr, bytes, stream);
     Py_END_ALLOW_THREADS
     return finish(rc);
 }
@@ -456,6 +645,11 @@ PyMethodDef methods[] = {
     {"attention_bwd", (PyCFunction)(void (*)(void))attention_bwd, METH_FASTCALL, "lb_attention_bwd_scratch / lb_attention_bwd_atomic on tensors"},
     {"attention_bwd_scratch_bytes", (PyCFunction)(void (*)(void))attention_bwd_scratch_bytes, METH_FASTCALL, "lb_attention_bwd_scratch_bytes of tensors"},
     {"gemm", (PyCFunction)(void (*)(void))gemm, METH_FASTCALL, "lb_gemm on tensors"},
+    {"qk_norm_rope", (PyCFunction)(void (*)(void))qk_norm_rope, METH_FASTCALL, "lb_qk_norm_rope on tensors"},
+    {"qk_norm_rope_bwd", (PyCFunction)(void (*)(void))qk_norm_rope_bwd, METH_FASTCALL, "lb_qk_norm_rope_bwd on tensors"},
+    {"gated_mlp_fwd", (PyCFunction)(void (*)(void))gated_mlp_fwd, METH_FASTCALL, "lb_gated_mlp_fwd on tensors"},
+    {"gated_mlp_bwd", (PyCFunction)(void (*)(void))gated_mlp_bwd, METH_FASTCALL, "lb_gated_mlp_bwd on tensors"},
+    {"clip_grad_norm", (PyCFunction)(void (*)(void))clip_grad_norm, METH_FASTCALL, "lb_grad_norm / lb_clip_grad_norm on sequences of tensors"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "the call path of lumen_b200 over the C ABI", -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -470,6 +664,7 @@ PyMODINIT_FUNC PyInit__host(void) {
     names.is_cuda = PyUnicode_InternFromString("is_cuda");
     names.is_contiguous = PyUnicode_InternFromString("is_contiguous");
     names.get_device = PyUnicode_InternFromString("get_device");
+    names.numel = PyUnicode_InternFromString("numel");
     table_type.tp_name = "lumen_b200._host.CallTable";
     table_type.tp_basicsize = sizeof(CallTable);
     table_type.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_GC;

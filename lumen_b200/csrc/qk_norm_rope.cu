@@ -1,0 +1,333 @@
+// Norms of queries and keys for each head and the position rotation, in one pass over both, forward and backward.
+//
+// A row x is one head's H elements at one position. With r = 1 / sqrt(mean(x^2) + eps) and z = x r w, the pairs (a, b) of the first R
+// elements - (i, i + R/2), or neighbours (2i, 2i + 1) - turn by the angle of their token: y_a = z_a c - z_b s, y_b = z_b c + z_a s, where c and s
+// are row `position` of two float32 tables; the rest is y = z. Backward: dz by the transposed turn (dz_a = dy_a c + dy_b s,
+// dz_b = dy_b c - dy_a s), dw = sum over rows of dz x r, and with u = dz w: dx = r (u - x r^2 mean(u x)). Statistics, products and
+// sums are float32; each result is rounded once. Nothing is kept between the passes: r is found again from the row, which the backward
+// pass reads anyway.
+//
+// The weight gradients add up in registers over the rows of a thread, over a block's threads in shared memory, and over the blocks
+// in a second kernel: always in the same order, so that results repeat bit for bit.
+#include <algorithm>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "launch.cuh"
+
+namespace lb {
+namespace {
+
+constexpr int kMaxDim = 256;
+
+// One of the two operands: queries or keys.
+struct RopeSide {
+    const void* x;
+    const void* dy;  // backward
+    void* out;       // y, or dx
+    const void* w;   // null: all ones
+    void* dw;
+    float* partial;  // [blocks][H]: the blocks' sums of dw
+    long long x_b, x_s, x_n, x_h, dy_b, dy_s, dy_n, dy_h, out_b, out_s, out_n, out_h;
+    int heads, blocks;
+    int w_f32;       // w and dw are float32, whatever the rows' type
+};
+struct RopeArgs {
+    RopeSide side[2];
+    const float *cos, *sin;
+    long long ld_cos, ld_sin, cos_i, sin_i;
+    const void* positions;  // null: 0, 1, 2 ...
+    int positions_64;
+    long long pos_b, pos_s;
+    int table, batch, seq, H, R, interleaved;
+    float eps;
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <class T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// The row of the tables that a token turns by: its position, clamped into them.
+__device__ __forceinline__ int table_row(const RopeArgs& p, int b, int s) {
+    if (!p.positions) return s;
+    const long long at = b * p.pos_b + s * p.pos_s;
+    const long long pos = p.positions_64 ? ((const long long*)p.positions)[at] : (long long)((const int*)p.positions)[at];
+    return (int)(pos < 0 ? 0 : (pos >= p.table ? p.table - 1 : pos));
+}
+
+template <class T>
+__device__ __forceinline__ float weight(const RopeSide& q, int i) {
+    return !q.w ? 1.0f : q.w_f32 ? ((const float*)q.w)[i] : to_float(((const T*)q.w)[i]);
+}
+
+// Any head dim, strides and alignment: a warp a row, its elements lane by lane; the row waits in shared memory, so that a pair's
+// members find one another and results may go where the operand was.
+constexpr int kRowWarps = 8;
+template <class T, bool BWD>
+__global__ void __launch_bounds__(kRowWarps * 32) rope_rows_kernel(const RopeArgs p) {
+    __shared__ float held[kRowWarps][2][kMaxDim];
+    grid_wait();
+    const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
+    const RopeSide& q = p.side[side];
+    const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, H = p.H, R = p.R;
+    float *x = held[warp][0], *dy = held[warp][1];
+    float sum[kMaxDim / 32] = {};
+    const long long rows = (long long)p.batch * p.seq * q.heads;
+    for (long long row = (long long)block * kRowWarps + warp; row < rows; row += (long long)q.blocks * kRowWarps) {
+        const long long token = row / q.heads;
+        const int n = (int)(row - token * q.heads), b = (int)(token / p.seq), s = (int)(token - (long long)b * p.seq);
+        const T* from = (const T*)q.x + b * q.x_b + s * q.x_s + n * q.x_n;
+        float ss = 0.0f;
+        __syncwarp();
+        for (int i = lane; i < H; i += 32) {
+            const float v = to_float(from[i * q.x_h]);
+            x[i] = v, ss += v * v;
+        }
+        if (BWD) {
+            const T* g = (const T*)q.dy + b * q.dy_b + s * q.dy_s + n * q.dy_n;
+            for (int i = lane; i < H; i += 32) dy[i] = to_float(g[i * q.dy_h]);
+        }
+        __syncwarp();
+        for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        const float r = 1.0f / sqrtf(ss / H + p.eps);
+        const int at = table_row(p, b, s);
+        const float *cos = p.cos + at * p.ld_cos, *sin = p.sin + at * p.ld_sin;
+        T* to = (T*)q.out + b * q.out_b + s * q.out_s + n * q.out_n;
+        float u[kMaxDim / 32], mean = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kMaxDim / 32; j++) {
+            const int i = lane + 32 * j;
+            if (i >= H) break;
+            float c = 1.0f, sn = 0.0f;  // y_i = z_i c + z_other sn
+            int other = i;
+            if (i < R) {
+                const int pair = p.interleaved ? i / 2 : (i < R / 2 ? i : i - R / 2);
+                const bool first = p.interleaved ? i % 2 == 0 : i < R / 2;
+                other = p.interleaved ? i ^ 1 : (first ? i + R / 2 : i - R / 2);
+                c = cos[pair * p.cos_i], sn = sin[pair * p.sin_i];
+                if (first != BWD) sn = -sn;
+            }
+            if (!BWD) {
+                const float turned = i < R ? x[other] * r * weight<T>(q, other) * sn : 0.0f;
+                to[i * q.out_h] = from_float<T>(x[i] * r * weight<T>(q, i) * c + turned);
+            } else {
+                const float dz = i < R ? dy[i] * c + dy[other] * sn : dy[i];
+                sum[j] += dz * (x[i] * r);
+                u[j] = dz * weight<T>(q, i);
+                mean += u[j] * (x[i] * r);
+            }
+        }
+        if (BWD) {
+            for (int d = 16; d; d >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, d);
+            mean /= H;
+#pragma unroll
+            for (int j = 0; j < kMaxDim / 32; j++)
+                if (lane + 32 * j < H) to[(lane + 32 * j) * q.out_h] = from_float<T>(r * (u[j] - x[lane + 32 * j] * r * mean));
+        }
+    }
+    if (BWD && q.w) {
+        __syncthreads();
+        float* sums = &held[0][0][0];  // [warp][H]
+#pragma unroll
+        for (int j = 0; j < kMaxDim / 32; j++)
+            if (lane + 32 * j < H) sums[warp * kMaxDim + lane + 32 * j] = sum[j];
+        __syncthreads();
+        for (int i = threadIdx.x; i < H; i += blockDim.x) {
+            float t = 0.0f;
+            for (int k = 0; k < kRowWarps; k++) t += sums[k * kMaxDim + i];
+            q.partial[(long long)block * H + i] = t;
+        }
+    }
+}
+
+// dw: the blocks' sums, 32 columns a block, eight of its rows beside one another.
+template <class T>
+__global__ void __launch_bounds__(256) rope_weights_kernel(const RopeArgs p) {
+    __shared__ float held[8][33];
+    grid_wait();
+    const RopeSide& q = p.side[blockIdx.y];
+    if (!q.w) return;
+    const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+    float sum = 0.0f;
+    if (i < p.H)
+        for (int k = part; k < q.blocks; k += 8) sum += q.partial[(long long)k * p.H + i];
+    held[part][lane] = sum;
+    __syncthreads();
+    if (part == 0 && i < p.H) {
+        for (int k = 1; k < 8; k++) sum += held[k][lane];
+        if (q.w_f32) ((float*)q.dw)[i] = sum;
+        else ((T*)q.dw)[i] = from_float<T>(sum);
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+[[noreturn]] void refuse(const std::string& why) { fail(LB_ERR_INVALID, "qk_norm_rope: " + why); }
+
+void same_shape(const lb_tensor& a, const lb_tensor& b, const char* what) {
+    bool same = a.rank == b.rank && a.dtype == b.dtype;
+    for (int d = 0; same && d < a.rank; d++) same = a.shape[d] == b.shape[d];
+    if (!same) refuse(format("%s must have its operand's shape and dtype", what));
+}
+// Every element of a result has a place of its own (as far as the strides of one dimension say).
+void written(const lb_tensor& t, const char* what) {
+    for (int d = 0; d < t.rank; d++)
+        if (t.shape[d] > 1 && t.stride[d] == 0) refuse(format("%s is written and cannot be a broadcast view", what));
+}
+long long elements(const lb_tensor& t) {
+    long long n = 1;
+    for (int d = 0; d < t.rank; d++) n *= t.shape[d];
+    return n;
+}
+
+void weights(RopeSide& side, const lb_tensor* w, int H, int dtype, const char* what) {
+    if (!w) return;
+    if (w->rank != 1 || w->shape[0] != H || (w->dtype != dtype && w->dtype != LB_F32)) refuse(format("%s must be [%d] of the rows' dtype or float32", what, H));
+    if (H > 1 && w->stride[0] != 1) refuse(format("%s must be dense", what));
+    side.w = w->ptr, side.w_f32 = w->dtype == LB_F32;
+}
+
+// Both sides' blocks, in proportion to their rows: at most what fills the GPU once, at least one where a side has rows.
+constexpr int kBlocksPerSm = 4;
+void share_blocks(RopeArgs& p, long long rows_per_block, int sms) {
+    const long long tokens = (long long)p.batch * p.seq;
+    const long long need[2] = {(tokens * p.side[0].heads + rows_per_block - 1) / rows_per_block, (tokens * p.side[1].heads + rows_per_block - 1) / rows_per_block};
+    const long long all = need[0] + need[1], most = (long long)sms * kBlocksPerSm;
+    for (int k = 0; k < 2; k++) p.side[k].blocks = (int)(all <= most ? need[k] : need[k] ? std::max(1LL, most * need[k] / all) : 0);
+}
+
+struct RopeCall {
+    RopeArgs p{};
+    int dtype = 0;
+    long long rows = 0;
+};
+
+RopeCall check_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tensor* k, const lb_tensor* cos, const lb_tensor* sin, const lb_tensor* positions,
+                    const lb_tensor* wq, const lb_tensor* wk) {
+    if (!desc || !q || !k || !cos || !sin) refuse("null argument");
+    RopeCall c;
+    RopeArgs& p = c.p;
+    if (q->rank != 4 || k->rank != 4) refuse("queries and keys must be [batch, sequence, heads, head dim]");
+    if (q->dtype != k->dtype || (q->dtype != LB_F32 && q->dtype != LB_BF16 && q->dtype != LB_F16)) refuse("queries and keys must share a dtype: float16, bfloat16 or float32");
+    if (q->shape[0] != k->shape[0] || q->shape[1] != k->shape[1] || q->shape[3] != k->shape[3]) refuse("queries and keys must share batch, sequence and head dim");
+    for (int d = 0; d < 4; d++)
+        if (q->shape[d] < 0 || k->shape[d] < 0) refuse("negative size");
+    if (q->shape[3] < 1 || q->shape[3] > kMaxDim) refuse(format("head dims of 1 to %d", kMaxDim));
+    if (elements(*q) / q->shape[3] > INT32_MAX || elements(*k) / k->shape[3] > INT32_MAX || q->shape[0] * q->shape[1] > INT32_MAX)
+        fail(LB_ERR_UNSUPPORTED, "qk_norm_rope: more than 2^31 - 1 rows in one call");
+    c.dtype = q->dtype;
+    p.batch = (int)q->shape[0], p.seq = (int)q->shape[1], p.H = (int)q->shape[3];
+    if (cos->rank != 2 || sin->rank != 2 || cos->dtype != LB_F32 || sin->dtype != LB_F32 || cos->shape[0] != sin->shape[0] || cos->shape[1] != sin->shape[1])
+        refuse("cos and sin must be float32 tables of one shape [positions, rotated pairs]");
+    if (cos->shape[1] < 1 || 2 * cos->shape[1] > p.H) refuse(format("the tables' %lld pairs must be 1 to %d for a head dim of %d", (long long)cos->shape[1], p.H / 2, p.H));
+    if (cos->shape[0] > INT32_MAX) refuse("tables of at most 2^31 - 1 positions");
+    p.table = (int)cos->shape[0], p.R = (int)(2 * cos->shape[1]);
+    p.cos = (const float*)cos->ptr, p.sin = (const float*)sin->ptr;
+    p.ld_cos = cos->stride[0], p.cos_i = cos->stride[1], p.ld_sin = sin->stride[0], p.sin_i = sin->stride[1];
+    if (cos->shape[1] == 1) p.cos_i = p.sin_i = 1;
+    const long long tokens = (long long)p.batch * p.seq;
+    if (tokens && p.table < 1) refuse("the tables have no position");
+    if (positions) {
+        if (positions->dtype != LB_I32 && positions->dtype != LB_I64) refuse("positions must be int32 or int64");
+        const bool flat = positions->rank == 1;
+        if ((!flat && positions->rank != 2) || positions->shape[positions->rank - 1] != p.seq || (!flat && positions->shape[0] != p.batch))
+            refuse("positions must be [sequence] or [batch, sequence]");
+        p.positions = positions->ptr, p.positions_64 = positions->dtype == LB_I64;
+        p.pos_b = flat ? 0 : positions->stride[0], p.pos_s = positions->stride[flat ? 0 : 1];
+    } else if (p.table < p.seq) {
+        refuse(format("the tables hold %d positions, the sequence has %d", p.table, p.seq));
+    }
+    if (!(desc->eps >= 0.0f)) refuse("eps must not be negative");
+    p.eps = desc->eps, p.interleaved = desc->interleaved != 0;
+    const lb_tensor* x[2] = {q, k};
+    for (int s = 0; s < 2; s++) {
+        RopeSide& side = p.side[s];
+        side.x = x[s]->ptr, side.heads = (int)x[s]->shape[2];
+        side.x_b = x[s]->stride[0], side.x_s = x[s]->stride[1], side.x_n = x[s]->stride[2], side.x_h = x[s]->stride[3];
+    }
+    weights(p.side[0], wq, p.H, c.dtype, "the queries' weight");
+    weights(p.side[1], wk, p.H, c.dtype, "the keys' weight");
+    c.rows = elements(*q) / p.H + elements(*k) / p.H;
+    return c;
+}
+
+template <class T, bool BWD>
+void launch_rope(RopeCall& c, cudaStream_t stream) {
+    RopeArgs& p = c.p;
+    share_blocks(p, kRowWarps, device_info().sms);
+    const int blocks = p.side[0].blocks + p.side[1].blocks;
+    if (blocks) launch_overlapped(rope_rows_kernel<T, BWD>, dim3((unsigned)blocks), dim3(kRowWarps * 32), 0, stream, 0, p);
+    if (BWD && (p.side[0].w || p.side[1].w)) launch_overlapped(rope_weights_kernel<T>, dim3((unsigned)((p.H + 31) / 32), 2), dim3(256), 0, stream, 0, p);
+}
+template <bool BWD>
+void run_rope(RopeCall& c, void* stream) {
+    driver();
+    cudaStream_t s = (cudaStream_t)stream;
+    if (c.dtype == LB_F32) launch_rope<float, BWD>(c, s);
+    else if (c.dtype == LB_BF16) launch_rope<__nv_bfloat16, BWD>(c, s);
+    else launch_rope<__half, BWD>(c, s);
+}
+
+size_t scratch_bytes(int H) { return (size_t)sm_count_hint() * kBlocksPerSm * H * sizeof(float) * 2; }
+
+}  // namespace
+}  // namespace lb
+
+extern "C" {
+
+int lb_qk_norm_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tensor* k, const lb_tensor* cos, const lb_tensor* sin, const lb_tensor* positions,
+                    const lb_tensor* q_weight, const lb_tensor* k_weight, const lb_tensor* q_out, const lb_tensor* k_out, void* stream) {
+    return lb::guarded([&] {
+        lb::RopeCall c = lb::check_rope(desc, q, k, cos, sin, positions, q_weight, k_weight);
+        if (!q_out || !k_out) lb::refuse("null argument");
+        const lb_tensor *in[2] = {q, k}, *out[2] = {q_out, k_out};
+        for (int s = 0; s < 2; s++) {
+            lb::same_shape(*in[s], *out[s], "a result");
+            lb::written(*out[s], "a result");
+            lb::RopeSide& side = c.p.side[s];
+            side.out = out[s]->ptr, side.out_b = out[s]->stride[0], side.out_s = out[s]->stride[1], side.out_n = out[s]->stride[2], side.out_h = out[s]->stride[3];
+        }
+        if (c.rows) lb::run_rope<false>(c, stream);
+    });
+}
+
+size_t lb_qk_norm_rope_bwd_scratch_bytes(int head_dim) { return head_dim > 0 ? lb::scratch_bytes(head_dim) : 0; }
+
+int lb_qk_norm_rope_bwd(const lb_rope_desc* desc, const lb_tensor* d_q_out, const lb_tensor* d_k_out, const lb_tensor* q, const lb_tensor* k,
+                        const lb_tensor* cos, const lb_tensor* sin, const lb_tensor* positions, const lb_tensor* q_weight, const lb_tensor* k_weight,
+                        const lb_tensor* d_q, const lb_tensor* d_k, const lb_tensor* d_q_weight, const lb_tensor* d_k_weight, void* scratch,
+                        size_t scratch_bytes, void* stream) {
+    return lb::guarded([&] {
+        lb::RopeCall c = lb::check_rope(desc, q, k, cos, sin, positions, q_weight, k_weight);
+        if (!d_q_out || !d_k_out || !d_q || !d_k) lb::refuse("null argument");
+        const lb_tensor *in[2] = {q, k}, *dy[2] = {d_q_out, d_k_out}, *dx[2] = {d_q, d_k}, *w[2] = {q_weight, k_weight}, *dw[2] = {d_q_weight, d_k_weight};
+        for (int s = 0; s < 2; s++) {
+            lb::same_shape(*in[s], *dy[s], "a gradient");
+            lb::same_shape(*in[s], *dx[s], "a gradient");
+            lb::written(*dx[s], "a gradient");
+            lb::RopeSide& side = c.p.side[s];
+            side.dy = dy[s]->ptr, side.dy_b = dy[s]->stride[0], side.dy_s = dy[s]->stride[1], side.dy_n = dy[s]->stride[2], side.dy_h = dy[s]->stride[3];
+            side.out = dx[s]->ptr, side.out_b = dx[s]->stride[0], side.out_s = dx[s]->stride[1], side.out_n = dx[s]->stride[2], side.out_h = dx[s]->stride[3];
+            if (!w[s] != !dw[s]) lb::refuse("a weight has a gradient, and no weight has none");
+            if (dw[s]) {
+                lb::same_shape(*w[s], *dw[s], "a weight's gradient");
+                if (c.p.H > 1 && dw[s]->stride[0] != 1) lb::refuse("a weight's gradient must be dense");
+                side.dw = dw[s]->ptr;
+            }
+        }
+        if (c.p.side[0].w || c.p.side[1].w) {
+            const size_t need = lb::scratch_bytes(c.p.H);
+            if (!scratch || scratch_bytes < need || (uintptr_t)scratch % 16) lb::refuse(lb::format("the weights' gradients need %zu bytes of scratch, 16-byte aligned", need));
+            c.p.side[0].partial = (float*)scratch;
+            c.p.side[1].partial = (float*)((char*)scratch + need / 2);
+        }
+        if (c.rows || c.p.side[0].w || c.p.side[1].w) lb::run_rope<true>(c, stream);
+    });
+}
+}

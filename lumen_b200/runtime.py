@@ -348,3 +348,98 @@ def scatter_add_rows(x, ids, updates, deterministic=True, stream=None):
     _lib.check(lib.lb_scatter_add_rows(ctypes.byref(dx), ctypes.byref(di), ctypes.byref(du), ctypes.byref(do), scratch.data_ptr(),
                                        nbytes, int(deterministic), current_stream() if stream is None else stream))
     return out
+
+
+def _outputs(like, stream, *wanted):
+    """New dense tensors of `(shape, dtype name)` each, None for None."""
+    if _Torch.takes(like, stream):  # 1.5 us a tensor less than through `_empty_like_input`
+        return [None if w is None else like.new_empty(w[0], dtype=TORCH_DTYPES[w[1]]) for w in wanted]
+    return [None if w is None else _empty_like_input(like, *w) for w in wanted]
+
+
+def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None, stream=None):
+    """Norms of queries and keys for each head and the position rotation, in one pass through `lb_qk_norm_rope`. `q` `[B, S, N, H]` and `k`
+    `[B, S, Nkv, H]` are views of float16, bfloat16 or float32 (of a packed projection, say), H up to 256. Each head's row becomes
+    `z = x / sqrt(mean(x^2) + eps) * weight`; then its first `2 * pairs` elements turn, `y_a = z_a cos - z_b sin`, `y_b = z_b cos + z_a sin`, in pairs
+    `(i, i + pairs)`, or `(2i, 2i + 1)` with `interleaved`, by the float32 tables `cos` and `sin` `[positions, pairs]`. `positions`: int32 or int64,
+    `[S]` or `[B, S]`, clamped into the tables; None is 0, 1, 2 ... Weights: `[H]` of `q`'s dtype or float32; None is all ones. Returns `(q, k)`
+    of the operands' dtype, in `out` if given (which may be `(q, k)`)."""
+    require_cuda()
+    if out is None:
+        out = _outputs(q, stream, (tuple(q.shape), dtype_name(q.dtype)), (tuple(k.shape), dtype_name(k.dtype)))
+    _lib.host().qk_norm_rope(eps, bool(interleaved), q, k, cos, sin, positions, q_weight, k_weight, out[0], out[1], _stream(stream))
+    return out[0], out[1]
+
+
+def qk_norm_rope_backward(d_q_out, d_k_out, q, k, cos, sin, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None,
+                          stream=None):
+    """The backward pass of `qk_norm_rope` on the same operands: returns `(d_q, d_k, d_q_weight, d_k_weight)`, the last two of their weight's dtype and
+    None without one. `out` takes `d_q` and `d_k`, which may be `(d_q_out, d_k_out)`. Bit-identical from call to call."""
+    require_cuda()
+    wanted = [None if w is None else (tuple(w.shape), dtype_name(w.dtype)) for w in (q_weight, k_weight)]
+    if out is None:
+        out = _outputs(q, stream, (tuple(q.shape), dtype_name(q.dtype)), (tuple(k.shape), dtype_name(k.dtype)))
+    dwq, dwk = _outputs(q, stream, *wanted)
+    _lib.host().qk_norm_rope_bwd(eps, bool(interleaved), d_q_out, d_k_out, q, k, cos, sin, positions, q_weight, k_weight, out[0], out[1], dwq, dwk,
+                                 lambda nbytes: _workspace(q, (nbytes,), "uint8", stream), _stream(stream))
+    return out[0], out[1], dwq, dwk
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+
+
+def _activation(name) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {name!r}")
+    return ACTIVATIONS[name]
+
+
+def gated_mlp_forward(x, w_gate_up, w_down, activation="silu", residual=None, save=True, stream=None):
+    """The gated feed-forward block through `lb_gated_mlp_fwd`: `y = (f(x Wg^T) * (x Wu^T)) Wd^T` for the rows of `x` `[.., D]`, with `w_gate_up`
+    `[2 F, D]` (the F rows of Wg, then those of Wu), `w_down` `[D, F]` and `f` "silu", "gelu" (its tanh form) or "relu". Returns `(y, gate_up, h)`:
+    `gate_up` `[.., 2 F]`, the two projections (None with `save=False`), and `h` `[.., F]`, their gated product, are what the backward pass
+    reads. Sums are float32, and `h` is computed from them. `residual` (16-bit dtypes, shaped like `y`) is added to the rounded product. float16,
+    bfloat16 or float32; the tensor cores take 16-bit operands whose rows are 16-byte aligned, the CUDA cores the others. Bit-identical from call to
+    call; the same rows among others may differ by a rounding."""
+    require_cuda()
+    act, lead, dtype, f = _activation(activation), tuple(x.shape[:-1]), dtype_name(x.dtype), w_gate_up.shape[0] // 2
+    y, gate_up, h = _outputs(x, stream, (tuple(x.shape), dtype), ((*lead, 2 * f), dtype) if save else None, ((*lead, f), dtype))
+    _lib.host().gated_mlp_fwd(act, x, w_gate_up, w_down, residual, y, gate_up, h, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream), _stream(stream))
+    return y, gate_up, h
+
+
+def gated_mlp_backward(d_y, x, w_gate_up, w_down, gate_up, h, activation="silu", stream=None):
+    """The backward pass of `gated_mlp_forward` through `lb_gated_mlp_bwd`: returns `(d_x, d_w_gate_up, d_w_down)` of the operands' dtype. (A residual's
+    gradient is `d_y` itself.) Bit-identical from call to call."""
+    require_cuda()
+    act, dtype = _activation(activation), dtype_name(x.dtype)
+    d_x, d_wgu, d_wd = _outputs(x, stream, *((tuple(t.shape), dtype) for t in (x, w_gate_up, w_down)))
+    _lib.host().gated_mlp_bwd(act, d_y, x, w_gate_up, w_down, gate_up, h, d_x, d_wgu, d_wd, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream),
+                              _stream(stream))
+    return d_x, d_wgu, d_wd
+
+
+def _norm(tensors, out, max_norm, like, stream):
+    require_cuda()
+    if like is None:
+        if len(tensors) == 0:
+            raise ValueError("the norm of no tensors needs `like`, a tensor on the GPU")
+        like = tensors[0]
+    (norm,) = _outputs(like, stream, ((), "float32"))
+    _lib.host().clip_grad_norm(tensors, out, max_norm, norm, lambda nbytes: _workspace(like, (nbytes,), "uint8", stream), _stream(stream))
+    return norm
+
+
+def grad_norm(tensors, like=None, stream=None):
+    """The 2-norm of all elements of a list of tensors (float16, bfloat16 and float32 in any mix; each dense, in any order of its dimensions), as a
+    0-d float32 tensor on the device, through `lb_grad_norm`. A tensor listed twice counts twice. `like` says where the result goes if the list may
+    be empty. The sum of squares is held in 64 bits; the same bits from call to call."""
+    return _norm(tensors, None, None, like, stream)
+
+
+def clip_grad_norm(tensors, max_norm, out=None, like=None, stream=None):
+    """`grad_norm`, and every tensor times `min(1, max_norm / (norm + 1e-6))`: in place, or into `out`, a list of tensors of the same dtypes and
+    layouts that share no memory with one another or with `tensors`. Returns the norm before clipping (0-d float32, on the device); nothing
+    waits for it. In place, tensors of a norm within the bound are read once and left alone. An infinite or NaN norm makes every tensor 0 or NaN, as
+    the quotient says."""
+    return _norm(tensors, out, float(max_norm), like, stream)
