@@ -91,7 +91,10 @@ void run_gate(const GateArgs& p, int act, cudaStream_t s) {
     const unsigned gx = (unsigned)((cols + tx - 1) / tx);
     const long long rows = (p.M + block.y - 1) / block.y;
     const dim3 grid(gx, (unsigned)std::min<long long>(rows, std::max(1u, (unsigned)device_info().sms * 16 / gx)));
-    auto go = [&](auto kernel4, auto kernel1) { launch_overlapped(whole ? kernel4 : kernel1, grid, block, 0, s, 0, p); };
+    auto go = [&](auto kernel4, auto kernel1) {
+        auto kernel = whole ? kernel4 : kernel1;
+        launch_overlapped(kernel, grid, block, 0, s, 0, p);
+    };
     if (act == ACT_SILU) go(gate_kernel<T, 4, ACT_SILU, BWD>, gate_kernel<T, 1, ACT_SILU, BWD>);
     else if (act == ACT_GELU) go(gate_kernel<T, 4, ACT_GELU, BWD>, gate_kernel<T, 1, ACT_GELU, BWD>);
     else go(gate_kernel<T, 4, ACT_RELU, BWD>, gate_kernel<T, 1, ACT_RELU, BWD>);

@@ -40,7 +40,7 @@ struct RopeArgs {
     const void* positions;  // null: 0, 1, 2 ...
     int positions_64;
     long long pos_b, pos_s;
-    int table, batch, seq, H, R, interleaved;
+    int table, batch, seq, H, R, interleaved, lanes;
     float eps;
 };
 
@@ -146,6 +146,157 @@ __global__ void __launch_bounds__(kRowWarps * 32) rope_rows_kernel(const RopeArg
     }
 }
 
+// A thread's four pairs turned, (v[j], v[4 + j]) or neighbours; BACK: the other way.
+__device__ __forceinline__ void turn(float* v, const float* c, const float* s, bool neighbours, bool back) {
+    if (neighbours) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float a = v[2 * j], b = v[2 * j + 1], n = back ? -s[j] : s[j];
+            v[2 * j] = a * c[j] - b * n, v[2 * j + 1] = b * c[j] + a * n;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float a = v[j], b = v[4 + j], n = back ? -s[j] : s[j];
+            v[j] = a * c[j] - b * n, v[4 + j] = b * c[j] + a * n;
+        }
+    }
+}
+
+// Four elements of a row as float32 and back; the address is a multiple of their size.
+template <class T> struct Four;
+template <> struct Four<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = *(const float4*)p; }
+    __device__ __forceinline__ void widen(float* x) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+    __device__ __forceinline__ static void store(float* p, const float* x) { *(float4*)p = make_float4(x[0], x[1], x[2], x[3]); }
+};
+template <> struct Four<__nv_bfloat16> {
+    uint2 v;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *(const uint2*)p; }
+    __device__ __forceinline__ void widen(float* x) const {
+        x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u), x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+    __device__ __forceinline__ static void store(__nv_bfloat16* p, const float* x) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+        *(uint2*)p = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+    }
+};
+template <> struct Four<__half> {
+    uint2 v;
+    __device__ __forceinline__ void load(const __half* p) { v = *(const uint2*)p; }
+    __device__ __forceinline__ void widen(float* x) const {
+        const float2 lo = __half22float2(*(const __half2*)&v.x), hi = __half22float2(*(const __half2*)&v.y);
+        x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+    }
+    __device__ __forceinline__ static void store(__half* p, const float* x) {
+        const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
+        *(uint2*)p = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+    }
+};
+
+// Head dims and rotated parts that are multiples of 8, rows of aligned pieces of four elements: `p.lanes` lanes of a warp a row (a power of two), eight elements
+// each, both members of four pairs among them, so that a row is in registers once and its elements meet only in the sums of its statistics. A group
+// of lanes takes HEADS heads of a token at a time, whose loads are in flight together and whose angles are the same.
+constexpr int kGroupThreads = 256, kGroupBlocks = 3;
+template <class T, bool BWD, int HEADS>
+__global__ void __launch_bounds__(kGroupThreads, kGroupBlocks) rope_groups_kernel(const RopeArgs p) {
+    __shared__ float held[BWD ? kGroupThreads * 8 : 1];
+    grid_wait();
+    const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
+    const RopeSide& q = p.side[side];
+    const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x;
+    const int lanes = p.lanes, c = threadIdx.x & (lanes - 1), turning = p.R / 8;
+    const bool live = c * 8 < p.H, turns = c < turning;
+    // the thread's two runs of four elements
+    const int e0 = p.interleaved || !turns ? 8 * c : 4 * c, e1 = p.interleaved || !turns ? e0 + 4 : p.R / 2 + 4 * c;
+    float w[8], sum[BWD ? 8 : 1] = {};
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = live ? weight<T>(q, e0 + j) : 0.0f, w[4 + j] = live ? weight<T>(q, e1 + j) : 0.0f;
+    const int chunks = (q.heads + HEADS - 1) / HEADS, groups = kGroupThreads / lanes;
+    const long long tasks = (long long)p.batch * p.seq * chunks;
+    const float per = 1.0f / (float)p.H;
+    for (long long base = (long long)block * groups; base < tasks; base += (long long)q.blocks * groups) {
+        const long long mine = base + threadIdx.x / lanes;
+        const bool there = mine < tasks && live;
+        const unsigned task = (unsigned)(mine < tasks ? mine : tasks - 1), token = task / chunks;
+        const int n0 = (int)(task - token * chunks) * HEADS, b = (int)(token / p.seq), s = (int)(token - (unsigned)b * p.seq);
+        const T* from = (const T*)q.x + b * q.x_b + s * q.x_s + n0 * q.x_n;
+        const T* grad = BWD ? (const T*)q.dy + b * q.dy_b + s * q.dy_s + n0 * q.dy_n : nullptr;
+        Four<T> x_in[HEADS][2], g_in[BWD ? HEADS : 1][2];
+#pragma unroll
+        for (int k = 0; k < HEADS; k++)
+            if (there && n0 + k < q.heads) {
+                x_in[k][0].load(from + k * q.x_n + e0), x_in[k][1].load(from + k * q.x_n + e1);
+                if (BWD) g_in[k][0].load(grad + k * q.dy_n + e0), g_in[k][1].load(grad + k * q.dy_n + e1);
+            }
+        float cs[4], sn[4];
+        if (there && turns) {
+            const long long at = table_row(p, b, s);
+            Four<float> t;
+            t.load(p.cos + at * p.ld_cos + 4 * c), t.widen(cs);
+            t.load(p.sin + at * p.ld_sin + 4 * c), t.widen(sn);
+        }
+        T* to = (T*)q.out + b * q.out_b + s * q.out_s + n0 * q.out_n;
+#pragma unroll
+        for (int k = 0; k < HEADS; k++) {
+            const bool past = n0 + k >= q.heads;  // every lane of the warp votes
+            if (__all_sync(0xffffffffu, past)) break;
+            const bool row = there && n0 + k < q.heads;
+            float x[8], y[8], ss = 0.0f, dot = 0.0f;
+            if (row) {
+                x_in[k][0].widen(x), x_in[k][1].widen(x + 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) ss += x[j] * x[j];
+            if (BWD) {  // y: dz
+                if (row) g_in[k][0].widen(y), g_in[k][1].widen(y + 4);
+                if (row && turns) turn(y, cs, sn, p.interleaved, true);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (!row) y[j] = 0.0f;
+                    dot += y[j] * w[j] * x[j];
+                }
+            }
+            for (int d = lanes >> 1; d; d >>= 1) {
+                ss += __shfl_xor_sync(0xffffffffu, ss, d);
+                if (BWD) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+            }
+            const float r = 1.0f / sqrtf(ss * per + p.eps);
+            if (!BWD) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = x[j] * r * w[j];
+                if (turns) turn(y, cs, sn, p.interleaved, false);
+            } else {
+                const float mean = dot * r * per;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float unit = x[j] * r;
+                    sum[j] += row ? y[j] * unit : 0.0f;
+                    y[j] = r * (y[j] * w[j] - unit * mean);
+                }
+            }
+            if (row) Four<T>::store(to + k * q.out_n + e0, y), Four<T>::store(to + k * q.out_n + e1, y + 4);
+        }
+    }
+    if (BWD && q.w) {  // [group][H]
+        const int g = threadIdx.x / lanes;
+        if (live) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) held[g * p.H + e0 + j] = sum[j], held[g * p.H + e1 + j] = sum[4 + j];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.H; i += kGroupThreads) {
+            float t = 0.0f;
+            for (int k = 0; k < groups; k++) t += held[k * p.H + i];
+            q.partial[(long long)block * p.H + i] = t;
+        }
+    }
+}
+
 // dw: the blocks' sums, 32 columns a block, eight of its rows beside one another.
 template <class T>
 __global__ void __launch_bounds__(256) rope_weights_kernel(const RopeArgs p) {
@@ -194,12 +345,27 @@ void weights(RopeSide& side, const lb_tensor* w, int H, int dtype, const char* w
 }
 
 // Both sides' blocks, in proportion to their rows: at most what fills the GPU once, at least one where a side has rows.
-constexpr int kBlocksPerSm = 4;
-void share_blocks(RopeArgs& p, long long rows_per_block, int sms) {
-    const long long tokens = (long long)p.batch * p.seq;
-    const long long need[2] = {(tokens * p.side[0].heads + rows_per_block - 1) / rows_per_block, (tokens * p.side[1].heads + rows_per_block - 1) / rows_per_block};
-    const long long all = need[0] + need[1], most = (long long)sms * kBlocksPerSm;
+constexpr int kBlocksPerSm = 4;  // at most; the scratch holds a sum for each
+void share_blocks(RopeArgs& p, int groups, int heads, int sms, int per_sm) {
+    const long long tokens = (long long)p.batch * p.seq, most = (long long)sms * per_sm;
+    long long need[2];
+    for (int k = 0; k < 2; k++) need[k] = (tokens * ((p.side[k].heads + heads - 1) / heads) + groups - 1) / groups;
+    const long long all = need[0] + need[1];
     for (int k = 0; k < 2; k++) p.side[k].blocks = (int)(all <= most ? need[k] : need[k] ? std::max(1LL, most * need[k] / all) : 0);
+}
+
+// Whether rows can be taken in pieces of four elements by groups of lanes.
+bool in_pieces(const RopeArgs& p, int dtype, bool bwd) {
+    if (p.H % 8 || p.R % 8 || p.cos_i != 1 || p.sin_i != 1 || p.ld_cos % 4 || p.ld_sin % 4 || (uintptr_t)p.cos % 16 || (uintptr_t)p.sin % 16) return false;
+    const int per = 4, bytes = 4 * dtype_size(dtype);
+    auto fits = [&](const void* ptr, long long b, long long s, long long n, long long h, int heads) {
+        return (uintptr_t)ptr % bytes == 0 && (b % per == 0 || p.batch == 1) && (s % per == 0 || p.seq == 1) && (n % per == 0 || heads <= 1) && h == 1;
+    };
+    for (const RopeSide& q : p.side)
+        if (q.heads && (!fits(q.x, q.x_b, q.x_s, q.x_n, q.x_h, q.heads) || !fits(q.out, q.out_b, q.out_s, q.out_n, q.out_h, q.heads) ||
+                        (bwd && !fits(q.dy, q.dy_b, q.dy_s, q.dy_n, q.dy_h, q.heads))))
+            return false;
+    return true;
 }
 
 struct RopeCall {
@@ -260,9 +426,24 @@ RopeCall check_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tenso
 template <class T, bool BWD>
 void launch_rope(RopeCall& c, cudaStream_t stream) {
     RopeArgs& p = c.p;
-    share_blocks(p, kRowWarps, device_info().sms);
-    const int blocks = p.side[0].blocks + p.side[1].blocks;
-    if (blocks) launch_overlapped(rope_rows_kernel<T, BWD>, dim3((unsigned)blocks), dim3(kRowWarps * 32), 0, stream, 0, p);
+    const int sms = device_info().sms;
+    auto blocks = [&] { return dim3((unsigned)(p.side[0].blocks + p.side[1].blocks)); };
+    if (c.rows && in_pieces(p, c.dtype, BWD)) {
+        p.lanes = 1;
+        while (p.lanes * 8 < p.H) p.lanes *= 2;
+        constexpr int kHeads = BWD ? 2 : 4, kPerSm = kGroupBlocks;
+        const int groups = kGroupThreads / p.lanes;
+        if (c.rows >= (long long)sms * kPerSm * groups * kHeads) {
+            share_blocks(p, groups, kHeads, sms, kPerSm);
+            launch_overlapped(rope_groups_kernel<T, BWD, kHeads>, blocks(), dim3(kGroupThreads), 0, stream, 0, p);
+        } else {
+            share_blocks(p, groups, 1, sms, kPerSm);
+            launch_overlapped(rope_groups_kernel<T, BWD, 1>, blocks(), dim3(kGroupThreads), 0, stream, 0, p);
+        }
+    } else if (c.rows) {
+        share_blocks(p, kRowWarps, 1, sms, kBlocksPerSm);
+        launch_overlapped(rope_rows_kernel<T, BWD>, blocks(), dim3(kRowWarps * 32), 0, stream, 0, p);
+    }
     if (BWD && (p.side[0].w || p.side[1].w)) launch_overlapped(rope_weights_kernel<T>, dim3((unsigned)((p.H + 31) / 32), 2), dim3(256), 0, stream, 0, p);
 }
 template <bool BWD>

@@ -217,22 +217,25 @@ def test_gradients_against_differences(cuda, h, interleaved):
             assert abs((up - down) / (2 * step) - parts.sum()) <= 4 * STEPS32 * parts.abs().sum() * 8 + 1e-7 * parts.abs().sum()
 
 
-def test_many_rows_repeat_bit_for_bit_and_agree_with_few(cuda):
-    """More rows than the grid has threads: weights' gradients add up in a fixed order, and a row's result does not depend on the rows beside it."""
-    q, k, dq, dk, g = case(cuda, 3, 2501, 16, 4, 64, torch.bfloat16)
-    cos, sin = tables(2501, 32, cuda)
-    w = (1 + 0.3 * torch.randn(64, generator=g, device=cuda)).to(torch.bfloat16)
-    first = qk_norm_rope_backward(dq, dk, q, k, cos, sin, q_weight=w, k_weight=w)
+@pytest.mark.parametrize("n, nk, h, pairs, interleaved, dtype", [(16, 4, 64, 32, False, torch.bfloat16), (7, 5, 128, 64, False, torch.float16), (15, 1, 80, 16, True, torch.float32),
+                                                                 (13, 3, 256, 128, False, torch.bfloat16), (9, 3, 31, 15, False, torch.bfloat16)])  # fmt: skip
+def test_many_rows_repeat_bit_for_bit_and_agree_with_few(cuda, n, nk, h, pairs, interleaved, dtype):
+    """More rows than the grid has threads, numbers of heads that nothing divides: weights' gradients add up in a fixed order, and a row's result does not
+    depend on the rows beside it."""
+    q, k, dq, dk, g = case(cuda, 3, 2501, n, nk, h, dtype)
+    cos, sin = tables(2501, pairs, cuda)
+    w = (1 + 0.3 * torch.randn(h, generator=g, device=cuda)).to(dtype)
+    first = qk_norm_rope_backward(dq, dk, q, k, cos, sin, q_weight=w, k_weight=w, interleaved=interleaved)
     for _ in range(3):
-        assert all(torch.equal(a, b) for a, b in zip(first, qk_norm_rope_backward(dq, dk, q, k, cos, sin, q_weight=w, k_weight=w)))
+        assert all(torch.equal(a, b) for a, b in zip(first, qk_norm_rope_backward(dq, dk, q, k, cos, sin, q_weight=w, k_weight=w, interleaved=interleaved)))
     rows = torch.arange(2501, device=cuda).expand(3, 2501)
     for x, dy, dx, dw in ((q, dq, first[0], first[2]), (k, dk, first[1], first[3])):
-        (want_dx, dx_size), (want_dw, dw_size) = backward64(dy, x, w, cos, sin, rows, False)
+        (want_dx, dx_size), (want_dw, dw_size) = backward64(dy, x, w, cos, sin, rows, interleaved)
         close(dx, want_dx, dx_size)
         close(dw, want_dw, dw_size, chain=4.0)
-    whole = qk_norm_rope(q, k, cos, sin, q_weight=w, k_weight=w)
+    whole = qk_norm_rope(q, k, cos, sin, q_weight=w, k_weight=w, interleaved=interleaved)
     for at in (0, 1, 1250, 2500):
-        one = qk_norm_rope(q[1:2, at : at + 1], k[1:2, at : at + 1], cos, sin, positions=torch.tensor([at], device=cuda), q_weight=w, k_weight=w)
+        one = qk_norm_rope(q[1:2, at : at + 1], k[1:2, at : at + 1], cos, sin, positions=torch.tensor([at], device=cuda), q_weight=w, k_weight=w, interleaved=interleaved)
         assert torch.equal(one[0][0, 0], whole[0][1, at]) and torch.equal(one[1][0, 0], whole[1][1, at])
 
 
