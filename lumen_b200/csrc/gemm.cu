@@ -17,6 +17,7 @@
 #include <map>
 #include <mutex>
 
+#include "divide.cuh"
 #include "gemm.h"
 #include "launch.cuh"
 #include "sm100.cuh"
@@ -33,17 +34,6 @@ constexpr int kStageBytesA = BM * BK * 2, kStageBytesB = BN * BK * 2;
 constexpr int kEpilogueStageBytes = 8 * 4096;  // one 4 KB staging area per epilogue warp (store_rows_coalesced)
 constexpr int kSmemBytes = STAGES * (kStageBytesA + kStageBytesB) + 1024 /*alignment slack*/ + 256 /*barriers*/ + kEpilogueStageBytes;
 
-// n / d for 0 <= n < 2^31 as a multiply and a shift (Granlund and Montgomery's round-up method): where a tile lies is worked out by
-// every warp between two tiles, and six integer divisions took 1200 cycles there.
-struct Divisor {
-    uint32_t d = 1, mul = 1, shift = 0;
-    void set(uint32_t by) {
-        d = by, shift = 0;
-        while ((1ull << shift) < d) shift++;
-        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
 struct GemmArgs {
     int M, N, K, batch;
     int a_mn_major, b_mn_major;

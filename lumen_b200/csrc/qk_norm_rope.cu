@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "divide.cuh"
 #include "launch.cuh"
 
 namespace lb {
@@ -31,6 +32,7 @@ struct RopeSide {
     float* partial;  // [blocks][H]: the blocks' sums of dw
     long long x_b, x_s, x_n, x_h, dy_b, dy_s, dy_n, dy_h, out_b, out_s, out_n, out_h;
     int heads, blocks;
+    Divisor by_chunks;  // of a token's heads
     int w_f32;       // w and dw are float32, whatever the rows' type
 };
 struct RopeArgs {
@@ -42,6 +44,7 @@ struct RopeArgs {
     long long pos_b, pos_s;
     int table, batch, seq, H, R, interleaved, lanes;
     float eps;
+    Divisor by_seq;
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -196,94 +199,61 @@ template <> struct Four<__half> {
 };
 
 // Head dims and rotated parts that are multiples of 8, rows of aligned pieces of four elements: `p.lanes` lanes of a warp a row (a power of two), eight elements
-// each, both members of four pairs among them, so that a row is in registers once and its elements meet only in the sums of its statistics. A group
-// of lanes takes HEADS heads of a token at a time, whose loads are in flight together and whose angles are the same.
-constexpr int kGroupThreads = 256, kGroupBlocks = 3;
-template <class T, bool BWD, int HEADS>
-__global__ void __launch_bounds__(kGroupThreads, kGroupBlocks) rope_groups_kernel(const RopeArgs p) {
-    __shared__ float held[BWD ? kGroupThreads * 8 : 1];
-    grid_wait();
-    const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
-    const RopeSide& q = p.side[side];
-    const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x;
-    const int lanes = p.lanes, c = threadIdx.x & (lanes - 1), turning = p.R / 8;
-    const bool live = c * 8 < p.H, turns = c < turning;
-    // the thread's two runs of four elements
-    const int e0 = p.interleaved || !turns ? 8 * c : 4 * c, e1 = p.interleaved || !turns ? e0 + 4 : p.R / 2 + 4 * c;
-    float w[8], sum[BWD ? 8 : 1] = {};
+// each, both members of four pairs among them, so that a row is in registers once and its elements meet only in the sums of its statistics.
+constexpr int kGroupThreads = 256;
+
+// What a thread keeps for all its rows.
+template <class T, bool BWD>
+struct Lane {
+    int c, e0, e1;  // its place in the row, its two runs of four elements
+    bool live, turns;
+    float w[8], sum[BWD ? 8 : 1];
+
+    __device__ __forceinline__ Lane(const RopeArgs& p, const RopeSide& q) {
+        c = threadIdx.x & (p.lanes - 1), live = c * 8 < p.H, turns = c < p.R / 8;
+        const bool beside = p.interleaved || !turns;
+        e0 = beside ? 8 * c : 4 * c, e1 = beside ? e0 + 4 : p.R / 2 + 4 * c;
 #pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = live ? weight<T>(q, e0 + j) : 0.0f, w[4 + j] = live ? weight<T>(q, e1 + j) : 0.0f;
-    const int chunks = (q.heads + HEADS - 1) / HEADS, groups = kGroupThreads / lanes;
-    const long long tasks = (long long)p.batch * p.seq * chunks;
-    const float per = 1.0f / (float)p.H;
-    for (long long base = (long long)block * groups; base < tasks; base += (long long)q.blocks * groups) {
-        const long long mine = base + threadIdx.x / lanes;
-        const bool there = mine < tasks && live;
-        const unsigned task = (unsigned)(mine < tasks ? mine : tasks - 1), token = task / chunks;
-        const int n0 = (int)(task - token * chunks) * HEADS, b = (int)(token / p.seq), s = (int)(token - (unsigned)b * p.seq);
-        const T* from = (const T*)q.x + b * q.x_b + s * q.x_s + n0 * q.x_n;
-        const T* grad = BWD ? (const T*)q.dy + b * q.dy_b + s * q.dy_s + n0 * q.dy_n : nullptr;
-        Four<T> x_in[HEADS][2], g_in[BWD ? HEADS : 1][2];
+        for (int j = 0; j < 4; j++) w[j] = live ? weight<T>(q, e0 + j) : 0.0f, w[4 + j] = live ? weight<T>(q, e1 + j) : 0.0f;
+        if (BWD) {
 #pragma unroll
-        for (int k = 0; k < HEADS; k++)
-            if (there && n0 + k < q.heads) {
-                x_in[k][0].load(from + k * q.x_n + e0), x_in[k][1].load(from + k * q.x_n + e1);
-                if (BWD) g_in[k][0].load(grad + k * q.dy_n + e0), g_in[k][1].load(grad + k * q.dy_n + e1);
-            }
-        float cs[4], sn[4];
-        if (there && turns) {
-            const long long at = table_row(p, b, s);
-            Four<float> t;
-            t.load(p.cos + at * p.ld_cos + 4 * c), t.widen(cs);
-            t.load(p.sin + at * p.ld_sin + 4 * c), t.widen(sn);
-        }
-        T* to = (T*)q.out + b * q.out_b + s * q.out_s + n0 * q.out_n;
-#pragma unroll
-        for (int k = 0; k < HEADS; k++) {
-            const bool past = n0 + k >= q.heads;  // every lane of the warp votes
-            if (__all_sync(0xffffffffu, past)) break;
-            const bool row = there && n0 + k < q.heads;
-            float x[8], y[8], ss = 0.0f, dot = 0.0f;
-            if (row) {
-                x_in[k][0].widen(x), x_in[k][1].widen(x + 4);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) ss += x[j] * x[j];
-            if (BWD) {  // y: dz
-                if (row) g_in[k][0].widen(y), g_in[k][1].widen(y + 4);
-                if (row && turns) turn(y, cs, sn, p.interleaved, true);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (!row) y[j] = 0.0f;
-                    dot += y[j] * w[j] * x[j];
-                }
-            }
-            for (int d = lanes >> 1; d; d >>= 1) {
-                ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                if (BWD) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-            }
-            const float r = 1.0f / sqrtf(ss * per + p.eps);
-            if (!BWD) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = x[j] * r * w[j];
-                if (turns) turn(y, cs, sn, p.interleaved, false);
-            } else {
-                const float mean = dot * r * per;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float unit = x[j] * r;
-                    sum[j] += row ? y[j] * unit : 0.0f;
-                    y[j] = r * (y[j] * w[j] - unit * mean);
-                }
-            }
-            if (row) Four<T>::store(to + k * q.out_n + e0, y), Four<T>::store(to + k * q.out_n + e1, y + 4);
+            for (int j = 0; j < 8; j++) sum[j] = 0.0f;
         }
     }
-    if (BWD && q.w) {  // [group][H]
-        const int g = threadIdx.x / lanes;
+    // One row, executed by the whole warp: x and, backward, y = dy go in (zeros where `there` is none), y = the result comes out.
+    __device__ __forceinline__ void row(const RopeArgs& p, bool there, float* x, float* y, const float* cs, const float* sn) {
+        const float per = 1.0f / (float)p.H;
+        float ss = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) ss += x[j] * x[j];
+        if (BWD) {
+            if (turns) turn(y, cs, sn, p.interleaved, true);  // dz
+#pragma unroll
+            for (int j = 0; j < 8; j++) dot += y[j] * w[j] * x[j];
+        }
+        for (int d = p.lanes >> 1; d; d >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, d);
+            if (BWD) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        }
+        const float r = there ? 1.0f / sqrtf(ss * per + p.eps) : 0.0f;  // (no row leaves no sum, with eps = 0 either)
+        if (!BWD) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = x[j] * r * w[j];
+            if (turns) turn(y, cs, sn, p.interleaved, false);
+        } else {
+            const float mean = dot * r * per;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float unit = x[j] * r;
+                sum[j] += y[j] * unit;
+                y[j] = r * (y[j] * w[j] - unit * mean);
+            }
+        }
+    }
+    // A block's sums of dw, all threads: [group][H] in shared memory, its rows added up.
+    __device__ __forceinline__ void leave(const RopeArgs& p, const RopeSide& q, int block, float* held) {
+        __syncthreads();
+        const int groups = kGroupThreads / p.lanes, g = threadIdx.x / p.lanes;
         if (live) {
 #pragma unroll
             for (int j = 0; j < 4; j++) held[g * p.H + e0 + j] = sum[j], held[g * p.H + e1 + j] = sum[4 + j];
@@ -294,6 +264,144 @@ __global__ void __launch_bounds__(kGroupThreads, kGroupBlocks) rope_groups_kerne
             for (int k = 0; k < groups; k++) t += held[k * p.H + i];
             q.partial[(long long)block * p.H + i] = t;
         }
+    }
+};
+
+// Few rows: one a group of lanes at a time, its loads straight into registers.
+template <class T, bool BWD>
+__global__ void __launch_bounds__(kGroupThreads, 3) rope_few_kernel(const RopeArgs p) {
+    __shared__ float held[BWD ? kGroupThreads * 8 : 1];
+    grid_wait();
+    const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
+    const RopeSide& q = p.side[side];
+    const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
+    Lane<T, BWD> lane(p, q);
+    const long long rows = (long long)p.batch * p.seq * q.heads;
+    for (long long base = (long long)block * groups; base < rows; base += (long long)q.blocks * groups) {
+        const long long mine = base + threadIdx.x / p.lanes;
+        const bool there = mine < rows && lane.live;
+        const unsigned row = (unsigned)(mine < rows ? mine : rows - 1), token = row / q.heads;
+        const int n = (int)(row - token * q.heads), b = (int)(token / p.seq), s = (int)(token - (unsigned)b * p.seq);
+        float x[8] = {}, y[8] = {}, cs[4] = {}, sn[4] = {};  // (zeros turn zeros into zeros)
+        Four<T> in[2], grad[2];
+        Four<float> turned[2];
+        if (there) {
+            const T* from = (const T*)q.x + b * q.x_b + s * q.x_s + n * q.x_n;
+            in[0].load(from + lane.e0), in[1].load(from + lane.e1);
+            if (BWD) {
+                const T* g = (const T*)q.dy + b * q.dy_b + s * q.dy_s + n * q.dy_n;
+                grad[0].load(g + lane.e0), grad[1].load(g + lane.e1);
+            }
+            if (lane.turns) {
+                const long long at = table_row(p, b, s);
+                turned[0].load(p.cos + at * p.ld_cos + 4 * lane.c), turned[1].load(p.sin + at * p.ld_sin + 4 * lane.c);
+            }
+            in[0].widen(x), in[1].widen(x + 4);
+            if (BWD) grad[0].widen(y), grad[1].widen(y + 4);
+            if (lane.turns) turned[0].widen(cs), turned[1].widen(sn);
+        }
+        lane.row(p, there, x, y, cs, sn);
+        if (there) {
+            T* to = (T*)q.out + b * q.out_b + s * q.out_s + n * q.out_n;
+            Four<T>::store(to + lane.e0, y), Four<T>::store(to + lane.e1, y + 4);
+        }
+    }
+    if (BWD && q.w) lane.leave(p, q, block, held);
+}
+
+// Many rows: a group of lanes takes HEADS heads of a token at a time, which turn by the same angles, and has the next token's (or the next
+// heads') rows on their way into shared memory meanwhile: every thread copies what it reads itself, so that it waits for nobody else.
+__device__ __forceinline__ void copy_async(void* to, const void* from, int bytes) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+    const size_t src = __cvta_generic_to_global(from);
+    if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(src) : "memory");
+}
+template <class T, bool BWD>
+constexpr int many_heads() { return sizeof(T) == 2 ? 4 : 2; }
+template <class T, bool BWD>
+constexpr int many_smem() { return 2 * many_heads<T, BWD>() * (BWD ? 4 : 2) * kGroupThreads * (int)sizeof(Four<T>); }
+template <class T, bool BWD>
+__global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeArgs p) {
+    constexpr int HEADS = many_heads<T, BWD>(), RUNS = BWD ? 4 : 2, STAGE = HEADS * RUNS * kGroupThreads;
+    extern __shared__ __align__(16) uint8_t smem[];
+    Four<T>* ring = (Four<T>*)smem + threadIdx.x;  // [stage][head][run][thread]
+    grid_wait();
+    const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
+    const RopeSide& q = p.side[side];
+    const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
+    Lane<T, BWD> lane(p, q);
+    const unsigned chunks = q.by_chunks.d, tasks = (unsigned)(p.batch * p.seq) * chunks, step = (unsigned)(q.blocks * groups);
+    unsigned task = (unsigned)(block * groups + threadIdx.x / p.lanes);
+    const unsigned rounds = (tasks - min(tasks, (unsigned)(block * groups)) + step - 1) / step;  // the same for the whole block
+
+    struct Place {
+        int b, s, n0;
+    };
+    auto place = [&](unsigned t) {
+        const unsigned token = q.by_chunks.div(t), b = p.by_seq.div(token);
+        return Place{(int)b, (int)(token - b * p.seq), (int)(t - token * chunks) * HEADS};
+    };
+    auto fetch = [&](const Place& at, int stage) {
+        const T* from = (const T*)q.x + at.b * q.x_b + at.s * q.x_s + at.n0 * q.x_n;
+        const T* grad = BWD ? (const T*)q.dy + at.b * q.dy_b + at.s * q.dy_s + at.n0 * q.dy_n : nullptr;
+        Four<T>* to = ring + stage * STAGE;
+#pragma unroll
+        for (int k = 0; k < HEADS; k++)
+            if (lane.live && at.n0 + k < q.heads) {
+                copy_async(to + (k * RUNS + 0) * kGroupThreads, from + k * q.x_n + lane.e0, sizeof(Four<T>));
+                copy_async(to + (k * RUNS + 1) * kGroupThreads, from + k * q.x_n + lane.e1, sizeof(Four<T>));
+                if (BWD) {
+                    copy_async(to + (k * RUNS + RUNS - 2) * kGroupThreads, grad + k * q.dy_n + lane.e0, sizeof(Four<T>));
+                    copy_async(to + (k * RUNS + RUNS - 1) * kGroupThreads, grad + k * q.dy_n + lane.e1, sizeof(Four<T>));
+                }
+            }
+    };
+    // angles one task ahead, the position that they are found by two
+    Four<float> cs_next{make_float4(0.0f, 0.0f, 0.0f, 0.0f)}, sn_next = cs_next;
+    auto angles = [&](int at) {
+        if (lane.turns) cs_next.load(p.cos + at * p.ld_cos + 4 * lane.c), sn_next.load(p.sin + at * p.ld_sin + 4 * lane.c);
+    };
+    auto position = [&](unsigned t) {
+        const Place at = place(t);
+        return table_row(p, at.b, at.s);
+    };
+    Place here = {}, next = {};
+    int after = 0;
+    if (task < tasks) next = place(task), fetch(next, 0), angles(position(task));
+    if (task < tasks && tasks - task > step) after = position(task + step);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (unsigned round = 0; round < rounds; round++, task += step) {
+        const bool there = task < tasks && lane.live;
+        here = next;
+        float cs[4], sn[4];
+        cs_next.widen(cs), sn_next.widen(sn);
+        if (task < tasks && tasks - task > step) {
+            next = place(task + step);
+            fetch(next, (round + 1) & 1);
+            angles(after);
+            if (tasks - task - step > step) after = position(task + 2 * step);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        T* to = (T*)q.out + here.b * q.out_b + here.s * q.out_s + here.n0 * q.out_n;
+        const Four<T>* held = ring + (round & 1) * STAGE;
+#pragma unroll
+        for (int k = 0; k < HEADS; k++) {
+            const bool row = there && here.n0 + k < q.heads;
+            if (!__any_sync(0xffffffffu, row)) break;
+            float x[8] = {}, y[8] = {};
+            if (row) {
+                held[(k * RUNS + 0) * kGroupThreads].widen(x), held[(k * RUNS + 1) * kGroupThreads].widen(x + 4);
+                if (BWD) held[(k * RUNS + RUNS - 2) * kGroupThreads].widen(y), held[(k * RUNS + RUNS - 1) * kGroupThreads].widen(y + 4);
+            }
+            lane.row(p, row, x, y, cs, sn);
+            if (row) Four<T>::store(to + k * q.out_n + lane.e0, y), Four<T>::store(to + k * q.out_n + lane.e1, y + 4);
+        }
+    }
+    if (BWD && q.w) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        lane.leave(p, q, block, (float*)smem);
     }
 }
 
@@ -431,14 +539,18 @@ void launch_rope(RopeCall& c, cudaStream_t stream) {
     if (c.rows && in_pieces(p, c.dtype, BWD)) {
         p.lanes = 1;
         while (p.lanes * 8 < p.H) p.lanes *= 2;
-        constexpr int kHeads = BWD ? 2 : 4, kPerSm = kGroupBlocks;
+        constexpr int kHeads = many_heads<T, BWD>(), kPerSm = 3;
         const int groups = kGroupThreads / p.lanes;
         if (c.rows >= (long long)sms * kPerSm * groups * kHeads) {
+            if (first_use_on_device((const void*)rope_many_kernel<T, BWD>))
+                LB_CUDA(cudaFuncSetAttribute(rope_many_kernel<T, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, many_smem<T, BWD>()));
             share_blocks(p, groups, kHeads, sms, kPerSm);
-            launch_overlapped(rope_groups_kernel<T, BWD, kHeads>, blocks(), dim3(kGroupThreads), 0, stream, 0, p);
+            p.by_seq.set((uint32_t)std::max(p.seq, 1));
+            for (RopeSide& q : p.side) q.by_chunks.set((uint32_t)std::max((q.heads + kHeads - 1) / kHeads, 1));
+            launch_overlapped(rope_many_kernel<T, BWD>, blocks(), dim3(kGroupThreads), (many_smem<T, BWD>()), stream, 0, p);
         } else {
             share_blocks(p, groups, 1, sms, kPerSm);
-            launch_overlapped(rope_groups_kernel<T, BWD, 1>, blocks(), dim3(kGroupThreads), 0, stream, 0, p);
+            launch_overlapped(rope_few_kernel<T, BWD>, blocks(), dim3(kGroupThreads), 0, stream, 0, p);
         }
     } else if (c.rows) {
         share_blocks(p, kRowWarps, 1, sms, kBlocksPerSm);

@@ -199,6 +199,18 @@ def test_nothing_to_do(cuda, shape):
     assert bool((dwk == 0).all()) and (q.numel() > 0 or bool((dwq == 0).all()))  # an empty sum
 
 
+@pytest.mark.parametrize("s", [3, 3001])
+@pytest.mark.parametrize("h", [64, 72, 31])
+def test_no_eps(cuda, h, s):
+    """eps = 0, heads that no group divides: what has no row adds nothing to the weights' gradients."""
+    q, k, dq, dk, g = case(cuda, 1, s, 9, 3, h, torch.float32)
+    cos, sin = tables(s, h // 2 // 4 * 4, cuda)
+    w = 1 + 0.3 * torch.randn(h, generator=g, device=cuda)
+    zero = qk_norm_rope_backward(dq, dk, q, k, cos, sin, q_weight=w, k_weight=w, eps=0.0)
+    some = qk_norm_rope_backward(dq, dk, q, k, cos, sin, q_weight=w, k_weight=w, eps=1e-30)  # float32 sees no difference
+    assert all(torch.equal(a, b) and bool(a.isfinite().all()) for a, b in zip(zero, some))
+
+
 @pytest.mark.parametrize("h, interleaved", [(64, False), (80, True), (31, False)])
 def test_gradients_against_differences(cuda, h, interleaved):
     q, k, dq, dk, g = case(cuda, 2, 3, 2, 1, h, torch.float32)
