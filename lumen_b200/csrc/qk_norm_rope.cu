@@ -149,54 +149,86 @@ __global__ void __launch_bounds__(kRowWarps * 32) rope_rows_kernel(const RopeArg
     }
 }
 
-// A thread's four pairs turned, (v[j], v[4 + j]) or neighbours; BACK: the other way.
-__device__ __forceinline__ void turn(float* v, const float* c, const float* s, bool neighbours, bool back) {
-    if (neighbours) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float a = v[2 * j], b = v[2 * j + 1], n = back ? -s[j] : s[j];
-            v[2 * j] = a * c[j] - b * n, v[2 * j + 1] = b * c[j] + a * n;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float a = v[j], b = v[4 + j], n = back ? -s[j] : s[j];
-            v[j] = a * c[j] - b * n, v[4 + j] = b * c[j] + a * n;
-        }
-    }
+// Two float32 values in one register pair: an instruction for both (fused multiply-add, product), each rounded as by itself.
+struct Pair {
+    unsigned long long v;
+};
+__device__ __forceinline__ Pair both(float lo, float hi) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
 }
+__device__ __forceinline__ float2 apart(Pair a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator-(Pair a) { return {a.v ^ 0x8000000080000000ull}; }
 
-// Four elements of a row as float32 and back; the address is a multiple of their size.
+// Four elements of a row, as two pairs of float32 and back; the address is a multiple of their size.
 template <class T> struct Four;
 template <> struct Four<float> {
     float4 v;
     __device__ __forceinline__ void load(const float* p) { v = *(const float4*)p; }
-    __device__ __forceinline__ void widen(float* x) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
-    __device__ __forceinline__ static void store(float* p, const float* x) { *(float4*)p = make_float4(x[0], x[1], x[2], x[3]); }
+    __device__ __forceinline__ void widen(Pair* x) const { x[0] = both(v.x, v.y), x[1] = both(v.z, v.w); }
+    __device__ __forceinline__ static void store(float* p, const Pair* x) {
+        const float2 lo = apart(x[0]), hi = apart(x[1]);
+        *(float4*)p = make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
 };
 template <> struct Four<__nv_bfloat16> {
     uint2 v;
     __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *(const uint2*)p; }
-    __device__ __forceinline__ void widen(float* x) const {
-        x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u), x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+    __device__ __forceinline__ void widen(Pair* x) const {
+        x[0] = both(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u)), x[1] = both(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
     }
-    __device__ __forceinline__ static void store(__nv_bfloat16* p, const float* x) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+    __device__ __forceinline__ static void store(__nv_bfloat16* p, const Pair* x) {
+        const __nv_bfloat162 lo = __float22bfloat162_rn(apart(x[0])), hi = __float22bfloat162_rn(apart(x[1]));
         *(uint2*)p = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
     }
 };
 template <> struct Four<__half> {
     uint2 v;
     __device__ __forceinline__ void load(const __half* p) { v = *(const uint2*)p; }
-    __device__ __forceinline__ void widen(float* x) const {
+    __device__ __forceinline__ void widen(Pair* x) const {
         const float2 lo = __half22float2(*(const __half2*)&v.x), hi = __half22float2(*(const __half2*)&v.y);
-        x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+        x[0] = both(lo.x, lo.y), x[1] = both(hi.x, hi.y);
     }
-    __device__ __forceinline__ static void store(__half* p, const float* x) {
-        const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
+    __device__ __forceinline__ static void store(__half* p, const Pair* x) {
+        const __half2 lo = __float22half2_rn(apart(x[0])), hi = __float22half2_rn(apart(x[1]));
         *(uint2*)p = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
     }
 };
+
+// A thread's four pairs turned: the first of two pairs in v[0], v[1], the seconds in v[2], v[3], or neighbours in one register pair each; BACK: the
+// other way.
+template <bool BACK>
+__device__ __forceinline__ void turn(Pair* v, const Pair* c, const Pair* s, bool neighbours) {
+    if (neighbours) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 x = apart(v[j]), cc = apart(c[j / 2]), ss = apart(s[j / 2]);
+            const float cj = j % 2 ? cc.y : cc.x, sj = BACK ? -(j % 2 ? ss.y : ss.x) : (j % 2 ? ss.y : ss.x);
+            v[j] = fma2(both(x.y, x.x), both(-sj, sj), v[j] * both(cj, cj));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const Pair a = v[j], b = v[2 + j], n = BACK ? -s[j] : s[j];
+            v[j] = fma2(-n, b, a * c[j]), v[2 + j] = fma2(n, a, b * c[j]);
+        }
+    }
+}
 
 // Head dims and rotated parts that are multiples of 8, rows of aligned pieces of four elements: `p.lanes` lanes of a warp a row (a power of two), eight elements
 // each, both members of four pairs among them, so that a row is in registers once and its elements meet only in the sums of its statistics.
@@ -207,46 +239,55 @@ template <class T, bool BWD>
 struct Lane {
     int c, e0, e1;  // its place in the row, its two runs of four elements
     bool live, turns;
-    float w[8], sum[BWD ? 8 : 1];
+    Pair w[4], sum[BWD ? 4 : 1];
 
     __device__ __forceinline__ Lane(const RopeArgs& p, const RopeSide& q) {
         c = threadIdx.x & (p.lanes - 1), live = c * 8 < p.H, turns = c < p.R / 8;
         const bool beside = p.interleaved || !turns;
         e0 = beside ? 8 * c : 4 * c, e1 = beside ? e0 + 4 : p.R / 2 + 4 * c;
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = live ? weight<T>(q, e0 + j) : 0.0f, w[4 + j] = live ? weight<T>(q, e1 + j) : 0.0f;
-        if (BWD) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) sum[j] = 0.0f;
+        for (int j = 0; j < 4; j++) {
+            const int i = j < 2 ? e0 + 2 * j : e1 + 2 * (j - 2);
+            w[j] = live ? both(weight<T>(q, i), weight<T>(q, i + 1)) : both(0.0f, 0.0f);
+            if (BWD) sum[j] = both(0.0f, 0.0f);
         }
     }
-    // One row, executed by the whole warp: x and, backward, y = dy go in (zeros where `there` is none), y = the result comes out.
-    __device__ __forceinline__ void row(const RopeArgs& p, bool there, float* x, float* y, const float* cs, const float* sn) {
-        const float per = 1.0f / (float)p.H;
-        float ss = 0.0f, dot = 0.0f;
+    // One row, executed by the whole warp: x and, backward, y = dy go in, y = the result comes out. Zeros go in where a lane has no part of its row;
+    // where there is no row (`there`), whatever goes in stays among the lanes that would have it. 1 / sqrt by the hardware's 2^-22 and a Newton step.
+    __device__ __forceinline__ void row(const RopeArgs& p, float per, bool there, const Pair* x, Pair* y, const Pair* cs, const Pair* sn) {
+        Pair squares = x[0] * x[0], products;
 #pragma unroll
-        for (int j = 0; j < 8; j++) ss += x[j] * x[j];
+        for (int j = 1; j < 4; j++) squares = fma2(x[j], x[j], squares);
         if (BWD) {
-            if (turns) turn(y, cs, sn, p.interleaved, true);  // dz
+            if (turns) turn<true>(y, cs, sn, p.interleaved);  // dz
+            products = y[0] * w[0] * x[0];
 #pragma unroll
-            for (int j = 0; j < 8; j++) dot += y[j] * w[j] * x[j];
+            for (int j = 1; j < 4; j++) products = fma2(y[j] * w[j], x[j], products);
         }
-        for (int d = p.lanes >> 1; d; d >>= 1) {
+        const float2 s2 = apart(squares), d2 = BWD ? apart(products) : make_float2(0.0f, 0.0f);
+        float ss = s2.x + s2.y, dot = d2.x + d2.y;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            if (d >= p.lanes) continue;
             ss += __shfl_xor_sync(0xffffffffu, ss, d);
             if (BWD) dot += __shfl_xor_sync(0xffffffffu, dot, d);
         }
-        const float r = there ? 1.0f / sqrtf(ss * per + p.eps) : 0.0f;  // (no row leaves no sum, with eps = 0 either)
+        const float v = ss * per + p.eps;
+        float r = rsqrtf(v);
+        if (v > 1e-30f && v < 1e30f) r *= 1.5f - 0.5f * v * r * r;
+        const Pair rr = both(r, r);
         if (!BWD) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = x[j] * r * w[j];
-            if (turns) turn(y, cs, sn, p.interleaved, false);
+            for (int j = 0; j < 4; j++) y[j] = x[j] * rr * w[j];
+            if (turns) turn<false>(y, cs, sn, p.interleaved);
         } else {
-            const float mean = dot * r * per;
+            const float mean = -dot * r * per * r;
+            const Pair mm = both(mean, mean);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float unit = x[j] * r;
-                sum[j] += y[j] * unit;
-                y[j] = r * (y[j] * w[j] - unit * mean);
+            for (int j = 0; j < 4; j++) {
+                const Pair unit = x[j] * rr;
+                if (there) sum[j] = fma2(y[j], unit, sum[j]);
+                y[j] = fma2(unit, mm, y[j] * w[j] * rr);
             }
         }
     }
@@ -256,7 +297,7 @@ struct Lane {
         const int groups = kGroupThreads / p.lanes, g = threadIdx.x / p.lanes;
         if (live) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) held[g * p.H + e0 + j] = sum[j], held[g * p.H + e1 + j] = sum[4 + j];
+            for (int j = 0; j < 4; j++) *(float2*)(held + g * p.H + (j < 2 ? e0 + 2 * j : e1 + 2 * (j - 2))) = apart(sum[j]);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < p.H; i += kGroupThreads) {
@@ -276,13 +317,14 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_few_kernel(const RopeAr
     const RopeSide& q = p.side[side];
     const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
     Lane<T, BWD> lane(p, q);
+    const float per = 1.0f / (float)p.H;
     const long long rows = (long long)p.batch * p.seq * q.heads;
     for (long long base = (long long)block * groups; base < rows; base += (long long)q.blocks * groups) {
         const long long mine = base + threadIdx.x / p.lanes;
         const bool there = mine < rows && lane.live;
         const unsigned row = (unsigned)(mine < rows ? mine : rows - 1), token = row / q.heads;
         const int n = (int)(row - token * q.heads), b = (int)(token / p.seq), s = (int)(token - (unsigned)b * p.seq);
-        float x[8] = {}, y[8] = {}, cs[4] = {}, sn[4] = {};  // (zeros turn zeros into zeros)
+        Pair x[4] = {}, y[4] = {}, cs[2] = {}, sn[2] = {};
         Four<T> in[2], grad[2];
         Four<float> turned[2];
         if (there) {
@@ -296,14 +338,14 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_few_kernel(const RopeAr
                 const long long at = table_row(p, b, s);
                 turned[0].load(p.cos + at * p.ld_cos + 4 * lane.c), turned[1].load(p.sin + at * p.ld_sin + 4 * lane.c);
             }
-            in[0].widen(x), in[1].widen(x + 4);
-            if (BWD) grad[0].widen(y), grad[1].widen(y + 4);
+            in[0].widen(x), in[1].widen(x + 2);
+            if (BWD) grad[0].widen(y), grad[1].widen(y + 2);
             if (lane.turns) turned[0].widen(cs), turned[1].widen(sn);
         }
-        lane.row(p, there, x, y, cs, sn);
+        lane.row(p, per, there, x, y, cs, sn);
         if (there) {
             T* to = (T*)q.out + b * q.out_b + s * q.out_s + n * q.out_n;
-            Four<T>::store(to + lane.e0, y), Four<T>::store(to + lane.e1, y + 4);
+            Four<T>::store(to + lane.e0, y), Four<T>::store(to + lane.e1, y + 2);
         }
     }
     if (BWD && q.w) lane.leave(p, q, block, held);
@@ -331,6 +373,7 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
     const RopeSide& q = p.side[side];
     const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
     Lane<T, BWD> lane(p, q);
+    const float per = 1.0f / (float)p.H;
     const unsigned chunks = q.by_chunks.d, tasks = (unsigned)(p.batch * p.seq) * chunks, step = (unsigned)(q.blocks * groups);
     unsigned task = (unsigned)(block * groups + threadIdx.x / p.lanes);
     const unsigned rounds = (tasks - min(tasks, (unsigned)(block * groups)) + step - 1) / step;  // the same for the whole block
@@ -366,6 +409,8 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
         const Place at = place(t);
         return table_row(p, at.b, at.s);
     };
+    if (!lane.live)  // nothing is copied for lanes behind the row's end
+        for (int k = 0; k < 2 * HEADS * RUNS; k++) ring[k * kGroupThreads] = Four<T>{};
     Place here = {}, next = {};
     int after = 0;
     if (task < tasks) next = place(task), fetch(next, 0), angles(position(task));
@@ -374,7 +419,7 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
     for (unsigned round = 0; round < rounds; round++, task += step) {
         const bool there = task < tasks && lane.live;
         here = next;
-        float cs[4], sn[4];
+        Pair cs[2], sn[2];
         cs_next.widen(cs), sn_next.widen(sn);
         if (task < tasks && tasks - task > step) {
             next = place(task + step);
@@ -390,13 +435,11 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
         for (int k = 0; k < HEADS; k++) {
             const bool row = there && here.n0 + k < q.heads;
             if (!__any_sync(0xffffffffu, row)) break;
-            float x[8] = {}, y[8] = {};
-            if (row) {
-                held[(k * RUNS + 0) * kGroupThreads].widen(x), held[(k * RUNS + 1) * kGroupThreads].widen(x + 4);
-                if (BWD) held[(k * RUNS + RUNS - 2) * kGroupThreads].widen(y), held[(k * RUNS + RUNS - 1) * kGroupThreads].widen(y + 4);
-            }
-            lane.row(p, row, x, y, cs, sn);
-            if (row) Four<T>::store(to + k * q.out_n + lane.e0, y), Four<T>::store(to + k * q.out_n + lane.e1, y + 4);
+            Pair x[4], y[4];
+            held[(k * RUNS + 0) * kGroupThreads].widen(x), held[(k * RUNS + 1) * kGroupThreads].widen(x + 2);
+            if (BWD) held[(k * RUNS + RUNS - 2) * kGroupThreads].widen(y), held[(k * RUNS + RUNS - 1) * kGroupThreads].widen(y + 2);
+            lane.row(p, per, row, x, y, cs, sn);
+            if (row) Four<T>::store(to + k * q.out_n + lane.e0, y), Four<T>::store(to + k * q.out_n + lane.e1, y + 2);
         }
     }
     if (BWD && q.w) {
