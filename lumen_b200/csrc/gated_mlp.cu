@@ -148,6 +148,9 @@ void sized(const lb_tensor& t, long long rows, long long cols, int dtype, const 
     if (rows && cols && (uintptr_t)t.ptr % dtype_size(dtype)) refuse(format("%s is not aligned to its elements", what));
 }
 
+// Whether the products with the gate in their epilogue are taken, where the layouts are theirs.
+bool gated_tiles(long long M) { return M > 128; }
+
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 size_t product_scratch(const lb_tensor& a, const lb_tensor& b) { return lb_gemm_operands_scratch_bytes(&a, &b); }
 
@@ -176,7 +179,7 @@ struct Block {
 
 struct Forward : Block {
     lb_tensor y, gate_up{}, h;
-    bool keeps;
+    bool keeps, fused = false;
     size_t sums = 0;  // bytes of [a b] in float32
 
     Forward(int act, const lb_tensor* x_t, const lb_tensor* wgu_t, const lb_tensor* wd_t, const lb_tensor* y_t, const lb_tensor* gate_up_t, const lb_tensor* h_t)
@@ -184,12 +187,18 @@ struct Forward : Block {
         sized(y, M, D, dtype, "y"), written(y, "y"), sized(h, M, F, dtype, "h"), written(h, "h");
         if (keeps) gate_up = as_rows(gate_up_t, "gate_up"), sized(gate_up, M, 2 * F, dtype, "gate_up"), written(gate_up, "gate_up");
         if (M == 0) return;
-        if (dtype != LB_F32 || !keeps) sums = up((size_t)M * 2 * F * 4);
-        products = std::max(product_scratch(x, transposed(wgu)), product_scratch(h, transposed(wd)));
+        fused = gated_tiles(M) && gemm_gated_takes(x, wgu, h, keeps ? &gate_up : nullptr);
+        if (!fused && (dtype != LB_F32 || !keeps)) sums = up((size_t)M * 2 * F * 4);
+        products = std::max(fused ? 0 : product_scratch(x, transposed(wgu)), product_scratch(h, transposed(wd)));
     }
     size_t bytes() const { return sums + products; }
     void run(const lb_tensor* residual, void* stream) {
         char* more = (char*)scratch + sums;
+        if (fused) {
+            gemm_gated(x, wgu, h, keeps ? &gate_up : nullptr, act, stream);
+            gemm(h, transposed(wd), y, residual ? EPI_ADD : EPI_NONE, 0, stream, more, products, residual, nullptr);
+            return;
+        }
         const lb_tensor pre = sums ? matrix(scratch, LB_F32, M, 2 * F, 2 * F) : gate_up;
         gemm(x, transposed(wgu), pre, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
         GateArgs g{};
@@ -202,6 +211,7 @@ struct Forward : Block {
 
 struct Backward : Block {
     lb_tensor dy, gate_up, h, dx, dwgu, dwd;
+    bool fused = false;
     size_t sums = 0, slopes = 0;  // bytes of dh in float32 and of [da db]
 
     Backward(int act, const lb_tensor* dy_t, const lb_tensor* x_t, const lb_tensor* wgu_t, const lb_tensor* wd_t, const lb_tensor* gate_up_t, const lb_tensor* h_t,
@@ -212,19 +222,25 @@ struct Backward : Block {
         if (gate_up.stride[1] != 1) fail(LB_ERR_UNSUPPORTED, "gated_mlp: gate_up must be row-major");
         sized(dx, M, D, dtype, "d_x"), written(dx, "d_x");
         sized(dwgu, 2 * F, D, dtype, "d_w_gate_up"), written(dwgu, "d_w_gate_up"), sized(dwd, D, F, dtype, "d_w_down"), written(dwd, "d_w_down");
-        sums = up((size_t)M * F * 4), slopes = up((size_t)M * 2 * F * dtype_size(dtype));
+        fused = M && gated_tiles(M) && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F));
+        sums = fused ? 0 : up((size_t)M * F * 4), slopes = up((size_t)M * 2 * F * dtype_size(dtype));
         const lb_tensor d = slope();
-        products = std::max(std::max(product_scratch(dy, wd), product_scratch(d, wgu)), std::max(product_scratch(transposed(d), x), product_scratch(transposed(dy), h)));
+        products = std::max(std::max(fused ? 0 : product_scratch(dy, wd), product_scratch(d, wgu)), std::max(product_scratch(transposed(d), x), product_scratch(transposed(dy), h)));
     }
     lb_tensor slope() const { return matrix((char*)scratch + sums, dtype, M, 2 * F, 2 * F); }
     size_t bytes() const { return sums + slopes + products; }
     void run(void* stream) {
         char* more = (char*)scratch + sums + slopes;
-        const lb_tensor dh = matrix(scratch, LB_F32, M, F, F), d = slope();
-        gemm(dy, wd, dh, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
-        GateArgs g{};
-        g.in = scratch, g.ld_in = F, g.gate_up = gate_up.ptr, g.ld_gate_up = gate_up.stride[0], g.gate_up_out = d.ptr, g.ld_out = 2 * F, g.M = (int)M, g.F = (int)F;
-        run_gate<true>(dtype, g, act, (cudaStream_t)stream);
+        const lb_tensor d = slope();
+        if (fused) {
+            gemm_sloped(dy, wd, gate_up, d, act, stream);
+        } else {
+            const lb_tensor dh = matrix(scratch, LB_F32, M, F, F);
+            gemm(dy, wd, dh, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
+            GateArgs g{};
+            g.in = scratch, g.ld_in = F, g.gate_up = gate_up.ptr, g.ld_gate_up = gate_up.stride[0], g.gate_up_out = d.ptr, g.ld_out = 2 * F, g.M = (int)M, g.F = (int)F;
+            run_gate<true>(dtype, g, act, (cudaStream_t)stream);
+        }
         gemm(d, wgu, dx, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
         gemm(transposed(d), x, dwgu, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
         gemm(transposed(dy), h, dwd, EPI_NONE, 0, stream, more, products, nullptr, nullptr);

@@ -18,6 +18,7 @@
 #include <mutex>
 
 #include "divide.cuh"
+#include "gate.cuh"
 #include "gemm.h"
 #include "launch.cuh"
 #include "sm100.cuh"
@@ -52,6 +53,27 @@ struct GemmArgs {
     // unit writes a float32 partial tile to `partial` [splits][batch][M][N] and splitk_reduce adds them in order
     int splits, kb_per_split;
     float* partial;
+};
+
+// What the kernel for CTA pairs does with a tile: the epilogues of lb_gemm, or one half of the gated feed-forward block. In its forward products
+// the leader's half of the B columns are rows of one weight and the other CTA's the same rows of another, so that each CTA's accumulator holds both
+// projections of 128 columns side by side; in its backward product the epilogue reads what the forward pass has kept.
+enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED };
+struct PlainArgs : GemmArgs {
+    static constexpr int mode = PAIR_PLAIN;
+};
+struct alignas(64) GatedArgs : GemmArgs {
+    static constexpr int mode = PAIR_GATED;
+    CUtensorMap map_up;  // the other weight; N, d, ldd: the gated product's
+    int act;
+    void* kept;          // [gate, up], rows ld_kept apart; null: not kept
+    long long ld_kept;
+};
+struct SlopedArgs : GemmArgs {
+    static constexpr int mode = PAIR_SLOPED;
+    int act;
+    const void* kept;    // d, ldd: the gradient of both projections side by side
+    long long ld_kept;
 };
 
 // Unit `unit` of the grid: split * tiles + tile, neighbours share a K range.
@@ -237,6 +259,107 @@ __device__ __forceinline__ void drain_tile_aux(const GemmArgs& p, uint32_t tbase
             }
         }
         store_rows_coalesced<4>(stage, packed, out0 + c * 64, p.ldd * 2, 32, lane);
+    }
+}
+
+// ---- the gated feed-forward block's tiles ---------------------------------------------------------------------------
+// 32 float32 values rounded to 16 bits, two a word.
+__device__ __forceinline__ void round_columns(const uint32_t* v, uint32_t* w, bool f16) {
+    if (LB_RARELY(f16)) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+            w[j] = *(const uint32_t*)&h;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+            w[j] = *(const uint32_t*)&h;
+        }
+    }
+}
+template <int ACT>
+__device__ __forceinline__ void gate_columns(uint32_t* a, const uint32_t* b) {
+#pragma unroll
+    for (int j = 0; j < 32; j++) a[j] = __float_as_uint(activation<ACT, true>(__uint_as_float(a[j])) * __uint_as_float(b[j]));
+}
+// 64 columns of both projections (the gate's at `tbase`, the other's 128 columns further), their gated product, whole 128-byte row pieces each.
+// Rows are 16-byte aligned and N is a multiple of 8 (checked by the host).
+template <class Release>
+__device__ __forceinline__ void drain_gated(const GatedArgs& p, uint32_t tbase, int row, int col0, uint4* stage, int lane, Release release) {
+    uint4 gate[8], up[8], h[8];
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        uint32_t v[64];
+        tmem_ld_32x32(tbase + c * 32, v);
+        tmem_ld_32x32(tbase + BN / 2 + c * 32, v + 32);
+        tmem_ld_wait();
+        if (c == 1) release();
+        round_columns(v, (uint32_t*)(gate + 4 * c), p.d_f16), round_columns(v + 32, (uint32_t*)(up + 4 * c), p.d_f16);
+        if (p.act == ACT_SILU) gate_columns<ACT_SILU>(v, v + 32);
+        else if (p.act == ACT_GELU) gate_columns<ACT_GELU>(v, v + 32);
+        else gate_columns<ACT_RELU>(v, v + 32);
+        round_columns(v, (uint32_t*)(h + 4 * c), p.d_f16);
+    }
+    const int first = row - lane, rows = p.M - first, segs = (p.N - col0) / 8;
+    if (rows <= 0 || segs <= 0) return;
+    store_rows_coalesced<8>(stage, h, (uint8_t*)((uint16_t*)p.d + first * p.ldd + col0), p.ldd * 2, rows, lane, segs);
+    if (p.kept) {
+        uint16_t* out = (uint16_t*)p.kept + first * p.ld_kept + col0;
+        store_rows_coalesced<8>(stage, gate, (uint8_t*)out, p.ld_kept * 2, rows, lane, segs);
+        store_rows_coalesced<8>(stage, up, (uint8_t*)(out + p.N), p.ld_kept * 2, rows, lane, segs);
+    }
+}
+
+// Both projections' 32 columns of the warp's rows, as aux_load spreads them; zeros outside the matrix.
+__device__ __forceinline__ void kept_load(const SlopedArgs& p, int first, int col, int lane, uint4* gate, uint4* up) {
+    const uint16_t* at = (const uint16_t*)p.kept + first * p.ld_kept + col + (lane & 3) * 8;
+    const bool inside = col + (lane & 3) * 8 < p.N;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const int r = t * 8 + (lane >> 2);
+        const bool live = inside && first + r < p.M;
+        gate[t] = live ? *(const uint4*)(at + r * p.ld_kept) : make_uint4(0u, 0u, 0u, 0u);
+        up[t] = live ? *(const uint4*)(at + r * p.ld_kept + p.N) : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+__device__ __forceinline__ float half_of(uint32_t w, int k, bool f16) {
+    if (f16) return __half2float(__ushort_as_half((unsigned short)(w >> (16 * k))));
+    return __uint_as_float(k ? w & 0xffff0000u : w << 16);
+}
+// dh in v, both projections in a and b: v becomes the gate's gradient, w the other's.
+template <int ACT>
+__device__ __forceinline__ void slope_columns(uint32_t* v, const uint32_t* a, const uint32_t* b, uint32_t* w, bool f16) {
+#pragma unroll
+    for (int j = 0; j < 32; j++) {
+        float slope;
+        const float dh = __uint_as_float(v[j]), value = activation_slope<ACT, true>(half_of(a[j / 2], j % 2, f16), slope);
+        v[j] = __float_as_uint(dh * half_of(b[j / 2], j % 2, f16) * slope), w[j] = __float_as_uint(dh * value);
+    }
+}
+template <class Release>
+__device__ __forceinline__ void drain_sloped(const SlopedArgs& p, uint32_t tbase, int row, int col_base, uint4* gate, uint4* up, uint4* stage, int lane, Release release) {
+    const int first = row - lane, rows = p.M - first;
+    uint16_t* out = (uint16_t*)p.d + first * p.ldd + col_base;
+#pragma unroll 1
+    for (int c = 0; c < BN / 2 / 32; c++) {
+        uint32_t v[32], a[16], b[16], w[32];
+        tmem_ld_32x32(tbase + c * 32, v);
+        aux_to_rows(stage + 128, gate, a, lane), aux_to_rows(stage + 128, up, b, lane);
+        if (c + 1 < BN / 2 / 32) kept_load(p, first, col_base + (c + 1) * 32, lane, gate, up);
+        tmem_ld_wait();
+        if (c == BN / 2 / 32 - 1) release();
+        if (p.act == ACT_SILU) slope_columns<ACT_SILU>(v, a, b, w, p.d_f16);
+        else if (p.act == ACT_GELU) slope_columns<ACT_GELU>(v, a, b, w, p.d_f16);
+        else slope_columns<ACT_RELU>(v, a, b, w, p.d_f16);
+        const int segs = (p.N - col_base - c * 32) / 8;
+        if (rows <= 0 || segs <= 0) continue;
+        uint4 packed[4];
+        round_columns(v, (uint32_t*)packed, p.d_f16);
+        store_rows_coalesced<4>(stage, packed, (uint8_t*)(out + c * 32), p.ldd * 2, rows, lane, segs);
+        round_columns(w, (uint32_t*)packed, p.d_f16);
+        store_rows_coalesced<4>(stage, packed, (uint8_t*)(out + c * 32 + p.N), p.ldd * 2, rows, lane, segs);
     }
 }
 
@@ -434,8 +557,9 @@ constexpr int PSTAGES = 6;
 constexpr int kPairStageBytesA = BM * BK * 2, kPairStageBytesB = (BN / 2) * BK * 2;
 constexpr int kPairSmemBytes = PSTAGES * (kPairStageBytesA + kPairStageBytesB) + 1024 + 256 + kEpilogueStageBytes;
 
+template <class Args>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
+gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Args p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
     uint8_t* smem_a = smem;
@@ -467,6 +591,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         fence_barrier_init();
         tma_prefetch_desc(&map_a);
         tma_prefetch_desc(&map_b);
+        if constexpr (Args::mode == PAIR_GATED) tma_prefetch_desc(&p.map_up);
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_base_slot, 512);
@@ -488,7 +613,13 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             for (int unit = pair; unit < num_units && ok; unit += num_pairs) {
                 int b, m_blk, n_blk;
                 const int kb0 = tile_coords(p, unit, b, m_blk, n_blk) * p.kb_per_split;
-                const int row0 = m_blk * 2 * BM + (int)rank * BM, col0 = n_blk * BN + (int)rank * (BN / 2);
+                const int row0 = m_blk * 2 * BM + (int)rank * BM;
+                int col0 = n_blk * BN + (int)rank * (BN / 2);
+                const CUtensorMap* operand_b = &map_b;
+                if constexpr (Args::mode == PAIR_GATED) {
+                    col0 = n_blk * (BN / 2);
+                    if (rank) operand_b = &p.map_up;
+                }
                 const int kb1 = min(total_kb, kb0 + p.kb_per_split);
                 for (int kb = kb0; kb < kb1; kb++) {
                     if (!(ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag))) break;
@@ -502,10 +633,10 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                             tma_load_3d_pair(sa + j * (64 * BK * 2), &map_a, &full[stage], row0 + j * 64, kb * BK, b);
                     }
                     if (!p.b_mn_major) {
-                        tma_load_3d_pair(sb, &map_b, &full[stage], kb * BK, col0, b);  // box {64 k, 128 n}
+                        tma_load_3d_pair(sb, operand_b, &full[stage], kb * BK, col0, b);  // box {64 k, 128 n}
                     } else {
                         for (int j = 0; j < BN / 2 / 64; j++)  // boxes {64 n, 64 k}
-                            tma_load_3d_pair(sb + j * (64 * BK * 2), &map_b, &full[stage], col0 + j * 64, kb * BK, b);
+                            tma_load_3d_pair(sb + j * (64 * BK * 2), operand_b, &full[stage], col0 + j * 64, kb * BK, b);
                     }
                     if (++stage == PSTAGES) {
                         stage = 0;
@@ -568,24 +699,41 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             int b, m_blk, n_blk;
             const int split = tile_coords(p, unit, b, m_blk, n_blk);
             const int row = m_blk * 2 * BM + (int)rank * BM + quarter * 32 + lane;
-            const int col_base = n_blk * BN + col_half * (BN / 2);
-            const long long row_off = (long long)b * p.d_batch_stride + (long long)row * p.ldd;
-            const bool fast = __all_sync(0xffffffffu, aux_fast_path(p, row, col_base, vec_ok));  // warp-uniform: both drains load tensor memory warp-wide
-            const uint16_t* ax_warp = (const uint16_t*)p.aux + (long long)b * p.aux_batch_stride + (long long)(row - lane) * p.ld_aux + col_base;
-            uint4 raw[4];
-            if (fast) aux_load(ax_warp, p.ld_aux, lane, raw);
-            if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
-            __syncwarp();
-            tc_fence_after();
-            const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
             auto release = [&] {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(&tmem_empty[buf], 0);
             };
-            if (fast) drain_tile_aux(p, tbase, row_off + col_base, ax_warp, raw, stage, lane, release);
-            else if (LB_RARELY(p.splits > 1)) drain_partial(p, tbase, row, col_base, b, split, stage, lane, release);
-            else drain_tile(p, tbase, row, row_off, col_base, b, vec_ok, stage, lane, release);
+            if constexpr (Args::mode == PAIR_GATED) {
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 4));
+                drain_gated(p, tbase, row, n_blk * (BN / 2) + col_half * (BN / 4), stage, lane, release);
+            } else if constexpr (Args::mode == PAIR_SLOPED) {
+                const int col_base = n_blk * BN + col_half * (BN / 2);
+                uint4 gate[4], up[4];
+                kept_load(p, row - lane, col_base, lane, gate, up);
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                drain_sloped(p, tbase, row, col_base, gate, up, stage, lane, release);
+            } else {
+                const int col_base = n_blk * BN + col_half * (BN / 2);
+                const long long row_off = (long long)b * p.d_batch_stride + (long long)row * p.ldd;
+                const bool fast = __all_sync(0xffffffffu, aux_fast_path(p, row, col_base, vec_ok));  // warp-uniform: both drains load tensor memory warp-wide
+                const uint16_t* ax_warp = (const uint16_t*)p.aux + (long long)b * p.aux_batch_stride + (long long)(row - lane) * p.ld_aux + col_base;
+                uint4 raw[4];
+                if (fast) aux_load(ax_warp, p.ld_aux, lane, raw);
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                if (fast) drain_tile_aux(p, tbase, row_off + col_base, ax_warp, raw, stage, lane, release);
+                else if (LB_RARELY(p.splits > 1)) drain_partial(p, tbase, row, col_base, b, split, stage, lane, release);
+                else drain_tile(p, tbase, row, row_off, col_base, b, vec_ok, stage, lane, release);
+            }
         }
     }
 
@@ -792,7 +940,7 @@ static int resident_pairs(const DeviceInfo& dev) {
     int pairs = 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (dev.sms / 2), 1, 1), cfg.blockDim = dim3(kThreads, 1, 1), cfg.dynamicSmemBytes = kPairSmemBytes;
-    if (cudaOccupancyMaxActiveClusters(&pairs, gemm_tcgen05_pair, &cfg) != cudaSuccess || pairs <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&pairs, gemm_tcgen05_pair<PlainArgs>, &cfg) != cudaSuccess || pairs <= 0) {
         cudaGetLastError();
         pairs = 0;
     }
@@ -849,6 +997,14 @@ static bool tensor_core_operands(const View3& a, const View3& b, bool& a_cols, b
            a.rows <= INT32_MAX && b.cols <= INT32_MAX && a.cols <= INT32_MAX;
 }
 
+// The divisions by which a tile is found.
+static void set_raster(GemmArgs& p, long long tiles) {
+    p.by_tiles.set((uint32_t)tiles), p.by_batch.set((uint32_t)(p.tiles_m * p.tiles_n));
+    p.group_m = std::min(p.group_m, p.tiles_m);
+    p.by_group.set((uint32_t)(p.group_m * p.tiles_n)), p.by_rows.set((uint32_t)p.group_m);
+    p.by_last_rows.set((uint32_t)(p.tiles_m % p.group_m ? p.tiles_m % p.group_m : p.group_m));
+}
+
 // Kernels that gemm launches.
 int gemm_launches(const lb_tensor& a_t, const lb_tensor& b_t, size_t scratch_bytes, int kernel_choice, const GemmTuning* tuning) {
     const View3 a = view3(a_t, "a"), b = view3(b_t, "b");
@@ -896,7 +1052,7 @@ bool gemm(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& d_t, int 
     if (kernel_choice == 1 && !tc_ok) fail(LB_ERR_UNSUPPORTED, "gemm: the tcgen05 kernels need bfloat16 or float16 operands with a unit stride and 16-byte aligned rows");
 
     if (tc_ok) {
-        GemmArgs p{};
+        PlainArgs p{};
         p.M = (int)M, p.N = (int)N, p.K = (int)K, p.batch = (int)batch;
         p.a_mn_major = !a_cols;  // A [M, K]: contiguous columns = K-major
         p.b_mn_major = b_cols;   // B [K, N]: contiguous columns = N-major
@@ -933,9 +1089,9 @@ bool gemm(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& d_t, int 
             gemm_small(map_a, p.b_mn_major ? map_b : make_map(bt, true, BK, 64), q, (int)batch, dev.sms, s);
             return false;
         }
-        if (first_use_on_device((const void*)gemm_tcgen05_pair)) {
+        if (first_use_on_device((const void*)gemm_tcgen05_pair<PlainArgs>)) {
             LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
-            LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
+            LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<PlainArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
         }
         const int max_pairs = resident_pairs(dev);
         long long tiles = (long long)p.tiles_m * p.tiles_n * batch;
@@ -943,14 +1099,11 @@ bool gemm(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& d_t, int 
         p.splits = route.splits, p.kb_per_split = route.kb_per_split;
         p.partial = (float*)scratch;
         if (tiles * p.splits > INT32_MAX) fail(LB_ERR_UNSUPPORTED, "gemm: too many output tiles for one launch");
-        p.by_tiles.set((uint32_t)tiles), p.by_batch.set((uint32_t)(p.tiles_m * p.tiles_n));
-        p.group_m = std::min(p.group_m, p.tiles_m);
-        p.by_group.set((uint32_t)(p.group_m * p.tiles_n)), p.by_rows.set((uint32_t)p.group_m);
-        p.by_last_rows.set((uint32_t)(p.tiles_m % p.group_m ? p.tiles_m % p.group_m : p.group_m));
+        set_raster(p, tiles);
         if (pairs) {
             const int resident = max_pairs > 0 ? max_pairs : sms / 2;
             int grid = 2 * (int)std::min<long long>(tiles * p.splits, resident);
-            launch_overlapped(gemm_tcgen05_pair, dim3((unsigned)grid), dim3(kThreads), kPairSmemBytes, s, 0, map_a, map_b, p);
+            launch_overlapped(gemm_tcgen05_pair<PlainArgs>, dim3((unsigned)grid), dim3(kThreads), kPairSmemBytes, s, 0, map_a, map_b, p);
         } else {
             int grid = (int)std::min<long long>(tiles * p.splits, sms);
             launch_overlapped(gemm_tcgen05, dim3((unsigned)grid), dim3(kThreads), kSmemBytes, s, 0, map_a, map_b, p);
@@ -986,6 +1139,75 @@ bool gemm(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& d_t, int 
     }
     gemm_simt(a.ptr, b.ptr, a.dtype, p, device_info().sms, s);
     return false;
+}
+
+static View3 turned(View3 v) {
+    std::swap(v.rows, v.cols), std::swap(v.sr, v.sc);
+    return v;
+}
+// Rows of a result (or of what an epilogue reads) that the gated kernels take in 16-byte pieces.
+static bool in_pieces(const lb_tensor& t) { return (uintptr_t)t.ptr % 16 == 0 && (t.shape[0] <= 1 || t.stride[0] % 8 == 0) && t.stride[1] == 1; }
+
+// What both of the gated block's products set up: x [M, K] times w [N, K] transposed on CTA pairs, tiles of `tile_n` columns.
+static void pair_args(GemmArgs& p, const View3& x, const View3& w, bool x_cols, bool w_cols, int tile_n, long long& tiles) {
+    p.M = (int)x.rows, p.N = (int)w.rows, p.K = (int)x.cols, p.batch = 1;
+    p.a_mn_major = !x_cols, p.b_mn_major = !w_cols;
+    p.in_bf16 = p.d_bf16 = x.dtype == LB_BF16, p.d_f16 = x.dtype == LB_F16;
+    p.status = status_word();
+    p.tiles_m = (p.M + 2 * BM - 1) / (2 * BM), p.tiles_n = (p.N + tile_n - 1) / tile_n, p.group_m = 8;
+    p.splits = 1, p.kb_per_split = (p.K + BK - 1) / BK;
+    tiles = (long long)p.tiles_m * p.tiles_n;
+    if (tiles > INT32_MAX) fail(LB_ERR_UNSUPPORTED, "gemm: too many output tiles for one launch");
+    set_raster(p, tiles);
+}
+template <class Args>
+static void launch_pairs(const CUtensorMap& map_a, const CUtensorMap& map_b, const Args& p, long long tiles, void* stream) {
+    const DeviceInfo& dev = device_info();
+    if (first_use_on_device((const void*)gemm_tcgen05_pair<Args>))
+        LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
+    const int max_pairs = resident_pairs(dev), grid = 2 * (int)std::min<long long>(tiles, max_pairs > 0 ? max_pairs : dev.sms / 2);
+    launch_overlapped(gemm_tcgen05_pair<Args>, dim3((unsigned)grid), dim3(kThreads), kPairSmemBytes, (cudaStream_t)stream, 0, map_a, map_b, p);
+}
+
+bool gemm_gated_takes(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept) {
+    View3 half = view3(w, "w");
+    half.rows /= 2;
+    bool a_cols, b_cols;
+    return h.shape[1] % 8 == 0 && tensor_core_operands(view3(x, "x"), turned(half), a_cols, b_cols) && in_pieces(h) && (!kept || in_pieces(*kept));
+}
+void gemm_gated(const lb_tensor& x_t, const lb_tensor& w_t, const lb_tensor& h, const lb_tensor* kept, int act, void* stream) {
+    driver();
+    View3 x = view3(x_t, "x"), w = view3(w_t, "w");
+    w.rows /= 2;
+    View3 up = w;
+    up.ptr = (uint16_t*)w.ptr + w.rows * w.sr;
+    bool x_cols, w_rows;
+    tensor_core_operands(x, turned(w), x_cols, w_rows);
+    GatedArgs p{};
+    long long tiles;
+    pair_args(p, x, w, x_cols, !w_rows, BN / 2, tiles);
+    p.d = h.ptr, p.ldd = h.stride[0], p.act = act;
+    if (kept) p.kept = kept->ptr, p.ld_kept = kept->stride[0];
+    auto weight = [&](const View3& v) { return p.b_mn_major ? make_map(v, false, 64, BK) : make_map(v, true, BK, BN / 2); };
+    p.map_up = weight(up);
+    launch_pairs(p.a_mn_major ? make_map(x, false, 64, BK) : make_map(x, true, BK, BM), weight(w), p, tiles, stream);
+}
+
+bool gemm_sloped_takes(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d) {
+    bool a_cols, b_cols;
+    return w.shape[1] % 8 == 0 && tensor_core_operands(view3(dy, "dy"), view3(w, "w"), a_cols, b_cols) && in_pieces(kept) && in_pieces(d);
+}
+void gemm_sloped(const lb_tensor& dy_t, const lb_tensor& w_t, const lb_tensor& kept, const lb_tensor& d, int act, void* stream) {
+    driver();
+    const View3 dy = view3(dy_t, "dy"), b = view3(w_t, "w"), w = turned(b);
+    bool dy_cols, b_cols;
+    tensor_core_operands(dy, b, dy_cols, b_cols);
+    SlopedArgs p{};
+    long long tiles;
+    pair_args(p, dy, w, dy_cols, !b_cols, BN, tiles);
+    p.d = d.ptr, p.ldd = d.stride[0], p.act = act, p.kept = kept.ptr, p.ld_kept = kept.stride[0];
+    launch_pairs(p.a_mn_major ? make_map(dy, false, 64, BK) : make_map(dy, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p,
+                 tiles, stream);
 }
 
 }  // namespace lb

@@ -70,4 +70,12 @@ struct SmallGemmArgs {
 
 void gemm_small(const CUtensorMap& map_a, const CUtensorMap& map_b, SmallGemmArgs p, int batch, int sms, cudaStream_t s);
 
+// The gated feed-forward block's products with their epilogues, 16-bit operands on CTA pairs. Forward, x [M, K] and w [2 N, K]: h [M, N] = f(a) b with a and
+// b the products with the two halves of w's rows, and kept = [a b] unless it is null. Backward, dy [M, K] and w [K, N]: d = [dh b f'(a), dh f(a)] with
+// dh = dy w and kept = [a b]. `_takes`: whether the operands' layouts are theirs.
+bool gemm_gated_takes(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept);
+void gemm_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept, int act, void* stream);
+bool gemm_sloped_takes(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d);
+void gemm_sloped(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d, int act, void* stream);
+
 }  // namespace lb
