@@ -263,30 +263,29 @@ __device__ __forceinline__ void drain_tile_aux(const GemmArgs& p, uint32_t tbase
 }
 
 // ---- the gated feed-forward block's tiles ---------------------------------------------------------------------------
-// 32 float32 values rounded to 16 bits, two a word.
-__device__ __forceinline__ void round_columns(const uint32_t* v, uint32_t* w, bool f16) {
-    if (LB_RARELY(f16)) {
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-            w[j] = *(const uint32_t*)&h;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-            w[j] = *(const uint32_t*)&h;
-        }
+// Two float32 values rounded to 16 bits in a word, and a word's two.
+template <bool F16>
+__device__ __forceinline__ uint32_t narrow(Pair x) {
+    if (F16) {
+        const __half2 h = __float22half2_rn(apart(x));
+        return *(const uint32_t*)&h;
     }
+    const __nv_bfloat162 h = __float22bfloat162_rn(apart(x));
+    return *(const uint32_t*)&h;
 }
-template <int ACT>
-__device__ __forceinline__ void gate_columns(uint32_t* a, const uint32_t* b) {
-#pragma unroll
-    for (int j = 0; j < 32; j++) a[j] = __float_as_uint(activation<ACT, true>(__uint_as_float(a[j])) * __uint_as_float(b[j]));
+template <bool F16>
+__device__ __forceinline__ Pair widen(uint32_t w) {
+    if (F16) {
+        const float2 f = __half22float2(*(const __half2*)&w);
+        return both(f.x, f.y);
+    }
+    return both(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
+__device__ __forceinline__ Pair columns(const uint32_t* v, int j) { return both(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])); }
+
 // 64 columns of both projections (the gate's at `tbase`, the other's 128 columns further), their gated product, whole 128-byte row pieces each.
 // Rows are 16-byte aligned and N is a multiple of 8 (checked by the host).
-template <class Release>
+template <int ACT, bool F16, class Release>
 __device__ __forceinline__ void drain_gated(const GatedArgs& p, uint32_t tbase, int row, int col0, uint4* stage, int lane, Release release) {
     uint4 gate[8], up[8], h[8];
 #pragma unroll
@@ -296,11 +295,12 @@ __device__ __forceinline__ void drain_gated(const GatedArgs& p, uint32_t tbase, 
         tmem_ld_32x32(tbase + BN / 2 + c * 32, v + 32);
         tmem_ld_wait();
         if (c == 1) release();
-        round_columns(v, (uint32_t*)(gate + 4 * c), p.d_f16), round_columns(v + 32, (uint32_t*)(up + 4 * c), p.d_f16);
-        if (p.act == ACT_SILU) gate_columns<ACT_SILU>(v, v + 32);
-        else if (p.act == ACT_GELU) gate_columns<ACT_GELU>(v, v + 32);
-        else gate_columns<ACT_RELU>(v, v + 32);
-        round_columns(v, (uint32_t*)(h + 4 * c), p.d_f16);
+        uint32_t *g = (uint32_t*)(gate + 4 * c), *u = (uint32_t*)(up + 4 * c), *r = (uint32_t*)(h + 4 * c);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const Pair a = columns(v, j), b = columns(v + 32, j);
+            g[j] = narrow<F16>(a), u[j] = narrow<F16>(b), r[j] = narrow<F16>(activation<ACT>(a) * b);
+        }
     }
     const int first = row - lane, rows = p.M - first, segs = (p.N - col0) / 8;
     if (rows <= 0 || segs <= 0) return;
@@ -324,45 +324,32 @@ __device__ __forceinline__ void kept_load(const SlopedArgs& p, int first, int co
         up[t] = live ? *(const uint4*)(at + r * p.ld_kept + p.N) : make_uint4(0u, 0u, 0u, 0u);
     }
 }
-__device__ __forceinline__ float half_of(uint32_t w, int k, bool f16) {
-    if (f16) return __half2float(__ushort_as_half((unsigned short)(w >> (16 * k))));
-    return __uint_as_float(k ? w & 0xffff0000u : w << 16);
-}
-// dh in v, both projections in a and b: v becomes the gate's gradient, w the other's.
-template <int ACT>
-__device__ __forceinline__ void slope_columns(uint32_t* v, const uint32_t* a, const uint32_t* b, uint32_t* w, bool f16) {
-#pragma unroll
-    for (int j = 0; j < 32; j++) {
-        float slope;
-        const float dh = __uint_as_float(v[j]), value = activation_slope<ACT, true>(half_of(a[j / 2], j % 2, f16), slope);
-        v[j] = __float_as_uint(dh * half_of(b[j / 2], j % 2, f16) * slope), w[j] = __float_as_uint(dh * value);
-    }
-}
-template <class Release>
+// 128 columns of dh and of both projections, 32 at a time: the gradients of both.
+template <int ACT, bool F16, class Release>
 __device__ __forceinline__ void drain_sloped(const SlopedArgs& p, uint32_t tbase, int row, int col_base, uint4* gate, uint4* up, uint4* stage, int lane, Release release) {
     const int first = row - lane, rows = p.M - first;
     uint16_t* out = (uint16_t*)p.d + first * p.ldd + col_base;
 #pragma unroll 1
     for (int c = 0; c < BN / 2 / 32; c++) {
-        uint32_t v[32], a[16], b[16], w[32];
+        uint32_t v[32], a[16], b[16];
         tmem_ld_32x32(tbase + c * 32, v);
         aux_to_rows(stage + 128, gate, a, lane), aux_to_rows(stage + 128, up, b, lane);
         if (c + 1 < BN / 2 / 32) kept_load(p, first, col_base + (c + 1) * 32, lane, gate, up);
         tmem_ld_wait();
         if (c == BN / 2 / 32 - 1) release();
-        if (p.act == ACT_SILU) slope_columns<ACT_SILU>(v, a, b, w, p.d_f16);
-        else if (p.act == ACT_GELU) slope_columns<ACT_GELU>(v, a, b, w, p.d_f16);
-        else slope_columns<ACT_RELU>(v, a, b, w, p.d_f16);
+        uint4 da[4], db[4];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            Pair slope;
+            const Pair dh = columns(v, j), value = activation_slope<ACT>(widen<F16>(a[j]), slope);
+            ((uint32_t*)da)[j] = narrow<F16>(dh * widen<F16>(b[j]) * slope), ((uint32_t*)db)[j] = narrow<F16>(dh * value);
+        }
         const int segs = (p.N - col_base - c * 32) / 8;
         if (rows <= 0 || segs <= 0) continue;
-        uint4 packed[4];
-        round_columns(v, (uint32_t*)packed, p.d_f16);
-        store_rows_coalesced<4>(stage, packed, (uint8_t*)(out + c * 32), p.ldd * 2, rows, lane, segs);
-        round_columns(w, (uint32_t*)packed, p.d_f16);
-        store_rows_coalesced<4>(stage, packed, (uint8_t*)(out + c * 32 + p.N), p.ldd * 2, rows, lane, segs);
+        store_rows_coalesced<4>(stage, da, (uint8_t*)(out + c * 32), p.ldd * 2, rows, lane, segs);
+        store_rows_coalesced<4>(stage, db, (uint8_t*)(out + c * 32 + p.N), p.ldd * 2, rows, lane, segs);
     }
 }
-
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
     extern __shared__ uint8_t smem_raw[];
@@ -709,7 +696,13 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 4));
-                drain_gated(p, tbase, row, n_blk * (BN / 2) + col_half * (BN / 4), stage, lane, release);
+                const int col0 = n_blk * (BN / 2) + col_half * (BN / 4);
+                if (!p.d_f16 && p.act == ACT_SILU) drain_gated<ACT_SILU, false>(p, tbase, row, col0, stage, lane, release);
+                else if (!p.d_f16 && p.act == ACT_GELU) drain_gated<ACT_GELU, false>(p, tbase, row, col0, stage, lane, release);
+                else if (!p.d_f16) drain_gated<ACT_RELU, false>(p, tbase, row, col0, stage, lane, release);
+                else if (p.act == ACT_SILU) drain_gated<ACT_SILU, true>(p, tbase, row, col0, stage, lane, release);
+                else if (p.act == ACT_GELU) drain_gated<ACT_GELU, true>(p, tbase, row, col0, stage, lane, release);
+                else drain_gated<ACT_RELU, true>(p, tbase, row, col0, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_SLOPED) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 uint4 gate[4], up[4];
@@ -718,7 +711,12 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                drain_sloped(p, tbase, row, col_base, gate, up, stage, lane, release);
+                if (!p.d_f16 && p.act == ACT_SILU) drain_sloped<ACT_SILU, false>(p, tbase, row, col_base, gate, up, stage, lane, release);
+                else if (!p.d_f16 && p.act == ACT_GELU) drain_sloped<ACT_GELU, false>(p, tbase, row, col_base, gate, up, stage, lane, release);
+                else if (!p.d_f16) drain_sloped<ACT_RELU, false>(p, tbase, row, col_base, gate, up, stage, lane, release);
+                else if (p.act == ACT_SILU) drain_sloped<ACT_SILU, true>(p, tbase, row, col_base, gate, up, stage, lane, release);
+                else if (p.act == ACT_GELU) drain_sloped<ACT_GELU, true>(p, tbase, row, col_base, gate, up, stage, lane, release);
+                else drain_sloped<ACT_RELU, true>(p, tbase, row, col_base, gate, up, stage, lane, release);
             } else {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 const long long row_off = (long long)b * p.d_batch_stride + (long long)row * p.ldd;

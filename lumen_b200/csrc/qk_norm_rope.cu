@@ -16,6 +16,7 @@
 
 #include "divide.cuh"
 #include "launch.cuh"
+#include "pair.cuh"
 
 namespace lb {
 namespace {
@@ -148,32 +149,6 @@ __global__ void __launch_bounds__(kRowWarps * 32) rope_rows_kernel(const RopeArg
         }
     }
 }
-
-// Two float32 values in one register pair: an instruction for both (fused multiply-add, product), each rounded as by itself.
-struct Pair {
-    unsigned long long v;
-};
-__device__ __forceinline__ Pair both(float lo, float hi) {
-    Pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 apart(Pair a) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-    return r;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-    Pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ Pair operator-(Pair a) { return {a.v ^ 0x8000000080000000ull}; }
 
 // Four elements of a row, as two pairs of float32 and back; the address is a multiple of their size.
 template <class T> struct Four;
