@@ -179,7 +179,7 @@ struct Block {
 
 struct Forward : Block {
     lb_tensor y, gate_up{}, h;
-    bool keeps, fused = false;
+    bool keeps, few = false, fused = false;
     size_t sums = 0;  // bytes of [a b] in float32
 
     Forward(int act, const lb_tensor* x_t, const lb_tensor* wgu_t, const lb_tensor* wd_t, const lb_tensor* y_t, const lb_tensor* gate_up_t, const lb_tensor* h_t)
@@ -187,6 +187,8 @@ struct Forward : Block {
         sized(y, M, D, dtype, "y"), written(y, "y"), sized(h, M, F, dtype, "h"), written(h, "h");
         if (keeps) gate_up = as_rows(gate_up_t, "gate_up"), sized(gate_up, M, 2 * F, dtype, "gate_up"), written(gate_up, "gate_up");
         if (M == 0) return;
+        few = skinny_takes(x, wgu) && skinny_takes(h, wd);
+        if (few) return;
         fused = gated_tiles(M) && gemm_gated_takes(x, wgu, h, keeps ? &gate_up : nullptr);
         if (!fused && (dtype != LB_F32 || !keeps)) sums = up((size_t)M * 2 * F * 4);
         products = std::max(fused ? 0 : product_scratch(x, transposed(wgu)), product_scratch(h, transposed(wd)));
@@ -194,6 +196,11 @@ struct Forward : Block {
     size_t bytes() const { return sums + products; }
     void run(const lb_tensor* residual, void* stream) {
         char* more = (char*)scratch + sums;
+        if (few) {
+            skinny_gated(x, wgu, h, keeps ? &gate_up : nullptr, act, stream);
+            skinny_product(h, wd, y, residual, stream);
+            return;
+        }
         if (fused) {
             gemm_gated(x, wgu, h, keeps ? &gate_up : nullptr, act, stream);
             gemm(h, transposed(wd), y, residual ? EPI_ADD : EPI_NONE, 0, stream, more, products, residual, nullptr);

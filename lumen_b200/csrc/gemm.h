@@ -78,4 +78,9 @@ void gemm_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, cons
 bool gemm_sloped_takes(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d);
 void gemm_sloped(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d, int act, void* stream);
 
+// A few tokens (gemm_skinny.cu): out [M, N] = x [M, K] w^T with w [N, K], plus `add` [M, N] once rounded (null: nothing); h and kept as in gemm_gated.
+bool skinny_takes(const lb_tensor& x, const lb_tensor& w);
+void skinny_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept, int act, void* stream);
+void skinny_product(const lb_tensor& x, const lb_tensor& w, const lb_tensor& out, const lb_tensor* add, void* stream);
+
 }  // namespace lb

@@ -81,15 +81,7 @@ bool truth(PyObject* b, bool* out) {  // steals b
     return v >= 0;
 }
 
-bool describe(PyObject* t, lb_tensor* out) {
-    PyObject* cuda = PyObject_GetAttr(t, names.is_cuda);
-    bool on_gpu = true;
-    if (!cuda) PyErr_Clear();  // a tensor type without the attribute answers for itself
-    else if (!truth(cuda, &on_gpu)) return false;
-    if (!on_gpu) {
-        PyErr_SetString(PyExc_ValueError, "expected a CUDA tensor");
-        return false;
-    }
+bool describe_view(PyObject* t, lb_tensor* out) {
     int32_t strides = 0;
     if (!dtype_code(t, &out->dtype) || !read_pointer(t, &out->ptr)) return false;
     if (!read_longs(PyObject_GetAttr(t, names.shape), out->shape, &out->rank, "shape")) return false;
@@ -99,6 +91,18 @@ bool describe(PyObject* t, lb_tensor* out) {
         return false;
     }
     return true;
+}
+
+bool describe(PyObject* t, lb_tensor* out) {
+    PyObject* cuda = PyObject_GetAttr(t, names.is_cuda);
+    bool on_gpu = true;
+    if (!cuda) PyErr_Clear();  // a tensor type without the attribute answers for itself
+    else if (!truth(cuda, &on_gpu)) return false;
+    if (!on_gpu) {
+        PyErr_SetString(PyExc_ValueError, "expected a CUDA tensor");
+        return false;
+    }
+    return describe_view(t, out);
 }
 
 PyObject* finish(int status) {
@@ -225,7 +229,10 @@ int is_here(PyObject* t, Here& here) {
     else if (here.current(&device) && at != device) PyErr_Format(PyExc_ValueError, "a tensor is on GPU %ld, the current one is GPU %d", at, device);
     return PyErr_Occurred() ? -1 : 1;
 }
-bool describe_here(PyObject* t, lb_tensor* out, Here& here) { return is_here(t, here) >= 0 && describe(t, out); }
+bool describe_here(PyObject* t, lb_tensor* out, Here& here) {
+    const int torch = is_here(t, here);
+    return torch > 0 ? describe_view(t, out) : torch == 0 && describe(t, out);
+}
 
 // A call's workspace, from `take(bytes)` where it needs any; held until the call's kernels are queued.
 struct Scratch {
@@ -334,7 +341,7 @@ bool describe_dense(PyObject* t, lb_tensor* out, Here& here) {
     if (torch < 0) return false;
     bool contiguous = false;
     if (torch && !truth(PyObject_CallMethodNoArgs(t, names.is_contiguous), &contiguous)) return false;
-    if (!contiguous) return describe(t, out);
+    if (!contiguous) return torch ? describe_view(t, out) : describe(t, out);
     PyObject* count = PyObject_CallMethodNoArgs(t, names.numel);
     if (!count) return false;
     out->rank = 1, out->shape[0] = PyLong_AsLongLong(count), out->stride[0] = 1;
