@@ -22,20 +22,21 @@
 namespace lb {
 namespace {
 
-constexpr int kThreads = 256, kBlocksPerSm = 4;
-constexpr int kUnroll = 4;                                  // 16-byte loads of a thread in flight
-constexpr int kChunkBytes = kThreads * 16 * kUnroll;        // 16 KB of the operand
-constexpr int kMost = 240;                                  // tensors of one launch
+constexpr int kThreads = 256, kBlocksPerSm = 3;
+constexpr int kReads = 8, kScales = 4;                      // 16-byte loads of a thread in flight: squares, scaling (which holds its results too)
+constexpr int kChunkBytes = kThreads * 16 * kReads;         // 32 KB of the operand
+constexpr int kMost = 240, kFew = 32;                       // tensors of one launch: two sizes of table, the smaller the cheaper to hand over
 
+template <int MOST>
 struct NormTable {
-    const void* x[kMost];
-    void* out[kMost];
-    long long n[kMost];
-    int first[kMost + 1];  // first chunk of each tensor
-    uint8_t dtype[kMost];
+    const void* x[MOST];
+    void* out[MOST];
+    long long n[MOST];
+    int first[MOST + 1];  // first chunk of each tensor
+    uint8_t dtype[MOST];
     int count;
 };
-static_assert(sizeof(NormTable) <= 32000, "kernel parameters");
+static_assert(sizeof(NormTable<kMost>) <= 32000, "kernel parameters");
 
 template <class T> struct Of;
 template <> struct Of<float> {
@@ -111,7 +112,8 @@ __device__ __forceinline__ double block_sum(double v, double* held) {  // to all
 }
 
 // The tensor that chunk `c` lies in: the last whose first chunk is not behind it (an empty tensor has none).
-__device__ __forceinline__ int tensor_of(const NormTable& t, int c) {
+template <int MOST>
+__device__ __forceinline__ int tensor_of(const NormTable<MOST>& t, int c) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -127,12 +129,12 @@ __device__ __forceinline__ double chunk_squares(const T* x, int n) {
     const int head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T)), vecs = (n - head) / per;
     const uint4* v = (const uint4*)(x + head);
     double sum = 0.0;
-    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kUnroll) {
-        uint4 w[kUnroll];
+    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kReads) {
+        uint4 w[kReads];
 #pragma unroll
-        for (int k = 0; k < kUnroll; k++) w[k] = i0 + k * kThreads < vecs ? v[i0 + k * kThreads] : make_uint4(0u, 0u, 0u, 0u);
+        for (int k = 0; k < kReads; k++) w[k] = i0 + k * kThreads < vecs ? v[i0 + k * kThreads] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int k = 0; k < kUnroll; k++) {
+        for (int k = 0; k < kReads; k++) {
             float f[per];
             Of<T>::widen(w[k], f);
             sum += squares<per>(f);
@@ -153,13 +155,13 @@ __device__ __forceinline__ void chunk_scale(const T* x, T* out, int n, float c, 
     if ((((uintptr_t)x ^ (uintptr_t)out) & 15) == 0) head = min(n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T)), vecs = (n - head) / per;
     const uint4* v = (const uint4*)(x + head);
     uint4* o = (uint4*)(out + head);
-    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kUnroll) {
-        uint4 w[kUnroll];
+    for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kScales) {
+        uint4 w[kScales];
 #pragma unroll
-        for (int k = 0; k < kUnroll; k++)
+        for (int k = 0; k < kScales; k++)
             if (i0 + k * kThreads < vecs) w[k] = v[i0 + k * kThreads];
 #pragma unroll
-        for (int k = 0; k < kUnroll; k++)
+        for (int k = 0; k < kScales; k++)
             if (i0 + k * kThreads < vecs) {
                 float f[per];
                 Of<T>::widen(w[k], f);
@@ -174,7 +176,8 @@ __device__ __forceinline__ void chunk_scale(const T* x, T* out, int n, float c, 
     }
 }
 
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_squares_kernel(const __grid_constant__ NormTable t, double* partial) {
+template <int MOST>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_squares_kernel(const __grid_constant__ NormTable<MOST> t, double* partial) {
     __shared__ double held[kThreads / 32];
     grid_wait();
     double sum = 0.0;
@@ -205,7 +208,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* partial, i
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_scale_kernel(const __grid_constant__ NormTable t, const double* partial, int parts, double max_norm, float* norm) {
+template <int MOST>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_scale_kernel(const __grid_constant__ NormTable<MOST> t, const double* partial, int parts, double max_norm, float* norm) {
     __shared__ double held[kThreads / 32];
     grid_wait();
     const double n = total_norm(partial, parts, held);
@@ -261,6 +265,44 @@ struct Range {
 
 size_t scratch_bytes(int n) { return (size_t)((n + kMost - 1) / kMost) * sm_count_hint() * kBlocksPerSm * sizeof(double); }
 
+// The launches for tensors that have been looked at, MOST of them (those with elements) a table.
+template <int MOST>
+void launch_norm(const lb_tensor* xs, const lb_tensor* outs, int n, const std::vector<long long>& count, double max_norm, float* norm, double* partial, cudaStream_t s) {
+    const int grid = device_info().sms * kBlocksPerSm;
+    std::vector<NormTable<MOST>> tables;
+    std::vector<int> blocks;
+    int parts = 0;
+    for (int k = 0; k < n;) {
+        tables.emplace_back();
+        NormTable<MOST>& t = tables.back();
+        t.count = 0;
+        long long chunks = 0;
+        for (; k < n && t.count < MOST; k++) {
+            if (!count[k]) continue;
+            const int i = t.count++;
+            t.x[i] = xs[k].ptr, t.out[i] = outs ? outs[k].ptr : nullptr, t.n[i] = count[k], t.dtype[i] = (uint8_t)xs[k].dtype;
+            t.first[i] = (int)chunks;
+            const int per = kChunkBytes / dtype_size(xs[k].dtype);
+            chunks += (count[k] + per - 1) / per;
+        }
+        t.first[t.count] = (int)chunks;
+        blocks.push_back((int)std::min<long long>(chunks, grid));
+        if (!chunks) continue;
+        launch_overlapped(norm_squares_kernel<MOST>, dim3((unsigned)blocks.back()), dim3(kThreads), 0, s, 0, t, partial + parts);
+        parts += blocks.back();
+    }
+    if (!outs || !parts) {
+        launch_overlapped(norm_kernel, dim3(1), dim3(kThreads), 0, s, 0, (const double*)partial, parts, norm);
+        return;
+    }
+    bool first = true;
+    for (size_t k = tables.size(); k-- > 0;) {
+        if (!blocks[k]) continue;
+        launch_overlapped(norm_scale_kernel<MOST>, dim3((unsigned)blocks[k]), dim3(kThreads), 0, s, 0, tables[k], (const double*)partial, parts, max_norm, first ? norm : nullptr);
+        first = false;
+    }
+}
+
 // `outs` null: the norm alone.
 void run_norm(const lb_tensor* xs, const lb_tensor* outs, int n, double max_norm, const lb_tensor* norm, void* scratch, size_t bytes, void* stream) {
     if (n < 0 || (n && !xs) || !norm) refuse("null argument");
@@ -294,42 +336,10 @@ void run_norm(const lb_tensor* xs, const lb_tensor* outs, int n, double max_norm
     const size_t need = scratch_bytes(n);
     if (n && (!scratch || bytes < need || (uintptr_t)scratch % 16)) refuse(format("%zu bytes of scratch are needed, 16-byte aligned", need));
     driver();
-    cudaStream_t s = (cudaStream_t)stream;
-    const int grid = device_info().sms * kBlocksPerSm;
-    double* partial = (double*)scratch;
-    std::vector<NormTable> tables;
-    std::vector<int> blocks;
-    int parts = 0;
-    for (int k0 = 0; k0 < n; k0 += kMost) {
-        tables.emplace_back();
-        NormTable& t = tables.back();
-        t.count = 0;
-        long long chunks = 0;
-        for (int k = k0; k < std::min(n, k0 + kMost); k++) {
-            if (!count[k]) continue;
-            const int i = t.count++;
-            t.x[i] = xs[k].ptr, t.out[i] = outs ? outs[k].ptr : nullptr, t.n[i] = count[k], t.dtype[i] = (uint8_t)xs[k].dtype;
-            t.first[i] = (int)chunks;
-            const int per = kChunkBytes / dtype_size(xs[k].dtype);
-            chunks += (count[k] + per - 1) / per;
-        }
-        t.first[t.count] = (int)chunks;
-        blocks.push_back((int)std::min<long long>(chunks, grid));
-        if (!chunks) continue;
-        launch_overlapped(norm_squares_kernel, dim3((unsigned)blocks.back()), dim3(kThreads), 0, s, 0, t, partial + parts);
-        parts += blocks.back();
-    }
-    float* result = (float*)norm->ptr;
-    if (!outs || !parts) {
-        launch_overlapped(norm_kernel, dim3(1), dim3(kThreads), 0, s, 0, (const double*)partial, parts, result);
-        return;
-    }
-    bool first = true;
-    for (size_t k = tables.size(); k-- > 0;) {
-        if (!blocks[k]) continue;
-        launch_overlapped(norm_scale_kernel, dim3((unsigned)blocks[k]), dim3(kThreads), 0, s, 0, tables[k], (const double*)partial, parts, max_norm, first ? result : nullptr);
-        first = false;
-    }
+    int live = 0;
+    for (int k = 0; k < n; k++) live += count[k] > 0;
+    if (live <= kFew) launch_norm<kFew>(xs, outs, n, count, max_norm, (float*)norm->ptr, (double*)scratch, (cudaStream_t)stream);
+    else launch_norm<kMost>(xs, outs, n, count, max_norm, (float*)norm->ptr, (double*)scratch, (cudaStream_t)stream);
 }
 
 }  // namespace

@@ -351,10 +351,19 @@ def scatter_add_rows(x, ids, updates, deterministic=True, stream=None):
 
 
 def _outputs(like, stream, *wanted):
-    """New dense tensors of `(shape, dtype name)` each, None for None."""
-    if _Torch.takes(like, stream):  # 1.5 us a tensor less than through `_empty_like_input`
-        return [None if w is None else like.new_empty(w[0], dtype=TORCH_DTYPES[w[1]]) for w in wanted]
-    return [None if w is None else _empty_like_input(like, *w) for w in wanted]
+    """New dense tensors of `(shape, dtype name)` each, None for None, and the handle of the stream."""
+    if _Torch.takes(like, stream):
+        return [None if w is None else like.new_empty(w[0], dtype=TORCH_DTYPES[w[1]]) for w in wanted], _Torch.stream()
+    return [None if w is None else _empty_like_input(like, *w) for w in wanted], _stream(stream)
+
+
+def _results_like(tensors, out, stream):
+    """`out`, or new dense tensors like each of `tensors`, and the handle of the stream."""
+    if out is not None:
+        return out, _stream(stream)
+    if _Torch.takes(tensors[0], stream):
+        return [_Torch.like(t) for t in tensors], _Torch.stream()
+    return [_empty_like_input(t, tuple(t.shape), dtype_name(t.dtype)) for t in tensors], _stream(stream)
 
 
 def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None, stream=None):
@@ -365,10 +374,9 @@ def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, e
     `[S]` or `[B, S]`, clamped into the tables; None is 0, 1, 2 ... Weights: `[H]` of `q`'s dtype or float32; None is all ones. Returns `(q, k)`
     of the operands' dtype, in `out` if given (which may be `(q, k)`)."""
     require_cuda()
-    if out is None:
-        out = _outputs(q, stream, (tuple(q.shape), dtype_name(q.dtype)), (tuple(k.shape), dtype_name(k.dtype)))
-    _lib.host().qk_norm_rope(eps, bool(interleaved), q, k, cos, sin, positions, q_weight, k_weight, out[0], out[1], _stream(stream))
-    return out[0], out[1]
+    (q_out, k_out), handle = _results_like((q, k), out, stream)
+    _lib.host().qk_norm_rope(eps, bool(interleaved), q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out, handle)
+    return q_out, k_out
 
 
 def qk_norm_rope_backward(d_q_out, d_k_out, q, k, cos, sin, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None,
@@ -376,13 +384,13 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, cos, sin, positions=None, q_we
     """The backward pass of `qk_norm_rope` on the same operands: returns `(d_q, d_k, d_q_weight, d_k_weight)`, the last two of their weight's dtype and
     None without one. `out` takes `d_q` and `d_k`, which may be `(d_q_out, d_k_out)`. Bit-identical from call to call."""
     require_cuda()
-    wanted = [None if w is None else (tuple(w.shape), dtype_name(w.dtype)) for w in (q_weight, k_weight)]
-    if out is None:
-        out = _outputs(q, stream, (tuple(q.shape), dtype_name(q.dtype)), (tuple(k.shape), dtype_name(k.dtype)))
-    dwq, dwk = _outputs(q, stream, *wanted)
-    _lib.host().qk_norm_rope_bwd(eps, bool(interleaved), d_q_out, d_k_out, q, k, cos, sin, positions, q_weight, k_weight, out[0], out[1], dwq, dwk,
-                                 lambda nbytes: _workspace(q, (nbytes,), "uint8", stream), _stream(stream))
-    return out[0], out[1], dwq, dwk
+    (d_q, d_k), handle = _results_like((q, k), out, stream)
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    grads = _results_like(weights, None, stream)[0] if weights else []
+    d_q_weight, d_k_weight = grads.pop(0) if q_weight is not None else None, grads.pop() if k_weight is not None else None
+    _lib.host().qk_norm_rope_bwd(eps, bool(interleaved), d_q_out, d_k_out, q, k, cos, sin, positions, q_weight, k_weight, d_q, d_k, d_q_weight, d_k_weight,
+                                 lambda nbytes: _workspace(q, (nbytes,), "uint8", stream), handle)
+    return d_q, d_k, d_q_weight, d_k_weight
 
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
@@ -402,9 +410,13 @@ def gated_mlp_forward(x, w_gate_up, w_down, activation="silu", residual=None, sa
     bfloat16 or float32; the tensor cores take 16-bit operands whose rows are 16-byte aligned, the CUDA cores the others. Bit-identical from call to
     call; the same rows among others may differ by a rounding."""
     require_cuda()
-    act, lead, dtype, f = _activation(activation), tuple(x.shape[:-1]), dtype_name(x.dtype), w_gate_up.shape[0] // 2
-    y, gate_up, h = _outputs(x, stream, (tuple(x.shape), dtype), ((*lead, 2 * f), dtype) if save else None, ((*lead, f), dtype))
-    _lib.host().gated_mlp_fwd(act, x, w_gate_up, w_down, residual, y, gate_up, h, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream), _stream(stream))
+    act, lead, f = _activation(activation), x.shape[:-1], w_gate_up.shape[0] // 2
+    if _Torch.takes(x, stream):
+        y, gate_up, h, handle = _Torch.like(x), x.new_empty((*lead, 2 * f)) if save else None, x.new_empty((*lead, f)), _Torch.stream()
+    else:
+        dtype = dtype_name(x.dtype)
+        (y, gate_up, h), handle = _outputs(x, stream, (tuple(x.shape), dtype), ((*lead, 2 * f), dtype) if save else None, ((*lead, f), dtype))
+    _lib.host().gated_mlp_fwd(act, x, w_gate_up, w_down, residual, y, gate_up, h, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream), handle)
     return y, gate_up, h
 
 
@@ -412,10 +424,9 @@ def gated_mlp_backward(d_y, x, w_gate_up, w_down, gate_up, h, activation="silu",
     """The backward pass of `gated_mlp_forward` through `lb_gated_mlp_bwd`: returns `(d_x, d_w_gate_up, d_w_down)` of the operands' dtype. (A residual's
     gradient is `d_y` itself.) Bit-identical from call to call."""
     require_cuda()
-    act, dtype = _activation(activation), dtype_name(x.dtype)
-    d_x, d_wgu, d_wd = _outputs(x, stream, *((tuple(t.shape), dtype) for t in (x, w_gate_up, w_down)))
-    _lib.host().gated_mlp_bwd(act, d_y, x, w_gate_up, w_down, gate_up, h, d_x, d_wgu, d_wd, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream),
-                              _stream(stream))
+    act = _activation(activation)
+    (d_x, d_wgu, d_wd), handle = _results_like((x, w_gate_up, w_down), None, stream)
+    _lib.host().gated_mlp_bwd(act, d_y, x, w_gate_up, w_down, gate_up, h, d_x, d_wgu, d_wd, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream), handle)
     return d_x, d_wgu, d_wd
 
 
@@ -425,8 +436,8 @@ def _norm(tensors, out, max_norm, like, stream):
         if len(tensors) == 0:
             raise ValueError("the norm of no tensors needs `like`, a tensor on the GPU")
         like = tensors[0]
-    (norm,) = _outputs(like, stream, ((), "float32"))
-    _lib.host().clip_grad_norm(tensors, out, max_norm, norm, lambda nbytes: _workspace(like, (nbytes,), "uint8", stream), _stream(stream))
+    (norm,), handle = _outputs(like, stream, ((), "float32"))
+    _lib.host().clip_grad_norm(tensors, out, max_norm, norm, lambda nbytes: _workspace(like, (nbytes,), "uint8", stream), handle)
     return norm
 
 

@@ -188,7 +188,8 @@ def test_gated_block_in_order():
     ({"residual": Array((10, 96), "bfloat16")}, "residual must be"),
     ({"residual": Array((10, 64), "bfloat16", strides=[1, 10])}, "residual must be row-major"),
     ({"x": Array((3, 4, 64), "bfloat16", strides=[1000, 64, 1])}, "not evenly spaced"),
-    ({"take": lambda nbytes: At((nbytes,), "uint8", 8)}, "16-byte aligned"),
+    ({"x": Array((100, 64), "bfloat16"), "y": Array((100, 64), "bfloat16"), "gate_up": Array((100, 192), "bfloat16"), "h": Array((100, 96), "bfloat16"),
+      "take": lambda nbytes: At((nbytes,), "uint8", 8)}, "16-byte aligned"),
 ])  # fmt: skip
 def test_gated_block_refusals(change, match):
     with refused(match):
@@ -269,6 +270,13 @@ def test_more_clipping_refusals():
         clip([At((5,))], norm=At((), "bfloat16", 1 << 20))
     with refused("16-byte aligned"):
         clip([At((5,))], take=lambda nbytes: At((nbytes,), "uint8", 8))
+
+
+@pytest.mark.parametrize("tensor", [torch.zeros(5), torch.zeros(4, 6).t(), torch.nn.Parameter(torch.zeros(3)), torch.zeros(0, 3, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.complex64)])
+def test_torch_tensors_on_the_host(tensor):
+    """What torch's exchange table tells is refused like what its methods tell."""
+    with pytest.raises((ValueError, TypeError), match="expected a CUDA tensor|no lumen dtype"):
+        clip([tensor])
 
 
 def test_tensors_on_the_host():
