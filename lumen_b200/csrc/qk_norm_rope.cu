@@ -185,44 +185,58 @@ template <> struct Four<__half> {
     }
 };
 
-// A thread's four pairs turned: the first of two pairs in v[0], v[1], the seconds in v[2], v[3], or neighbours in one register pair each; BACK: the
+// N elements of a row, four or (16-bit types) eight.
+template <class T, int N> struct Run;
+template <class T> struct Run<T, 4> : Four<T> {};
+template <class T> struct Run<T, 8> {
+    uint4 v;
+    __device__ __forceinline__ void load(const T* p) { v = *(const uint4*)p; }
+    __device__ __forceinline__ void widen(Pair* x) const { Four<T>{make_uint2(v.x, v.y)}.widen(x), Four<T>{make_uint2(v.z, v.w)}.widen(x + 2); }
+    __device__ __forceinline__ static void store(T* p, const Pair* x) {
+        uint2 h[2];
+        Four<T>::store((T*)&h[0], x), Four<T>::store((T*)&h[1], x + 2);
+        *(uint4*)p = make_uint4(h[0].x, h[0].y, h[1].x, h[1].y);
+    }
+};
+
+// A thread's N pairs turned: the first members in the first half of v, the second ones in the other, or neighbours in one register pair each; BACK: the
 // other way.
-template <bool BACK>
+template <bool BACK, int N>
 __device__ __forceinline__ void turn(Pair* v, const Pair* c, const Pair* s, bool neighbours) {
     if (neighbours) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < N; j++) {
             const float2 x = apart(v[j]), cc = apart(c[j / 2]), ss = apart(s[j / 2]);
             const float cj = j % 2 ? cc.y : cc.x, sj = BACK ? -(j % 2 ? ss.y : ss.x) : (j % 2 ? ss.y : ss.x);
             v[j] = fma2(both(x.y, x.x), both(-sj, sj), v[j] * both(cj, cj));
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const Pair a = v[j], b = v[2 + j], n = BACK ? -s[j] : s[j];
-            v[j] = fma2(-n, b, a * c[j]), v[2 + j] = fma2(n, a, b * c[j]);
+        for (int j = 0; j < N / 2; j++) {
+            const Pair a = v[j], b = v[N / 2 + j], n = BACK ? -s[j] : s[j];
+            v[j] = fma2(-n, b, a * c[j]), v[N / 2 + j] = fma2(n, a, b * c[j]);
         }
     }
 }
 
-// Head dims and rotated parts that are multiples of 8, rows of aligned pieces of four elements: `p.lanes` lanes of a warp a row (a power of two), eight elements
-// each, both members of four pairs among them, so that a row is in registers once and its elements meet only in the sums of its statistics.
+// Head dims and rotated parts that are multiples of 2 N (N: 4 or 8), rows of aligned pieces of N elements: `p.lanes` lanes of a warp a row (a power of two), 2 N
+// elements each, both members of N pairs among them, so that a row is in registers once and its elements meet only in the sums of its statistics.
 constexpr int kGroupThreads = 256;
 
 // What a thread keeps for all its rows.
-template <class T, bool BWD>
+template <class T, bool BWD, int N>
 struct Lane {
-    int c, e0, e1;  // its place in the row, its two runs of four elements
+    int c, e0, e1;  // its place in the row, its two runs of N elements
     bool live, turns;
-    Pair w[4], sum[BWD ? 4 : 1];
+    Pair w[N], sum[BWD ? N : 1];
 
     __device__ __forceinline__ Lane(const RopeArgs& p, const RopeSide& q) {
-        c = threadIdx.x & (p.lanes - 1), live = c * 8 < p.H, turns = c < p.R / 8;
+        c = threadIdx.x & (p.lanes - 1), live = c * 2 * N < p.H, turns = c < p.R / (2 * N);
         const bool beside = p.interleaved || !turns;
-        e0 = beside ? 8 * c : 4 * c, e1 = beside ? e0 + 4 : p.R / 2 + 4 * c;
+        e0 = beside ? 2 * N * c : N * c, e1 = beside ? e0 + N : p.R / 2 + N * c;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int i = j < 2 ? e0 + 2 * j : e1 + 2 * (j - 2);
+        for (int j = 0; j < N; j++) {
+            const int i = j < N / 2 ? e0 + 2 * j : e1 + 2 * j - N;
             w[j] = live ? both(weight<T>(q, i), weight<T>(q, i + 1)) : both(0.0f, 0.0f);
             if (BWD) sum[j] = both(0.0f, 0.0f);
         }
@@ -232,12 +246,12 @@ struct Lane {
     __device__ __forceinline__ void row(const RopeArgs& p, float per, bool there, const Pair* x, Pair* y, const Pair* cs, const Pair* sn) {
         Pair squares = x[0] * x[0], products;
 #pragma unroll
-        for (int j = 1; j < 4; j++) squares = fma2(x[j], x[j], squares);
+        for (int j = 1; j < N; j++) squares = fma2(x[j], x[j], squares);
         if (BWD) {
-            if (turns) turn<true>(y, cs, sn, p.interleaved);  // dz
+            if (turns) turn<true, N>(y, cs, sn, p.interleaved);  // dz
             products = y[0] * w[0] * x[0];
 #pragma unroll
-            for (int j = 1; j < 4; j++) products = fma2(y[j] * w[j], x[j], products);
+            for (int j = 1; j < N; j++) products = fma2(y[j] * w[j], x[j], products);
         }
         const float2 s2 = apart(squares), d2 = BWD ? apart(products) : make_float2(0.0f, 0.0f);
         float ss = s2.x + s2.y, dot = d2.x + d2.y;
@@ -253,13 +267,13 @@ struct Lane {
         const Pair rr = both(r, r);
         if (!BWD) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = x[j] * rr * w[j];
-            if (turns) turn<false>(y, cs, sn, p.interleaved);
+            for (int j = 0; j < N; j++) y[j] = x[j] * rr * w[j];
+            if (turns) turn<false, N>(y, cs, sn, p.interleaved);
         } else {
             const float mean = -dot * r * per * r;
             const Pair mm = both(mean, mean);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < N; j++) {
                 const Pair unit = x[j] * rr;
                 if (there) sum[j] = fma2(y[j], unit, sum[j]);
                 y[j] = fma2(unit, mm, y[j] * w[j] * rr);
@@ -272,7 +286,7 @@ struct Lane {
         const int groups = kGroupThreads / p.lanes, g = threadIdx.x / p.lanes;
         if (live) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) *(float2*)(held + g * p.H + (j < 2 ? e0 + 2 * j : e1 + 2 * (j - 2))) = apart(sum[j]);
+            for (int j = 0; j < N; j++) *(float2*)(held + g * p.H + (j < N / 2 ? e0 + 2 * j : e1 + 2 * j - N)) = apart(sum[j]);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < p.H; i += kGroupThreads) {
@@ -291,7 +305,7 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_few_kernel(const RopeAr
     const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
     const RopeSide& q = p.side[side];
     const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
-    Lane<T, BWD> lane(p, q);
+    Lane<T, BWD, 4> lane(p, q);
     const float per = 1.0f / (float)p.H;
     const long long rows = (long long)p.batch * p.seq * q.heads;
     for (long long base = (long long)block * groups; base < rows; base += (long long)q.blocks * groups) {
@@ -334,20 +348,23 @@ __device__ __forceinline__ void copy_async(void* to, const void* from, int bytes
     if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(src) : "memory");
 }
-template <class T, bool BWD>
-constexpr int many_heads() { return sizeof(T) == 2 ? 4 : 2; }
-template <class T, bool BWD>
-constexpr int many_smem() { return 2 * many_heads<T, BWD>() * (BWD ? 4 : 2) * kGroupThreads * (int)sizeof(Four<T>); }
-template <class T, bool BWD>
-__global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeArgs p) {
-    constexpr int HEADS = many_heads<T, BWD>(), RUNS = BWD ? 4 : 2, STAGE = HEADS * RUNS * kGroupThreads;
+// Heads of a group at a time, blocks of an SM, bytes of its ring.
+template <class T, bool BWD, int N>
+constexpr int many_heads() { return sizeof(T) == 4 || (BWD && N == 8) ? 2 : 4; }
+template <int N>
+constexpr int many_per_sm() { return N == 8 ? 2 : 3; }
+template <class T, bool BWD, int N>
+constexpr int many_smem() { return 2 * many_heads<T, BWD, N>() * (BWD ? 4 : 2) * kGroupThreads * (int)sizeof(Run<T, N>); }
+template <class T, bool BWD, int N>
+__global__ void __launch_bounds__(kGroupThreads, many_per_sm<N>()) rope_many_kernel(const RopeArgs p) {
+    constexpr int HEADS = many_heads<T, BWD, N>(), RUNS = BWD ? 4 : 2, STAGE = HEADS * RUNS * kGroupThreads;
     extern __shared__ __align__(16) uint8_t smem[];
-    Four<T>* ring = (Four<T>*)smem + threadIdx.x;  // [stage][head][run][thread]
+    Run<T, N>* ring = (Run<T, N>*)smem + threadIdx.x;  // [stage][head][run][thread]
     grid_wait();
     const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
     const RopeSide& q = p.side[side];
     const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
-    Lane<T, BWD> lane(p, q);
+    Lane<T, BWD, N> lane(p, q);
     const float per = 1.0f / (float)p.H;
     const unsigned chunks = q.by_chunks.d, tasks = (unsigned)(p.batch * p.seq) * chunks, step = (unsigned)(q.blocks * groups);
     unsigned task = (unsigned)(block * groups + threadIdx.x / p.lanes);
@@ -363,29 +380,32 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
     auto fetch = [&](const Place& at, int stage) {
         const T* from = (const T*)q.x + at.b * q.x_b + at.s * q.x_s + at.n0 * q.x_n;
         const T* grad = BWD ? (const T*)q.dy + at.b * q.dy_b + at.s * q.dy_s + at.n0 * q.dy_n : nullptr;
-        Four<T>* to = ring + stage * STAGE;
+        Run<T, N>* to = ring + stage * STAGE;
 #pragma unroll
         for (int k = 0; k < HEADS; k++)
             if (lane.live && at.n0 + k < q.heads) {
-                copy_async(to + (k * RUNS + 0) * kGroupThreads, from + k * q.x_n + lane.e0, sizeof(Four<T>));
-                copy_async(to + (k * RUNS + 1) * kGroupThreads, from + k * q.x_n + lane.e1, sizeof(Four<T>));
+                copy_async(to + (k * RUNS + 0) * kGroupThreads, from + k * q.x_n + lane.e0, sizeof(Run<T, N>));
+                copy_async(to + (k * RUNS + 1) * kGroupThreads, from + k * q.x_n + lane.e1, sizeof(Run<T, N>));
                 if (BWD) {
-                    copy_async(to + (k * RUNS + RUNS - 2) * kGroupThreads, grad + k * q.dy_n + lane.e0, sizeof(Four<T>));
-                    copy_async(to + (k * RUNS + RUNS - 1) * kGroupThreads, grad + k * q.dy_n + lane.e1, sizeof(Four<T>));
+                    copy_async(to + (k * RUNS + RUNS - 2) * kGroupThreads, grad + k * q.dy_n + lane.e0, sizeof(Run<T, N>));
+                    copy_async(to + (k * RUNS + RUNS - 1) * kGroupThreads, grad + k * q.dy_n + lane.e1, sizeof(Run<T, N>));
                 }
             }
     };
     // angles one task ahead, the position that they are found by two
-    Four<float> cs_next{make_float4(0.0f, 0.0f, 0.0f, 0.0f)}, sn_next = cs_next;
+    Four<float> cs_next[N / 4] = {}, sn_next[N / 4] = {};
     auto angles = [&](int at) {
-        if (lane.turns) cs_next.load(p.cos + at * p.ld_cos + 4 * lane.c), sn_next.load(p.sin + at * p.ld_sin + 4 * lane.c);
+        if (!lane.turns) return;
+#pragma unroll
+        for (int j = 0; j < N / 4; j++)
+            cs_next[j].load(p.cos + at * p.ld_cos + N * lane.c + 4 * j), sn_next[j].load(p.sin + at * p.ld_sin + N * lane.c + 4 * j);
     };
     auto position = [&](unsigned t) {
         const Place at = place(t);
         return table_row(p, at.b, at.s);
     };
     if (!lane.live)  // nothing is copied for lanes behind the row's end
-        for (int k = 0; k < 2 * HEADS * RUNS; k++) ring[k * kGroupThreads] = Four<T>{};
+        for (int k = 0; k < 2 * HEADS * RUNS; k++) ring[k * kGroupThreads] = Run<T, N>{};
     Place here = {}, next = {};
     int after = 0;
     if (task < tasks) next = place(task), fetch(next, 0), angles(position(task));
@@ -394,8 +414,9 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
     for (unsigned round = 0; round < rounds; round++, task += step) {
         const bool there = task < tasks && lane.live;
         here = next;
-        Pair cs[2], sn[2];
-        cs_next.widen(cs), sn_next.widen(sn);
+        Pair cs[N / 2], sn[N / 2];
+#pragma unroll
+        for (int j = 0; j < N / 4; j++) cs_next[j].widen(cs + 2 * j), sn_next[j].widen(sn + 2 * j);
         if (task < tasks && tasks - task > step) {
             next = place(task + step);
             fetch(next, (round + 1) & 1);
@@ -405,16 +426,16 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
         asm volatile("cp.async.commit_group;" ::: "memory");
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         T* to = (T*)q.out + here.b * q.out_b + here.s * q.out_s + here.n0 * q.out_n;
-        const Four<T>* held = ring + (round & 1) * STAGE;
+        const Run<T, N>* held = ring + (round & 1) * STAGE;
 #pragma unroll
         for (int k = 0; k < HEADS; k++) {
             const bool row = there && here.n0 + k < q.heads;
             if (!__any_sync(0xffffffffu, row)) break;
-            Pair x[4], y[4];
-            held[(k * RUNS + 0) * kGroupThreads].widen(x), held[(k * RUNS + 1) * kGroupThreads].widen(x + 2);
-            if (BWD) held[(k * RUNS + RUNS - 2) * kGroupThreads].widen(y), held[(k * RUNS + RUNS - 1) * kGroupThreads].widen(y + 2);
+            Pair x[N], y[N];
+            held[(k * RUNS + 0) * kGroupThreads].widen(x), held[(k * RUNS + 1) * kGroupThreads].widen(x + N / 2);
+            if (BWD) held[(k * RUNS + RUNS - 2) * kGroupThreads].widen(y), held[(k * RUNS + RUNS - 1) * kGroupThreads].widen(y + N / 2);
             lane.row(p, per, row, x, y, cs, sn);
-            if (row) Four<T>::store(to + k * q.out_n + lane.e0, y), Four<T>::store(to + k * q.out_n + lane.e1, y + 2);
+            if (row) Run<T, N>::store(to + k * q.out_n + lane.e0, y), Run<T, N>::store(to + k * q.out_n + lane.e1, y + N / 2);
         }
     }
     if (BWD && q.w) {
@@ -423,21 +444,24 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_many_kernel(const RopeA
     }
 }
 
-// dw: the blocks' sums, 32 columns a block, eight of its rows beside one another.
+// dw: the blocks' sums, 32 columns a block, 32 of its rows beside one another, four loads of each in flight.
 template <class T>
-__global__ void __launch_bounds__(256) rope_weights_kernel(const RopeArgs p) {
-    __shared__ float held[8][33];
+__global__ void __launch_bounds__(1024) rope_weights_kernel(const RopeArgs p) {
+    __shared__ float held[32][33];
     grid_wait();
     const RopeSide& q = p.side[blockIdx.y];
     if (!q.w) return;
     const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
     float sum = 0.0f;
-    if (i < p.H)
-        for (int k = part; k < q.blocks; k += 8) sum += q.partial[(long long)k * p.H + i];
+    if (i < p.H) {
+#pragma unroll 4
+        for (int k = part; k < q.blocks; k += 32) sum += q.partial[(long long)k * p.H + i];
+    }
     held[part][lane] = sum;
     __syncthreads();
     if (part == 0 && i < p.H) {
-        for (int k = 1; k < 8; k++) sum += held[k][lane];
+#pragma unroll
+        for (int k = 1; k < 32; k++) sum += held[k][lane];
         if (q.w_f32) ((float*)q.dw)[i] = sum;
         else ((T*)q.dw)[i] = from_float<T>(sum);
     }
@@ -480,10 +504,10 @@ void share_blocks(RopeArgs& p, int groups, int heads, int sms, int per_sm) {
     for (int k = 0; k < 2; k++) p.side[k].blocks = (int)(all <= most ? need[k] : need[k] ? std::max(1LL, most * need[k] / all) : 0);
 }
 
-// Whether rows can be taken in pieces of four elements by groups of lanes.
-bool in_pieces(const RopeArgs& p, int dtype, bool bwd) {
-    if (p.H % 8 || p.R % 8 || p.cos_i != 1 || p.sin_i != 1 || p.ld_cos % 4 || p.ld_sin % 4 || (uintptr_t)p.cos % 16 || (uintptr_t)p.sin % 16) return false;
-    const int per = 4, bytes = 4 * dtype_size(dtype);
+// Whether rows can be taken in pieces of `run` elements by groups of lanes.
+bool in_pieces(const RopeArgs& p, int dtype, bool bwd, int run) {
+    if (p.H % (2 * run) || p.R % (2 * run) || p.cos_i != 1 || p.sin_i != 1 || p.ld_cos % 4 || p.ld_sin % 4 || (uintptr_t)p.cos % 16 || (uintptr_t)p.sin % 16) return false;
+    const int per = run, bytes = run * dtype_size(dtype);
     auto fits = [&](const void* ptr, long long b, long long s, long long n, long long h, int heads) {
         return (uintptr_t)ptr % bytes == 0 && (b % per == 0 || p.batch == 1) && (s % per == 0 || p.seq == 1) && (n % per == 0 || heads <= 1) && h == 1;
     };
@@ -549,32 +573,40 @@ RopeCall check_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tenso
     return c;
 }
 
+template <class T, bool BWD, int N>
+void launch_many(RopeArgs& p, int sms, cudaStream_t stream) {
+    constexpr int kHeads = many_heads<T, BWD, N>();
+    p.lanes = 1;
+    while (p.lanes * 2 * N < p.H) p.lanes *= 2;
+    if (first_use_on_device((const void*)rope_many_kernel<T, BWD, N>))
+        LB_CUDA(cudaFuncSetAttribute(rope_many_kernel<T, BWD, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, many_smem<T, BWD, N>()));
+    share_blocks(p, kGroupThreads / p.lanes, kHeads, sms, many_per_sm<N>());
+    p.by_seq.set((uint32_t)std::max(p.seq, 1));
+    for (RopeSide& q : p.side) q.by_chunks.set((uint32_t)std::max((q.heads + kHeads - 1) / kHeads, 1));
+    launch_overlapped(rope_many_kernel<T, BWD, N>, dim3((unsigned)(p.side[0].blocks + p.side[1].blocks)), dim3(kGroupThreads), (many_smem<T, BWD, N>()), stream, 0, p);
+}
 template <class T, bool BWD>
 void launch_rope(RopeCall& c, cudaStream_t stream) {
     RopeArgs& p = c.p;
     const int sms = device_info().sms;
     auto blocks = [&] { return dim3((unsigned)(p.side[0].blocks + p.side[1].blocks)); };
-    if (c.rows && in_pieces(p, c.dtype, BWD)) {
+    if (c.rows && in_pieces(p, c.dtype, BWD, 4)) {
         p.lanes = 1;
         while (p.lanes * 8 < p.H) p.lanes *= 2;
-        constexpr int kHeads = many_heads<T, BWD>(), kPerSm = 3;
         const int groups = kGroupThreads / p.lanes;
-        if (c.rows >= (long long)sms * kPerSm * groups * kHeads) {
-            if (first_use_on_device((const void*)rope_many_kernel<T, BWD>))
-                LB_CUDA(cudaFuncSetAttribute(rope_many_kernel<T, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, many_smem<T, BWD>()));
-            share_blocks(p, groups, kHeads, sms, kPerSm);
-            p.by_seq.set((uint32_t)std::max(p.seq, 1));
-            for (RopeSide& q : p.side) q.by_chunks.set((uint32_t)std::max((q.heads + kHeads - 1) / kHeads, 1));
-            launch_overlapped(rope_many_kernel<T, BWD>, blocks(), dim3(kGroupThreads), (many_smem<T, BWD>()), stream, 0, p);
-        } else {
-            share_blocks(p, groups, 1, sms, kPerSm);
+        if (c.rows < (long long)sms * 3 * groups * 4) {
+            share_blocks(p, groups, 1, sms, 3);
             launch_overlapped(rope_few_kernel<T, BWD>, blocks(), dim3(kGroupThreads), 0, stream, 0, p);
+        } else if (sizeof(T) == 2 && in_pieces(p, c.dtype, BWD, 8)) {
+            if constexpr (sizeof(T) == 2) launch_many<T, BWD, 8>(p, sms, stream);
+        } else {
+            launch_many<T, BWD, 4>(p, sms, stream);
         }
     } else if (c.rows) {
         share_blocks(p, kRowWarps, 1, sms, kBlocksPerSm);
         launch_overlapped(rope_rows_kernel<T, BWD>, blocks(), dim3(kRowWarps * 32), 0, stream, 0, p);
     }
-    if (BWD && (p.side[0].w || p.side[1].w)) launch_overlapped(rope_weights_kernel<T>, dim3((unsigned)((p.H + 31) / 32), 2), dim3(256), 0, stream, 0, p);
+    if (BWD && (p.side[0].w || p.side[1].w)) launch_overlapped(rope_weights_kernel<T>, dim3((unsigned)((p.H + 31) / 32), 2), dim3(1024), 0, stream, 0, p);
 }
 template <bool BWD>
 void run_rope(RopeCall& c, void* stream) {

@@ -232,8 +232,8 @@ def test_gradients_against_differences(cuda, h, interleaved):
 @pytest.mark.parametrize("n, nk, h, pairs, interleaved, dtype", [(16, 4, 64, 32, False, torch.bfloat16), (7, 5, 128, 64, False, torch.float16), (15, 1, 80, 16, True, torch.float32),
                                                                  (13, 3, 256, 128, False, torch.bfloat16), (9, 3, 31, 15, False, torch.bfloat16)])  # fmt: skip
 def test_many_rows_repeat_bit_for_bit_and_agree_with_few(cuda, n, nk, h, pairs, interleaved, dtype):
-    """More rows than the grid has threads, numbers of heads that nothing divides: weights' gradients add up in a fixed order, and a row's result does not
-    depend on the rows beside it."""
+    """More rows than the grid has threads, numbers of heads that nothing divides: weights' gradients add up in a fixed order, and a row alone
+    is what it is among others, to a rounding."""
     q, k, dq, dk, g = case(cuda, 3, 2501, n, nk, h, dtype)
     cos, sin = tables(2501, pairs, cuda)
     w = (1 + 0.3 * torch.randn(h, generator=g, device=cuda)).to(dtype)
@@ -248,7 +248,10 @@ def test_many_rows_repeat_bit_for_bit_and_agree_with_few(cuda, n, nk, h, pairs, 
     whole = qk_norm_rope(q, k, cos, sin, q_weight=w, k_weight=w, interleaved=interleaved)
     for at in (0, 1, 1250, 2500):
         one = qk_norm_rope(q[1:2, at : at + 1], k[1:2, at : at + 1], cos, sin, positions=torch.tensor([at], device=cuda), q_weight=w, k_weight=w, interleaved=interleaved)
-        assert torch.equal(one[0][0, 0], whole[0][1, at]) and torch.equal(one[1][0, 0], whole[1][1, at])
+        for a, b, x in ((one[0][0, 0], whole[0][1, at], q[1, at]), (one[1][0, 0], whole[1][1, at], k[1, at])):  # another kernel adds a row up in another order
+            want, size = forward64(x, w, cos, sin, torch.tensor(at, device=cuda), interleaved)
+            close(a, want, size)
+            close(b, want, size)
 
 
 def test_streams_graphs_and_overlapping_calls(cuda):
