@@ -148,8 +148,13 @@ void sized(const lb_tensor& t, long long rows, long long cols, int dtype, const 
     if (rows && cols && (uintptr_t)t.ptr % dtype_size(dtype)) refuse(format("%s is not aligned to its elements", what));
 }
 
-// Whether the products with the gate in their epilogue are taken, where the layouts are theirs.
-bool gated_tiles(long long M) { return M > 128; }
+// Whether the products with the gate in their epilogue are taken, where the layouts are theirs: where enough SMs get a tile (of 128 rows by 128 columns of
+// h, backward by 256), since lb_gemm's own choices cut K and take narrower tiles. us of a pass in a graph, products apart -> these, bfloat16, width x hidden:
+// forward 200 tokens 512 x 2048 (32 tiles) 17.6 -> 20.3, 128 of 1024 x 4096 (32) 20.6 -> 24.4, 384 of 512 x 2048 (48) 17.4 -> 16.0, 200 of 1024 x 4096 (64)
+// 21.4 -> 20.1, 128 of 2048 x 8192 (64) 36.1 -> 31.5, 1024 of 1024 x 4096 41.7 -> 34.4; backward 200 of 1024 x 4096 (32) 35.1 -> 39.3, 384 (48) 46.5 -> 47.1,
+// 512 (64) 51.5 -> 50.8, 1024 of 512 x 2048 (64) 39.4 -> 38.9, 200 of 2048 x 8192 (64) 77.9 -> 79.6, 1024 of it 177 -> 174, 16384 of 1024 x 4096 837 -> 761.
+bool gated_tiles(long long M, long long F) { return (M + 127) / 128 * ((F + 127) / 128) >= 48; }
+bool sloped_tiles(long long M, long long F) { return (M + 127) / 128 * ((F + 255) / 256) >= 64; }
 
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 size_t product_scratch(const lb_tensor& a, const lb_tensor& b) { return lb_gemm_operands_scratch_bytes(&a, &b); }
@@ -189,7 +194,7 @@ struct Forward : Block {
         if (M == 0) return;
         few = skinny_takes(x, wgu) && skinny_takes(h, wd);
         if (few) return;
-        fused = gated_tiles(M) && gemm_gated_takes(x, wgu, h, keeps ? &gate_up : nullptr);
+        fused = gated_tiles(M, F) && gemm_gated_takes(x, wgu, h, keeps ? &gate_up : nullptr);
         if (!fused && (dtype != LB_F32 || !keeps)) sums = up((size_t)M * 2 * F * 4);
         products = std::max(fused ? 0 : product_scratch(x, transposed(wgu)), product_scratch(h, transposed(wd)));
     }
@@ -229,7 +234,7 @@ struct Backward : Block {
         if (gate_up.stride[1] != 1) fail(LB_ERR_UNSUPPORTED, "gated_mlp: gate_up must be row-major");
         sized(dx, M, D, dtype, "d_x"), written(dx, "d_x");
         sized(dwgu, 2 * F, D, dtype, "d_w_gate_up"), written(dwgu, "d_w_gate_up"), sized(dwd, D, F, dtype, "d_w_down"), written(dwd, "d_w_down");
-        fused = M && gated_tiles(M) && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F));
+        fused = M && sloped_tiles(M, F) && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F));
         sums = fused ? 0 : up((size_t)M * F * 4), slopes = up((size_t)M * 2 * F * dtype_size(dtype));
         const lb_tensor d = slope();
         products = std::max(std::max(fused ? 0 : product_scratch(dy, wd), product_scratch(d, wgu)), std::max(product_scratch(transposed(d), x), product_scratch(transposed(dy), h)));

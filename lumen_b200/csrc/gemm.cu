@@ -69,11 +69,10 @@ struct alignas(64) GatedArgs : GemmArgs {
     void* kept;          // [gate, up], rows ld_kept apart; null: not kept
     long long ld_kept;
 };
-struct SlopedArgs : GemmArgs {
+struct alignas(64) SlopedArgs : GemmArgs {
     static constexpr int mode = PAIR_SLOPED;
+    CUtensorMap map_gate, map_up, map_d_gate, map_d_up;  // both projections as kept, and their gradients: 32 x 32 pieces
     int act;
-    const void* kept;    // d, ldd: the gradient of both projections side by side
-    long long ld_kept;
 };
 
 // Unit `unit` of the grid: split * tiles + tile, neighbours share a K range.
@@ -312,44 +311,106 @@ __device__ __forceinline__ void drain_gated(const GatedArgs& p, uint32_t tbase, 
     }
 }
 
-// Both projections' 32 columns of the warp's rows, as aux_load spreads them; zeros outside the matrix.
-__device__ __forceinline__ void kept_load(const SlopedArgs& p, int first, int col, int lane, uint4* gate, uint4* up) {
-    const uint16_t* at = (const uint16_t*)p.kept + first * p.ld_kept + col + (lane & 3) * 8;
-    const bool inside = col + (lane & 3) * 8 < p.N;
+// The backward's way out. A warp's rows of a tile leave 32 columns at a time: both projections' pieces of 32 x 32 arrive by TMA in one of three places,
+// each lane turns its row of them and of dh into their gradients where they lie, and TMA takes those away; two pieces ahead are on their way
+// meanwhile, the next tile's among them. Rows and columns outside the matrices arrive as zeros and do not leave.
+//
+// Bound by what passes between an SM and the L2: a tile's operands, 512 KB a CTA at K = 1024, and 128 KB either way for the pieces (without the stores it takes
+// 119 us, without the arithmetic no less, and the plain product of these sizes, which stores a quarter of that, 95): 16384 x 4096 x 1024 through registers and
+// the staging area 165 us, so 148.
+constexpr int kPieceBytes = 4096, kPieces = 3;  // a warp's: 32 rows of 64 bytes of either projection
+template <int ACT, bool F16>
+__device__ __forceinline__ void slope_piece(uint32_t piece, const uint32_t* v, int lane) {
+    const uint32_t row = piece + lane * 64, turn = (lane >> 1) & 3;  // 16-byte pieces of a row as TMA's 64-byte swizzle puts them
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const int r = t * 8 + (lane >> 2);
-        const bool live = inside && first + r < p.M;
-        gate[t] = live ? *(const uint4*)(at + r * p.ld_kept) : make_uint4(0u, 0u, 0u, 0u);
-        up[t] = live ? *(const uint4*)(at + r * p.ld_kept + p.N) : make_uint4(0u, 0u, 0u, 0u);
-    }
-}
-// 128 columns of dh and of both projections, 32 at a time: the gradients of both.
-template <int ACT, bool F16, class Release>
-__device__ __forceinline__ void drain_sloped(const SlopedArgs& p, uint32_t tbase, int row, int col_base, uint4* gate, uint4* up, uint4* stage, int lane, Release release) {
-    const int first = row - lane, rows = p.M - first;
-    uint16_t* out = (uint16_t*)p.d + first * p.ldd + col_base;
-#pragma unroll 1
-    for (int c = 0; c < BN / 2 / 32; c++) {
-        uint32_t v[32], a[16], b[16];
-        tmem_ld_32x32(tbase + c * 32, v);
-        aux_to_rows(stage + 128, gate, a, lane), aux_to_rows(stage + 128, up, b, lane);
-        if (c + 1 < BN / 2 / 32) kept_load(p, first, col_base + (c + 1) * 32, lane, gate, up);
-        tmem_ld_wait();
-        if (c == BN / 2 / 32 - 1) release();
-        uint4 da[4], db[4];
+    for (int q = 0; q < 4; q++) {
+        const uint32_t at = row + ((q ^ turn) << 4);
+        const uint4 g = ld_shared(at), u = ld_shared(at + kPieceBytes / 2);
+        const uint32_t a[4] = {g.x, g.y, g.z, g.w}, b[4] = {u.x, u.y, u.z, u.w};
+        uint32_t da[4], db[4];
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
+        for (int j = 0; j < 4; j++) {
             Pair slope;
-            const Pair dh = columns(v, j), value = activation_slope<ACT>(widen<F16>(a[j]), slope);
-            ((uint32_t*)da)[j] = narrow<F16>(dh * widen<F16>(b[j]) * slope), ((uint32_t*)db)[j] = narrow<F16>(dh * value);
+            const Pair dh = columns(v, 4 * q + j), value = activation_slope<ACT>(widen<F16>(a[j]), slope);
+            da[j] = narrow<F16>(dh * widen<F16>(b[j]) * slope), db[j] = narrow<F16>(dh * value);
         }
-        const int segs = (p.N - col_base - c * 32) / 8;
-        if (rows <= 0 || segs <= 0) continue;
-        store_rows_coalesced<4>(stage, da, (uint8_t*)(out + c * 32), p.ldd * 2, rows, lane, segs);
-        store_rows_coalesced<4>(stage, db, (uint8_t*)(out + c * 32 + p.N), p.ldd * 2, rows, lane, segs);
+        st_shared(at, make_uint4(da[0], da[1], da[2], da[3])), st_shared(at + kPieceBytes / 2, make_uint4(db[0], db[1], db[2], db[3]));
     }
 }
+template <class Args>
+__device__ __forceinline__ void sloped_way_out(const Args& p, uint8_t* pieces, uint64_t* landed, uint64_t* tmem_full, uint64_t* tmem_empty, uint32_t tmem_base, int pair,
+                                               int num_pairs, int num_units, int rank, int quarter, int col_half, int lane, volatile int* abort_flag) {
+    auto first_row = [&](int m_blk) { return m_blk * 2 * BM + rank * BM + quarter * 32; };
+    auto first_col = [&](int n_blk) { return n_blk * BN + col_half * (BN / 2); };
+    auto pieces_of = [&](int row, int col) { return row < p.M ? max(0, min(BN / 2 / 32, (p.N - col + 31) / 32)) : 0; };
+    // the pieces to come: where the next one to be fetched lies
+    int load_unit = pair - num_pairs, load_row = 0, load_col = 0, load_left = 0;
+    uint32_t loaded = 0;
+    auto fetch = [&] {
+        while (load_left == 0) {
+            load_unit += num_pairs;
+            if (load_unit >= num_units) return;
+            int b, m_blk, n_blk;
+            tile_coords(p, load_unit, b, m_blk, n_blk);
+            load_row = first_row(m_blk), load_col = first_col(n_blk), load_left = pieces_of(load_row, load_col);
+        }
+        if (lane == 0) {
+            uint64_t* bar = landed + loaded % kPieces;
+            uint8_t* to = pieces + loaded % kPieces * kPieceBytes;
+            mbar_expect_tx(bar, kPieceBytes);
+            tma_load_3d(to, &p.map_gate, bar, load_col, load_row, 0);
+            tma_load_3d(to + kPieceBytes / 2, &p.map_up, bar, load_col, load_row, 0);
+        }
+        loaded++, load_left--, load_col += 32;
+    };
+    fetch(), fetch();
+    uint32_t done = 0;
+    int local = 0;
+    bool ok = true;
+    for (int unit = pair; unit < num_units && ok; unit += num_pairs, local++) {
+        const int buf = local & 1;
+        int b, m_blk, n_blk;
+        tile_coords(p, unit, b, m_blk, n_blk);
+        const int row = first_row(m_blk), col = first_col(n_blk), count = pieces_of(row, col);
+        if (!(ok = mbar_wait_warp(&tmem_full[buf], (uint32_t)(local >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+        auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(&tmem_empty[buf], 0);
+        };
+        if (count == 0) release();
+#pragma unroll 1
+        for (int c = 0; c < count && ok; c++, done++) {
+            uint32_t v[32];
+            tmem_ld_32x32(tbase + c * 32, v);
+            ok = mbar_wait_warp(&landed[done % kPieces], done / kPieces & 1, abort_flag);
+            tmem_ld_wait();
+            if (c == count - 1) release();
+            if (!ok) break;
+            uint8_t* piece = pieces + done % kPieces * kPieceBytes;
+            const uint32_t at = smem_u32(piece);
+            if (!p.d_f16 && p.act == ACT_SILU) slope_piece<ACT_SILU, false>(at, v, lane);
+            else if (!p.d_f16 && p.act == ACT_GELU) slope_piece<ACT_GELU, false>(at, v, lane);
+            else if (!p.d_f16) slope_piece<ACT_RELU, false>(at, v, lane);
+            else if (p.act == ACT_SILU) slope_piece<ACT_SILU, true>(at, v, lane);
+            else if (p.act == ACT_GELU) slope_piece<ACT_GELU, true>(at, v, lane);
+            else slope_piece<ACT_RELU, true>(at, v, lane);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) bulk_wait_read();  // the piece before this one has left: its place is the one fetched into next
+            fetch();
+            if (lane == 0) {
+                tma_store_3d(&p.map_d_gate, piece, col + c * 32, row, 0);
+                tma_store_3d(&p.map_d_up, piece + kPieceBytes / 2, col + c * 32, row, 0);
+                bulk_commit();
+            }
+        }
+    }
+    if (lane == 0) bulk_wait();
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
     extern __shared__ uint8_t smem_raw[];
@@ -543,20 +604,28 @@ gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 constexpr int PSTAGES = 6;
 constexpr int kPairStageBytesA = BM * BK * 2, kPairStageBytesB = (BN / 2) * BK * 2;
 constexpr int kPairSmemBytes = PSTAGES * (kPairStageBytesA + kPairStageBytesB) + 1024 + 256 + kEpilogueStageBytes;
+// The gated block's backward product has a larger way out and four stages beside it.
+constexpr int pair_stages(int mode) { return mode == PAIR_SLOPED ? 4 : PSTAGES; }
+constexpr int pair_smem(int mode) {
+    return mode == PAIR_SLOPED ? 4 * (kPairStageBytesA + kPairStageBytesB) + kEpilogueWarps * kPieces * kPieceBytes + 1024 + 512 : kPairSmemBytes;
+}
+static_assert(pair_smem(PAIR_SLOPED) <= 227 * 1024, "shared memory");
 
 template <class Args>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Args p) {
+    constexpr int STAGES_ = pair_stages(Args::mode);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
     uint8_t* smem_a = smem;
-    uint8_t* smem_b = smem + PSTAGES * kPairStageBytesA;
-    uint64_t* full = (uint64_t*)(smem + PSTAGES * (kPairStageBytesA + kPairStageBytesB));
-    uint64_t* empty = full + PSTAGES;
-    uint64_t* tmem_full = empty + PSTAGES;
+    uint8_t* smem_b = smem + STAGES_ * kPairStageBytesA;
+    uint64_t* full = (uint64_t*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + (Args::mode == PAIR_SLOPED ? kEpilogueWarps * kPieces * kPieceBytes : 0));
+    uint64_t* empty = full + STAGES_;
+    uint64_t* tmem_full = empty + STAGES_;
     uint64_t* tmem_empty = tmem_full + 2;
     uint32_t* tmem_base_slot = (uint32_t*)(tmem_empty + 2);
     volatile int* abort_flag = (volatile int*)(tmem_base_slot + 1);
+    [[maybe_unused]] uint64_t* landed = (uint64_t*)(tmem_base_slot + 2);  // pieces of the backward's way out, each warp's
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp-uniform for the compiler too
     const uint32_t rank = cluster_ctarank();
@@ -566,7 +635,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const int num_units = num_tiles * p.splits;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < PSTAGES; s++) {
+        for (int s = 0; s < STAGES_; s++) {
             mbar_init(&full[s], 1);   // the leader's expect_tx arrival; bytes of both CTAs
             mbar_init(&empty[s], 1);  // one commit from the leader's MMA thread
         }
@@ -574,6 +643,8 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             mbar_init(&tmem_full[s], 1);
             mbar_init(&tmem_empty[s], 2 * kEpilogueWarps);  // used in the leader only: every epilogue warp of the pair
         }
+        if constexpr (Args::mode == PAIR_SLOPED)
+            for (int s = 0; s < kEpilogueWarps * kPieces; s++) mbar_init(&landed[s], 1);
         *abort_flag = 0;
         fence_barrier_init();
         tma_prefetch_desc(&map_a);
@@ -625,13 +696,13 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                         for (int j = 0; j < BN / 2 / 64; j++)  // boxes {64 n, 64 k}
                             tma_load_3d_pair(sb + j * (64 * BK * 2), operand_b, &full[stage], col0 + j * 64, kb * BK, b);
                     }
-                    if (++stage == PSTAGES) {
+                    if (++stage == STAGES_) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
             }
-            if (ok) mbar_wait_ring<PSTAGES>(empty, phase * PSTAGES + stage, abort_flag);
+            if (ok) mbar_wait_ring<STAGES_>(empty, phase * STAGES_ + stage, abort_flag);
         }
     } else if (warp == 1) {
         // ---- MMA issuer (leader CTA only): the whole warp, so that the operands stay in uniform registers ----
@@ -663,7 +734,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                         da = desc_advance(da, a_step), db = desc_advance(db, b_step);
                     }
                     mma_commit_pair(&empty[stage], 3, leader);  // frees the stage in both CTAs
-                    if (++stage == PSTAGES) {
+                    if (++stage == STAGES_) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -675,7 +746,12 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         // ---- epilogue: warps 2..9 of both CTAs, each CTA on its own 128 rows ----
         const int quarter = warp & 3;
         const int col_half = (warp - 2) >> 2;
-        uint4* stage = (uint4*)(smem + PSTAGES * (kPairStageBytesA + kPairStageBytesB) + 256) + (warp - 2) * (kStageBytesPerWarp / 16);
+        if constexpr (Args::mode == PAIR_SLOPED) {
+            uint8_t* pieces = smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB);
+            sloped_way_out(p, pieces + (warp - 2) * kPieces * kPieceBytes, landed + (warp - 2) * kPieces, tmem_full, tmem_empty, tmem_base, pair, num_pairs, num_units,
+                           (int)rank, quarter, col_half, lane, abort_flag);
+        } else {
+        uint4* stage = (uint4*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + 256) + (warp - 2) * (kStageBytesPerWarp / 16);
         int local = 0;
         bool ok = true;
         const bool vec_ok = p.d_bf16 || p.d_f16 ? (p.ldd % 8 == 0 && p.d_batch_stride % 8 == 0 && ((uintptr_t)p.d & 15) == 0)
@@ -703,20 +779,6 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else if (p.act == ACT_SILU) drain_gated<ACT_SILU, true>(p, tbase, row, col0, stage, lane, release);
                 else if (p.act == ACT_GELU) drain_gated<ACT_GELU, true>(p, tbase, row, col0, stage, lane, release);
                 else drain_gated<ACT_RELU, true>(p, tbase, row, col0, stage, lane, release);
-            } else if constexpr (Args::mode == PAIR_SLOPED) {
-                const int col_base = n_blk * BN + col_half * (BN / 2);
-                uint4 gate[4], up[4];
-                kept_load(p, row - lane, col_base, lane, gate, up);
-                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
-                __syncwarp();
-                tc_fence_after();
-                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                if (!p.d_f16 && p.act == ACT_SILU) drain_sloped<ACT_SILU, false>(p, tbase, row, col_base, gate, up, stage, lane, release);
-                else if (!p.d_f16 && p.act == ACT_GELU) drain_sloped<ACT_GELU, false>(p, tbase, row, col_base, gate, up, stage, lane, release);
-                else if (!p.d_f16) drain_sloped<ACT_RELU, false>(p, tbase, row, col_base, gate, up, stage, lane, release);
-                else if (p.act == ACT_SILU) drain_sloped<ACT_SILU, true>(p, tbase, row, col_base, gate, up, stage, lane, release);
-                else if (p.act == ACT_GELU) drain_sloped<ACT_GELU, true>(p, tbase, row, col_base, gate, up, stage, lane, release);
-                else drain_sloped<ACT_RELU, true>(p, tbase, row, col_base, gate, up, stage, lane, release);
             } else {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 const long long row_off = (long long)b * p.d_batch_stride + (long long)row * p.ldd;
@@ -732,6 +794,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else if (LB_RARELY(p.splits > 1)) drain_partial(p, tbase, row, col_base, b, split, stage, lane, release);
                 else drain_tile(p, tbase, row, row_off, col_base, b, vec_ok, stage, lane, release);
             }
+        }
         }
     }
 
@@ -825,7 +888,7 @@ View3 view3(const lb_tensor& t, const char* what) {
     return v;
 }
 
-CUtensorMap make_map(const View3& v, bool contiguous_is_cols, int box_inner, int box_outer) {
+CUtensorMap make_map(const View3& v, bool contiguous_is_cols, int box_inner, int box_outer, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     // dims innermost first: {contiguous, strided, batch}
     long long inner = contiguous_is_cols ? v.cols : v.rows, outer = contiguous_is_cols ? v.rows : v.cols;
     long long outer_stride = contiguous_is_cols ? v.sr : v.sc;
@@ -837,7 +900,7 @@ CUtensorMap make_map(const View3& v, bool contiguous_is_cols, int box_inner, int
     CUtensorMap map;
     check_cu(driver().cuTensorMapEncodeTiled(&map, v.dtype == LB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                                              3, v.ptr, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
              "cuTensorMapEncodeTiled");
     return map;
@@ -1162,9 +1225,9 @@ template <class Args>
 static void launch_pairs(const CUtensorMap& map_a, const CUtensorMap& map_b, const Args& p, long long tiles, void* stream) {
     const DeviceInfo& dev = device_info();
     if (first_use_on_device((const void*)gemm_tcgen05_pair<Args>))
-        LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
+        LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(Args::mode)));
     const int max_pairs = resident_pairs(dev), grid = 2 * (int)std::min<long long>(tiles, max_pairs > 0 ? max_pairs : dev.sms / 2);
-    launch_overlapped(gemm_tcgen05_pair<Args>, dim3((unsigned)grid), dim3(kThreads), kPairSmemBytes, (cudaStream_t)stream, 0, map_a, map_b, p);
+    launch_overlapped(gemm_tcgen05_pair<Args>, dim3((unsigned)grid), dim3(kThreads), pair_smem(Args::mode), (cudaStream_t)stream, 0, map_a, map_b, p);
 }
 
 bool gemm_gated_takes(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept) {
@@ -1203,7 +1266,12 @@ void gemm_sloped(const lb_tensor& dy_t, const lb_tensor& w_t, const lb_tensor& k
     SlopedArgs p{};
     long long tiles;
     pair_args(p, dy, w, dy_cols, !b_cols, BN, tiles);
-    p.d = d.ptr, p.ldd = d.stride[0], p.act = act, p.kept = kept.ptr, p.ld_kept = kept.stride[0];
+    p.act = act;
+    auto half = [&](const lb_tensor& t, int k) {
+        const View3 v{(uint16_t*)t.ptr + (long long)k * p.N, t.dtype, 1, p.M, p.N, 0, t.stride[0], 1};
+        return make_map(v, true, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+    };
+    p.map_gate = half(kept, 0), p.map_up = half(kept, 1), p.map_d_gate = half(d, 0), p.map_d_up = half(d, 1);
     launch_pairs(p.a_mn_major ? make_map(dy, false, 64, BK) : make_map(dy, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p,
                  tiles, stream);
 }

@@ -1,4 +1,4 @@
-// Products of a few tokens (up to 16) with a weight matrix, and the gated block's: the weights are read once, and that is what a call costs.
+// Products of a few tokens (up to 32) with a weight matrix, and the gated block's: the weights are read once, and that is what a call costs.
 //
 // out [M, N] = x [M, K] w^T with w [N, K], rows along K. A block takes 16 rows of w (of the gated block eight of each weight) or, where that leaves SMs
 // without a block, eight, its warps a range of K each; partial sums meet in shared memory and are added in the warps' order. The rows go from
@@ -6,7 +6,8 @@
 // short side, and no tile of a tcgen05 product is shorter than 128 rows): which eight elements along K a lane holds is free as long as both sides
 // agree, so that each of its loads is 16 contiguous bytes. Up to 24 loads of a lane are in flight.
 //
-// Bound by the bytes of w and the time a load takes to arrive; what it measured is said where its launch is chosen.
+// Bound by the bytes of w, the time a load takes to arrive and, with more tokens, by reading those from the L2: 4 tokens with weights of 1024 x 4096 take 5.7 us
+// for both halves of the gated block where the weights' 25 MB are in the L2, 4.5 TB/s.
 #include <algorithm>
 
 #include "gate.cuh"
@@ -16,8 +17,9 @@
 namespace lb {
 namespace {
 
-constexpr int kMaxWarps = 16;
-constexpr int ahead(int tokens) { return tokens == 8 ? 8 : 4; }  // 32-wide blocks of K a warp has in flight: 96 registers of each lane
+constexpr int kMaxWarps = 16, kMaxTokens = 32;
+// 32-wide blocks of K a warp has in flight: 96 registers of each lane, 64 and 96
+constexpr int ahead(int tokens) { return tokens == 8 ? 8 : 4; }
 
 // 16 bytes, or zeros; in the order that these are written in, ahead of the products. STREAM: not to be read again soon.
 template <bool STREAM>
@@ -68,7 +70,7 @@ __device__ __forceinline__ float widen16(uint16_t x) {
     return F16 ? __half2float(__ushort_as_half(x)) : __uint_as_float((uint32_t)x << 16);
 }
 
-// GATED: rows 0..7 of a tile are the gate's, 8..15 the other projection's. ROWS: 16, or 8 with the tile's second half empty. TOKENS: 8 or 16.
+// GATED: rows 0..7 of a tile are the gate's, 8..15 the other projection's. ROWS: 16, or 8 with the tile's second half empty. TOKENS: 8, 16 or 32.
 template <bool GATED, bool F16, int ROWS, int TOKENS>
 __global__ void __launch_bounds__(kMaxWarps * 32, 1) skinny_kernel(const SkinnyArgs p) {
     __shared__ float sums[kMaxWarps][16][TOKENS + 1];
@@ -142,7 +144,7 @@ template <bool GATED, bool F16>
 void launch_skinny(SkinnyArgs& p, int sms, cudaStream_t s) {
     const int blocks = (p.K + 31) / 32;
     // a warp takes some blocks of K at a time, all of them in flight: as many warps as that needs
-    const int at_once = ahead(p.M <= 8 ? 8 : 16);
+    const int at_once = ahead(p.M <= 8 ? 8 : p.M <= 16 ? 16 : 32);
     p.warps = std::min(kMaxWarps, (blocks + at_once - 1) / at_once);
     p.per_warp = (blocks + p.warps - 1) / p.warps;
     const int rows = GATED ? 8 : (p.N + 15) / 16 >= sms ? 16 : 8;
@@ -150,10 +152,12 @@ void launch_skinny(SkinnyArgs& p, int sms, cudaStream_t s) {
     auto go = [&](auto kernel) { launch_overlapped(kernel, grid, block, 0, s, 0, p); };
     if (GATED || rows == 16) {
         if (p.M <= 8) go(skinny_kernel<GATED, F16, 16, 8>);
-        else go(skinny_kernel<GATED, F16, 16, 16>);
+        else if (p.M <= 16) go(skinny_kernel<GATED, F16, 16, 16>);
+        else go(skinny_kernel<GATED, F16, 16, 32>);
     } else {
         if (p.M <= 8) go(skinny_kernel<false, F16, 8, 8>);
-        else go(skinny_kernel<false, F16, 8, 16>);
+        else if (p.M <= 16) go(skinny_kernel<false, F16, 8, 16>);
+        else go(skinny_kernel<false, F16, 8, 32>);
     }
 }
 
@@ -169,8 +173,13 @@ SkinnyArgs skinny_args(const lb_tensor& x, const lb_tensor& w, const lb_tensor& 
 
 }  // namespace
 
+// Every block reads all tokens, from the L2: with more than eight of them that is what grows, and beyond 64 MB of it 128-row tiles are the better choice.
+// us of a gated block in a graph, bfloat16, width x hidden, tiles -> these: 4 tokens 1024 x 4096 22.4 -> 5.7, 16 (17 MB) 22.2 -> 9.1, 32 (34 MB) 22.1 -> 12.9,
+// 32 of 512 x 2048 12.8 -> 6.4, 4 of 2048 x 8192 33.5 -> 22.0; 9 of it (38 MB) 32 -> 29.8, 16 (67 MB) 31.9 -> 32.6, 32 (134 MB) 28.8 -> 47.0.
 bool skinny_takes(const lb_tensor& x, const lb_tensor& w) {
-    return x.shape[0] <= 16 && x.shape[1] % 8 == 0 && (x.dtype == LB_BF16 || x.dtype == LB_F16) && rows_in_pieces(x) && rows_in_pieces(w);
+    const long long M = x.shape[0], K = x.shape[1], N = w.shape[0];
+    return M <= kMaxTokens && K % 8 == 0 && (x.dtype == LB_BF16 || x.dtype == LB_F16) && rows_in_pieces(x) && rows_in_pieces(w) &&
+           (M <= 8 || M * K * 2 * (N / 16) < 64LL << 20);
 }
 void skinny_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept, int act, void* stream) {
     driver();
