@@ -223,7 +223,7 @@ struct Forward : Block {
 
 struct Backward : Block {
     lb_tensor dy, gate_up, h, dx, dwgu, dwd;
-    bool fused = false;
+    bool fused = false, grouped = false;
     size_t sums = 0, slopes = 0;  // bytes of dh in float32 and of [da db]
 
     Backward(int act, const lb_tensor* dy_t, const lb_tensor* x_t, const lb_tensor* wgu_t, const lb_tensor* wd_t, const lb_tensor* gate_up_t, const lb_tensor* h_t,
@@ -236,8 +236,10 @@ struct Backward : Block {
         sized(dwgu, 2 * F, D, dtype, "d_w_gate_up"), written(dwgu, "d_w_gate_up"), sized(dwd, D, F, dtype, "d_w_down"), written(dwd, "d_w_down");
         fused = M && sloped_tiles(M, F) && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F));
         sums = fused ? 0 : up((size_t)M * F * 4), slopes = up((size_t)M * 2 * F * dtype_size(dtype));
-        const lb_tensor d = slope();
-        products = std::max(std::max(fused ? 0 : product_scratch(dy, wd), product_scratch(d, wgu)), std::max(product_scratch(transposed(d), x), product_scratch(transposed(dy), h)));
+        const lb_tensor d = slope(), a[] = {d, transposed(d), transposed(dy)}, b[] = {wgu, x, h};
+        grouped = M && gemm_group_pays(a, b, 3);
+        products = fused ? 0 : product_scratch(dy, wd);
+        for (int k = 0; k < 3 && !grouped; k++) products = std::max(products, product_scratch(a[k], b[k]));
     }
     lb_tensor slope() const { return matrix((char*)scratch + sums, dtype, M, 2 * F, 2 * F); }
     size_t bytes() const { return sums + slopes + products; }
@@ -253,9 +255,9 @@ struct Backward : Block {
             g.in = scratch, g.ld_in = F, g.gate_up = gate_up.ptr, g.ld_gate_up = gate_up.stride[0], g.gate_up_out = d.ptr, g.ld_out = 2 * F, g.M = (int)M, g.F = (int)F;
             run_gate<true>(dtype, g, act, (cudaStream_t)stream);
         }
-        gemm(d, wgu, dx, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
-        gemm(transposed(d), x, dwgu, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
-        gemm(transposed(dy), h, dwd, EPI_NONE, 0, stream, more, products, nullptr, nullptr);
+        const lb_tensor a[] = {d, transposed(d), transposed(dy)}, b[] = {wgu, x, h}, out[] = {dx, dwgu, dwd};
+        if (grouped) return gemm_group(a, b, out, 3, stream);
+        for (int k = 0; k < 3; k++) gemm(a[k], b[k], out[k], EPI_NONE, 0, stream, more, products, nullptr, nullptr);
     }
 };
 

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <vector>
 
 #include "divide.cuh"
 #include "gate.cuh"
@@ -58,7 +59,7 @@ struct GemmArgs {
 // What the kernel for CTA pairs does with a tile: the epilogues of lb_gemm, or one half of the gated feed-forward block. In its forward products
 // the leader's half of the B columns are rows of one weight and the other CTA's the same rows of another, so that each CTA's accumulator holds both
 // projections of 128 columns side by side; in its backward product the epilogue reads what the forward pass has kept.
-enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED };
+enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED, PAIR_GROUP };
 struct PlainArgs : GemmArgs {
     static constexpr int mode = PAIR_PLAIN;
 };
@@ -74,6 +75,29 @@ struct alignas(64) SlopedArgs : GemmArgs {
     CUtensorMap map_gate, map_up, map_d_gate, map_d_up;  // both projections as kept, and their gradients: 32 x 32 pieces
     int act;
 };
+
+// Up to three products of one launch, one after another in the grid, each without an epilogue and its K whole.
+constexpr int kGroup = 3;
+struct alignas(64) GroupArgs : GemmArgs {
+    static constexpr int mode = PAIR_GROUP;
+    CUtensorMap map_a[kGroup], map_b[kGroup];
+    GemmArgs product[kGroup];
+    int first[kGroup + 1];  // first unit of each, those that there are not beginning at the end
+};
+// The product that a unit belongs to; `unit` becomes its number in it.
+template <class Args>
+__device__ __forceinline__ const GemmArgs& product_of(const Args& p, int& unit, int& which) {
+    which = 0;
+    if constexpr (Args::mode == PAIR_GROUP) {
+#pragma unroll
+        for (int k = 1; k < kGroup; k++)
+            if (unit >= p.first[k]) which = k;
+        unit -= p.first[which];
+        return p.product[which];
+    } else {
+        return p;
+    }
+}
 
 // Unit `unit` of the grid: split * tiles + tile, neighbours share a K range.
 __device__ __forceinline__ int tile_coords(const GemmArgs& p, int unit, int& b, int& m_blk, int& n_blk) {
@@ -630,9 +654,9 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp-uniform for the compiler too
     const uint32_t rank = cluster_ctarank();
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-    const int num_tiles = p.tiles_m * p.tiles_n * p.batch;  // tiles_m counts 256-row pair tiles here
-    const int total_kb = (p.K + BK - 1) / BK;
-    const int num_units = num_tiles * p.splits;
+    int num_units;  // tiles_m counts 256-row pair tiles here
+    if constexpr (Args::mode == PAIR_GROUP) num_units = p.first[kGroup];
+    else num_units = p.tiles_m * p.tiles_n * p.batch * p.splits;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES_; s++) {
@@ -647,8 +671,12 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             for (int s = 0; s < kEpilogueWarps * kPieces; s++) mbar_init(&landed[s], 1);
         *abort_flag = 0;
         fence_barrier_init();
-        tma_prefetch_desc(&map_a);
-        tma_prefetch_desc(&map_b);
+        if constexpr (Args::mode == PAIR_GROUP) {
+            for (int k = 0; k < kGroup; k++) tma_prefetch_desc(&p.map_a[k]), tma_prefetch_desc(&p.map_b[k]);
+        } else {
+            tma_prefetch_desc(&map_a);
+            tma_prefetch_desc(&map_b);
+        }
         if constexpr (Args::mode == PAIR_GATED) tma_prefetch_desc(&p.map_up);
     }
     if (warp == 1) {
@@ -669,28 +697,30 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             uint32_t phase = 0;
             bool ok = true;
             for (int unit = pair; unit < num_units && ok; unit += num_pairs) {
-                int b, m_blk, n_blk;
-                const int kb0 = tile_coords(p, unit, b, m_blk, n_blk) * p.kb_per_split;
+                int at = unit, which, b, m_blk, n_blk;
+                const GemmArgs& q = product_of(p, at, which);
+                const int total_kb = (q.K + BK - 1) / BK, kb0 = tile_coords(q, at, b, m_blk, n_blk) * q.kb_per_split;
                 const int row0 = m_blk * 2 * BM + (int)rank * BM;
                 int col0 = n_blk * BN + (int)rank * (BN / 2);
-                const CUtensorMap* operand_b = &map_b;
+                const CUtensorMap *operand_a = &map_a, *operand_b = &map_b;
+                if constexpr (Args::mode == PAIR_GROUP) operand_a = &p.map_a[which], operand_b = &p.map_b[which];
                 if constexpr (Args::mode == PAIR_GATED) {
                     col0 = n_blk * (BN / 2);
                     if (rank) operand_b = &p.map_up;
                 }
-                const int kb1 = min(total_kb, kb0 + p.kb_per_split);
+                const int kb1 = min(total_kb, kb0 + q.kb_per_split);
                 for (int kb = kb0; kb < kb1; kb++) {
                     if (!(ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag))) break;
                     if (rank == 0) mbar_expect_tx(&full[stage], 2 * (kPairStageBytesA + kPairStageBytesB));
                     uint8_t* sa = smem_a + stage * kPairStageBytesA;
                     uint8_t* sb = smem_b + stage * kPairStageBytesB;
-                    if (!p.a_mn_major) {
-                        tma_load_3d_pair(sa, &map_a, &full[stage], kb * BK, row0, b);  // box {64 k, 128 m}
+                    if (!q.a_mn_major) {
+                        tma_load_3d_pair(sa, operand_a, &full[stage], kb * BK, row0, b);  // box {64 k, 128 m}
                     } else {
                         for (int j = 0; j < BM / 64; j++)  // boxes {64 m, 64 k}
-                            tma_load_3d_pair(sa + j * (64 * BK * 2), &map_a, &full[stage], row0 + j * 64, kb * BK, b);
+                            tma_load_3d_pair(sa + j * (64 * BK * 2), operand_a, &full[stage], row0 + j * 64, kb * BK, b);
                     }
-                    if (!p.b_mn_major) {
+                    if (!q.b_mn_major) {
                         tma_load_3d_pair(sb, operand_b, &full[stage], kb * BK, col0, b);  // box {64 k, 128 n}
                     } else {
                         for (int j = 0; j < BN / 2 / 64; j++)  // boxes {64 n, 64 k}
@@ -708,10 +738,15 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         // ---- MMA issuer (leader CTA only): the whole warp, so that the operands stay in uniform registers ----
         if (rank == 0) {
             const bool leader = elect_one();
-            const uint32_t idesc = make_idesc(2 * BM, BN, p.in_bf16 != 0, p.a_mn_major, p.b_mn_major);
-            const uint64_t da0 = p.a_mn_major ? make_smem_desc(smem_u32(smem_a), 64 * BK * 2, 1024) : make_smem_desc(smem_u32(smem_a), 16, 1024);
-            const uint64_t db0 = p.b_mn_major ? make_smem_desc(smem_u32(smem_b), 64 * BK * 2, 1024) : make_smem_desc(smem_u32(smem_b), 16, 1024);
-            const uint32_t a_step = p.a_mn_major ? 2048u : 32u, b_step = p.b_mn_major ? 2048u : 32u;
+            uint32_t idesc, a_step, b_step;
+            uint64_t da0, db0;
+            auto operands = [&](const GemmArgs& q) {
+                idesc = make_idesc(2 * BM, BN, q.in_bf16 != 0, q.a_mn_major, q.b_mn_major);
+                da0 = q.a_mn_major ? make_smem_desc(smem_u32(smem_a), 64 * BK * 2, 1024) : make_smem_desc(smem_u32(smem_a), 16, 1024);
+                db0 = q.b_mn_major ? make_smem_desc(smem_u32(smem_b), 64 * BK * 2, 1024) : make_smem_desc(smem_u32(smem_b), 16, 1024);
+                a_step = q.a_mn_major ? 2048u : 32u, b_step = q.b_mn_major ? 2048u : 32u;
+            };
+            if constexpr (Args::mode != PAIR_GROUP) operands(p);
             int stage = 0;
             uint32_t phase = 0;
             int local = 0;
@@ -722,8 +757,11 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 if (!(ok = mbar_wait_cluster_warp(&tmem_empty[buf], (use & 1) ^ 1, abort_flag))) break;
                 tc_fence_after();
                 const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
-                const int kb0 = (int)p.by_tiles.div(unit) * p.kb_per_split;
-                const int num_kb = min(total_kb, kb0 + p.kb_per_split) - kb0;
+                int at = unit, which;
+                const GemmArgs& q = product_of(p, at, which);
+                if constexpr (Args::mode == PAIR_GROUP) operands(q);
+                const int total_kb = (q.K + BK - 1) / BK, kb0 = (int)q.by_tiles.div(at) * q.kb_per_split;
+                const int num_kb = min(total_kb, kb0 + q.kb_per_split) - kb0;
                 for (int kb = 0; kb < num_kb; kb++) {
                     if (!(ok = mbar_wait_warp(&full[stage], phase, abort_flag))) break;
                     tc_fence_after();
@@ -754,13 +792,18 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         uint4* stage = (uint4*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + 256) + (warp - 2) * (kStageBytesPerWarp / 16);
         int local = 0;
         bool ok = true;
-        const bool vec_ok = p.d_bf16 || p.d_f16 ? (p.ldd % 8 == 0 && p.d_batch_stride % 8 == 0 && ((uintptr_t)p.d & 15) == 0)
-                                                : (p.ldd % 4 == 0 && p.d_batch_stride % 4 == 0 && ((uintptr_t)p.d & 15) == 0);
+        auto in_vectors = [](const GemmArgs& q) {
+            return q.d_bf16 || q.d_f16 ? (q.ldd % 8 == 0 && q.d_batch_stride % 8 == 0 && ((uintptr_t)q.d & 15) == 0)
+                                       : (q.ldd % 4 == 0 && q.d_batch_stride % 4 == 0 && ((uintptr_t)q.d & 15) == 0);
+        };
+        bool vec_ok = false;
+        if constexpr (Args::mode == PAIR_PLAIN) vec_ok = in_vectors(p);
         for (int unit = pair; unit < num_units && ok; unit += num_pairs, local++) {
             const int buf = local & 1;
             const uint32_t use = (uint32_t)(local >> 1);
-            int b, m_blk, n_blk;
-            const int split = tile_coords(p, unit, b, m_blk, n_blk);
+            int at = unit, which, b, m_blk, n_blk;
+            const GemmArgs& q = product_of(p, at, which);
+            const int split = tile_coords(q, at, b, m_blk, n_blk);
             const int row = m_blk * 2 * BM + (int)rank * BM + quarter * 32 + lane;
             auto release = [&] {
                 tc_fence_before();
@@ -779,6 +822,13 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else if (p.act == ACT_SILU) drain_gated<ACT_SILU, true>(p, tbase, row, col0, stage, lane, release);
                 else if (p.act == ACT_GELU) drain_gated<ACT_GELU, true>(p, tbase, row, col0, stage, lane, release);
                 else drain_gated<ACT_RELU, true>(p, tbase, row, col0, stage, lane, release);
+            } else if constexpr (Args::mode == PAIR_GROUP) {
+                const int col_base = n_blk * BN + col_half * (BN / 2);
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                drain_tile(q, tbase, row, (long long)row * q.ldd, col_base, 0, in_vectors(q), stage, lane, release);
             } else {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 const long long row_off = (long long)b * p.d_batch_stride + (long long)row * p.ldd;
@@ -938,16 +988,17 @@ static int gemm_tile_splits(long long M, long long N, long long K, long long bat
 // this model puts another less than a tenth below it is no better line: 64 such shapes, every operand major, 0.84 - 1.14 of these counts' time for a product alone,
 // 1.007 in the mean, and 0.84 - 1.37, 0.99, one after another under the power cap.) Which products stay on narrow tiles is left to the model above, which
 // that line was measured with.
+static double pairs_us(long long tiles, long long total_kb, int s, int pairs, double millions) {
+    const double kb = (double)((total_kb + s - 1) / s), waves = (double)((tiles * s + pairs - 1) / pairs);
+    return 3.0 + waves * (0.3 * kb + 2.0) + 0.1 * kb * (double)(tiles * s) / pairs + (s > 1 ? 3.5 + millions * (0.45 * s + 0.6) : 0.0);
+}
 int gemm_splits(long long M, long long N, long long K, long long batch, int sms) {
     if (M <= BM) return gemm_tile_splits(M, N, K, batch, sms);
     const int pairs = sms / 2;
     const long long tiles = ((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN) * batch, total_kb = (K + BK - 1) / BK;
     if (tiles >= 4LL * pairs || total_kb < 32) return 1;
     const double millions = (double)(batch * M * N) * 1e-6;
-    auto cost = [&](int s) {
-        const double kb = (double)((total_kb + s - 1) / s), waves = (double)((tiles * s + pairs - 1) / pairs);
-        return 3.0 + waves * (0.3 * kb + 2.0) + 0.1 * kb * (double)(tiles * s) / pairs + (s > 1 ? 3.5 + millions * (0.45 * s + 0.6) : 0.0);
-    };
+    auto cost = [&](int s) { return pairs_us(tiles, total_kb, s, pairs, millions); };
     int best = 1;
     double best_us = cost(1) * 0.9;
     for (int s = 2; s <= 32 && total_kb / s >= 16; s++)
@@ -1228,6 +1279,58 @@ static void launch_pairs(const CUtensorMap& map_a, const CUtensorMap& map_b, con
         LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(Args::mode)));
     const int max_pairs = resident_pairs(dev), grid = 2 * (int)std::min<long long>(tiles, max_pairs > 0 ? max_pairs : dev.sms / 2);
     launch_overlapped(gemm_tcgen05_pair<Args>, dim3((unsigned)grid), dim3(kThreads), pair_smem(Args::mode), (cudaStream_t)stream, 0, map_a, map_b, p);
+}
+
+// Products that do not depend on one another in one launch, the longest K first, where the model of pairs says that they take a tenth less so than one
+// after another: each alone leaves SMs without a tile in its last round, and together they have one last round. Pairs take units in turn.
+bool gemm_group_pays(const lb_tensor* a, const lb_tensor* b, int n) {
+    const int sms = sm_count_hint(), pairs = sms / 2;
+    if (n > kGroup) return false;
+    double alone = 0.0, shared = 0.0;
+    long long units = 0, order[kGroup], tiles[kGroup], blocks[kGroup];
+    for (int k = 0; k < n; k++) {
+        const View3 x = view3(a[k], "a"), y = view3(b[k], "b");
+        bool a_cols, b_cols;
+        const long long M = x.rows, N = y.cols, K = x.cols;
+        if (M <= BM || N == 0 || !tensor_core_operands(x, y, a_cols, b_cols)) return false;
+        const int split = gemm_splits(M, N, K, 1, sms);
+        if (gemm_route(M, N, K, 1, sms, 0, split > 1 ? gemm_scratch_bytes(M, N, K, 1) : 0, nullptr).ranges) return false;
+        order[k] = k, tiles[k] = (M + 2 * BM - 1) / (2 * BM) * ((N + BN - 1) / BN), blocks[k] = (K + BK - 1) / BK;
+        alone += pairs_us(tiles[k], blocks[k], split, pairs, (double)(M * N) * 1e-6);
+        shared += 0.1 * (double)(blocks[k] * tiles[k]) / pairs, units += tiles[k];
+    }
+    if (units > 16LL * pairs) return false;  // (the last round's idle SMs are no tenth any more)
+    std::sort(order, order + n, [&](long long x, long long y) { return blocks[x] > blocks[y]; });
+    std::vector<double> load((size_t)pairs, 0.0);
+    long long at = 0;
+    for (int k = 0; k < n; k++)
+        for (long long i = 0; i < tiles[order[k]]; i++) load[(size_t)(at++ % pairs)] += 0.3 * (double)blocks[order[k]] + 2.0;
+    return 3.0 + *std::max_element(load.begin(), load.end()) + shared < 0.9 * alone;
+}
+void gemm_group(const lb_tensor* a, const lb_tensor* b, const lb_tensor* d, int n, void* stream) {
+    driver();
+    GroupArgs p{};
+    int order[kGroup];
+    for (int k = 0; k < n; k++) order[k] = k;
+    std::sort(order, order + n, [&](int x, int y) { return a[x].shape[1] > a[y].shape[1]; });
+    long long units = 0;
+    for (int k = 0; k < kGroup; k++) {
+        p.first[k] = (int)units;
+        const int i = order[std::min(k, n - 1)];
+        const View3 x = view3(a[i], "a"), y = view3(b[i], "b"), w = turned(y);
+        bool a_cols, b_cols;
+        tensor_core_operands(x, y, a_cols, b_cols);
+        GemmArgs& q = p.product[k];
+        long long tiles;
+        pair_args(q, x, w, a_cols, !b_cols, BN, tiles);
+        q.d = d[i].ptr, q.ldd = d[i].stride[0];
+        p.map_a[k] = q.a_mn_major ? make_map(x, false, 64, BK) : make_map(x, true, BK, BM);
+        p.map_b[k] = q.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2);
+        if (k < n) units += tiles;
+    }
+    p.first[kGroup] = (int)units;
+    p.status = status_word();
+    launch_pairs(p.map_a[0], p.map_b[0], p, units, stream);
 }
 
 bool gemm_gated_takes(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept) {

@@ -78,6 +78,10 @@ void gemm_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, cons
 bool gemm_sloped_takes(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d);
 void gemm_sloped(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d, int act, void* stream);
 
+// d[k] = a[k] b[k] for up to three products of 16-bit operands that do not depend on one another, in one launch; `_pays`: whether they can and gain by it.
+bool gemm_group_pays(const lb_tensor* a, const lb_tensor* b, int n);
+void gemm_group(const lb_tensor* a, const lb_tensor* b, const lb_tensor* d, int n, void* stream);
+
 // A few tokens (gemm_skinny.cu): out [M, N] = x [M, K] w^T with w [N, K], plus `add` [M, N] once rounded (null: nothing); h and kept as in gemm_gated.
 bool skinny_takes(const lb_tensor& x, const lb_tensor& w);
 void skinny_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept, int act, void* stream);

@@ -276,7 +276,7 @@ int read_dl(PyObject* t, lb_tensor* out, Here& here) {
     out->ptr = (char*)d.data + d.byte_offset, out->dtype = dtype, out->rank = d.ndim;
     int64_t step = 1;
     for (int k = d.ndim; k-- > 0; step *= d.shape[k]) out->shape[k] = d.shape[k], out->stride[k] = d.strides ? d.strides[k] : step;
-    return 1;
+    return out->ptr || step == 0;  // (a wrapper around other tensors has elements and no memory: its own methods have the say)
 }
 bool describe_here(PyObject* t, lb_tensor* out, Here& here) {
     if (const int read = read_dl(t, out, here)) return read > 0;

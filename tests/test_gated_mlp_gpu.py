@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from lumen_b200 import device as D
-from lumen_b200.runtime import device_status, gated_mlp_backward, gated_mlp_forward
+from lumen_b200.runtime import device_status, gated_mlp_backward, gated_mlp_forward, gemm
 
 pytestmark = pytest.mark.gpu
 
@@ -102,7 +102,7 @@ SHAPES = [
     # tokens, width, hidden
     (1, 64, 64), (1, 1024, 512), (2, 136, 264), (4, 1024, 1000), (7, 512, 128), (8, 96, 2048), (9, 256, 192), (16, 328, 520), (17, 128, 128),
     (32, 512, 256), (33, 256, 200), (100, 64, 72), (128, 256, 256), (129, 520, 136), (255, 128, 1032), (257, 264, 384), (300, 72, 128), (512, 256, 640),
-    (700, 8, 8), (1000, 320, 1160), (5, 15, 9), (40, 33, 70), (130, 100, 61),
+    (700, 8, 8), (1000, 320, 1160), (1500, 840, 2056), (1921, 1000, 1504), (8300, 40, 8), (5, 2400, 64), (12, 2400, 72), (20, 2400, 64), (24, 512, 264), (5, 15, 9), (40, 33, 70), (130, 100, 61),
 ]  # fmt: skip
 
 
@@ -260,6 +260,17 @@ def test_repeats_streams_and_graphs(cuda, m):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for out, w in zip(outs, want) for a, b in zip(out, w))
     device_status()
+
+
+@pytest.mark.parametrize("shape", [(2600, 840, 2056), (1500, 840, 2056), (1777, 1096, 1288)])
+def test_products_of_one_launch_are_those_of_several(cuda, shape):
+    """The backward's last products, whether they share a launch or not, give the bits of lb_gemm's with K whole."""
+    m, d, f = shape
+    x, wgu, wd, dy = operands(cuda, m, d, f, torch.bfloat16)
+    _, gate_up, h = gated_mlp_forward(x, wgu, wd)
+    dx, dwgu, dwd = gated_mlp_backward(dy, x, wgu, wd, gate_up, h)
+    assert torch.equal(dwd, gemm(dy.t(), h, torch.empty_like(wd), kernel="tcgen05"))
+    check_backward(dy, x, wgu, wd, gate_up, h, "silu", dx, dwgu, dwd)
 
 
 def test_on_the_packages_own_tensors(cuda):

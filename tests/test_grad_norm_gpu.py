@@ -185,6 +185,44 @@ def test_repeats_bit_for_bit_on_any_stream_and_in_graphs(cuda):
         assert torch.equal(norms[k], want[k][0]) and all(torch.equal(a, b) for a, b in zip(outs[k], want[k][1]))
 
 
+def test_a_tensor_on_another_gpu_is_refused(cuda):
+    """A stand-in that says it lives on GPU 1 while GPU 0 is current: nothing is launched."""
+
+    class Elsewhere:
+        shape, dtype, is_cuda = (4,), "float32", True
+        get_device = staticmethod(lambda: 1)
+        data_ptr = staticmethod(lambda: 1 << 20)
+        stride = staticmethod(lambda: (1,))
+
+    x = torch.ones(4, device=cuda)
+    for call in (lambda: clip_grad_norm([x, Elsewhere()], 1.0), lambda: clip_grad_norm([x], 1.0, out=[Elsewhere()]), lambda: grad_norm([x, Elsewhere()])):
+        with pytest.raises(ValueError, match="a tensor is on GPU 1, the current one is GPU 0"):
+            call()
+    assert torch.equal(x, torch.ones_like(x))
+
+
+def test_from_several_threads(cuda):
+    """Two threads, each on a stream of its own, clip their own tensors at once."""
+    import threading
+
+    sets = [tensors(cuda, [70001, 333, 4096], seed=k) for k in range(2)]
+    want = [float(grad_norm(xs)) for xs in sets]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[k] = [float(clip_grad_norm(sets[k], 1e9)) for _ in range(50)]
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(set(g) == {w} for g, w in zip(got, want))
+
+
 def test_on_the_packages_own_tensors(cuda):
     xs = tensors(cuda, [1000, 33], dtypes=[torch.float32])
     region = D.Region(32 << 20)
