@@ -82,7 +82,8 @@ struct alignas(64) GroupArgs : GemmArgs {
     static constexpr int mode = PAIR_GROUP;
     CUtensorMap map_a[kGroup], map_b[kGroup];
     GemmArgs product[kGroup];
-    int first[kGroup + 1];  // first unit of each, those that there are not beginning at the end
+    int first[kGroup];  // first unit of each, those that there are not beginning at the end
+    int units;
 };
 // The product that a unit belongs to; `unit` becomes its number in it.
 template <class Args>
@@ -655,7 +656,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const uint32_t rank = cluster_ctarank();
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
     int num_units;  // tiles_m counts 256-row pair tiles here
-    if constexpr (Args::mode == PAIR_GROUP) num_units = p.first[kGroup];
+    if constexpr (Args::mode == PAIR_GROUP) num_units = p.units;
     else num_units = p.tiles_m * p.tiles_n * p.batch * p.splits;
 
     if (threadIdx.x == 0) {
@@ -671,12 +672,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             for (int s = 0; s < kEpilogueWarps * kPieces; s++) mbar_init(&landed[s], 1);
         *abort_flag = 0;
         fence_barrier_init();
-        if constexpr (Args::mode == PAIR_GROUP) {
-            for (int k = 0; k < kGroup; k++) tma_prefetch_desc(&p.map_a[k]), tma_prefetch_desc(&p.map_b[k]);
-        } else {
-            tma_prefetch_desc(&map_a);
-            tma_prefetch_desc(&map_b);
-        }
+        if constexpr (Args::mode != PAIR_GROUP) tma_prefetch_desc(&map_a), tma_prefetch_desc(&map_b);
         if constexpr (Args::mode == PAIR_GATED) tma_prefetch_desc(&p.map_up);
     }
     if (warp == 1) {
@@ -1328,7 +1324,7 @@ void gemm_group(const lb_tensor* a, const lb_tensor* b, const lb_tensor* d, int 
         p.map_b[k] = q.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2);
         if (k < n) units += tiles;
     }
-    p.first[kGroup] = (int)units;
+    p.units = (int)units;
     p.status = status_word();
     launch_pairs(p.map_a[0], p.map_b[0], p, units, stream);
 }
