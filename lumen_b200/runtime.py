@@ -225,7 +225,7 @@ class _Torch:
             torch = sys.modules["torch"]
             if not hasattr(torch._C, "_cuda_getCurrentRawStream"):
                 return False
-            cls.empty_like, cls.dense, cls.float32 = torch.empty_like, torch.contiguous_format, torch.float32
+            cls.empty_like, cls.dense, cls.float32, cls.bytes = torch.empty_like, torch.contiguous_format, torch.float32, torch.uint8
             cls.raw_stream, cls.device, cls.tensor = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, torch.Tensor
         return type(t) is cls.tensor and stream is None and _current[0] == 0 and t.is_cuda
 
@@ -357,6 +357,13 @@ def _outputs(like, stream, *wanted):
     return [None if w is None else _empty_like_input(like, *w) for w in wanted], _stream(stream)
 
 
+def _scratch(like, stream):
+    """What the native path calls for a call's workspace: `nbytes` -> memory for the kernels queued on `stream` (see `_workspace`)."""
+    if _Torch.takes(like, stream):
+        return lambda nbytes: like.new_empty(nbytes, dtype=_Torch.bytes)
+    return lambda nbytes: _workspace(like, (nbytes,), "uint8", stream)
+
+
 def _results_like(tensors, out, stream):
     """`out`, or new dense tensors like each of `tensors`, and the handle of the stream."""
     if out is not None:
@@ -390,7 +397,7 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, cos, sin, positions=None, q_we
     grads = _results_like(weights, None, stream)[0] if weights else []
     d_q_weight, d_k_weight = grads.pop(0) if q_weight is not None else None, grads.pop() if k_weight is not None else None
     _lib.host().qk_norm_rope_bwd(eps, bool(interleaved), d_q_out, d_k_out, q, k, cos, sin, positions, q_weight, k_weight, d_q, d_k, d_q_weight, d_k_weight,
-                                 lambda nbytes: _workspace(q, (nbytes,), "uint8", stream), handle)
+                                 _scratch(q, stream), handle)
     return d_q, d_k, d_q_weight, d_k_weight
 
 
@@ -417,7 +424,7 @@ def gated_mlp_forward(x, w_gate_up, w_down, activation="silu", residual=None, sa
     else:
         dtype = dtype_name(x.dtype)
         (y, gate_up, h), handle = _outputs(x, stream, (tuple(x.shape), dtype), ((*lead, 2 * f), dtype) if save else None, ((*lead, f), dtype))
-    _lib.host().gated_mlp_fwd(act, x, w_gate_up, w_down, residual, y, gate_up, h, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream), handle)
+    _lib.host().gated_mlp_fwd(act, x, w_gate_up, w_down, residual, y, gate_up, h, _scratch(x, stream), handle)
     return y, gate_up, h
 
 
@@ -427,7 +434,7 @@ def gated_mlp_backward(d_y, x, w_gate_up, w_down, gate_up, h, activation="silu",
     require_cuda()
     act = _activation(activation)
     (d_x, d_wgu, d_wd), handle = _results_like((x, w_gate_up, w_down), None, stream)
-    _lib.host().gated_mlp_bwd(act, d_y, x, w_gate_up, w_down, gate_up, h, d_x, d_wgu, d_wd, lambda nbytes: _workspace(x, (nbytes,), "uint8", stream), handle)
+    _lib.host().gated_mlp_bwd(act, d_y, x, w_gate_up, w_down, gate_up, h, d_x, d_wgu, d_wd, _scratch(x, stream), handle)
     return d_x, d_wgu, d_wd
 
 
@@ -438,7 +445,7 @@ def _norm(tensors, out, max_norm, like, stream):
             raise ValueError("the norm of no tensors needs `like`, a tensor on the GPU")
         like = tensors[0]
     (norm,), handle = _outputs(like, stream, ((), "float32"))
-    _lib.host().clip_grad_norm(tensors, out, max_norm, norm, lambda nbytes: _workspace(like, (nbytes,), "uint8", stream), handle)
+    _lib.host().clip_grad_norm(tensors, out, max_norm, norm, _scratch(like, stream), handle)
     return norm
 
 
