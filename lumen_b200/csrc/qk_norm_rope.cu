@@ -350,7 +350,7 @@ __device__ __forceinline__ void copy_async(void* to, const void* from, int bytes
 }
 // Heads of a group at a time, blocks of an SM, bytes of its ring.
 template <class T, bool BWD, int N>
-constexpr int many_heads() { return sizeof(T) == 4 || (BWD && N == 8) ? 2 : 4; }
+constexpr int many_heads() { return sizeof(T) == 4 || N == 8 ? 2 : 4; }
 template <int N>
 constexpr int many_per_sm() { return N == 8 ? 2 : 3; }
 template <class T, bool BWD, int N>
