@@ -308,7 +308,8 @@ __device__ __forceinline__ Pair widen(uint32_t w) {
 __device__ __forceinline__ Pair columns(const uint32_t* v, int j) { return both(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])); }
 
 // 64 columns of both projections (the gate's at `tbase`, the other's 128 columns further), their gated product, whole 128-byte row pieces each.
-// Rows are 16-byte aligned and N is a multiple of 8 (checked by the host).
+// Rows are 16-byte aligned and N is a multiple of 8 (checked by the host). 16384 x 4096 (twice) x 1024 with all three results 195 us, 1410 TFLOP/s; the plain
+// product of that many FLOPs, with a result of two thirds the size, 187. Packed arithmetic is what brought it from 200.
 template <int ACT, bool F16, class Release>
 __device__ __forceinline__ void drain_gated(const GatedArgs& p, uint32_t tbase, int row, int col0, uint4* stage, int lane, Release release) {
     uint4 gate[8], up[8], h[8];
@@ -776,15 +777,14 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 if (ok) mma_commit_pair(&tmem_full[buf], 3, leader);
             }
         }
+    } else if constexpr (Args::mode == PAIR_SLOPED) {
+        uint8_t* pieces = smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB);
+        sloped_way_out(p, pieces + (warp - 2) * kPieces * kPieceBytes, landed + (warp - 2) * kPieces, tmem_full, tmem_empty, tmem_base, pair, num_pairs, num_units, (int)rank,
+                       warp & 3, (warp - 2) >> 2, lane, abort_flag);
     } else {
         // ---- epilogue: warps 2..9 of both CTAs, each CTA on its own 128 rows ----
         const int quarter = warp & 3;
         const int col_half = (warp - 2) >> 2;
-        if constexpr (Args::mode == PAIR_SLOPED) {
-            uint8_t* pieces = smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB);
-            sloped_way_out(p, pieces + (warp - 2) * kPieces * kPieceBytes, landed + (warp - 2) * kPieces, tmem_full, tmem_empty, tmem_base, pair, num_pairs, num_units,
-                           (int)rank, quarter, col_half, lane, abort_flag);
-        } else {
         uint4* stage = (uint4*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + 256) + (warp - 2) * (kStageBytesPerWarp / 16);
         int local = 0;
         bool ok = true;
@@ -840,7 +840,6 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else if (LB_RARELY(p.splits > 1)) drain_partial(p, tbase, row, col_base, b, split, stage, lane, release);
                 else drain_tile(p, tbase, row, row_off, col_base, b, vec_ok, stage, lane, release);
             }
-        }
         }
     }
 
@@ -1278,7 +1277,10 @@ static void launch_pairs(const CUtensorMap& map_a, const CUtensorMap& map_b, con
 }
 
 // Products that do not depend on one another in one launch, the longest K first, where the model of pairs says that they take a tenth less so than one
-// after another: each alone leaves SMs without a tile in its last round, and together they have one last round. Pairs take units in turn.
+// after another: each alone leaves SMs without a tile in its last round, and together they have one last round. Pairs take units in turn. us of the gated
+// block's backward, three launches -> one, bfloat16: 2600 x 840 x 2056 (36 + 68 + 44 tiles on 74 pairs) 95.3 -> 79.5; in a graph 4096 tokens of 512 x 2048 80 -> 69,
+// 8192 of 1024 x 4096 338 -> 319, 8192 of 512 x 2048 110 -> 104; where the model says no: 512 of 1024 x 4096 50.9 -> 65.4, 1024 65.4 -> 74.0, 2048 99 -> 106,
+// 16384 742 -> 779.
 bool gemm_group_pays(const lb_tensor* a, const lb_tensor* b, int n) {
     const int sms = sm_count_hint(), pairs = sms / 2;
     if (n > kGroup) return false;
