@@ -369,7 +369,10 @@ def _results_like(tensors, out, stream):
     if out is not None:
         return out, _stream(stream)
     if _Torch.takes(tensors[0], stream):
-        return [_Torch.like(t) for t in tensors], _Torch.stream()
+        try:
+            return [_Torch.like(t) for t in tensors], _Torch.stream()
+        except TypeError:  # one of them is another framework's
+            pass
     return [_empty_like_input(t, tuple(t.shape), dtype_name(t.dtype)) for t in tensors], _stream(stream)
 
 

@@ -102,7 +102,7 @@ SHAPES = [
     # tokens, width, hidden
     (1, 64, 64), (1, 1024, 512), (2, 136, 264), (4, 1024, 1000), (7, 512, 128), (8, 96, 2048), (9, 256, 192), (16, 328, 520), (17, 128, 128),
     (32, 512, 256), (33, 256, 200), (100, 64, 72), (128, 256, 256), (129, 520, 136), (255, 128, 1032), (257, 264, 384), (300, 72, 128), (512, 256, 640),
-    (700, 8, 8), (1000, 320, 1160), (1500, 840, 2056), (1921, 1000, 1504), (8300, 40, 8), (5, 2400, 64), (12, 2400, 72), (20, 2400, 64), (24, 512, 264), (5, 15, 9), (40, 33, 70), (130, 100, 61),
+    (700, 8, 8), (1000, 320, 1160), (1500, 840, 2056), (1921, 1000, 1504), (8300, 40, 8), (5, 2400, 64), (12, 2400, 72), (20, 2400, 64), (24, 512, 264), (64, 40, 6200), (40, 24, 16400), (3, 64, 4200), (30, 8, 5000), (5, 15, 9), (40, 33, 70), (130, 100, 61),
 ]  # fmt: skip
 
 
@@ -191,6 +191,18 @@ def test_nan_stays_in_its_row(cuda, m):
         assert bool(got[1].isnan().all())
         keep = torch.arange(m, device=cuda) != 1
         assert torch.equal(got[keep], was[keep])
+
+
+def test_parameters_and_results_of_autograd(cuda):
+    """Weights as torch's parameters: results are plain tensors, and the weights stay what they were."""
+    x, wgu, wd, dy = operands(cuda, 40, 64, 96, torch.bfloat16)
+    want = gated_mlp_forward(x, wgu, wd)
+    grads = gated_mlp_backward(dy, x, wgu, wd, want[1], want[2])
+    p, q = torch.nn.Parameter(wgu), torch.nn.Parameter(wd)
+    got = gated_mlp_forward(torch.nn.Parameter(x), p, q)
+    again = gated_mlp_backward(dy, x, p, q, got[1], got[2])
+    for a, b in zip((*got, *again), (*want, *grads)):
+        assert torch.equal(a, b) and not a.requires_grad and type(a) is torch.Tensor
 
 
 def test_no_tokens(cuda):
