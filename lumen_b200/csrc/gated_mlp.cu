@@ -194,7 +194,7 @@ struct Forward : Block {
         if (M == 0) return;
         few = skinny_takes(x, wgu) && skinny_takes(h, wd);
         if (few) return;
-        fused = gated_tiles(M, F) && gemm_gated_takes(x, wgu, h, keeps ? &gate_up : nullptr);
+        fused = gemm_gated_takes(x, wgu, h, keeps ? &gate_up : nullptr) && (gemm_gated_ranges(x, wgu) || gated_tiles(M, F));
         if (!fused && (dtype != LB_F32 || !keeps)) sums = up((size_t)M * 2 * F * 4);
         products = std::max(fused ? 0 : product_scratch(x, transposed(wgu)), product_scratch(h, transposed(wd)));
     }

@@ -1337,6 +1337,9 @@ bool gemm_gated_takes(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h
     bool a_cols, b_cols;
     return h.shape[1] % 8 == 0 && tensor_core_operands(view3(x, "x"), turned(half), a_cols, b_cols) && in_pieces(h) && (!kept || in_pieces(*kept));
 }
+int gemm_gated_ranges(const lb_tensor& x, const lb_tensor& w) {
+    return w.stride[1] == 1 ? gemm_small_splits(x.shape[0], w.shape[0], x.shape[1], 1, sm_count_hint(), 1) : 0;
+}
 void gemm_gated(const lb_tensor& x_t, const lb_tensor& w_t, const lb_tensor& h, const lb_tensor* kept, int act, void* stream) {
     driver();
     View3 x = view3(x_t, "x"), w = view3(w_t, "w");
@@ -1345,6 +1348,14 @@ void gemm_gated(const lb_tensor& x_t, const lb_tensor& w_t, const lb_tensor& h, 
     up.ptr = (uint16_t*)w.ptr + w.rows * w.sr;
     bool x_cols, w_rows;
     tensor_core_operands(x, turned(w), x_cols, w_rows);
+    if (const int ranges = w_rows ? 0 : gemm_gated_ranges(x_t, w_t)) {
+        SmallGemmArgs q{};
+        q.M = (int)x.rows, q.N = (int)w.rows, q.K = (int)x.cols, q.a_mn_major = !x_cols, q.in_bf16 = q.d_bf16 = x.dtype == LB_BF16, q.d_f16 = x.dtype == LB_F16;
+        q.d = h.ptr, q.ldd = h.stride[0], q.status = status_word(), q.splits = ranges;
+        gemm_small_gated(q.a_mn_major ? make_map(x, false, 64, BK) : make_map(x, true, BK, BM), make_map(w, true, BK, 32), make_map(up, true, BK, 32), q, act,
+                         kept ? kept->ptr : nullptr, kept ? kept->stride[0] : 0, device_info().sms, (cudaStream_t)stream);
+        return;
+    }
     GatedArgs p{};
     long long tiles;
     pair_args(p, x, w, x_cols, !w_rows, BN / 2, tiles);

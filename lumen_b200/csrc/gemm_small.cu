@@ -15,6 +15,7 @@
 // 128 x 8192 K 1024 8.5 -> 6.3, 1024^3 8.5 -> 6.2; with ranges 704 x 1024 K 4096 16.8 -> 14.6, 200 x 1024 K 4096 9.1 -> 8.5.
 #include <cuda_fp16.h>
 
+#include "gate.cuh"
 #include "gemm.h"
 #include "launch.cuh"
 #include "sm100.cuh"
@@ -47,10 +48,43 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr, uint32_t rank) {
 // byte offset of 16-byte chunk `c` of row `r` of the partial tile: eight rows' equal chunks fall in different banks
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * BN * 4 + ((c ^ (r & 7)) << 4)); }
 
+// What the kernel does with a tile: lb_gemm's epilogues, or the gated feed-forward block's, whose tile is 32 columns of both projections: rows of two weights
+// one after the other in B's place, and in the partial tile their columns.
+struct SmallPlain : SmallGemmArgs {
+    static constexpr bool gated = false;
+};
+struct alignas(64) SmallGated : SmallGemmArgs {
+    static constexpr bool gated = true;
+    CUtensorMap map_up;  // the other weight; N, d, ldd: the gated product's
+    int act;
+    void* kept;  // both projections side by side; null: not kept
+    long long ld_kept;
+};
+__device__ __forceinline__ uint32_t round_pair(Pair x, bool bf16) {
+    const float2 v = apart(x);
+    if (bf16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(v.x, v.y);
+        return *(const uint32_t*)&t;
+    }
+    const __half2 t = __floats2half2_rn(v.x, v.y);
+    return *(const uint32_t*)&t;
+}
+__device__ __forceinline__ uint4 round_eight(const float* x, bool bf16) {
+    return make_uint4(round_pair(both(x[0], x[1]), bf16), round_pair(both(x[2], x[3]), bf16), round_pair(both(x[4], x[5]), bf16), round_pair(both(x[6], x[7]), bf16));
+}
+template <int ACT>
+__device__ __forceinline__ void gate_eight(float* a, const float* b) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const float2 h = apart(activation<ACT>(both(a[j], a[j + 1])) * both(b[j], b[j + 1]));
+        a[j] = h.x, a[j + 1] = h.y;
+    }
+}
+
 // RANKS: a tile's K range is cut over a cluster
-template <int STAGES, bool RANKS>
+template <int STAGES, bool RANKS, class Args>
 __global__ void __launch_bounds__(kThreads, 8 / STAGES)
-gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const SmallGemmArgs p) {
+gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Args p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
     uint8_t *sa = smem, *sb = smem + STAGES * kStageA;
@@ -103,7 +137,10 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 } else {
                     for (int j = 0; j < BM / 64; j++) tma_load_3d(sa + st * kStageA + j * (64 * BK * 2), &map_a, &full[st], m_blk * BM + j * 64, k, b);
                 }
-                if (!p.b_mn_major) tma_load_3d(sb + st * kStageB, &map_b, &full[st], k, n_blk * BN, b);  // box {64 k, 64 n}
+                if constexpr (Args::gated) {  // boxes {64 k, 32 n}
+                    tma_load_3d(sb + st * kStageB, &map_b, &full[st], k, n_blk * (BN / 2), b);
+                    tma_load_3d(sb + st * kStageB + kStageB / 2, &p.map_up, &full[st], k, n_blk * (BN / 2), b);
+                } else if (!p.b_mn_major) tma_load_3d(sb + st * kStageB, &map_b, &full[st], k, n_blk * BN, b);  // box {64 k, 64 n}
                 else tma_load_3d(sb + st * kStageB, &map_b, &full[st], n_blk * BN, k, b);                 // box {64 n, 64 k}
             }
             if (ok) mbar_wait_ring<STAGES>(empty, (uint32_t)num_kb, abort_flag);
@@ -154,29 +191,13 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     // this CTA's share of the rows: eight columns per thread
     const int rows = BM / splits;
     const bool good = !*abort_flag;
-    for (int i = threadIdx.x; i < rows * (BN / 8); i += kThreads) {
-        const int r = rank * rows + i / (BN / 8), q = i % (BN / 8);
-        const long long row = (long long)m_blk * BM + r;
-        const int col = n_blk * BN + q * 8;
-        const int live = good && row < p.M ? min(8, p.N - col) : 0;
-        if (live <= 0) continue;
-        const bool whole = p.vec && live == 8;
-        uint32_t a[4] = {0u, 0u, 0u, 0u};  // the epilogue's operand is on its way while the ranks' sums are
-        if (p.epilogue >= EPI_ADD && live > 0) {
-            const uint16_t* aux = (const uint16_t*)p.aux + (long long)b * p.aux_batch_stride + row * p.ld_aux + col;
-            if (p.aux_vec && live == 8) {
-                const uint4 t = *(const uint4*)aux;
-                a[0] = t.x, a[1] = t.y, a[2] = t.z, a[3] = t.w;
-            } else {
+    // Eight columns of row `local` of them, row r of the tile: the ranks' sums.
+    auto total = [&](int local, int r, int q, float* x) {
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (j < live) a[j / 2] |= (uint32_t)aux[j] << (j % 2 * 16);
-            }
-        }
+        for (int j = 0; j < 8; j++) x[j] = 0.0f;
         const uint32_t at0 = smem_u32(smem) + chunk_at(r, 2 * q), at1 = smem_u32(smem) + chunk_at(r, 2 * q + 1);
-        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (PUSH) {
-            const uint32_t at = chunk_at(i / (BN / 8), 2 * q), beside = at ^ 16;
+            const uint32_t at = chunk_at(local, 2 * q), beside = at ^ 16;
             for (int s = 0; s < splits; s++) {
                 const uint32_t from = s == rank ? smem_u32(smem) + rank * rows * (BN * 4) : smem_u32(landing) + (s < rank ? s : s - 1) * rows * (BN * 4);
                 const uint4 u = ld_shared(from + at), w = ld_shared(from + beside);
@@ -201,6 +222,45 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
             x[4] = __uint_as_float(w.x), x[5] = __uint_as_float(w.y), x[6] = __uint_as_float(w.z), x[7] = __uint_as_float(w.w);
         }
+    };
+    if constexpr (Args::gated) {
+        for (int i = threadIdx.x; i < rows * (BN / 16); i += kThreads) {
+            const int r = rank * rows + i / (BN / 16), q = i % (BN / 16), col = n_blk * (BN / 2) + q * 8;
+            const long long row = (long long)m_blk * BM + r;
+            if (!good || row >= p.M || col >= p.N) continue;  // (N is a multiple of eight, rows are 16-byte aligned)
+            float x[8], y[8];
+            total(i / (BN / 16), r, q, x), total(i / (BN / 16), r, q + BN / 16, y);
+            if (p.kept) {
+                uint16_t* kept = (uint16_t*)p.kept + row * p.ld_kept + col;
+                *(uint4*)kept = round_eight(x, p.d_bf16), *(uint4*)(kept + p.N) = round_eight(y, p.d_bf16);
+            }
+            if (p.act == ACT_SILU) gate_eight<ACT_SILU>(x, y);
+            else if (p.act == ACT_GELU) gate_eight<ACT_GELU>(x, y);
+            else gate_eight<ACT_RELU>(x, y);
+            *(uint4*)((uint16_t*)p.d + row * p.ldd + col) = round_eight(x, p.d_bf16);
+        }
+    }
+    for (int i = threadIdx.x; !Args::gated && i < rows * (BN / 8); i += kThreads) {
+        const int r = rank * rows + i / (BN / 8), q = i % (BN / 8);
+        const long long row = (long long)m_blk * BM + r;
+        const int col = n_blk * BN + q * 8;
+        const int live = good && row < p.M ? min(8, p.N - col) : 0;
+        if (live <= 0) continue;
+        const bool whole = p.vec && live == 8;
+        uint32_t a[4] = {0u, 0u, 0u, 0u};  // the epilogue's operand is on its way while the ranks' sums are
+        if (p.epilogue >= EPI_ADD && live > 0) {
+            const uint16_t* aux = (const uint16_t*)p.aux + (long long)b * p.aux_batch_stride + row * p.ld_aux + col;
+            if (p.aux_vec && live == 8) {
+                const uint4 t = *(const uint4*)aux;
+                a[0] = t.x, a[1] = t.y, a[2] = t.z, a[3] = t.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (j < live) a[j / 2] |= (uint32_t)aux[j] << (j % 2 * 16);
+            }
+        }
+        float x[8];
+        total(i / (BN / 8), r, q, x);
         if (p.epilogue == EPI_RELU) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = fmaxf(x[j], 0.0f);
@@ -266,22 +326,36 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 }  // namespace
 
-template <int STAGES, bool RANKS>
-static void launch_small(const CUtensorMap& map_a, const CUtensorMap& map_b, const SmallGemmArgs& p, int batch, cudaStream_t s) {
-    if (first_use_on_device((const void*)gemm_small_kernel<STAGES, RANKS>))
-        LB_CUDA(cudaFuncSetAttribute(gemm_small_kernel<STAGES, RANKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(STAGES, RANKS)));
-    launch_overlapped(gemm_small_kernel<STAGES, RANKS>, dim3((unsigned)((long long)p.tiles_m * p.tiles_n * batch * p.splits)), dim3(kThreads), smem_bytes(STAGES, RANKS), s,
+template <int STAGES, bool RANKS, class Args>
+static void launch_small(const CUtensorMap& map_a, const CUtensorMap& map_b, const Args& p, int batch, cudaStream_t s) {
+    if (first_use_on_device((const void*)gemm_small_kernel<STAGES, RANKS, Args>))
+        LB_CUDA(cudaFuncSetAttribute(gemm_small_kernel<STAGES, RANKS, Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(STAGES, RANKS)));
+    launch_overlapped(gemm_small_kernel<STAGES, RANKS, Args>, dim3((unsigned)((long long)p.tiles_m * p.tiles_n * batch * p.splits)), dim3(kThreads), smem_bytes(STAGES, RANKS), s,
                       (unsigned)p.splits, map_a, map_b, p);
 }
+template <class Args>
+static void launch_small(const CUtensorMap& map_a, const CUtensorMap& map_b, const Args& p, int batch, int sms, cudaStream_t s) {
+    if ((long long)p.tiles_m * p.tiles_n * batch * p.splits > sms) launch_small<4, true>(map_a, map_b, p, batch, s);
+    else if (p.splits > 1) launch_small<8, true>(map_a, map_b, p, batch, s);
+    else launch_small<8, false>(map_a, map_b, p, batch, s);
+}
 
-void gemm_small(const CUtensorMap& map_a, const CUtensorMap& map_b, SmallGemmArgs p, int batch, int sms, cudaStream_t s) {
+void gemm_small(const CUtensorMap& map_a, const CUtensorMap& map_b, SmallGemmArgs q, int batch, int sms, cudaStream_t s) {
+    SmallPlain p{};
+    (SmallGemmArgs&)p = q;
     p.tiles_m = (p.M + BM - 1) / BM, p.tiles_n = (p.N + BN - 1) / BN;
     const int per_line = p.d_bf16 || p.d_f16 ? 8 : 4;
     p.aux_vec = (uintptr_t)p.aux % 16 == 0 && p.ld_aux % 8 == 0 && p.aux_batch_stride % 8 == 0;
     p.vec = (uintptr_t)p.d % 16 == 0 && p.ldd % per_line == 0 && p.d_batch_stride % per_line == 0;
-    if ((long long)p.tiles_m * p.tiles_n * batch * p.splits > sms) launch_small<4, true>(map_a, map_b, p, batch, s);
-    else if (p.splits > 1) launch_small<8, true>(map_a, map_b, p, batch, s);
-    else launch_small<8, false>(map_a, map_b, p, batch, s);
+    launch_small(map_a, map_b, p, batch, sms, s);
+}
+void gemm_small_gated(const CUtensorMap& map_a, const CUtensorMap& map_gate, const CUtensorMap& map_up, SmallGemmArgs q, int act, void* kept, long long ld_kept, int sms,
+                      cudaStream_t s) {
+    SmallGated p{};
+    (SmallGemmArgs&)p = q;
+    p.tiles_m = (p.M + BM - 1) / BM, p.tiles_n = (p.N + BN / 2 - 1) / (BN / 2);
+    p.map_up = map_up, p.act = act, p.kept = kept, p.ld_kept = ld_kept;
+    launch_small(map_a, map_gate, p, 1, sms, s);
 }
 
 }  // namespace lb
