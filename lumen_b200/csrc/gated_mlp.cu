@@ -148,8 +148,8 @@ void sized(const lb_tensor& t, long long rows, long long cols, int dtype, const 
     if (rows && cols && (uintptr_t)t.ptr % dtype_size(dtype)) refuse(format("%s is not aligned to its elements", what));
 }
 
-// Whether the products with the gate in their epilogue are taken, where the layouts are theirs: where enough SMs get a tile (of 128 rows by 128 columns of
-// h, backward by 256), since lb_gemm's own choices cut K and take narrower tiles. us of a pass in a graph, products apart -> these, bfloat16, width x hidden:
+// Whether the pairs' products with the gate in their epilogue are taken, where the layouts are theirs and (forward) narrow tiles are too many: where enough SMs
+// get a tile (of 128 rows by 128 columns of h, backward by 256), since lb_gemm's own choices cut K and take narrower tiles. us of a pass in a graph, products apart -> these, bfloat16, width x hidden:
 // forward 200 tokens 512 x 2048 (32 tiles) 17.6 -> 20.3, 128 of 1024 x 4096 (32) 20.6 -> 24.4, 384 of 512 x 2048 (48) 17.4 -> 16.0, 200 of 1024 x 4096 (64)
 // 21.4 -> 20.1, 128 of 2048 x 8192 (64) 36.1 -> 31.5, 1024 of 1024 x 4096 41.7 -> 34.4; backward 200 of 1024 x 4096 (32) 35.1 -> 39.3, 384 (48) 46.5 -> 47.1,
 // 512 (64) 51.5 -> 50.8, 1024 of 512 x 2048 (64) 39.4 -> 38.9, 200 of 2048 x 8192 (64) 77.9 -> 79.6, 1024 of it 177 -> 174, 16384 of 1024 x 4096 837 -> 761.

@@ -49,7 +49,8 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * BN * 4 + ((c ^ (r & 7)) << 4)); }
 
 // What the kernel does with a tile: lb_gemm's epilogues, or the gated feed-forward block's, whose tile is 32 columns of both projections: rows of two weights
-// one after the other in B's place, and in the partial tile their columns.
+// one after the other in B's place, and in the partial tile their columns. us of a whole block in a graph, bfloat16, lb_gemm into float32 and an element-wise
+// kernel -> this: 64 tokens of 1024 x 4096 20.1 -> 18.3, of 512 x 2048 13.0 -> 11.9, 384 of 512 x 1024 12.2 -> 10.4, 200 of 512 x 2048 17.6 -> 15.7.
 struct SmallPlain : SmallGemmArgs {
     static constexpr bool gated = false;
 };
