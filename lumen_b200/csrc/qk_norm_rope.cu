@@ -13,8 +13,8 @@
 // Bound by memory with many rows, and before that by instructions: the arithmetic is packed, and what a row costs beside it (addresses, its sums' shuffles,
 // the root) is shared by as many elements a thread as registers hold. us of the backward of 32768 tokens x 40 heads x 128, bfloat16, 1.0 GB: a warp a
 // row, by the element 2227; rows in registers, eight elements a thread 304; the next rows on their way into shared memory 258; packed arithmetic and a hardware
-// root 217; sixteen elements a thread 191 (167 in a graph, 6.03 TB/s of 6.53; under the power cap 194). Forward in a graph 111 us, 6.07 TB/s; 3062 x 40 x 128
-// forward 15 us, 4.2 TB/s; 4 tokens x 32 heads x 64 3 us.
+// root 217; sixteen elements a thread 191 (165 in a graph, 6.09 TB/s of 6.53; under the power cap 194). Forward in a graph 109 us, 6.16 TB/s; 3062 x 40 x 128
+// forward 13.6 us, 4.6 TB/s (weights read behind the first rows, in vectors: before that 14.9); 512 tokens x 40 x 128 4.9 us.
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -41,6 +41,7 @@ struct RopeSide {
     int heads, blocks;
     Divisor by_chunks;  // of a token's heads
     int w_f32;       // w and dw are float32, whatever the rows' type
+    int w_vec;       // w is 16-byte aligned
 };
 struct RopeArgs {
     RopeSide side[2];
@@ -236,15 +237,35 @@ struct Lane {
     bool live, turns;
     Pair w[N], sum[BWD ? N : 1];
 
-    __device__ __forceinline__ Lane(const RopeArgs& p, const RopeSide& q) {
+    __device__ __forceinline__ explicit Lane(const RopeArgs& p) {
         c = threadIdx.x & (p.lanes - 1), live = c * 2 * N < p.H, turns = c < p.R / (2 * N);
         const bool beside = p.interleaved || !turns;
         e0 = beside ? 2 * N * c : N * c, e1 = beside ? e0 + N : p.R / 2 + N * c;
+        if (BWD) {
+#pragma unroll
+            for (int j = 0; j < N; j++) sum[j] = both(0.0f, 0.0f);
+        }
+    }
+    __device__ __forceinline__ void weights(const RopeSide& q) {
+        if (q.w && q.w_vec && live) {
+            if (q.w_f32) {
+#pragma unroll
+                for (int j = 0; j < N / 4; j++) {
+                    Four<float> lo, hi;
+                    lo.load((const float*)q.w + e0 + 4 * j), hi.load((const float*)q.w + e1 + 4 * j);
+                    lo.widen(w + 2 * j), hi.widen(w + N / 2 + 2 * j);
+                }
+            } else {
+                Run<T, N> lo, hi;
+                lo.load((const T*)q.w + e0), hi.load((const T*)q.w + e1);
+                lo.widen(w), hi.widen(w + N / 2);
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const int i = j < N / 2 ? e0 + 2 * j : e1 + 2 * j - N;
             w[j] = live ? both(weight<T>(q, i), weight<T>(q, i + 1)) : both(0.0f, 0.0f);
-            if (BWD) sum[j] = both(0.0f, 0.0f);
         }
     }
     // One row, executed by the whole warp: x and, backward, y = dy go in, y = the result comes out. Zeros go in where a lane has no part of its row;
@@ -311,7 +332,8 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_few_kernel(const RopeAr
     const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
     const RopeSide& q = p.side[side];
     const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
-    Lane<T, BWD, 4> lane(p, q);
+    Lane<T, BWD, 4> lane(p);
+    lane.weights(q);
     const float per = 1.0f / (float)p.H;
     const long long rows = (long long)p.batch * p.seq * q.heads;
     for (long long base = (long long)block * groups; base < rows; base += (long long)q.blocks * groups) {
@@ -372,7 +394,7 @@ __global__ void __launch_bounds__(kGroupThreads, many_per_sm<N>()) rope_many_ker
     const int side = blockIdx.x < p.side[0].blocks ? 0 : 1;
     const RopeSide& q = p.side[side];
     const int block = side ? blockIdx.x - p.side[0].blocks : blockIdx.x, groups = kGroupThreads / p.lanes;
-    Lane<T, BWD, N> lane(p, q);
+    Lane<T, BWD, N> lane(p);
     const float per = 1.0f / (float)p.H;
     const unsigned chunks = q.by_chunks.d, tasks = (unsigned)(p.batch * p.seq) * chunks, step = (unsigned)(q.blocks * groups);
     unsigned task = (unsigned)(block * groups + threadIdx.x / p.lanes);
@@ -419,6 +441,7 @@ __global__ void __launch_bounds__(kGroupThreads, many_per_sm<N>()) rope_many_ker
     if (task < tasks) next = place(task), fetch(next, 0), angles(position(task));
     if (task < tasks && tasks - task > step) after = position(task + step);
     asm volatile("cp.async.commit_group;" ::: "memory");
+    lane.weights(q);  // (behind the first rows, which are longer on their way)
     for (unsigned round = 0; round < rounds; round++, task += step) {
         const bool there = task < tasks && lane.live;
         here = next;
@@ -452,7 +475,7 @@ __global__ void __launch_bounds__(kGroupThreads, many_per_sm<N>()) rope_many_ker
     }
 }
 
-// dw: the blocks' sums, 32 columns a block, 32 of its rows beside one another, four loads of each in flight.
+// dw: the blocks' sums, 32 columns a block, 32 of its rows beside one another, sixteen loads of a thread in flight.
 template <class T>
 __global__ void __launch_bounds__(1024) rope_weights_kernel(const RopeArgs p) {
     __shared__ float held[32][33];
@@ -462,8 +485,13 @@ __global__ void __launch_bounds__(1024) rope_weights_kernel(const RopeArgs p) {
     const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
     float sum = 0.0f;
     if (i < p.H) {
-#pragma unroll 4
-        for (int k = part; k < q.blocks; k += 32) sum += q.partial[(long long)k * p.H + i];
+        for (int k0 = part; k0 < q.blocks; k0 += 32 * 16) {
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] = k0 + 32 * k < q.blocks ? q.partial[(long long)(k0 + 32 * k) * p.H + i] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 16; k++) sum += v[k];
+        }
     }
     held[part][lane] = sum;
     __syncthreads();
@@ -499,7 +527,7 @@ void weights(RopeSide& side, const lb_tensor* w, int H, int dtype, const char* w
     if (!w) return;
     if (w->rank != 1 || w->shape[0] != H || (w->dtype != dtype && w->dtype != LB_F32)) refuse(format("%s must be [%d] of the rows' dtype or float32", what, H));
     if (H > 1 && w->stride[0] != 1) refuse(format("%s must be dense", what));
-    side.w = w->ptr, side.w_f32 = w->dtype == LB_F32;
+    side.w = w->ptr, side.w_f32 = w->dtype == LB_F32, side.w_vec = (uintptr_t)w->ptr % 16 == 0;
 }
 
 // Both sides' blocks, in proportion to their rows: at most what fills the GPU once, at least one where a side has rows.
@@ -603,7 +631,7 @@ void launch_rope(RopeCall& c, cudaStream_t stream) {
         while (p.lanes * 8 < p.H) p.lanes *= 2;
         const int groups = kGroupThreads / p.lanes;
         // below four rows a group of the kernel for few, a second and third round of which cost less than the other kernel's start (512 tokens x 40
-        // heads x 128, forward: 20480 rows 5.6 us; 1024 tokens on the other 7.3)
+        // heads x 128, forward: 20480 rows 4.9 us; 1024 tokens on the other 5.8)
         if (c.rows < (long long)sms * 3 * groups * 4) {
             share_blocks(p, groups, 1, sms, 3);
             launch_overlapped(rope_few_kernel<T, BWD>, blocks(), dim3(kGroupThreads), 0, stream, 0, p);
