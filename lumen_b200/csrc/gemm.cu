@@ -72,7 +72,7 @@ struct alignas(64) GatedArgs : GemmArgs {
 };
 struct alignas(64) SlopedArgs : GemmArgs {
     static constexpr int mode = PAIR_SLOPED;
-    CUtensorMap map_gate, map_up, map_d_gate, map_d_up;  // both projections as kept, and their gradients: 32 x 32 pieces
+    CUtensorMap map_gate, map_up, map_d_gate, map_d_up;  // both projections as kept, and their gradients: pieces of 32 rows of 64
     int act;
 };
 
@@ -337,20 +337,20 @@ __device__ __forceinline__ void drain_gated(const GatedArgs& p, uint32_t tbase, 
     }
 }
 
-// The backward's way out. A warp's rows of a tile leave 32 columns at a time: both projections' pieces of 32 x 32 arrive by TMA in one of three places,
-// each lane turns its row of them and of dh into their gradients where they lie, and TMA takes those away; two pieces ahead are on their way
-// meanwhile, the next tile's among them. Rows and columns outside the matrices arrive as zeros and do not leave.
+// The backward's way out. 32 rows of a tile leave 64 columns at a time, by two warps: both projections' pieces of 32 x 64 arrive by TMA in one of three
+// places, each lane turns its half of a row of them and of dh into their gradients where they lie, and TMA takes those away; two pieces ahead
+// are on their way meanwhile, the next tile's among them. Rows and columns outside the matrices arrive as zeros and do not leave.
 //
-// Bound by what passes between an SM and the L2: a tile's operands, 512 KB a CTA at K = 1024, and 128 KB either way for the pieces (without the stores it takes
-// 119 us, without the arithmetic no less, and the plain product of these sizes, which stores a quarter of that, 95): 16384 x 4096 x 1024 through registers and
-// the staging area 165 us, so 148.
-constexpr int kPieceBytes = 4096, kPieces = 3;  // a warp's: 32 rows of 64 bytes of either projection
+// Bound by TMA, which takes a row of a box at a time: a tile's operands are 4096 rows of 128 bytes at K = 1024, the pieces 1024 either way. 16384 x 4096 x 1024: through
+// registers and the staging area 165 us; pieces of 64-byte rows 148 (without loads 115, without stores either 100, without arithmetic 89; three stages and a fourth
+// piece 168); of 128-byte rows 132 - 135.
+constexpr int kPieceBytes = 8192, kPieces = 3;  // two warps': 32 rows of 128 bytes of either projection
 template <int ACT, bool F16>
-__device__ __forceinline__ void slope_piece(uint32_t piece, const uint32_t* v, int lane) {
-    const uint32_t row = piece + lane * 64, turn = (lane >> 1) & 3;  // 16-byte pieces of a row as TMA's 64-byte swizzle puts them
+__device__ __forceinline__ void slope_piece(uint32_t piece, const uint32_t* v, int half, int lane) {
+    const uint32_t row = piece + lane * 128;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-        const uint32_t at = row + ((q ^ turn) << 4);
+        const uint32_t at = row + (((half * 4 + q) ^ (lane & 7)) << 4);  // 16-byte pieces of a row as TMA's 128-byte swizzle puts them
         const uint4 g = ld_shared(at), u = ld_shared(at + kPieceBytes / 2);
         const uint32_t a[4] = {g.x, g.y, g.z, g.w}, b[4] = {u.x, u.y, u.z, u.w};
         uint32_t da[4], db[4];
@@ -363,22 +363,36 @@ __device__ __forceinline__ void slope_piece(uint32_t piece, const uint32_t* v, i
         st_shared(at, make_uint4(da[0], da[1], da[2], da[3])), st_shared(at + kPieceBytes / 2, make_uint4(db[0], db[1], db[2], db[3]));
     }
 }
+// A barrier of the two warps with number `id`: whether both say yes.
+__device__ __forceinline__ bool both_warps(int id, bool yes) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "bar.red.and.pred p, %1, 64, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"(id), "r"((uint32_t)yes)
+        : "memory");
+    return all != 0;
+}
+// `pieces`, `landed`: those of the warp's quarter of the rows; `half`: which of its two warps. Where a wait has given up, both warps still meet at the
+// barrier of a piece before they leave.
 template <class Args>
 __device__ __forceinline__ void sloped_way_out(const Args& p, uint8_t* pieces, uint64_t* landed, uint64_t* tmem_full, uint64_t* tmem_empty, uint32_t tmem_base, int pair,
-                                               int num_pairs, int num_units, int rank, int quarter, int col_half, int lane, volatile int* abort_flag) {
+                                               int num_pairs, int num_units, int rank, int quarter, int half, int lane, volatile int* abort_flag) {
     auto first_row = [&](int m_blk) { return m_blk * 2 * BM + rank * BM + quarter * 32; };
-    auto first_col = [&](int n_blk) { return n_blk * BN + col_half * (BN / 2); };
-    auto pieces_of = [&](int row, int col) { return row < p.M ? max(0, min(BN / 2 / 32, (p.N - col + 31) / 32)) : 0; };
+    auto pieces_of = [&](int row, int col) { return row < p.M ? min(BN / 64, (p.N - col + 63) / 64) : 0; };
     // the pieces to come: where the next one to be fetched lies
     int load_unit = pair - num_pairs, load_row = 0, load_col = 0, load_left = 0;
     uint32_t loaded = 0;
-    auto fetch = [&] {
+    auto fetch = [&] {  // the first warp
         while (load_left == 0) {
             load_unit += num_pairs;
             if (load_unit >= num_units) return;
             int b, m_blk, n_blk;
             tile_coords(p, load_unit, b, m_blk, n_blk);
-            load_row = first_row(m_blk), load_col = first_col(n_blk), load_left = pieces_of(load_row, load_col);
+            load_row = first_row(m_blk), load_col = n_blk * BN, load_left = pieces_of(load_row, load_col);
         }
         if (lane == 0) {
             uint64_t* bar = landed + loaded % kPieces;
@@ -387,20 +401,20 @@ __device__ __forceinline__ void sloped_way_out(const Args& p, uint8_t* pieces, u
             tma_load_3d(to, &p.map_gate, bar, load_col, load_row, 0);
             tma_load_3d(to + kPieceBytes / 2, &p.map_up, bar, load_col, load_row, 0);
         }
-        loaded++, load_left--, load_col += 32;
+        loaded++, load_left--, load_col += 64;
     };
-    fetch(), fetch();
+    if (half == 0) fetch(), fetch();
     uint32_t done = 0;
     int local = 0;
-    bool ok = true;
-    for (int unit = pair; unit < num_units && ok; unit += num_pairs, local++) {
+    bool ok = true, on = true;
+    for (int unit = pair; unit < num_units && on; unit += num_pairs, local++) {
         const int buf = local & 1;
         int b, m_blk, n_blk;
         tile_coords(p, unit, b, m_blk, n_blk);
-        const int row = first_row(m_blk), col = first_col(n_blk), count = pieces_of(row, col);
-        if (!(ok = mbar_wait_warp(&tmem_full[buf], (uint32_t)(local >> 1) & 1, abort_flag))) break;
+        const int row = first_row(m_blk), col = n_blk * BN, count = pieces_of(row, col);
+        if (!mbar_wait_warp(&tmem_full[buf], (uint32_t)(local >> 1) & 1, abort_flag)) ok = false;
         tc_fence_after();
-        const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+        const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + half * 32);
         auto release = [&] {
             tc_fence_before();
             __syncwarp();
@@ -408,33 +422,37 @@ __device__ __forceinline__ void sloped_way_out(const Args& p, uint8_t* pieces, u
         };
         if (count == 0) release();
 #pragma unroll 1
-        for (int c = 0; c < count && ok; c++, done++) {
+        for (int c = 0; c < count && on; c++, done++) {
             uint32_t v[32];
-            tmem_ld_32x32(tbase + c * 32, v);
-            ok = mbar_wait_warp(&landed[done % kPieces], done / kPieces & 1, abort_flag);
+            tmem_ld_32x32(tbase + c * 64, v);
+            if (!mbar_wait_warp(&landed[done % kPieces], done / kPieces & 1, abort_flag)) ok = false;
             tmem_ld_wait();
             if (c == count - 1) release();
-            if (!ok) break;
             uint8_t* piece = pieces + done % kPieces * kPieceBytes;
             const uint32_t at = smem_u32(piece);
-            if (!p.d_f16 && p.act == ACT_SILU) slope_piece<ACT_SILU, false>(at, v, lane);
-            else if (!p.d_f16 && p.act == ACT_GELU) slope_piece<ACT_GELU, false>(at, v, lane);
-            else if (!p.d_f16) slope_piece<ACT_RELU, false>(at, v, lane);
-            else if (p.act == ACT_SILU) slope_piece<ACT_SILU, true>(at, v, lane);
-            else if (p.act == ACT_GELU) slope_piece<ACT_GELU, true>(at, v, lane);
-            else slope_piece<ACT_RELU, true>(at, v, lane);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) bulk_wait_read();  // the piece before this one has left: its place is the one fetched into next
-            fetch();
-            if (lane == 0) {
-                tma_store_3d(&p.map_d_gate, piece, col + c * 32, row, 0);
-                tma_store_3d(&p.map_d_up, piece + kPieceBytes / 2, col + c * 32, row, 0);
-                bulk_commit();
+            if (ok) {
+                if (!p.d_f16 && p.act == ACT_SILU) slope_piece<ACT_SILU, false>(at, v, half, lane);
+                else if (!p.d_f16 && p.act == ACT_GELU) slope_piece<ACT_GELU, false>(at, v, half, lane);
+                else if (!p.d_f16) slope_piece<ACT_RELU, false>(at, v, half, lane);
+                else if (p.act == ACT_SILU) slope_piece<ACT_SILU, true>(at, v, half, lane);
+                else if (p.act == ACT_GELU) slope_piece<ACT_GELU, true>(at, v, half, lane);
+                else slope_piece<ACT_RELU, true>(at, v, half, lane);
+                fence_proxy_async();
+            }
+            on = both_warps(1 + quarter, ok);
+            if (half == 0 && on) {
+                if (lane == 0) bulk_wait_read();  // the piece before this one has left: its place is the one fetched into next
+                fetch();
+                if (lane == 0) {
+                    tma_store_3d(&p.map_d_gate, piece, col + c * 64, row, 0);
+                    tma_store_3d(&p.map_d_up, piece + kPieceBytes / 2, col + c * 64, row, 0);
+                    bulk_commit();
+                }
+                __syncwarp();
             }
         }
     }
-    if (lane == 0) bulk_wait();
+    if (half == 0 && lane == 0) bulk_wait();
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -633,7 +651,7 @@ constexpr int kPairSmemBytes = PSTAGES * (kPairStageBytesA + kPairStageBytesB) +
 // The gated block's backward product has a larger way out and four stages beside it.
 constexpr int pair_stages(int mode) { return mode == PAIR_SLOPED ? 4 : PSTAGES; }
 constexpr int pair_smem(int mode) {
-    return mode == PAIR_SLOPED ? 4 * (kPairStageBytesA + kPairStageBytesB) + kEpilogueWarps * kPieces * kPieceBytes + 1024 + 512 : kPairSmemBytes;
+    return mode == PAIR_SLOPED ? 4 * (kPairStageBytesA + kPairStageBytesB) + 4 * kPieces * kPieceBytes + 1024 + 512 : kPairSmemBytes;
 }
 static_assert(pair_smem(PAIR_SLOPED) <= 227 * 1024, "shared memory");
 
@@ -645,13 +663,13 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     uint8_t* smem = align_1024(smem_raw);
     uint8_t* smem_a = smem;
     uint8_t* smem_b = smem + STAGES_ * kPairStageBytesA;
-    uint64_t* full = (uint64_t*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + (Args::mode == PAIR_SLOPED ? kEpilogueWarps * kPieces * kPieceBytes : 0));
+    uint64_t* full = (uint64_t*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + (Args::mode == PAIR_SLOPED ? 4 * kPieces * kPieceBytes : 0));
     uint64_t* empty = full + STAGES_;
     uint64_t* tmem_full = empty + STAGES_;
     uint64_t* tmem_empty = tmem_full + 2;
     uint32_t* tmem_base_slot = (uint32_t*)(tmem_empty + 2);
     volatile int* abort_flag = (volatile int*)(tmem_base_slot + 1);
-    [[maybe_unused]] uint64_t* landed = (uint64_t*)(tmem_base_slot + 2);  // pieces of the backward's way out, each warp's
+    [[maybe_unused]] uint64_t* landed = (uint64_t*)(tmem_base_slot + 2);  // pieces of the backward's way out, each quarter's
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp-uniform for the compiler too
     const uint32_t rank = cluster_ctarank();
@@ -670,7 +688,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             mbar_init(&tmem_empty[s], 2 * kEpilogueWarps);  // used in the leader only: every epilogue warp of the pair
         }
         if constexpr (Args::mode == PAIR_SLOPED)
-            for (int s = 0; s < kEpilogueWarps * kPieces; s++) mbar_init(&landed[s], 1);
+            for (int s = 0; s < 4 * kPieces; s++) mbar_init(&landed[s], 1);
         *abort_flag = 0;
         fence_barrier_init();
         if constexpr (Args::mode != PAIR_GROUP) tma_prefetch_desc(&map_a), tma_prefetch_desc(&map_b);
@@ -779,7 +797,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
     } else if constexpr (Args::mode == PAIR_SLOPED) {
         uint8_t* pieces = smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB);
-        sloped_way_out(p, pieces + (warp - 2) * kPieces * kPieceBytes, landed + (warp - 2) * kPieces, tmem_full, tmem_empty, tmem_base, pair, num_pairs, num_units, (int)rank,
+        sloped_way_out(p, pieces + (warp & 3) * kPieces * kPieceBytes, landed + (warp & 3) * kPieces, tmem_full, tmem_empty, tmem_base, pair, num_pairs, num_units, (int)rank,
                        warp & 3, (warp - 2) >> 2, lane, abort_flag);
     } else {
         // ---- epilogue: warps 2..9 of both CTAs, each CTA on its own 128 rows ----
@@ -933,7 +951,7 @@ View3 view3(const lb_tensor& t, const char* what) {
     return v;
 }
 
-CUtensorMap make_map(const View3& v, bool contiguous_is_cols, int box_inner, int box_outer, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+CUtensorMap make_map(const View3& v, bool contiguous_is_cols, int box_inner, int box_outer) {
     // dims innermost first: {contiguous, strided, batch}
     long long inner = contiguous_is_cols ? v.cols : v.rows, outer = contiguous_is_cols ? v.rows : v.cols;
     long long outer_stride = contiguous_is_cols ? v.sr : v.sc;
@@ -945,7 +963,7 @@ CUtensorMap make_map(const View3& v, bool contiguous_is_cols, int box_inner, int
     CUtensorMap map;
     check_cu(driver().cuTensorMapEncodeTiled(&map, v.dtype == LB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                                              3, v.ptr, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
              "cuTensorMapEncodeTiled");
     return map;
@@ -1381,7 +1399,7 @@ void gemm_sloped(const lb_tensor& dy_t, const lb_tensor& w_t, const lb_tensor& k
     p.act = act;
     auto half = [&](const lb_tensor& t, int k) {
         const View3 v{(uint16_t*)t.ptr + (long long)k * p.N, t.dtype, 1, p.M, p.N, 0, t.stride[0], 1};
-        return make_map(v, true, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+        return make_map(v, true, 64, 32);
     };
     p.map_gate = half(kept, 0), p.map_up = half(kept, 1), p.map_d_gate = half(d, 0), p.map_d_up = half(d, 1);
     launch_pairs(p.a_mn_major ? make_map(dy, false, 64, BK) : make_map(dy, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p,
