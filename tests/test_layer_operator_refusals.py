@@ -188,12 +188,22 @@ def test_gated_block_in_order():
     ({"residual": Array((10, 96), "bfloat16")}, "residual must be"),
     ({"residual": Array((10, 64), "bfloat16", strides=[1, 10])}, "residual must be row-major"),
     ({"x": Array((3, 4, 64), "bfloat16", strides=[1000, 64, 1])}, "not evenly spaced"),
-    ({"x": Array((100, 64), "bfloat16"), "y": Array((100, 64), "bfloat16"), "gate_up": Array((100, 192), "bfloat16"), "h": Array((100, 96), "bfloat16"),
-      "take": lambda nbytes: At((nbytes,), "uint8", 8)}, "16-byte aligned"),
 ])  # fmt: skip
 def test_gated_block_refusals(change, match):
     with refused(match):
         gated(**change)
+
+
+def test_gated_block_scratch():
+    """Float32 operands without what is kept: the projections need a place."""
+    t = "float32"
+    place = {"x": Array((10, 64), t), "wgu": Array((192, 64), t), "wd": Array((64, 96), t), "y": Array((10, 64), t), "gate_up": None, "h": Array((10, 96), t)}
+    with refused("bytes of scratch are needed, 16-byte aligned"):
+        gated(**place, take=lambda nbytes: At((nbytes,), "uint8", 8))
+    with refused("bytes of scratch are needed, 16-byte aligned"):
+        gated_back(take=lambda nbytes: At((nbytes,), "uint8", 8))
+    with reaches_the_gpu():
+        gated(**place)
 
 
 def test_a_residual_of_float32_is_refused():
