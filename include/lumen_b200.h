@@ -144,7 +144,7 @@ int lb_gemm(const lb_tensor* a, const lb_tensor* b, const lb_gemm_out* out, cons
  * `gate_up` [.., 2 F] = [a b] are what the backward pass reads; h is computed from the float32 sums. `residual` (nullable, 16-bit
  * dtypes) is added to the rounded product as LB_EPILOGUE_ADD does. Backward: dh = dy Wd, [da db] = [dh b f'(a), dh f(a)] rounded to the operands' dtype,
  * d_x = [da db] [Wg; Wu], d_w_gate_up = [da db]^T x, d_w_down = dy^T h, each with one float32 sum and one rounding. All tensors of a call
- * share a dtype (float16, bfloat16, float32); every call repeats bit for bit. Scratch: as many bytes as the _scratch_bytes call on the same
+ * share a dtype (float16, bfloat16, float32), and its results share no memory with one another or with its operands; every call repeats bit for bit. Scratch: as many bytes as the _scratch_bytes call on the same
  * tensors says (of their `ptr` only the alignment counts), 16-byte aligned; calls that may overlap on the GPU need scratch of their own. */
 typedef enum { LB_ACTIVATION_SILU = 0, LB_ACTIVATION_GELU_TANH = 1, LB_ACTIVATION_RELU = 2 } lb_activation;
 int lb_gated_mlp_fwd_scratch_bytes(int activation, const lb_tensor* x, const lb_tensor* w_gate_up, const lb_tensor* w_down, const lb_tensor* y,

@@ -5,6 +5,8 @@
 // backward pass in the operands' dtype; h is computed from the float32 sums, not from what was kept. [da db] is rounded to the operands'
 // dtype, as an operand of the tensor cores has to be.
 #include <algorithm>
+#include <cstdlib>
+#include <initializer_list>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -145,7 +147,28 @@ void written(const lb_tensor& t, const char* what) {
 void sized(const lb_tensor& t, long long rows, long long cols, int dtype, const char* what) {
     if (t.shape[0] != rows || t.shape[1] != cols || t.dtype != dtype)
         refuse(format("%s must be [%lld, %lld] of the operands' dtype, got %s[%lld, %lld]", what, rows, cols, dtype_name(t.dtype), (long long)t.shape[0], (long long)t.shape[1]));
-    if (rows && cols && (uintptr_t)t.ptr % dtype_size(dtype)) refuse(format("%s is not aligned to its elements", what));
+    if (rows && cols && (!t.ptr || (uintptr_t)t.ptr % dtype_size(dtype))) refuse(format("%s has no memory or is not aligned to its elements", what));
+}
+// Whether two matrices may share memory: their extents overlap, and they are not different columns of one.
+bool meet(const lb_tensor& a, const lb_tensor& b) {
+    auto bytes = [](const lb_tensor& t) {
+        return (((long long)t.shape[0] - 1) * std::abs(t.stride[0]) + (t.shape[1] - 1) * std::abs(t.stride[1]) + 1) * dtype_size(t.dtype);
+    };
+    if (a.shape[0] * a.shape[1] == 0 || b.shape[0] * b.shape[1] == 0) return false;
+    const long long x = (long long)(uintptr_t)a.ptr, y = (long long)(uintptr_t)b.ptr;
+    if (x + bytes(a) <= y || y + bytes(b) <= x) return false;
+    if (a.stride[0] != b.stride[0] || a.stride[1] != 1 || b.stride[1] != 1 || a.dtype != b.dtype || a.stride[0] <= 0) return true;
+    const long long item = dtype_size(a.dtype), row = a.stride[0] * item, apart = ((y - x) % row + row) % row;
+    return !(a.shape[1] * item <= apart && apart + b.shape[1] * item <= row);
+}
+// What is written shares no memory with what is read, or written.
+void keep_apart(std::initializer_list<const lb_tensor*> results, std::initializer_list<const lb_tensor*> operands) {
+    for (auto r = results.begin(); r != results.end(); ++r) {
+        for (const lb_tensor* o : operands)
+            if (meet(**r, *o)) refuse("a result shares memory with an operand");
+        for (auto other = r + 1; other != results.end(); ++other)
+            if (meet(**r, **other)) refuse("two results share memory");
+    }
 }
 
 // Whether the pairs' products with the gate in their epilogue are taken, where the layouts are theirs and (forward) narrow tiles are too many: where enough SMs
@@ -191,6 +214,8 @@ struct Forward : Block {
         : Block(act, x_t, wgu_t, wd_t), y(as_rows(y_t, "y")), h(as_rows(h_t, "h")), keeps(gate_up_t) {
         sized(y, M, D, dtype, "y"), written(y, "y"), sized(h, M, F, dtype, "h"), written(h, "h");
         if (keeps) gate_up = as_rows(gate_up_t, "gate_up"), sized(gate_up, M, 2 * F, dtype, "gate_up"), written(gate_up, "gate_up");
+        if (keeps) keep_apart({&y, &h, &gate_up}, {&x, &wgu, &wd});
+        else keep_apart({&y, &h}, {&x, &wgu, &wd});
         if (M == 0) return;
         few = skinny_takes(x, wgu) && skinny_takes(h, wd);
         if (few) return;
@@ -234,6 +259,7 @@ struct Backward : Block {
         if (gate_up.stride[1] != 1) fail(LB_ERR_UNSUPPORTED, "gated_mlp: gate_up must be row-major");
         sized(dx, M, D, dtype, "d_x"), written(dx, "d_x");
         sized(dwgu, 2 * F, D, dtype, "d_w_gate_up"), written(dwgu, "d_w_gate_up"), sized(dwd, D, F, dtype, "d_w_down"), written(dwd, "d_w_down");
+        keep_apart({&dx, &dwgu, &dwd}, {&dy, &x, &wgu, &wd, &gate_up, &h});
         fused = M && sloped_tiles(M, F) && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F));
         sums = fused ? 0 : up((size_t)M * F * 4), slopes = up((size_t)M * 2 * F * dtype_size(dtype));
         const lb_tensor d = slope(), a[] = {d, transposed(d), transposed(dy)}, b[] = {wgu, x, h};
@@ -289,6 +315,8 @@ int lb_gated_mlp_fwd(int activation, const lb_tensor* x, const lb_tensor* w_gate
             lb::sized(r, f.M, f.D, f.dtype, "residual");
             if (f.dtype == LB_F32) lb::fail(LB_ERR_UNSUPPORTED, "gated_mlp: a residual is added to 16-bit results");
             if (r.stride[1] != 1 && f.D > 1) lb::fail(LB_ERR_UNSUPPORTED, "gated_mlp: residual must be row-major");
+            if (f.keeps) lb::keep_apart({&f.y, &f.h, &f.gate_up}, {&r});
+            else lb::keep_apart({&f.y, &f.h}, {&r});
         }
         lb::give_scratch(f, f.bytes(), scratch, scratch_bytes);
         if (f.M) f.run(residual ? &r : nullptr, stream);

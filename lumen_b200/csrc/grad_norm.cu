@@ -277,7 +277,7 @@ long long dense_elements(const lb_tensor& t, int index) {
         if (t.shape[d] < 0) refuse(format("tensor %d has a negative size", index));
         n *= t.shape[d];
     }
-    if (n && (uintptr_t)t.ptr % dtype_size(t.dtype)) refuse(format("tensor %d is not aligned to its elements", index));
+    if (n && (!t.ptr || (uintptr_t)t.ptr % dtype_size(t.dtype))) refuse(format("tensor %d has no memory or is not aligned to its elements", index));
     if (n <= 1) return n;
     long long step = 1;
     bool used[LB_MAX_RANK] = {};
@@ -339,7 +339,7 @@ void launch_norm(const lb_tensor* xs, const lb_tensor* outs, int n, const std::v
 // `outs` null: the norm alone.
 void run_norm(const lb_tensor* xs, const lb_tensor* outs, int n, double max_norm, const lb_tensor* norm, void* scratch, size_t bytes, void* stream) {
     if (n < 0 || (n && !xs) || !norm) refuse("null argument");
-    if (norm->dtype != LB_F32 || norm->rank > LB_MAX_RANK) refuse("the norm is one float32 value");
+    if (norm->dtype != LB_F32 || norm->rank > LB_MAX_RANK || !norm->ptr || (uintptr_t)norm->ptr % 4) refuse("the norm is one float32 value");
     for (int d = 0; d < norm->rank; d++)
         if (norm->shape[d] != 1) refuse("the norm is one float32 value");
     std::vector<long long> count((size_t)n);
@@ -349,7 +349,7 @@ void run_norm(const lb_tensor* xs, const lb_tensor* outs, int n, double max_norm
         if (!outs) continue;
         bool same = outs[k].rank == xs[k].rank && outs[k].dtype == xs[k].dtype;
         for (int d = 0; same && d < xs[k].rank; d++) same = outs[k].shape[d] == xs[k].shape[d] && (outs[k].stride[d] == xs[k].stride[d] || xs[k].shape[d] == 1);
-        if (count[k] && (uintptr_t)outs[k].ptr % dtype_size(xs[k].dtype)) refuse(format("result %d is not aligned to its elements", k));
+        if (count[k] && (!outs[k].ptr || (uintptr_t)outs[k].ptr % dtype_size(xs[k].dtype))) refuse(format("result %d has no memory or is not aligned to its elements", k));
         if (!same) refuse(format("result %d must have its operand's shape, strides and dtype", k));
     }
     if (outs) {  // what is written is written once, and read by nothing else

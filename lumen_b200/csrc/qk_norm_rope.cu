@@ -507,22 +507,25 @@ __global__ void __launch_bounds__(1024) rope_weights_kernel(const RopeArgs p) {
 
 [[noreturn]] void refuse(const std::string& why) { fail(LB_ERR_INVALID, "qk_norm_rope: " + why); }
 
+long long elements(const lb_tensor& t) {
+    long long n = 1;
+    for (int d = 0; d < t.rank; d++) n *= t.shape[d];
+    return n;
+}
+void in_memory(const lb_tensor* t, const char* what) {
+    if (t && elements(*t) && (!t->ptr || (uintptr_t)t->ptr % dtype_size(t->dtype))) refuse(format("%s has no memory or is not aligned to its elements", what));
+}
 void same_shape(const lb_tensor& a, const lb_tensor& b, const char* what) {
     bool same = a.rank == b.rank && a.dtype == b.dtype;
     for (int d = 0; same && d < a.rank; d++) same = a.shape[d] == b.shape[d];
     if (!same) refuse(format("%s must have its operand's shape and dtype", what));
+    in_memory(&b, what);
 }
 // Every element of a result has a place of its own (as far as the strides of one dimension say).
 void written(const lb_tensor& t, const char* what) {
     for (int d = 0; d < t.rank; d++)
         if (t.shape[d] > 1 && t.stride[d] == 0) refuse(format("%s is written and cannot be a broadcast view", what));
 }
-long long elements(const lb_tensor& t) {
-    long long n = 1;
-    for (int d = 0; d < t.rank; d++) n *= t.shape[d];
-    return n;
-}
-
 void weights(RopeSide& side, const lb_tensor* w, int H, int dtype, const char* what) {
     if (!w) return;
     if (w->rank != 1 || w->shape[0] != H || (w->dtype != dtype && w->dtype != LB_F32)) refuse(format("%s must be [%d] of the rows' dtype or float32", what, H));
@@ -596,6 +599,8 @@ RopeCall check_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tenso
         refuse(format("the tables hold %d positions, the sequence has %d", p.table, p.seq));
     }
     if (!(desc->eps >= 0.0f)) refuse("eps must not be negative");
+    in_memory(q, "queries"), in_memory(k, "keys"), in_memory(cos, "cos"), in_memory(sin, "sin"), in_memory(positions, "positions"), in_memory(wq, "the queries' weight");
+    in_memory(wk, "the keys' weight");
     p.eps = desc->eps, p.interleaved = desc->interleaved != 0;
     const lb_tensor* x[2] = {q, k};
     for (int s = 0; s < 2; s++) {

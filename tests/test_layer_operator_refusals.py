@@ -139,20 +139,27 @@ def test_rotation_scratch():
 # ---- gated block ----------------------------------------------------------------------------------------------------
 
 
+def apart(a, change):
+    """The call's arguments with `change`, each stand-in in memory of its own unless it says where it is."""
+    a.update(change)
+    for k, t in enumerate(a.values()):
+        if type(t) is Array:
+            t.data_ptr = lambda at=(k + 1) << 24: at
+    return a.values()
+
+
 def gated(**change):
     t = "bfloat16"
     a = {"act": 0, "x": Array((10, 64), t), "wgu": Array((192, 64), t), "wd": Array((64, 96), t), "residual": None, "y": Array((10, 64), t),
          "gate_up": Array((10, 192), t), "h": Array((10, 96), t), "take": take}  # fmt: skip
-    a.update(change)
-    _lib.host().gated_mlp_fwd(*a.values(), 0)
+    _lib.host().gated_mlp_fwd(*apart(a, change), 0)
 
 
 def gated_back(**change):
     t = "bfloat16"
     a = {"act": 0, "dy": Array((10, 64), t), "x": Array((10, 64), t), "wgu": Array((192, 64), t), "wd": Array((64, 96), t), "gate_up": Array((10, 192), t),
          "h": Array((10, 96), t), "dx": Array((10, 64), t), "dwgu": Array((192, 64), t), "dwd": Array((64, 96), t), "take": take}  # fmt: skip
-    a.update(change)
-    _lib.host().gated_mlp_bwd(*a.values(), 0)
+    _lib.host().gated_mlp_bwd(*apart(a, change), 0)
 
 
 def test_gated_block_in_order():
@@ -204,6 +211,42 @@ def test_gated_block_scratch():
         gated_back(take=lambda nbytes: At((nbytes,), "uint8", 8))
     with reaches_the_gpu():
         gated(**place)
+
+
+def test_gated_block_results_in_operands_memory():
+    t = "bfloat16"
+    here = {"x": At((10, 64), t), "y": At((10, 64), t, 2 * 10 * 64)}
+    with reaches_the_gpu():  # one behind the other
+        gated(**here)
+    with reaches_the_gpu():  # columns of one matrix
+        gated(x=At((10, 64), t, strides=[128, 1]), y=At((10, 64), t, 128, strides=[128, 1]))
+    for change in ({"x": At((10, 64), t), "y": At((10, 64), t)}, {"x": At((10, 64), t), "y": At((10, 64), t, 2 * 10 * 64 - 16)},
+                   {"x": At((10, 64), t, strides=[128, 1]), "y": At((10, 64), t, 112, strides=[128, 1])}, {"wgu": At((192, 64), t), "h": At((10, 96), t, 4096)},
+                   {"residual": At((10, 64), t), "y": At((10, 64), t)}):  # fmt: skip
+        with refused("shares memory with an operand"):
+            gated(**change)
+    with refused("two results share memory"):
+        gated(h=At((10, 96), t), gate_up=At((10, 192), t, 1024))
+    with refused("shares memory with an operand"):
+        gated_back(x=At((10, 64), t), dx=At((10, 64), t))
+    with refused("two results share memory"):
+        gated_back(dwd=At((64, 96), t), dwgu=At((192, 64), t))
+
+
+def test_tensors_without_memory():
+    none, t = At((10, 64), "bfloat16", -(1 << 30)), "bfloat16"
+    with refused("x has no memory"):
+        gated(x=none)
+    with refused("queries has no memory"):
+        rope(q=At((2, 5, 4, 64), at=-(1 << 30)))
+    with refused("positions has no memory or is not aligned"):
+        rope(positions=At((5,), "int64", 4))
+    with refused("a result has no memory or is not aligned"):
+        rope(q_out=At((2, 5, 4, 64), at=2))
+    with refused("tensor 0 has no memory"):
+        clip([At((5,), at=-(1 << 30))])
+    with refused("one float32 value"):
+        clip([At((5,))], norm=At((), at=2))
 
 
 def test_a_residual_of_float32_is_refused():
