@@ -260,7 +260,7 @@ struct Backward : Block {
         sized(dx, M, D, dtype, "d_x"), written(dx, "d_x");
         sized(dwgu, 2 * F, D, dtype, "d_w_gate_up"), written(dwgu, "d_w_gate_up"), sized(dwd, D, F, dtype, "d_w_down"), written(dwd, "d_w_down");
         keep_apart({&dx, &dwgu, &dwd}, {&dy, &x, &wgu, &wd, &gate_up, &h});
-        fused = M && sloped_tiles(M, F) && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F));
+        fused = M && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F)) && (gemm_sloped_ranges(dy, wd) || sloped_tiles(M, F));
         sums = fused ? 0 : up((size_t)M * F * 4), slopes = up((size_t)M * 2 * F * dtype_size(dtype));
         const lb_tensor d = slope(), a[] = {d, transposed(d), transposed(dy)}, b[] = {wgu, x, h};
         grouped = M && gemm_group_pays(a, b, 3);

@@ -1388,11 +1388,22 @@ bool gemm_sloped_takes(const lb_tensor& dy, const lb_tensor& w, const lb_tensor&
     bool a_cols, b_cols;
     return w.shape[1] % 8 == 0 && tensor_core_operands(view3(dy, "dy"), view3(w, "w"), a_cols, b_cols) && in_pieces(kept) && in_pieces(d);
 }
+int gemm_sloped_ranges(const lb_tensor& dy, const lb_tensor& w) {
+    return gemm_small_splits(dy.shape[0], w.shape[1], dy.shape[1], 1, sm_count_hint(), 1);
+}
 void gemm_sloped(const lb_tensor& dy_t, const lb_tensor& w_t, const lb_tensor& kept, const lb_tensor& d, int act, void* stream) {
     driver();
     const View3 dy = view3(dy_t, "dy"), b = view3(w_t, "w"), w = turned(b);
     bool dy_cols, b_cols;
     tensor_core_operands(dy, b, dy_cols, b_cols);
+    if (const int ranges = gemm_sloped_ranges(dy_t, w_t)) {
+        SmallGemmArgs q{};
+        q.M = (int)dy.rows, q.N = (int)w.rows, q.K = (int)dy.cols, q.a_mn_major = !dy_cols, q.b_mn_major = b_cols, q.in_bf16 = q.d_bf16 = dy.dtype == LB_BF16;
+        q.d_f16 = dy.dtype == LB_F16, q.d = d.ptr, q.ldd = d.stride[0], q.status = status_word(), q.splits = ranges;
+        gemm_small_sloped(q.a_mn_major ? make_map(dy, false, 64, BK) : make_map(dy, true, BK, BM), q.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, 64), q, act,
+                          kept.ptr, kept.stride[0], device_info().sms, (cudaStream_t)stream);
+        return;
+    }
     SlopedArgs p{};
     long long tiles;
     pair_args(p, dy, w, dy_cols, !b_cols, BN, tiles);

@@ -72,15 +72,17 @@ void gemm_small(const CUtensorMap& map_a, const CUtensorMap& map_b, SmallGemmArg
 // The gated block's forward products on them: K-major weights, maps with boxes of 32 of their rows.
 void gemm_small_gated(const CUtensorMap& map_a, const CUtensorMap& map_gate, const CUtensorMap& map_up, SmallGemmArgs p, int act, void* kept, long long ld_kept, int sms,
                       cudaStream_t s);
+void gemm_small_sloped(const CUtensorMap& map_a, const CUtensorMap& map_b, SmallGemmArgs p, int act, const void* kept, long long ld_kept, int sms, cudaStream_t s);
 
 // The gated feed-forward block's products with their epilogues, 16-bit operands on CTA pairs. Forward, x [M, K] and w [2 N, K]: h [M, N] = f(a) b with a and
 // b the products with the two halves of w's rows, and kept = [a b] unless it is null. Backward, dy [M, K] and w [K, N]: d = [dh b f'(a), dh f(a)] with
-// dh = dy w and kept = [a b]. `_takes`: whether the operands' layouts are theirs. gemm_gated runs on narrow tiles where `_ranges` says in how many
-// K ranges (0: on CTA pairs).
+// dh = dy w and kept = [a b]. `_takes`: whether the operands' layouts are theirs. Both run on narrow tiles where `_ranges` says in how many K
+// ranges (0: on CTA pairs).
 bool gemm_gated_takes(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept);
 int gemm_gated_ranges(const lb_tensor& x, const lb_tensor& w);
 void gemm_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept, int act, void* stream);
 bool gemm_sloped_takes(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d);
+int gemm_sloped_ranges(const lb_tensor& dy, const lb_tensor& w);
 void gemm_sloped(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept, const lb_tensor& d, int act, void* stream);
 
 // d[k] = a[k] b[k] for up to three products of 16-bit operands that do not depend on one another, in one launch; `_pays`: whether they can and gain by it.

@@ -50,17 +50,30 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r
 
 // What the kernel does with a tile: lb_gemm's epilogues, or the gated feed-forward block's, whose tile is 32 columns of both projections: rows of two weights
 // one after the other in B's place, and in the partial tile their columns. us of a whole block in a graph, bfloat16, lb_gemm into float32 and an element-wise
-// kernel -> this: 64 tokens of 1024 x 4096 20.1 -> 18.3, of 512 x 2048 13.0 -> 11.9, 384 of 512 x 1024 12.2 -> 10.4, 200 of 512 x 2048 17.6 -> 15.7.
+// kernel -> this: 64 tokens of 1024 x 4096 20.1 -> 18.3, of 512 x 2048 13.0 -> 11.9, 384 of 512 x 1024 12.2 -> 10.4, 200 of 512 x 2048 17.6 -> 15.7;
+// backward 64 of 1024 x 4096 35.2 -> 34.3, 200 of 512 x 1024 26.8 -> 25.9, and dh needs no place of its own.
+// Its backward product has the gradients of both projections in its epilogue.
 struct SmallPlain : SmallGemmArgs {
-    static constexpr bool gated = false;
+    static constexpr bool gated = false, sloped = false;
 };
 struct alignas(64) SmallGated : SmallGemmArgs {
-    static constexpr bool gated = true;
+    static constexpr bool gated = true, sloped = false;
     CUtensorMap map_up;  // the other weight; N, d, ldd: the gated product's
     int act;
     void* kept;  // both projections side by side; null: not kept
     long long ld_kept;
 };
+struct SmallSloped : SmallGemmArgs {
+    static constexpr bool gated = false, sloped = true;
+    int act;
+    const void* kept;  // d, ldd: the gradients side by side
+    long long ld_kept;
+};
+__device__ __forceinline__ Pair widen_pair(uint32_t w, bool bf16) {
+    if (bf16) return both(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    const float2 f = __half22float2(*(const __half2*)&w);
+    return both(f.x, f.y);
+}
 __device__ __forceinline__ uint32_t round_pair(Pair x, bool bf16) {
     const float2 v = apart(x);
     if (bf16) {
@@ -79,6 +92,19 @@ __device__ __forceinline__ void gate_eight(float* a, const float* b) {
     for (int j = 0; j < 8; j += 2) {
         const float2 h = apart(activation<ACT>(both(a[j], a[j + 1])) * both(b[j], b[j + 1]));
         a[j] = h.x, a[j + 1] = h.y;
+    }
+}
+
+// dh in x, the projections in a and b: x becomes the gate's gradient, y the other's.
+template <int ACT>
+__device__ __forceinline__ void slope_eight(float* x, float* y, const uint4& a, const uint4& b, bool bf16) {
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        Pair slope;
+        const Pair dh = both(x[2 * j], x[2 * j + 1]), value = activation_slope<ACT>(widen_pair(aw[j], bf16), slope);
+        const float2 da = apart(dh * widen_pair(bw[j], bf16) * slope), db = apart(dh * value);
+        x[2 * j] = da.x, x[2 * j + 1] = da.y, y[2 * j] = db.x, y[2 * j + 1] = db.y;
     }
 }
 
@@ -241,7 +267,23 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             *(uint4*)((uint16_t*)p.d + row * p.ldd + col) = round_eight(x, p.d_bf16);
         }
     }
-    for (int i = threadIdx.x; !Args::gated && i < rows * (BN / 8); i += kThreads) {
+    if constexpr (Args::sloped) {
+        for (int i = threadIdx.x; i < rows * (BN / 8); i += kThreads) {
+            const int r = rank * rows + i / (BN / 8), q = i % (BN / 8), col = n_blk * BN + q * 8;
+            const long long row = (long long)m_blk * BM + r;
+            if (!good || row >= p.M || col >= p.N) continue;  // (N is a multiple of eight, rows are 16-byte aligned)
+            const uint16_t* kept = (const uint16_t*)p.kept + row * p.ld_kept + col;
+            const uint4 a = *(const uint4*)kept, b = *(const uint4*)(kept + p.N);
+            float x[8], y[8];
+            total(i / (BN / 8), r, q, x);
+            if (p.act == ACT_SILU) slope_eight<ACT_SILU>(x, y, a, b, p.d_bf16);
+            else if (p.act == ACT_GELU) slope_eight<ACT_GELU>(x, y, a, b, p.d_bf16);
+            else slope_eight<ACT_RELU>(x, y, a, b, p.d_bf16);
+            uint16_t* out = (uint16_t*)p.d + row * p.ldd + col;
+            *(uint4*)out = round_eight(x, p.d_bf16), *(uint4*)(out + p.N) = round_eight(y, p.d_bf16);
+        }
+    }
+    for (int i = threadIdx.x; !Args::gated && !Args::sloped && i < rows * (BN / 8); i += kThreads) {
         const int r = rank * rows + i / (BN / 8), q = i % (BN / 8);
         const long long row = (long long)m_blk * BM + r;
         const int col = n_blk * BN + q * 8;
@@ -357,6 +399,13 @@ void gemm_small_gated(const CUtensorMap& map_a, const CUtensorMap& map_gate, con
     p.tiles_m = (p.M + BM - 1) / BM, p.tiles_n = (p.N + BN / 2 - 1) / (BN / 2);
     p.map_up = map_up, p.act = act, p.kept = kept, p.ld_kept = ld_kept;
     launch_small(map_a, map_gate, p, 1, sms, s);
+}
+void gemm_small_sloped(const CUtensorMap& map_a, const CUtensorMap& map_b, SmallGemmArgs q, int act, const void* kept, long long ld_kept, int sms, cudaStream_t s) {
+    SmallSloped p{};
+    (SmallGemmArgs&)p = q;
+    p.tiles_m = (p.M + BM - 1) / BM, p.tiles_n = (p.N + BN - 1) / BN;
+    p.act = act, p.kept = kept, p.ld_kept = ld_kept;
+    launch_small(map_a, map_b, p, 1, sms, s);
 }
 
 }  // namespace lb
