@@ -147,7 +147,9 @@ void launch_skinny(SkinnyArgs& p, int sms, cudaStream_t s) {
     const int at_once = ahead(p.M <= 8 ? 8 : p.M <= 16 ? 16 : 32);
     p.warps = std::min(kMaxWarps, (blocks + at_once - 1) / at_once);
     p.per_warp = (blocks + p.warps - 1) / p.warps;
-    const int rows = GATED ? 8 : (p.N + 15) / 16 >= sms ? 16 : 8;
+    // rows of a block: 16 where three quarters of the SMs get one, else 8. us of a gated block of 1 and 8 tokens in a graph, 8 -> 16: 512 columns 3.7, 4.1 -> 4.1,
+    // 4.5; 1024 5.2, 6.2 -> 5.8, 6.9; 2048 21.6, 23.1 -> 20.0, 21.1; 2400 26.2, 25.3 -> 25.8, 24.5; 4096 72.2, 74.2 -> 67.3, 66.7
+    const int rows = GATED ? 8 : (p.N + 15) / 16 * 4 >= 3 * sms ? 16 : 8;
     const dim3 grid((unsigned)((p.N + rows - 1) / rows)), block((unsigned)p.warps * 32);
     auto go = [&](auto kernel) { launch_overlapped(kernel, grid, block, 0, s, 0, p); };
     if (GATED || rows == 16) {
@@ -175,7 +177,7 @@ SkinnyArgs skinny_args(const lb_tensor& x, const lb_tensor& w, const lb_tensor& 
 
 // Every block reads all tokens, from the L2: with more than eight of them that is what grows, and beyond 64 MB of it 128-row tiles are the better choice.
 // us of a gated block in a graph, bfloat16, width x hidden, tiles -> these: 4 tokens 1024 x 4096 22.4 -> 5.7, 16 (17 MB) 22.2 -> 9.1, 32 (34 MB) 22.1 -> 12.9,
-// 32 of 512 x 2048 12.8 -> 6.4, 4 of 2048 x 8192 33.5 -> 22.0; 9 of it (38 MB) 32 -> 29.8, 16 (67 MB) 31.9 -> 32.6, 32 (134 MB) 28.8 -> 47.0.
+// 32 of 512 x 2048 12.8 -> 6.4, 4 of 2048 x 8192 33.5 -> 20.5; 9 of it (38 MB) 32 -> 29.8, 16 (67 MB) 31.9 -> 32.6, 32 (134 MB) 28.8 -> 47.0.
 bool skinny_takes(const lb_tensor& x, const lb_tensor& w) {
     const long long M = x.shape[0], K = x.shape[1], N = w.shape[0];
     return M <= kMaxTokens && K % 8 == 0 && (x.dtype == LB_BF16 || x.dtype == LB_F16) && rows_in_pieces(x) && rows_in_pieces(w) &&

@@ -29,18 +29,17 @@ constexpr int kThreads = 256, kBlocksPerSm = 3;
 constexpr int kReads = 4, kScales = 2;                      // 32-byte loads of a thread in flight: squares, scaling (which holds its results too)
 constexpr int kChunkBytes = kThreads * 32 * kReads;         // 32 KB of the operand
 constexpr int kKeep = (64 << 20) / kChunkBytes;              // chunks whose second reading finds them in the L2
-constexpr int kMost = 240, kFew = 32;                       // tensors of one launch: two sizes of table, the smaller the cheaper to hand over
+constexpr int kMost = 240;                                  // tensors of one launch (a table for 32 is handed over 0.1 us faster, and is not worth its kernels)
 
-template <int MOST>
 struct NormTable {
-    const void* x[MOST];
-    void* out[MOST];
-    long long n[MOST];
-    int first[MOST + 1];  // first chunk of each tensor
-    uint8_t dtype[MOST];
+    const void* x[kMost];
+    void* out[kMost];
+    long long n[kMost];
+    int first[kMost + 1];  // first chunk of each tensor
+    uint8_t dtype[kMost];
     int count;
 };
-static_assert(sizeof(NormTable<kMost>) <= 32000, "kernel parameters");
+static_assert(sizeof(NormTable) <= 32000, "kernel parameters");
 
 template <class T> struct Of;
 template <> struct Of<float> {
@@ -139,8 +138,7 @@ __device__ __forceinline__ double block_sum(double v, double* held) {  // to all
 }
 
 // The tensor that chunk `c` lies in: the last whose first chunk is not behind it (an empty tensor has none).
-template <int MOST>
-__device__ __forceinline__ int tensor_of(const NormTable<MOST>& t, int c) {
+__device__ __forceinline__ int tensor_of(const NormTable& t, int c) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -203,8 +201,7 @@ __device__ __forceinline__ void chunk_scale(const T* x, T* out, int n, float c, 
     }
 }
 
-template <int MOST>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_squares_kernel(const __grid_constant__ NormTable<MOST> t, double* partial, int keep) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_squares_kernel(const __grid_constant__ NormTable t, double* partial, int keep) {
     __shared__ double held[kThreads / 32];
     grid_wait();
     double sum = 0.0;
@@ -241,8 +238,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* partial, i
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
-template <int MOST>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_scale_kernel(const __grid_constant__ NormTable<MOST> t, const double* partial, int parts, double max_norm, float* norm) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_scale_kernel(const __grid_constant__ NormTable t, const double* partial, int parts, double max_norm, float* norm) {
     __shared__ double held[kThreads / 32];
     grid_wait();
     const double n = total_norm(partial, parts, held);
@@ -298,19 +294,18 @@ struct Range {
 
 size_t scratch_bytes(int n) { return (size_t)((n + kMost - 1) / kMost) * sm_count_hint() * kBlocksPerSm * sizeof(double); }
 
-// The launches for tensors that have been looked at, MOST of them (those with elements) a table.
-template <int MOST>
+// The launches for tensors that have been looked at, kMost of them (those with elements) a table.
 void launch_norm(const lb_tensor* xs, const lb_tensor* outs, int n, const std::vector<long long>& count, double max_norm, float* norm, double* partial, cudaStream_t s) {
     const int grid = device_info().sms * kBlocksPerSm;
-    std::vector<NormTable<MOST>> tables;
+    std::vector<NormTable> tables;
     std::vector<int> blocks;
     int parts = 0;
     for (int k = 0; k < n;) {
         tables.emplace_back();
-        NormTable<MOST>& t = tables.back();
+        NormTable& t = tables.back();
         t.count = 0;
         long long chunks = 0;
-        for (; k < n && t.count < MOST; k++) {
+        for (; k < n && t.count < kMost; k++) {
             if (!count[k]) continue;
             const int i = t.count++;
             t.x[i] = xs[k].ptr, t.out[i] = outs ? outs[k].ptr : nullptr, t.n[i] = count[k], t.dtype[i] = (uint8_t)xs[k].dtype;
@@ -321,7 +316,7 @@ void launch_norm(const lb_tensor* xs, const lb_tensor* outs, int n, const std::v
         t.first[t.count] = (int)chunks;
         blocks.push_back((int)std::min<long long>(chunks, grid));
         if (!chunks) continue;
-        launch_overlapped(norm_squares_kernel<MOST>, dim3((unsigned)blocks.back()), dim3(kThreads), 0, s, 0, t, partial + parts, outs ? kKeep : 0);
+        launch_overlapped(norm_squares_kernel, dim3((unsigned)blocks.back()), dim3(kThreads), 0, s, 0, t, partial + parts, outs ? kKeep : 0);
         parts += blocks.back();
     }
     if (!outs || !parts) {
@@ -331,7 +326,7 @@ void launch_norm(const lb_tensor* xs, const lb_tensor* outs, int n, const std::v
     bool first = true;
     for (size_t k = tables.size(); k-- > 0;) {
         if (!blocks[k]) continue;
-        launch_overlapped(norm_scale_kernel<MOST>, dim3((unsigned)blocks[k]), dim3(kThreads), 0, s, 0, tables[k], (const double*)partial, parts, max_norm, first ? norm : nullptr);
+        launch_overlapped(norm_scale_kernel, dim3((unsigned)blocks[k]), dim3(kThreads), 0, s, 0, tables[k], (const double*)partial, parts, max_norm, first ? norm : nullptr);
         first = false;
     }
 }
@@ -369,10 +364,7 @@ void run_norm(const lb_tensor* xs, const lb_tensor* outs, int n, double max_norm
     const size_t need = scratch_bytes(n);
     if (n && (!scratch || bytes < need || (uintptr_t)scratch % 16)) refuse(format("%zu bytes of scratch are needed, 16-byte aligned", need));
     driver();
-    int live = 0;
-    for (int k = 0; k < n; k++) live += count[k] > 0;
-    if (live <= kFew) launch_norm<kFew>(xs, outs, n, count, max_norm, (float*)norm->ptr, (double*)scratch, (cudaStream_t)stream);
-    else launch_norm<kMost>(xs, outs, n, count, max_norm, (float*)norm->ptr, (double*)scratch, (cudaStream_t)stream);
+    launch_norm(xs, outs, n, count, max_norm, (float*)norm->ptr, (double*)scratch, (cudaStream_t)stream);
 }
 
 }  // namespace
