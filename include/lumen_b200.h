@@ -164,7 +164,8 @@ int lb_gated_mlp_bwd(int activation, const lb_tensor* d_y, const lb_tensor* x, c
  * z = x / sqrt(mean(x^2) + eps) * weight, then the first R = 2 * pairs elements turn in pairs, (i, i + R/2) or with `interleaved` (2i, 2i + 1):
  * y_a = z_a cos - z_b sin, y_b = z_b cos + z_a sin, by row `position` of the float32 tables `cos` and `sin` [positions, pairs]. `positions`
  * (int32 or int64, [S] or [B, S]; null: 0 .. S - 1) are clamped into the tables. Weights (nullable: ones) are [H] of the rows' dtype or float32.
- * Statistics and products are float32, each result is rounded once. Results may be the operands' own memory, row for row.
+ * Statistics and products are float32, each result is rounded once. Results may be the operands' own memory, row for
+ * row (the same address and strides); else they share none with one another or with any operand, as other heads, columns or rows of one buffer do not.
  * The backward pass reads the forward's operands and gives the gradients of both (d_q and d_k may take the place of d_q_out and d_k_out) and of
  * the weights (one each where there is a weight, of its dtype), bit-identical from run to run. Its scratch (weights only):
  * lb_qk_norm_rope_bwd_scratch_bytes, 16-byte aligned, not shared with a call that may overlap on the GPU. */

@@ -22,6 +22,7 @@
 
 #include "divide.cuh"
 #include "launch.cuh"
+#include "overlap.h"
 #include "pair.cuh"
 
 namespace lb {
@@ -521,7 +522,36 @@ void same_shape(const lb_tensor& a, const lb_tensor& b, const char* what) {
     if (!same) refuse(format("%s must have its operand's shape and dtype", what));
     in_memory(&b, what);
 }
-// Every element of a result has a place of its own (as far as the strides of one dimension say).
+// A result, and the operands whose memory it may be, row for row: every row is read by the threads that write it, before they do. Rows of other blocks are read
+// and written at any time, so all else that a call is given lies apart from it, and its elements from one another.
+struct Result {
+    const lb_tensor* t;
+    const char* what;
+    int own[2];  // numbers of operands
+};
+struct Operand {
+    const lb_tensor* t;
+    const char* what;
+};
+void keep_apart(const Result* results, int n_results, const Operand* operands, int n_operands) {
+    Extent written[4], read[9];
+    for (int k = 0; k < n_operands; k++)
+        if (operands[k].t) read[k] = extent(*operands[k].t);
+    for (int r = 0; r < n_results; r++) {
+        const Result& out = results[r];
+        if (!out.t) continue;
+        if (overlaps_itself(*out.t)) refuse(format("elements of %s share GPU memory with one another", out.what));
+        written[r] = extent(*out.t);
+        for (int k = 0; k < n_operands; k++) {
+            const lb_tensor* t = operands[k].t;
+            if (!t || !written[r].meets(read[k]) || ((k == out.own[0] || k == out.own[1]) && same_places(*out.t, *t))) continue;
+            if (share_memory(*out.t, *t)) refuse(format("%s shares GPU memory with %s", out.what, operands[k].what));
+        }
+        for (int k = 0; k < r; k++)
+            if (results[k].t && written[r].meets(written[k]) && share_memory(*out.t, *results[k].t)) refuse(format("%s shares GPU memory with %s", out.what, results[k].what));
+    }
+}
+// No dimension of a result is repeated.
 void written(const lb_tensor& t, const char* what) {
     for (int d = 0; d < t.rank; d++)
         if (t.shape[d] > 1 && t.stride[d] == 0) refuse(format("%s is written and cannot be a broadcast view", what));
@@ -679,6 +709,9 @@ int lb_qk_norm_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tenso
             lb::RopeSide& side = c.p.side[s];
             side.out = out[s]->ptr, side.out_b = out[s]->stride[0], side.out_s = out[s]->stride[1], side.out_n = out[s]->stride[2], side.out_h = out[s]->stride[3];
         }
+        const lb::Result results[] = {{q_out, "the queries' result", {0, 0}}, {k_out, "the keys' result", {1, 1}}};
+        const lb::Operand operands[] = {{q, "the queries"}, {k, "the keys"}, {cos, "cos"}, {sin, "sin"}, {positions, "positions"}, {q_weight, "the queries' weight"}, {k_weight, "the keys' weight"}};
+        lb::keep_apart(results, 2, operands, 7);
         if (c.rows) lb::run_rope<false>(c, stream);
     });
 }
@@ -713,6 +746,11 @@ int lb_qk_norm_rope_bwd(const lb_rope_desc* desc, const lb_tensor* d_q_out, cons
             c.p.side[0].partial = (float*)scratch;
             c.p.side[1].partial = (float*)((char*)scratch + need / 2);
         }
+        const lb::Result results[] = {{d_q, "the queries' gradient", {0, 2}}, {d_k, "the keys' gradient", {1, 3}}, {d_q_weight, "the queries' weight's gradient", {7, 7}},
+                                      {d_k_weight, "the keys' weight's gradient", {8, 8}}};  // (the weights' are written by a second kernel)
+        const lb::Operand operands[] = {{q, "the queries"}, {k, "the keys"}, {d_q_out, "the gradient of the queries' result"}, {d_k_out, "the gradient of the keys' result"}, {cos, "cos"},
+                                        {sin, "sin"}, {positions, "positions"}, {q_weight, "the queries' weight"}, {k_weight, "the keys' weight"}};
+        lb::keep_apart(results, 4, operands, 9);
         if (c.rows || c.p.side[0].w || c.p.side[1].w) lb::run_rope<true>(c, stream);
     });
 }

@@ -382,8 +382,8 @@ def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, e
     `z = x / sqrt(mean(x^2) + eps) * weight`; then its first `2 * pairs` elements turn, `y_a = z_a cos - z_b sin`, `y_b = z_b cos + z_a sin`, in pairs
     `(i, i + pairs)`, or `(2i, 2i + 1)` with `interleaved`, by the float32 tables `cos` and `sin` `[positions, pairs]`. `positions`: int32 or int64,
     `[S]` or `[B, S]`, clamped into the tables; None is 0, 1, 2 ... Weights: `[H]` of `q`'s dtype or float32; None is all ones. Returns `(q, k)`
-    of the operands' dtype, in `out` if given (which may be `(q, k)`). Bit-identical from call to call; the same rows among others may differ by a
-    rounding."""
+    of the operands' dtype, in `out` if given: `(q, k)` themselves, or memory that overlaps no tensor of the call. Bit-identical from call to call; the
+    same rows among others may differ by a rounding."""
     require_cuda()
     (q_out, k_out), handle = _results_like((q, k), out, stream)
     _lib.host().qk_norm_rope(eps, bool(interleaved), q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out, handle)
@@ -393,7 +393,8 @@ def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, e
 def qk_norm_rope_backward(d_q_out, d_k_out, q, k, cos, sin, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None,
                           stream=None):
     """The backward pass of `qk_norm_rope` on the same operands: returns `(d_q, d_k, d_q_weight, d_k_weight)`, the last two of their weight's dtype and
-    None without one. `out` takes `d_q` and `d_k`, which may be `(d_q_out, d_k_out)`. Bit-identical from call to call."""
+    None without one. `out` takes `d_q` and `d_k`, which may be `(d_q_out, d_k_out)` or memory that overlaps no tensor of the call. Bit-identical from
+    call to call."""
     require_cuda()
     (d_q, d_k), handle = _results_like((q, k), out, stream)
     weights = [w for w in (q_weight, k_weight) if w is not None]
