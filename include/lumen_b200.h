@@ -185,7 +185,7 @@ int lb_qk_norm_rope_bwd(const lb_rope_desc* desc, const lb_tensor* d_q_out, cons
 /* ---- global gradient norm and clipping -----------------------------------------------------------------------------
  * norm = sqrt(sum of squares over all tensors), one float32 value on the device; lb_clip_grad_norm also writes outputs[k] = tensors[k] * c with
  * c = min(1, max_norm / (norm + 1e-6)). Tensors of float16, bfloat16 and float32 in any mix, dense in any order of their dimensions; outputs of the
- * same shape, strides and dtype, the operand itself for in place (untouched where c is 1) or memory that overlaps no tensor of the call. A tensor given
+ * same shape, strides and dtype, the operand itself for in place (untouched where c is 1) or memory that overlaps no tensor of the call (nor the norm). A tensor given
  * twice counts twice, and is refused where it would be written twice. A norm that is infinite or NaN makes c 0 or NaN. The squares' sum is held in 64
  * bits; the same bits every time. Scratch: lb_grad_norm_scratch_bytes, 16-byte aligned, not shared with a call that may overlap on the GPU. */
 size_t lb_grad_norm_scratch_bytes(int n_tensors);

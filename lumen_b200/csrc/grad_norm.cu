@@ -347,7 +347,12 @@ void run_norm(const lb_tensor* xs, const lb_tensor* outs, int n, double max_norm
         if (count[k] && (!outs[k].ptr || (uintptr_t)outs[k].ptr % dtype_size(xs[k].dtype))) refuse(format("result %d has no memory or is not aligned to its elements", k));
         if (!same) refuse(format("result %d must have its operand's shape, strides and dtype", k));
     }
-    if (outs) {  // what is written is written once, and read by nothing else
+    if (outs) {  // what is written is written once, and read by nothing else; the norm among it
+        for (int k = 0; k < n; k++) {
+            const uintptr_t bytes = (uintptr_t)count[k] * dtype_size(xs[k].dtype), at = (uintptr_t)norm->ptr;
+            for (const uintptr_t from : {(uintptr_t)xs[k].ptr, (uintptr_t)outs[k].ptr})
+                if (bytes && at + 4 > from && at < from + bytes) refuse(format("the norm and %s %d share memory", from == (uintptr_t)xs[k].ptr ? "tensor" : "result", k));
+        }
         std::vector<Range> out;
         for (int k = 0; k < n; k++)
             if (count[k]) out.push_back({(uintptr_t)outs[k].ptr, (uintptr_t)outs[k].ptr + (size_t)count[k] * dtype_size(outs[k].dtype), k});

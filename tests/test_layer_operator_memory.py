@@ -153,3 +153,27 @@ def test_one_description_for_both_sides():
         _lib.check(lib.lb_qk_norm_rope(desc, q, q, table, table, None, None, None, q, other, None))
     with in_order():
         _lib.check(lib.lb_qk_norm_rope(desc, q, q, table, table, None, None, None, other, view(3 * ROOM, Q), None))
+
+
+# ---- clipping -------------------------------------------------------------------------------------------------------
+
+
+def clip(tensors, out, norm, most=1.0):
+    _lib.host().clip_grad_norm(tensors, out, most, norm, take, 0)
+
+
+def test_the_norms_place():
+    x, y, empty = At(0, (10,), dtype="float32"), At(ROOM, (9,)), At(64, (0, 3))
+    for at in (-4, 40, ROOM - 4, ROOM + 20, 64):
+        with in_order():
+            clip([x, y, empty], None, At(at, (), dtype="float32"))
+    with in_order():
+        clip([x], [At(2 * ROOM, (10,), dtype="float32")], At(40, (1,), dtype="float32"))
+    for at in (0, 36, ROOM, ROOM + 16):
+        with refused("the norm and tensor [01] share memory"):
+            clip([x, y], None, At(at, (), dtype="float32"))
+    for at in (4, 2 * ROOM + 36):
+        with refused("the norm and (tensor|result) 0 share memory"):
+            clip([x], [At(2 * ROOM, (10,), dtype="float32")], At(at, (), dtype="float32"))
+    with in_order():  # the norm alone is written behind the last read
+        clip([x], None, At(0, (), dtype="float32"), None)
