@@ -129,7 +129,9 @@ lb_tensor as_rows(const lb_tensor* t, const char* what) {
     long long rows = 1, step = 0;
     for (int d = 0; d < t->rank; d++)
         if (t->shape[d] < 0) refuse(format("%s has a negative size", what));
-    for (int d = last - 1; d >= 0; d--) {
+    for (int d = 0; d < last; d++)
+        if (t->shape[d] == 0) rows = 0;  // no rows: nothing about their spacing
+    for (int d = last - 1; d >= 0 && rows; d--) {
         if (t->shape[d] == 1) continue;
         if (rows != 1 && t->stride[d] != step * rows) fail(LB_ERR_UNSUPPORTED, format("gated_mlp: the rows of %s are not evenly spaced", what));
         if (rows == 1) step = t->stride[d];

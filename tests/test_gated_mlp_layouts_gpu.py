@@ -1,0 +1,20 @@
+"""The gated feed-forward block on batches and layouts that its kernels meet less often, against the formula in 64 bits."""
+
+import pytest
+import torch
+
+from lumen_b200.runtime import device_status, gated_mlp_backward, gated_mlp_forward
+from tests.test_gated_mlp_gpu import operands
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("lead", [(3, 0), (0, 3), (5, 0, 2), (1, 0)])
+def test_batches_without_tokens(cuda, lead):
+    _, wgu, wd, _ = operands(cuda, 1, 64, 72, torch.bfloat16)
+    x = torch.empty(*lead, 64, dtype=torch.bfloat16, device=cuda)
+    y, gate_up, h = gated_mlp_forward(x, wgu, wd)
+    assert y.shape == (*lead, 64) and gate_up.shape == (*lead, 144) and h.shape == (*lead, 72)
+    dx, dwgu, dwd = gated_mlp_backward(torch.empty_like(y), x, wgu, wd, gate_up, h)
+    device_status()
+    assert dx.shape == x.shape and bool((dwgu == 0).all()) and bool((dwd == 0).all())  # empty sums

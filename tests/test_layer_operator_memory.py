@@ -17,6 +17,10 @@ class At(Array):
     """A stand-in at byte `at`."""
 
     def __init__(self, at, shape, strides=None, dtype="bfloat16"):
+        if strides is None:
+            strides = [1] * len(shape)
+            for d in range(len(shape) - 2, -1, -1):
+                strides[d] = strides[d + 1] * max(shape[d + 1], 1)  # as torch counts them where there are no elements
         super().__init__(shape, dtype, strides)
         self.at = at
 
@@ -153,6 +157,35 @@ def test_one_description_for_both_sides():
         _lib.check(lib.lb_qk_norm_rope(desc, q, q, table, table, None, None, None, q, other, None))
     with in_order():
         _lib.check(lib.lb_qk_norm_rope(desc, q, q, table, table, None, None, None, other, view(3 * ROOM, Q), None))
+
+
+# ---- gated block ----------------------------------------------------------------------------------------------------
+
+D, F = 64, 96
+
+
+def gated(lead=(10,), **change):
+    a = {"act": 0, "x": At(0, (*lead, D)), "wgu": At(ROOM, (2 * F, D)), "wd": At(2 * ROOM, (D, F)), "residual": None, "y": At(3 * ROOM, (*lead, D)),
+         "gate_up": At(4 * ROOM, (*lead, 2 * F)), "h": At(5 * ROOM, (*lead, F)), "take": take}  # fmt: skip
+    assert not change.keys() - a.keys()
+    a.update(change)
+    _lib.host().gated_mlp_fwd(*a.values(), 0)
+
+
+def gated_back(lead=(10,), **change):
+    a = {"act": 0, "dy": At(0, (*lead, D)), "x": At(ROOM, (*lead, D)), "wgu": At(2 * ROOM, (2 * F, D)), "wd": At(3 * ROOM, (D, F)), "gate_up": At(4 * ROOM, (*lead, 2 * F)),
+         "h": At(5 * ROOM, (*lead, F)), "dx": At(6 * ROOM, (*lead, D)), "dwgu": At(7 * ROOM, (2 * F, D)), "dwd": At(8 * ROOM, (D, F)), "take": take}  # fmt: skip
+    assert not change.keys() - a.keys()
+    a.update(change)
+    _lib.host().gated_mlp_bwd(*a.values(), 0)
+
+
+@pytest.mark.parametrize("lead", [(0,), (3, 0), (0, 3), (5, 0, 2), (2, 5, 0), (0, 0), (1, 0, 7)])
+def test_batches_without_tokens(lead):
+    gated(lead)  # nothing to do
+    gated(lead, residual=At(6 * ROOM, (*lead, D)), gate_up=None)
+    with in_order():  # the weights' gradients are empty sums
+        gated_back(lead)
 
 
 # ---- clipping -------------------------------------------------------------------------------------------------------
