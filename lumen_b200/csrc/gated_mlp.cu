@@ -5,7 +5,6 @@
 // backward pass in the operands' dtype; h is computed from the float32 sums, not from what was kept. [da db] is rounded to the operands'
 // dtype, as an operand of the tensor cores has to be.
 #include <algorithm>
-#include <cstdlib>
 #include <initializer_list>
 
 #include <cuda_bf16.h>
@@ -14,6 +13,7 @@
 #include "gate.cuh"
 #include "gemm.h"
 #include "launch.cuh"
+#include "overlap.h"
 
 namespace lb {
 bool gemm(const lb_tensor& a, const lb_tensor& b, const lb_tensor& d, int epilogue, int kernel_choice, void* stream, void* scratch, size_t scratch_bytes,
@@ -151,25 +151,13 @@ void sized(const lb_tensor& t, long long rows, long long cols, int dtype, const 
         refuse(format("%s must be [%lld, %lld] of the operands' dtype, got %s[%lld, %lld]", what, rows, cols, dtype_name(t.dtype), (long long)t.shape[0], (long long)t.shape[1]));
     if (rows && cols && (!t.ptr || (uintptr_t)t.ptr % dtype_size(dtype))) refuse(format("%s has no memory or is not aligned to its elements", what));
 }
-// Whether two matrices may share memory: their extents overlap, and they are not different columns of one.
-bool meet(const lb_tensor& a, const lb_tensor& b) {
-    auto bytes = [](const lb_tensor& t) {
-        return (((long long)t.shape[0] - 1) * std::abs(t.stride[0]) + (t.shape[1] - 1) * std::abs(t.stride[1]) + 1) * dtype_size(t.dtype);
-    };
-    if (a.shape[0] * a.shape[1] == 0 || b.shape[0] * b.shape[1] == 0) return false;
-    const long long x = (long long)(uintptr_t)a.ptr, y = (long long)(uintptr_t)b.ptr;
-    if (x + bytes(a) <= y || y + bytes(b) <= x) return false;
-    if (a.stride[0] != b.stride[0] || a.stride[1] != 1 || b.stride[1] != 1 || a.dtype != b.dtype || a.stride[0] <= 0) return true;
-    const long long item = dtype_size(a.dtype), row = a.stride[0] * item, apart = ((y - x) % row + row) % row;
-    return !(a.shape[1] * item <= apart && apart + b.shape[1] * item <= row);
-}
 // What is written shares no memory with what is read, or written.
 void keep_apart(std::initializer_list<const lb_tensor*> results, std::initializer_list<const lb_tensor*> operands) {
     for (auto r = results.begin(); r != results.end(); ++r) {
         for (const lb_tensor* o : operands)
-            if (meet(**r, *o)) refuse("a result shares memory with an operand");
+            if (share_memory(**r, *o)) refuse("a result shares memory with an operand");
         for (auto other = r + 1; other != results.end(); ++other)
-            if (meet(**r, **other)) refuse("two results share memory");
+            if (share_memory(**r, **other)) refuse("two results share memory");
     }
 }
 

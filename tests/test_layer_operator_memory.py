@@ -188,6 +188,19 @@ def test_batches_without_tokens(lead):
         gated_back(lead)
 
 
+def test_operands_in_any_direction():
+    """Rows that go backwards through memory: what they cover lies in front of their first one."""
+    up, down = At(3 * ROOM, (10, D)), At(3 * ROOM + 2 * 9 * D, (10, D), [-D, 1])
+    with refused("shares memory with an operand"):
+        gated(x=down, y=up)
+    with in_order():
+        gated(x=At(3 * ROOM, (10, D), [-D, 1]), y=At(3 * ROOM + 2 * D, (10, D)))
+    with refused("shares memory with an operand"):
+        gated_back(h=At(6 * ROOM + 2 * 9 * F, (10, F), [-F, 1]), dx=At(6 * ROOM, (10, D)))
+    with in_order():  # every other row, and the rows between them
+        gated(x=At(0, (10, D), [2 * D, 1]), y=At(2 * D, (10, D), [2 * D, 1]))
+
+
 # ---- clipping -------------------------------------------------------------------------------------------------------
 
 
