@@ -204,8 +204,6 @@ struct Forward : Block {
         : Block(act, x_t, wgu_t, wd_t), y(as_rows(y_t, "y")), h(as_rows(h_t, "h")), keeps(gate_up_t) {
         sized(y, M, D, dtype, "y"), written(y, "y"), sized(h, M, F, dtype, "h"), written(h, "h");
         if (keeps) gate_up = as_rows(gate_up_t, "gate_up"), sized(gate_up, M, 2 * F, dtype, "gate_up"), written(gate_up, "gate_up");
-        if (keeps) keep_apart({&y, &h, &gate_up}, {&x, &wgu, &wd});
-        else keep_apart({&y, &h}, {&x, &wgu, &wd});
         if (M == 0) return;
         few = skinny_takes(x, wgu) && skinny_takes(h, wd);
         if (few) return;
@@ -249,7 +247,6 @@ struct Backward : Block {
         if (gate_up.stride[1] != 1) fail(LB_ERR_UNSUPPORTED, "gated_mlp: gate_up must be row-major");
         sized(dx, M, D, dtype, "d_x"), written(dx, "d_x");
         sized(dwgu, 2 * F, D, dtype, "d_w_gate_up"), written(dwgu, "d_w_gate_up"), sized(dwd, D, F, dtype, "d_w_down"), written(dwd, "d_w_down");
-        keep_apart({&dx, &dwgu, &dwd}, {&dy, &x, &wgu, &wd, &gate_up, &h});
         fused = M && gemm_sloped_takes(dy, wd, gate_up, matrix(nullptr, dtype, M, 2 * F, 2 * F)) && (gemm_sloped_ranges(dy, wd) || sloped_tiles(M, F));
         sums = fused ? 0 : up((size_t)M * F * 4), slopes = up((size_t)M * 2 * F * dtype_size(dtype));
         const lb_tensor d = slope(), a[] = {d, transposed(d), transposed(dy)}, b[] = {wgu, x, h};
@@ -305,9 +302,10 @@ int lb_gated_mlp_fwd(int activation, const lb_tensor* x, const lb_tensor* w_gate
             lb::sized(r, f.M, f.D, f.dtype, "residual");
             if (f.dtype == LB_F32) lb::fail(LB_ERR_UNSUPPORTED, "gated_mlp: a residual is added to 16-bit results");
             if (r.stride[1] != 1 && f.D > 1) lb::fail(LB_ERR_UNSUPPORTED, "gated_mlp: residual must be row-major");
-            if (f.keeps) lb::keep_apart({&f.y, &f.h, &f.gate_up}, {&r});
-            else lb::keep_apart({&f.y, &f.h}, {&r});
         }
+        const lb_tensor& add = residual ? r : f.x;
+        if (f.keeps) lb::keep_apart({&f.y, &f.h, &f.gate_up}, {&f.x, &f.wgu, &f.wd, &add});
+        else lb::keep_apart({&f.y, &f.h}, {&f.x, &f.wgu, &f.wd, &add});
         lb::give_scratch(f, f.bytes(), scratch, scratch_bytes);
         if (f.M) f.run(residual ? &r : nullptr, stream);
     });
@@ -327,6 +325,7 @@ int lb_gated_mlp_bwd(int activation, const lb_tensor* d_y, const lb_tensor* x, c
                      void* stream) {
     return lb::guarded([&] {
         lb::Backward b(activation, d_y, x, w_gate_up, w_down, gate_up, h, d_x, d_w_gate_up, d_w_down);
+        lb::keep_apart({&b.dx, &b.dwgu, &b.dwd}, {&b.dy, &b.x, &b.wgu, &b.wd, &b.gate_up, &b.h});
         lb::give_scratch(b, b.bytes(), scratch, scratch_bytes);
         b.run(stream);
     });

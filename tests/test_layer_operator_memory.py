@@ -201,6 +201,22 @@ def test_operands_in_any_direction():
         gated(x=At(0, (10, D), [2 * D, 1]), y=At(2 * D, (10, D), [2 * D, 1]))
 
 
+def test_sizes_of_scratch_do_not_ask_where_memory_is():
+    import ctypes
+
+    def view(*shape):
+        t = _lib.LbTensor()
+        t.ptr, t.dtype, t.rank = 4096, 10, 2
+        t.shape[0], t.shape[1], t.stride[0], t.stride[1] = *shape, shape[1], 1
+        return ctypes.byref(t)
+
+    lib, got = _lib.lib(), ctypes.c_size_t()
+    x, wgu, wd, gate_up, h = view(200, D), view(2 * F, D), view(D, F), view(200, 2 * F), view(200, F)
+    _lib.check(lib.lb_gated_mlp_fwd_scratch_bytes(0, x, wgu, wd, x, gate_up, h, ctypes.byref(got)))
+    _lib.check(lib.lb_gated_mlp_bwd_scratch_bytes(0, x, x, wgu, wd, gate_up, h, x, wgu, wd, ctypes.byref(got)))
+    assert got.value >= 200 * 2 * F * 2  # both projections' gradients
+
+
 # ---- clipping -------------------------------------------------------------------------------------------------------
 
 
