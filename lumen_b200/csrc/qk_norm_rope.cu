@@ -560,6 +560,7 @@ void weights(RopeSide& side, const lb_tensor* w, int H, int dtype, const char* w
     if (!w) return;
     if (w->rank != 1 || w->shape[0] != H || (w->dtype != dtype && w->dtype != LB_F32)) refuse(format("%s must be [%d] of the rows' dtype or float32", what, H));
     if (H > 1 && w->stride[0] != 1) refuse(format("%s must be dense", what));
+    in_memory(w, what);
     side.w = w->ptr, side.w_f32 = w->dtype == LB_F32, side.w_vec = (uintptr_t)w->ptr % 16 == 0;
 }
 
@@ -629,8 +630,7 @@ RopeCall check_rope(const lb_rope_desc* desc, const lb_tensor* q, const lb_tenso
         refuse(format("the tables hold %d positions, the sequence has %d", p.table, p.seq));
     }
     if (!(desc->eps >= 0.0f)) refuse("eps must not be negative");
-    in_memory(q, "queries"), in_memory(k, "keys"), in_memory(cos, "cos"), in_memory(sin, "sin"), in_memory(positions, "positions"), in_memory(wq, "the queries' weight");
-    in_memory(wk, "the keys' weight");
+    in_memory(q, "queries"), in_memory(k, "keys"), in_memory(cos, "cos"), in_memory(sin, "sin"), in_memory(positions, "positions");
     p.eps = desc->eps, p.interleaved = desc->interleaved != 0;
     const lb_tensor* x[2] = {q, k};
     for (int s = 0; s < 2; s++) {

@@ -159,6 +159,23 @@ def test_one_description_for_both_sides():
         _lib.check(lib.lb_qk_norm_rope(desc, q, q, table, table, None, None, None, other, view(3 * ROOM, Q), None))
 
 
+@pytest.mark.parametrize("rank", [-5, 0, 2, 9, 1 << 24])
+def test_weights_of_any_rank(rank):
+    """A description of more dimensions than there are places for is not read beyond them."""
+    import ctypes
+
+    def view(*shape, dtype=10, rank=None):
+        t, step = _lib.LbTensor(), 1
+        t.ptr, t.dtype, t.rank = 4096, dtype, len(shape) if rank is None else rank
+        for d in range(len(shape) - 1, -1, -1):
+            t.shape[d], t.stride[d], step = shape[d], step, step * shape[d]
+        return ctypes.byref(t)
+
+    lib, desc = _lib.lib(), (ctypes.c_float * 2)(1e-6, 0.0)
+    with refused("queries' weight must be \\[64\\]"):
+        _lib.check(lib.lb_qk_norm_rope(desc, view(*Q), view(*K), view(16, 32, dtype=11), view(16, 32, dtype=11), None, view(H, rank=rank), None, view(*Q), view(*K), None))
+
+
 # ---- gated block ----------------------------------------------------------------------------------------------------
 
 D, F = 64, 96
