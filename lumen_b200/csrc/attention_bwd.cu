@@ -595,8 +595,9 @@ template <int D, bool DKDV, int TILE>
 void launch_bwd_kernel(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& t1, const CUtensorMap& t2, dim3 grid, const BwdArgs& p,
                        cudaStream_t s) {
     using C = BwdConfig<D, DKDV, TILE>;
-    if (first_use_on_device((const void*)attention_bwd_kernel<D, DKDV, TILE>))
+    first_use_on_device((const void*)attention_bwd_kernel<D, DKDV, TILE>, [] {
         LB_CUDA(cudaFuncSetAttribute(attention_bwd_kernel<D, DKDV, TILE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes));
+    });
     launch_overlapped(attention_bwd_kernel<D, DKDV, TILE>, grid, dim3(C::kThreads), C::kBytes, s, 0, r1, r2, t1, t2, p);
 }
 

@@ -499,8 +499,9 @@ void attention_bwd_atomic_launch(const lb_attn_desc& desc, const CUtensorMap& mk
     if (regs != kLaunchRegs)
         fail(LB_ERR_UNSUPPORTED, format("attention backward: the single-kernel form was built with %d registers per thread, its register "
                                         "budgets assume %d", regs, kLaunchRegs));
-    if (first_use_on_device((const void*)attention_bwd_atomic_kernel))
+    first_use_on_device((const void*)attention_bwd_atomic_kernel, [] {
         LB_CUDA(cudaFuncSetAttribute(attention_bwd_atomic_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    });
     dim3 grid((unsigned)((Sk + BR - 1) / BR), (unsigned)Nkv, (unsigned)B);
     launch_overlapped(attention_bwd_atomic_kernel, grid, dim3(kThreads), kSmemBytes, s, 0, mk, mv, mq, mdo, make_acc_map(dq_acc, B, Sq, N), a);
     const long long rows = Sq * N;  // rows * 8 < 2^31 and B <= 65535: checked for attention_delta

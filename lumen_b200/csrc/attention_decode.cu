@@ -296,10 +296,10 @@ template <int D, int MT>
 void launch(const DecodeArgs& p, int batch, long long keys, cudaStream_t s) {
     auto kernel = attention_decode_kernel<D, MT>;
     constexpr int bytes = DecodeSmem<D, MT>::kBytes;
-    if (first_use_on_device((const void*)kernel)) {
+    first_use_on_device((const void*)kernel, [&] {
         LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    }
+    });
     const int splits = resident_splits<D, MT>(pick_splits(decode_cost(D, MT), (long long)batch * p.Nkv, keys, device_info().sms));
     launch_overlapped(kernel, dim3((unsigned)splits, (unsigned)p.Nkv, (unsigned)batch), dim3(kWarps * 32), bytes, s, (unsigned)splits, p);
 }

@@ -175,8 +175,9 @@ __global__ void __launch_bounds__(kThreads, 2) attention_dq_kernel(const __grid_
 
 template <int TILES>
 static void launch_dq(const CUtensorMap& keys, int batches, const DqArgs& p, cudaStream_t s) {
-    if (first_use_on_device((const void*)attention_dq_kernel<TILES>))
+    first_use_on_device((const void*)attention_dq_kernel<TILES>, [] {
         LB_CUDA(cudaFuncSetAttribute(attention_dq_kernel<TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqConfig<TILES>::kSmemBytes));
+    });
     launch_overlapped(attention_dq_kernel<TILES>, dim3((unsigned)((p.Sq + TILES * 128 - 1) / (TILES * 128)), (unsigned)p.heads, (unsigned)batches), dim3(kThreads),
                       DqConfig<TILES>::kSmemBytes, s, 0, keys, p);
 }

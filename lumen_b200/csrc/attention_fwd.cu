@@ -659,8 +659,9 @@ bool pair_has_registers() {
 template <int D>
 void launch_fwd_pair(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, FwdArgs p, cudaStream_t s) {
     constexpr int kBytes = FwdPairSmem<D>::kBytes;
-    if (first_use_on_device((const void*)attention_fwd_pair_kernel<D>))
+    first_use_on_device((const void*)attention_fwd_pair_kernel<D>, [] {
         LB_CUDA(cudaFuncSetAttribute(attention_fwd_pair_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+    });
     p.tiles = (p.Sq + 2 * BQ - 1) / (2 * BQ);
     const long long heads = (long long)p.B * p.N, bytes_per_head = std::max(1LL, (long long)p.Sk * D * 4 * p.Nkv / p.N);
     p.heads_at_once = (int)std::min(heads, std::max(1LL, (48LL << 20) / bytes_per_head));
@@ -796,12 +797,14 @@ void attention_fwd(const lb_attn_desc& desc, const lb_tensor& q, const lb_tensor
     }
     // One warpgroup, O in tensor memory, two CTAs per SM: two K/V stages at head dim 64, one at head dim 128 (96 KB per CTA)
     if (D == 128) {
-        if (first_use_on_device((const void*)attention_fwd_kernel<128, 1>))
+        first_use_on_device((const void*)attention_fwd_kernel<128, 1>, [] {
             LB_CUDA(cudaFuncSetAttribute(attention_fwd_kernel<128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<128, 1>::kBytes));
+        });
         launch_overlapped(attention_fwd_kernel<128, 1>, grid, dim3(kThreads), FwdSmem<128, 1>::kBytes, s, 0, mq, mk, mv, p);
     } else {
-        if (first_use_on_device((const void*)attention_fwd_kernel<64, 2>))
+        first_use_on_device((const void*)attention_fwd_kernel<64, 2>, [] {
             LB_CUDA(cudaFuncSetAttribute(attention_fwd_kernel<64, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<64, 2>::kBytes));
+        });
         launch_overlapped(attention_fwd_kernel<64, 2>, grid, dim3(kThreads), FwdSmem<64, 2>::kBytes, s, 0, mq, mk, mv, p);
     }
 }

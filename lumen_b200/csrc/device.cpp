@@ -5,7 +5,6 @@
 #include <cstdlib>
 #include <map>
 #include <mutex>
-#include <set>
 #include <vector>
 
 namespace lb {
@@ -70,7 +69,7 @@ const DeviceInfo& device_info() {
 static std::map<int, std::vector<int*>> g_status_words;
 static std::map<int, bool> g_has_main_word;
 
-static int current_device() {
+int current_device() {
     int dev = 0;
     LB_CUDA(cudaGetDevice(&dev));
     return dev;
@@ -119,11 +118,9 @@ int read_status() {
     return result;
 }
 
-bool first_use_on_device(const void* key) {
-    static std::set<std::pair<int, const void*>> seen;
-    const int dev = current_device();
-    std::lock_guard<std::mutex> lock(g_mutex);
-    return seen.emplace(dev, key).second;
+FirstUse& first_uses() {
+    static FirstUse uses;
+    return uses;
 }
 
 int launch_regs(const void* kernel) {

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "common.h"
+#include "first_use.h"
 
 namespace lb {
 
@@ -51,9 +52,14 @@ void register_status_word(int* word);
 // Synchronises the current device, then reads and clears every status word registered for it; the first non-zero
 // value, else 0. Allocates nothing.
 int read_status();
-// True the first time it is called with `key` while this device is current: one-time set-up per (device, kernel),
-// such as cudaFuncSetAttribute, which applies to the current device only.
-bool first_use_on_device(const void* key);
+// Runs `setup` the first time it is called with `key` while this device is current (first_use.h): one-time set-up per (device, kernel),
+// such as cudaFuncSetAttribute, which applies to the current device only. `setup` calls nothing that comes here.
+FirstUse& first_uses();
+int current_device();
+template <class F>
+void first_use_on_device(const void* key, F setup) {
+    first_uses().run(current_device(), key, setup);
+}
 // What an autotuner (or a caller) may fix for one GEMM instead of the built-in choices; 0 = choose.
 struct GemmTuning {
     int splits = 0;   // K ranges (needs scratch for that many float32 partial tiles)

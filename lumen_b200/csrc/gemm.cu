@@ -1214,10 +1214,10 @@ bool gemm(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& d_t, int 
             gemm_small(map_a, p.b_mn_major ? map_b : make_map(bt, true, BK, 64), q, (int)batch, dev.sms, s);
             return false;
         }
-        if (first_use_on_device((const void*)gemm_tcgen05_pair<PlainArgs>)) {
+        first_use_on_device((const void*)gemm_tcgen05_pair<PlainArgs>, [] {
             LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
             LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<PlainArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
-        }
+        });
         const int max_pairs = resident_pairs(dev);
         long long tiles = (long long)p.tiles_m * p.tiles_n * batch;
         const int sms = dev.sms;
@@ -1288,8 +1288,9 @@ static void pair_args(GemmArgs& p, const View3& x, const View3& w, bool x_cols, 
 template <class Args>
 static void launch_pairs(const CUtensorMap& map_a, const CUtensorMap& map_b, const Args& p, long long tiles, void* stream) {
     const DeviceInfo& dev = device_info();
-    if (first_use_on_device((const void*)gemm_tcgen05_pair<Args>))
+    first_use_on_device((const void*)gemm_tcgen05_pair<Args>, [] {
         LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(Args::mode)));
+    });
     const int max_pairs = resident_pairs(dev), grid = 2 * (int)std::min<long long>(tiles, max_pairs > 0 ? max_pairs : dev.sms / 2);
     launch_overlapped(gemm_tcgen05_pair<Args>, dim3((unsigned)grid), dim3(kThreads), pair_smem(Args::mode), (cudaStream_t)stream, 0, map_a, map_b, p);
 }

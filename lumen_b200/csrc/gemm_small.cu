@@ -371,8 +371,9 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 template <int STAGES, bool RANKS, class Args>
 static void launch_small(const CUtensorMap& map_a, const CUtensorMap& map_b, const Args& p, int batch, cudaStream_t s) {
-    if (first_use_on_device((const void*)gemm_small_kernel<STAGES, RANKS, Args>))
+    first_use_on_device((const void*)gemm_small_kernel<STAGES, RANKS, Args>, [] {
         LB_CUDA(cudaFuncSetAttribute(gemm_small_kernel<STAGES, RANKS, Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(STAGES, RANKS)));
+    });
     launch_overlapped(gemm_small_kernel<STAGES, RANKS, Args>, dim3((unsigned)((long long)p.tiles_m * p.tiles_n * batch * p.splits)), dim3(kThreads), smem_bytes(STAGES, RANKS), s,
                       (unsigned)p.splits, map_a, map_b, p);
 }

@@ -649,8 +649,9 @@ void launch_many(RopeArgs& p, int sms, cudaStream_t stream) {
     constexpr int kHeads = many_heads<T, BWD, N>();
     p.lanes = 1;
     while (p.lanes * 2 * N < p.H) p.lanes *= 2;
-    if (first_use_on_device((const void*)rope_many_kernel<T, BWD, N>))
+    first_use_on_device((const void*)rope_many_kernel<T, BWD, N>, [] {
         LB_CUDA(cudaFuncSetAttribute(rope_many_kernel<T, BWD, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, many_smem<T, BWD, N>()));
+    });
     share_blocks(p, kGroupThreads / p.lanes, kHeads, sms, many_per_sm<N>());
     p.by_seq.set((uint32_t)std::max(p.seq, 1));
     for (RopeSide& q : p.side) q.by_chunks.set((uint32_t)std::max((q.heads + kHeads - 1) / kHeads, 1));

@@ -896,8 +896,10 @@ unsigned attn_blocks(long long batch, long long heads, long long rows, int rw) {
 // `streamed`: the rows that the kernel walks per head
 template <int DU, int RW, class Kernel, class... Args>
 void launch_attn(Kernel kernel, unsigned blocks, int streamed, cudaStream_t st, AttnShape s, Args... args) {
-    if (AttnSmem<DU, RW>::bytes(kChunk) > 48 * 1024 && first_use_on_device((const void*)kernel))
-        LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnSmem<DU, RW>::bytes(kChunk)));
+    if (AttnSmem<DU, RW>::bytes(kChunk) > 48 * 1024)
+        first_use_on_device((const void*)kernel, [&] {
+            LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnSmem<DU, RW>::bytes(kChunk)));
+        });
     s.tile_rows = std::min(kChunk, (std::max(streamed, 1) + 3) / 4 * 4);
     launch_overlapped(kernel, dim3(blocks), dim3(kAttnWarps * 32), AttnSmem<DU, RW>::bytes(s.tile_rows), st, 0, args..., s);
 }
