@@ -1055,13 +1055,15 @@ int gemm_small_splits(long long M, long long N, long long K, long long batch, in
     return s;
 }
 
-// CTA pairs of gemm_tcgen05_pair that can be resident on `dev` at once (asked of the runtime once per device).
+// CTA pairs of gemm_tcgen05_pair that can be resident on `dev` at once (asked of the runtime once per device): one CTA fills an SM in each of its modes. The
+// runtime refuses to answer for a kernel whose limit of shared memory is still the default, whichever mode comes first.
 static int resident_pairs(const DeviceInfo& dev) {
     static std::mutex mutex;
     static std::map<int, int> cache;
     std::lock_guard<std::mutex> lock(mutex);
     auto it = cache.find(dev.device);
     if (it != cache.end()) return it->second;
+    LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<PlainArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
     int pairs = 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (dev.sms / 2), 1, 1), cfg.blockDim = dim3(kThreads, 1, 1), cfg.dynamicSmemBytes = kPairSmemBytes;

@@ -67,3 +67,11 @@ def test_every_set_up_runs_inside_it():
         if name.endswith((".cu", ".cpp", ".cuh", ".h")):
             text = open(os.path.join(CSRC, name)).read()
             assert "if (first_use_on_device(" not in text and "&& first_use_on_device(" not in text, name
+
+
+def test_pairs_are_counted_behind_their_kernels_set_up():
+    """The first launch of CTA pairs may be another mode's: what the runtime is asked about has its limit of shared memory by then."""
+    text = open(os.path.join(CSRC, "gemm.cu")).read()
+    body = text[text.index("static int resident_pairs(") :]
+    body = body[: body.index("\n}\n")]
+    assert 0 < body.index("cudaFuncSetAttribute(gemm_tcgen05_pair<PlainArgs>") < body.index("cudaOccupancyMaxActiveClusters")
