@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from lumen_b200.runtime import device_status, gated_mlp_backward, gated_mlp_forward
-from tests.test_gated_mlp_gpu import operands
+from tests.test_gated_mlp_gpu import check_backward, check_forward, operands
 
 pytestmark = pytest.mark.gpu
 
@@ -18,3 +18,16 @@ def test_batches_without_tokens(cuda, lead):
     dx, dwgu, dwd = gated_mlp_backward(torch.empty_like(y), x, wgu, wd, gate_up, h)
     device_status()
     assert dx.shape == x.shape and bool((dwgu == 0).all()) and bool((dwd == 0).all())  # empty sums
+
+
+@pytest.mark.parametrize("m, d, f", [(1500, 840, 2056), (200, 512, 1024), (40, 256, 520)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_that_lie_the_other_way_round(cuda, m, d, f, dtype):
+    """On tiles of CTA pairs and on narrow ones, with both projections' columns across and along the weights' rows."""
+    x, wgu, wd, dy = operands(cuda, m, d, f, dtype)
+    for a, b in ((wgu.t().contiguous().t(), wd.t().contiguous().t()), (wgu, wd.t().contiguous().t()), (wgu.t().contiguous().t(), wd)):
+        y, gate_up, h = gated_mlp_forward(x, a, b, activation="gelu")
+        check_forward(x, a, b, "gelu", y, gate_up, h)
+        grads = gated_mlp_backward(dy, x, a, b, gate_up, h, activation="gelu")
+        device_status()
+        check_backward(dy, x, a, b, gate_up, h, "gelu", *grads)
