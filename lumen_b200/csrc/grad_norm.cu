@@ -12,7 +12,10 @@
 // the operand's, nothing is left to do. The second pass walks the chunks backwards, and the last 64 MB that the first one reads stay in the L2 for it
 // (evict-last; all else goes first). 158 M bfloat16 values (317 MB): the squares take 47.6 us alone, 6.66 TB/s, clipping into other memory 147.5
 // us in all, 951 MB at 6.45 TB/s (nothing kept 152.2, 96 MB 148.5); loads of 16 bytes and four a thread in flight 159, 16-byte stores past the L2 no
-// gain, eight blocks to an SM 220. The norm of 60 M values of three types, 160 MB, 30 us with both launches, 5.3 TB/s.
+// gain, eight blocks to an SM 220; in place over the bound 157.6 in a graph (into other memory 149.5). Tables of one call share the 64 MB, the last ones first
+// (grad_norm.h): 300 tensors of 600 MB 291 us, 700 of 560 MB 279, with as much for every table 297 and 291. In place within the bound nothing reads what is kept: a
+// pass over the gradients behind the call is faster by it (158 M values from the end 216 -> 198 us), six passes over other data that just fits the L2 take 4 to 8 us longer
+// (80 MB 100 -> 108), and data that is smaller or larger than that no longer than before. The norm of 60 M values of three types, 160 MB, 30 us with both launches, 5.3 TB/s.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -20,6 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "grad_norm.h"
 #include "launch.cuh"
 
 namespace lb {
@@ -297,26 +301,29 @@ size_t scratch_bytes(int n) { return (size_t)((n + kMost - 1) / kMost) * sm_coun
 // The launches for tensors that have been looked at, kMost of them (those with elements) a table.
 void launch_norm(const lb_tensor* xs, const lb_tensor* outs, int n, const std::vector<long long>& count, double max_norm, float* norm, double* partial, cudaStream_t s) {
     const int grid = device_info().sms * kBlocksPerSm;
-    std::vector<NormTable> tables;
+    std::vector<long long> chunks((size_t)n);
+    for (int k = 0; k < n; k++) {
+        const int per = kChunkBytes / dtype_size(xs[k].dtype);
+        chunks[k] = (count[k] + per - 1) / per;
+    }
+    const std::vector<NormPass> passes = norm_passes(chunks, kMost, outs ? kKeep : 0);
+    std::vector<NormTable> tables(passes.size());
     std::vector<int> blocks;
     int parts = 0;
-    for (int k = 0; k < n;) {
-        tables.emplace_back();
-        NormTable& t = tables.back();
+    for (size_t at = 0; at < passes.size(); at++) {
+        NormTable& t = tables[at];
         t.count = 0;
-        long long chunks = 0;
-        for (; k < n && t.count < kMost; k++) {
+        int first = 0;
+        for (int k = passes[at].from; k < passes[at].to; k++) {
             if (!count[k]) continue;
             const int i = t.count++;
             t.x[i] = xs[k].ptr, t.out[i] = outs ? outs[k].ptr : nullptr, t.n[i] = count[k], t.dtype[i] = (uint8_t)xs[k].dtype;
-            t.first[i] = (int)chunks;
-            const int per = kChunkBytes / dtype_size(xs[k].dtype);
-            chunks += (count[k] + per - 1) / per;
+            t.first[i] = first, first += (int)chunks[k];
         }
-        t.first[t.count] = (int)chunks;
-        blocks.push_back((int)std::min<long long>(chunks, grid));
-        if (!chunks) continue;
-        launch_overlapped(norm_squares_kernel, dim3((unsigned)blocks.back()), dim3(kThreads), 0, s, 0, t, partial + parts, outs ? kKeep : 0);
+        t.first[t.count] = first;
+        blocks.push_back(std::min(first, grid));
+        if (!first) continue;
+        launch_overlapped(norm_squares_kernel, dim3((unsigned)blocks.back()), dim3(kThreads), 0, s, 0, t, partial + parts, passes[at].keep);
         parts += blocks.back();
     }
     if (!outs || !parts) {
