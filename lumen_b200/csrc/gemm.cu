@@ -1272,8 +1272,10 @@ static View3 turned(View3 v) {
     std::swap(v.rows, v.cols), std::swap(v.sr, v.sc);
     return v;
 }
-// Rows of a result (or of what an epilogue reads) that the gated kernels take in 16-byte pieces.
-static bool in_pieces(const lb_tensor& t) { return (uintptr_t)t.ptr % 16 == 0 && (t.shape[0] <= 1 || t.stride[0] % 8 == 0) && t.stride[1] == 1; }
+// Rows of a result (or of what an epilogue reads) that the gated kernels take in 16-byte pieces, by TMA among others: one behind the other in memory.
+static bool in_pieces(const lb_tensor& t) {
+    return (uintptr_t)t.ptr % 16 == 0 && (t.shape[0] <= 1 || (t.stride[0] % 8 == 0 && t.stride[0] >= t.shape[1])) && t.stride[1] == 1;
+}
 
 // What both of the gated block's products set up: x [M, K] times w [N, K] transposed on CTA pairs, tiles of `tile_n` columns.
 static void pair_args(GemmArgs& p, const View3& x, const View3& w, bool x_cols, bool w_cols, int tile_n, long long& tiles) {

@@ -31,3 +31,14 @@ def test_weights_that_lie_the_other_way_round(cuda, m, d, f, dtype):
         grads = gated_mlp_backward(dy, x, a, b, gate_up, h, activation="gelu")
         device_status()
         check_backward(dy, x, a, b, gate_up, h, "gelu", *grads)
+
+
+@pytest.mark.parametrize("m", [40, 300, 1500])
+def test_what_was_kept_in_rows_that_are_not_one_behind_the_other(cuda, m):
+    """One token repeated: its projections and their gated product as rows that share memory."""
+    x, wgu, wd, dy = operands(cuda, m, 840, 2056, torch.bfloat16)
+    x = x[:1].expand(m, 840)
+    y, gate_up, h = (t.expand(m, -1) for t in gated_mlp_forward(x[:1], wgu, wd))
+    grads = gated_mlp_backward(dy, x, wgu, wd, gate_up, h)
+    device_status()
+    check_backward(dy, x, wgu, wd, gate_up, h, "silu", *grads)
