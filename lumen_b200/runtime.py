@@ -376,6 +376,15 @@ def _results_like(tensors, out, stream):
     return [_empty_like_input(t, tuple(t.shape), dtype_name(t.dtype)) for t in tensors], _stream(stream)
 
 
+def _written(tensors):
+    """Tells autograd that the caller's `tensors` have other values now, so that a backward pass that kept one of them raises as it does for torch's
+    own in-place operations."""
+    torch = sys.modules.get("torch")
+    known = [t for t in tensors if isinstance(t, torch.Tensor)] if torch else ()
+    if known:
+        torch.autograd.graph.increment_version(known)
+
+
 def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None, stream=None):
     """Norms of queries and keys for each head and the position rotation, in one pass through `lb_qk_norm_rope`. `q` `[B, S, N, H]` and `k`
     `[B, S, Nkv, H]` are views of float16, bfloat16 or float32 (of a packed projection, say), H up to 256. Each head's row becomes
@@ -387,6 +396,8 @@ def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, e
     require_cuda()
     (q_out, k_out), handle = _results_like((q, k), out, stream)
     _lib.host().qk_norm_rope(eps, bool(interleaved), q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out, handle)
+    if out is not None:
+        _written(out)
     return q_out, k_out
 
 
@@ -402,6 +413,8 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, cos, sin, positions=None, q_we
     d_q_weight, d_k_weight = grads.pop(0) if q_weight is not None else None, grads.pop() if k_weight is not None else None
     _lib.host().qk_norm_rope_bwd(eps, bool(interleaved), d_q_out, d_k_out, q, k, cos, sin, positions, q_weight, k_weight, d_q, d_k, d_q_weight, d_k_weight,
                                  _scratch(q, stream), handle)
+    if out is not None:
+        _written(out)
     return d_q, d_k, d_q_weight, d_k_weight
 
 
@@ -450,6 +463,8 @@ def _norm(tensors, out, max_norm, like, stream):
         like = tensors[0]
     (norm,), handle = _outputs(like, stream, ((), "float32"))
     _lib.host().clip_grad_norm(tensors, out, max_norm, norm, _scratch(like, stream), handle)
+    if max_norm is not None:
+        _written(tensors if out is None else out)
     return norm
 
 
