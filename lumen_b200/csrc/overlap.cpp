@@ -86,6 +86,13 @@ bool overlaps_itself(const lb_tensor& t) {
     if (!places(t, base, [&](Wide s, Wide count) { step[dims] = s, n[dims++] = count; })) return false;
     for (int d = 0; d < t.rank; d++)
         if (t.shape[d] > 1 && t.stride[d] == 0) return true;
+    // where each dimension's step is beyond all that the smaller ones reach, as in any slice of a dense tensor, there is nothing to solve
+    for (int d = 1; d < dims; d++)
+        for (int k = d; k > 0 && step[k] < step[k - 1]; k--) std::swap(step[k], step[k - 1]), std::swap(n[k], n[k - 1]);
+    Wide reach = dtype_size(t.dtype);
+    bool nested = true;
+    for (int d = 0; d < dims && nested; d++) nested = step[d] >= reach, reach += step[d] * (n[d] - 1);
+    if (nested) return false;
     // two elements differ first in one dimension, the later of them by one or more there, and by anything in those behind it
     for (int first = 0; first < dims; first++) {
         Sum sum;

@@ -226,6 +226,7 @@ class _Torch:
             if not hasattr(torch._C, "_cuda_getCurrentRawStream"):
                 return False
             cls.empty_like, cls.dense, cls.float32, cls.bytes = torch.empty_like, torch.contiguous_format, torch.float32, torch.uint8
+            cls.changed = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
             cls.raw_stream, cls.device, cls.tensor = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, torch.Tensor
         return type(t) is cls.tensor and stream is None and _current[0] == 0 and t.is_cuda
 
@@ -379,6 +380,11 @@ def _results_like(tensors, out, stream):
 def _written(tensors):
     """Tells autograd that the caller's `tensors` have other values now, so that a backward pass that kept one of them raises as it does for torch's
     own in-place operations."""
+    if len(tensors) and type(tensors[0]) is _Torch.tensor:
+        try:
+            return _Torch.changed(tensors)
+        except RuntimeError:  # one of them is another framework's
+            pass
     torch = sys.modules.get("torch")
     known = [t for t in tensors if isinstance(t, torch.Tensor)] if torch else ()
     if known:
