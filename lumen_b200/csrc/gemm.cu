@@ -309,7 +309,8 @@ __device__ __forceinline__ Pair columns(const uint32_t* v, int j) { return both(
 
 // 64 columns of both projections (the gate's at `tbase`, the other's 128 columns further), their gated product, whole 128-byte row pieces each.
 // Rows are 16-byte aligned and N is a multiple of 8 (checked by the host). 16384 x 4096 (twice) x 1024 with all three results 195 us, 1410 TFLOP/s; the plain
-// product of that many FLOPs, with a result of two thirds the size, 187. Packed arithmetic is what brought it from 200.
+// product of that many FLOPs, with a result of two thirds the size, 187. Packed arithmetic is what brought it from 200. It takes 168 registers a
+// thread and spills 20 bytes (44 of loads).
 template <int ACT, bool F16, class Release>
 __device__ __forceinline__ void drain_gated(const GatedArgs& p, uint32_t tbase, int row, int col0, uint4* stage, int lane, Release release) {
     uint4 gate[8], up[8], h[8];
@@ -1301,8 +1302,8 @@ static void launch_pairs(const CUtensorMap& map_a, const CUtensorMap& map_b, con
 
 // Products that do not depend on one another in one launch, the longest K first, where the model of pairs says that they take a tenth less so than one
 // after another: each alone leaves SMs without a tile in its last round, and together they have one last round. Pairs take units in turn. us of the gated
-// block's backward, three launches -> one, bfloat16: 2600 x 840 x 2056 (36 + 68 + 44 tiles on 74 pairs) 95.3 -> 79.5; in a graph 4096 tokens of 512 x 2048 80 -> 69,
-// 8192 of 1024 x 4096 338 -> 319, 8192 of 512 x 2048 110 -> 104; where the model says no: 512 of 1024 x 4096 50.9 -> 65.4, 1024 65.4 -> 74.0, 2048 99 -> 106,
+// block's backward, three launches -> one, bfloat16: 2600 x 840 x 2056 (36 + 68 + 44 tiles on 74 pairs) 95.3 -> 79.5; in a graph 4096 tokens of 512 x 2048 80 -> 71,
+// 8192 of 512 x 2048 110 -> 103; where the model says no: 512 of 1024 x 4096 50.9 -> 65.4, 1024 65.4 -> 74.0, 2048 99 -> 106, 8192 (a fortieth by the model) 338 -> 332,
 // 16384 742 -> 779.
 bool gemm_group_pays(const lb_tensor* a, const lb_tensor* b, int n) {
     const int sms = sm_count_hint(), pairs = sms / 2;

@@ -77,7 +77,8 @@ __device__ __forceinline__ float weight(const RopeSide& q, int i) {
     return !q.w ? 1.0f : q.w_f32 ? ((const float*)q.w)[i] : to_float(((const T*)q.w)[i]);
 }
 
-// Any head dim, strides and alignment: a warp a row, its elements lane by lane; the row waits in shared memory, so that a pair's
+// Any head dim, strides and alignment, for the rows that the kernels below cannot take: right, not fast (32768 tokens x 40 heads x 128, bfloat16, rows that begin on 2
+// bytes: 1490 us forward, 2077 backward, of 103 and 154; it stays for odd head dims, element strides and tables that are not dense). A warp a row, its elements lane by lane; the row waits in shared memory, so that a pair's
 // members find one another and results may go where the operand was.
 constexpr int kRowWarps = 8;
 template <class T, bool BWD>
@@ -372,7 +373,8 @@ __global__ void __launch_bounds__(kGroupThreads, 3) rope_few_kernel(const RopeAr
 // Many rows: a group of lanes takes HEADS heads of a token at a time, which turn by the same angles, and has the next token's (or the next
 // heads') rows on their way into shared memory meanwhile: every thread copies what it reads itself, so that it waits for nobody else. Elements a thread, heads at a
 // time and blocks to an SM, us of that backward / forward: 8, 4, 3 217 / 144; 8, 4, 2 222; 8, 2, 3 243; 8, 2, 4 285; 16, 2, 2 191 / 111; 16, 4, 2 - / 131;
-// 16, 1, 2 - / 144.
+// 16, 1, 2 - / 144. At two blocks to an SM a thread has 128 registers, and the backward's sixteen elements spill 68 bytes (36 of loads); at
+// three, 80 registers, float32's eight spill 12 (16).
 __device__ __forceinline__ void copy_async(void* to, const void* from, int bytes) {
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
     const size_t src = __cvta_generic_to_global(from);

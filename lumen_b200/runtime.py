@@ -483,7 +483,7 @@ def grad_norm(tensors, like=None, stream=None):
 
 def clip_grad_norm(tensors, max_norm, out=None, like=None, stream=None):
     """`grad_norm`, and every tensor times `min(1, max_norm / (norm + 1e-6))`: in place, or into `out`, a list of tensors of the same dtypes and
-    layouts that share no memory with one another or with `tensors`. Returns the norm before clipping (0-d float32, on the device); nothing
-    waits for it. In place, tensors of a norm within the bound are read once and left alone. An infinite or NaN norm makes every tensor 0 or NaN, as
+    layouts that share no memory with one another or with `tensors`. `max_norm` is finite (`grad_norm` is the norm alone). Returns the norm before
+    clipping (0-d float32, on the device); nothing waits for it. In place, tensors of a norm within the bound are read once and left alone. An infinite or NaN norm makes every tensor 0 or NaN, as
     the quotient says."""
     return _norm(tensors, out, float(max_norm), like, stream)
