@@ -403,7 +403,7 @@ def qk_norm_rope(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, e
     (q_out, k_out), handle = _results_like((q, k), out, stream)
     _lib.host().qk_norm_rope(eps, bool(interleaved), q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out, handle)
     if out is not None:
-        _written(out)
+        _written((q_out, k_out))
     return q_out, k_out
 
 
@@ -420,7 +420,7 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, cos, sin, positions=None, q_we
     _lib.host().qk_norm_rope_bwd(eps, bool(interleaved), d_q_out, d_k_out, q, k, cos, sin, positions, q_weight, k_weight, d_q, d_k, d_q_weight, d_k_weight,
                                  _scratch(q, stream), handle)
     if out is not None:
-        _written(out)
+        _written((d_q, d_k))
     return d_q, d_k, d_q_weight, d_k_weight
 
 
@@ -463,6 +463,7 @@ def gated_mlp_backward(d_y, x, w_gate_up, w_down, gate_up, h, activation="silu",
 
 def _norm(tensors, out, max_norm, like, stream):
     require_cuda()
+    tensors, out = (t if t is None or type(t) in (list, tuple) else list(t) for t in (tensors, out))
     if like is None:
         if len(tensors) == 0:
             raise ValueError("the norm of no tensors needs `like`, a tensor on the GPU")

@@ -57,3 +57,26 @@ def test_in_inference_mode(cuda):
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is x
         clip_grad_norm([x, y], 0.5)
         assert abs(float(grad_norm([x, y])) - 0.5) < 1e-4
+
+
+def test_any_collection_of_tensors(cuda):
+    """A dictionary's values, a generator, the rows of a matrix: as a list of them."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x = [torch.randn(n, generator=g, device=cuda) for n in (5, 300, 7)]
+    want = [t.clone() for t in x]
+    norm = clip_grad_norm(want, 1.0)
+    for wrap in (lambda ts: dict(enumerate(ts)).values(), lambda ts: (t for t in ts), tuple):
+        got, out = [t.clone() for t in x], [torch.empty_like(t) for t in x]
+        assert torch.equal(grad_norm(wrap(got)), norm)
+        assert torch.equal(clip_grad_norm(wrap(got), 1.0, out=wrap(out)), norm) and all(torch.equal(a, b) for a, b in zip(out, want))
+        assert torch.equal(clip_grad_norm(wrap(got), 1.0, like=x[0]), norm) and all(torch.equal(a, b) for a, b in zip(got, want))
+    rows = torch.randn(4, 6, generator=g, device=cuda)
+    flat = rows.clone()
+    clip_grad_norm([flat], 0.5)
+    clip_grad_norm(rows, 0.5)
+    assert torch.allclose(rows, flat, rtol=1e-6, atol=0.0)  # sums of other groups
+    q = torch.randn(1, 3, 2, 64, generator=g, device=cuda)
+    cos, sin = torch.ones(3, 32, device=cuda), torch.zeros(3, 32, device=cuda)
+    want = qk_norm_rope(q, q, cos, sin)
+    got = qk_norm_rope(q, q, cos, sin, out=(torch.empty_like(q) for _ in range(2)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
