@@ -7,9 +7,7 @@
 #include <algorithm>
 #include <initializer_list>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+#include "convert.cuh"
 #include "gate.cuh"
 #include "gemm.h"
 #include "launch.cuh"
@@ -22,14 +20,6 @@ bool gemm(const lb_tensor& a, const lb_tensor& b, const lb_tensor& d, int epilog
 namespace {
 
 [[noreturn]] void refuse(const std::string& why) { fail(LB_ERR_INVALID, "gated_mlp: " + why); }
-
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <class T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
 template <class T, int V>
 struct alignas(sizeof(T) * V) Pack {

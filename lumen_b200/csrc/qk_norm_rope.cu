@@ -17,9 +17,7 @@
 // forward 13.6 us, 4.6 TB/s (weights read behind the first rows, in vectors: before that 14.9); 512 tokens x 40 x 128 4.9 us.
 #include <algorithm>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+#include "convert.cuh"
 #include "divide.cuh"
 #include "launch.cuh"
 #include "overlap.h"
@@ -55,14 +53,6 @@ struct RopeArgs {
     float eps;
     Divisor by_seq;
 };
-
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <class T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
 // The row of the tables that a token turns by: its position, clamped into them.
 __device__ __forceinline__ int table_row(const RopeArgs& p, int b, int s) {
