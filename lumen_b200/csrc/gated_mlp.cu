@@ -143,11 +143,17 @@ void sized(const lb_tensor& t, long long rows, long long cols, int dtype, const 
 }
 // What is written shares no memory with what is read, or written.
 void keep_apart(std::initializer_list<const lb_tensor*> results, std::initializer_list<const lb_tensor*> operands) {
-    for (auto r = results.begin(); r != results.end(); ++r) {
+    Extent read[8], written[4];
+    int k = 0, r = 0;
+    for (const lb_tensor* o : operands) read[k++] = extent(*o);
+    for (auto out = results.begin(); out != results.end(); ++out, r++) {
+        written[r] = extent(**out);
+        k = 0;
         for (const lb_tensor* o : operands)
-            if (share_memory(**r, *o)) refuse("a result shares memory with an operand");
-        for (auto other = r + 1; other != results.end(); ++other)
-            if (share_memory(**r, **other)) refuse("two results share memory");
+            if (written[r].meets(read[k++]) && share_memory(**out, *o)) refuse("a result shares memory with an operand");
+        k = 0;
+        for (auto other = results.begin(); other != out; ++other)
+            if (written[r].meets(written[k++]) && share_memory(**out, **other)) refuse("two results share memory");
     }
 }
 
