@@ -193,6 +193,49 @@ int lb_grad_norm(const lb_tensor* tensors, int n_tensors, const lb_tensor* norm,
 int lb_clip_grad_norm(const lb_tensor* tensors, const lb_tensor* outputs, int n_tensors, double max_norm, const lb_tensor* norm, void* scratch,
                       size_t scratch_bytes, void* stream);
 
+/* ---- softmax cross entropy of a projection to a vocabulary ------------------------------------------------------------
+ * z = x W^T for hidden states `x` [.., D] and `weight` [V, D] (any strides that lb_gemm takes; float16, bfloat16 or float32), lse = log sum exp(z) of each
+ * row and loss = lse - z[target], without keeping z. `targets` (int32 or int64, [..]) are clamped into the vocabulary; a row whose target is
+ * `ignore_index` does not count: its loss is 0, whatever stands in its x. `loss` is float32: [..], or one value, the sum or the mean over the
+ * rows that count (0 where none does). `lse` [..] float32 (of every row) is what the backward pass reads. Sums are float32 and more.
+ * Backward: `d_loss` is the gradient of `loss`, float32 of its shape (any even spacing of rows, 0 among them; null: ones); dz = (exp(z - lse) - [target]) g with
+ * each row's share g of it, computed anew for a piece of the vocabulary at a time and rounded to the operands' dtype; d_x = dz W and d_weight = dz^T x, of the
+ * operands' shapes and dtype, row-major, each with one float32 sum and one rounding; rows that do not count have a d_x of 0 and no part in d_weight. Results share
+ * no memory with one another or with an operand; every call repeats bit for bit. Scratch: as many bytes as the _scratch_bytes call on the same tensors
+ * says, 16-byte aligned; calls that may overlap on the GPU need scratch of their own. */
+typedef enum { LB_REDUCTION_NONE = 0, LB_REDUCTION_SUM = 1, LB_REDUCTION_MEAN = 2 } lb_reduction;
+typedef struct {
+    int32_t reduction;
+    int32_t reserved;
+    int64_t ignore_index;
+} lb_loss_desc;
+int lb_linear_cross_entropy_scratch_bytes(const lb_loss_desc* desc, const lb_tensor* x, const lb_tensor* weight, const lb_tensor* targets, size_t* bytes);
+int lb_linear_cross_entropy(const lb_loss_desc* desc, const lb_tensor* x, const lb_tensor* weight, const lb_tensor* targets, const lb_tensor* loss,
+                            const lb_tensor* lse, void* scratch, size_t scratch_bytes, void* stream);
+int lb_linear_cross_entropy_bwd_scratch_bytes(const lb_loss_desc* desc, const lb_tensor* x, const lb_tensor* weight, const lb_tensor* targets,
+                                              const lb_tensor* d_x, const lb_tensor* d_weight, size_t* bytes);
+int lb_linear_cross_entropy_bwd(const lb_loss_desc* desc, const lb_tensor* d_loss /* nullable */, const lb_tensor* x, const lb_tensor* weight,
+                                const lb_tensor* targets, const lb_tensor* lse, const lb_tensor* d_x, const lb_tensor* d_weight, void* scratch,
+                                size_t scratch_bytes, void* stream);
+
+/* ---- AdamW over a list of tensors ------------------------------------------------------------------------------------
+ * For each element, in float32: g' = g c, m = beta1 m + (1 - beta1) g', v = beta2 v + (1 - beta2) g'^2,
+ * w = w (1 - lr decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), rounded once to the parameter's type. With a `norm` (lb_grad_norm's)
+ * c = min(1, max_norm / (norm + 1e-6)), as lb_clip_grad_norm says, else c = 1. Parameters of float16, bfloat16 and float32 in any mix, dense in any order of
+ * their dimensions; gradients of the parameter's type or float32; moments of the parameter's shape and strides: float32, or, with `exp_avg_scale` and
+ * `exp_avg_sq_scale`, uint8: e4m3 codes of m / s and sqrt(v) / s, with a float32 scale s = max / 448 for each 256 elements in the order of memory (dense
+ * [ceil(elements / 256)]); codes and scales of zeros are a first step's moments. `masters` (nullable; an entry with a null ptr: none) are float32 copies of 16-bit
+ * parameters, which the step is then taken on. All but gradients, `step`, `lr` and `norm` are updated in place, and share no memory with anything else
+ * of the call; a gradient may be listed twice. `step`, which counts from 1 (float32, int32 or int64), `lr` and `norm` (float32) are single values on
+ * the device, read when the kernel runs; a null `step` or `lr` means the desc's. The same bits every time; the call takes no scratch. */
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    int64_t step;
+} lb_adamw_desc;
+int lb_adamw_step(const lb_adamw_desc* desc, const lb_tensor* params, const lb_tensor* grads, const lb_tensor* exp_avg, const lb_tensor* exp_avg_sq,
+                  const lb_tensor* exp_avg_scale /* nullable */, const lb_tensor* exp_avg_sq_scale /* nullable */, const lb_tensor* masters /* nullable */,
+                  int n_tensors, const lb_tensor* step /* nullable */, const lb_tensor* lr /* nullable */, const lb_tensor* norm /* nullable */, void* stream);
+
 /* ---- flash attention ----------------------------------------------------------------------------------------
  * Replaces the ATTENTION hook `fn(&Forward{operands, dtype, heads_per_kv, causal, scores, grid, heads}, tensors,
  * &Config)` (lumen/codegen/attention/cuda/mod.rs:33-62) and the Ampere FA-2 forward kernel behind it

@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "dense_lists.h"
 #include "grad_norm.h"
 #include "launch.cuh"
 
@@ -141,17 +142,6 @@ __device__ __forceinline__ double block_sum(double v, double* held) {  // to all
     return v;
 }
 
-// The tensor that chunk `c` lies in: the last whose first chunk is not behind it (an empty tensor has none).
-__device__ __forceinline__ int tensor_of(const NormTable& t, int c) {
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.first[mid] <= c) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
 template <class T, bool KEEP>
 __device__ __forceinline__ double chunk_squares(const T* x, int n) {
     constexpr int per = Of<T>::per;
@@ -268,26 +258,15 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_scale_kernel(cons
 
 [[noreturn]] void refuse(const std::string& why) { fail(LB_ERR_INVALID, "grad_norm: " + why); }
 
-// The number of elements of a tensor that fills its memory without gaps, in any order of its dimensions; refuses others.
-long long dense_elements(const lb_tensor& t, int index) {
+// The number of elements of a tensor of the call; refuses what is not dense.
+long long elements(const lb_tensor& t, int index) {
     if (t.rank < 0 || t.rank > LB_MAX_RANK) refuse(format("tensor %d has rank %d", index, t.rank));
     if (t.dtype != LB_F32 && t.dtype != LB_BF16 && t.dtype != LB_F16) refuse(format("tensor %d is %s: float16, bfloat16 or float32", index, dtype_name(t.dtype)));
-    long long n = 1;
-    for (int d = 0; d < t.rank; d++) {
+    for (int d = 0; d < t.rank; d++)
         if (t.shape[d] < 0) refuse(format("tensor %d has a negative size", index));
-        n *= t.shape[d];
-    }
+    const long long n = dense_elements(t);
     if (n && (!t.ptr || (uintptr_t)t.ptr % dtype_size(t.dtype))) refuse(format("tensor %d has no memory or is not aligned to its elements", index));
-    if (n <= 1) return n;
-    long long step = 1;
-    bool used[LB_MAX_RANK] = {};
-    for (int found = 0; step < n;) {  // the dimension that strides by what is filled so far
-        int next = -1;
-        for (int d = 0; d < t.rank && next < 0; d++)
-            if (!used[d] && t.shape[d] > 1 && t.stride[d] == step) next = d;
-        if (next < 0 || found++ > LB_MAX_RANK) refuse(format("tensor %d is not dense", index));
-        used[next] = true, step *= t.shape[next];
-    }
+    if (n < 0) refuse(format("tensor %d is not dense", index));
     return n;
 }
 
@@ -346,7 +325,7 @@ void run_norm(const lb_tensor* xs, const lb_tensor* outs, int n, double max_norm
         if (norm->shape[d] != 1) refuse("the norm is one float32 value");
     std::vector<long long> count((size_t)n);
     for (int k = 0; k < n; k++) {
-        count[k] = dense_elements(xs[k], k);
+        count[k] = elements(xs[k], k);
         if (count[k] / (kChunkBytes / 4) >= INT32_MAX / kMost) fail(LB_ERR_UNSUPPORTED, format("grad_norm: tensor %d has too many elements", k));
         if (!outs) continue;
         bool same = outs[k].rank == xs[k].rank && outs[k].dtype == xs[k].dtype;

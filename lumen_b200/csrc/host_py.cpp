@@ -392,6 +392,71 @@ PyObject* gated_mlp_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return finish(rc);
 }
 
+// linear_cross_entropy(reduction, ignore_index, x, weight, targets, loss, lse, take, stream)
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 9)) return nullptr;
+    lb_loss_desc d = {(int32_t)PyLong_AsLong(a[0]), 0, PyLong_AsLongLong(a[1])};
+    void* stream = PyLong_AsVoidPtr(a[8]);
+    if (PyErr_Occurred()) return nullptr;
+    lb_tensor t[5];
+    Here here;
+    for (int k = 0; k < 5; k++)
+        if (!describe_here(a[2 + k], &t[k], here)) return nullptr;
+    size_t bytes = 0;
+    int rc = lb_linear_cross_entropy_scratch_bytes(&d, &t[0], &t[1], &t[2], &bytes);
+    if (rc != LB_OK) return finish(rc);
+    Scratch scratch;
+    if (!scratch.get(a[7], bytes)) return nullptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lb_linear_cross_entropy(&d, &t[0], &t[1], &t[2], &t[3], &t[4], scratch.ptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// linear_cross_entropy_bwd(reduction, ignore_index, d_loss or None, x, weight, targets, lse, d_x, d_weight, take, stream)
+PyObject* linear_cross_entropy_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 11)) return nullptr;
+    lb_loss_desc d = {(int32_t)PyLong_AsLong(a[0]), 0, PyLong_AsLongLong(a[1])};
+    void* stream = PyLong_AsVoidPtr(a[10]);
+    if (PyErr_Occurred()) return nullptr;
+    lb_tensor t[7];
+    Here here;
+    for (int k = 0; k < 7; k++)
+        if ((k || a[2] != Py_None) && !describe_here(a[2 + k], &t[k], here)) return nullptr;
+    size_t bytes = 0;
+    int rc = lb_linear_cross_entropy_bwd_scratch_bytes(&d, &t[1], &t[2], &t[3], &t[5], &t[6], &bytes);
+    if (rc != LB_OK) return finish(rc);
+    Scratch scratch;
+    if (!scratch.get(a[9], bytes)) return nullptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lb_linear_cross_entropy_bwd(&d, a[2] == Py_None ? nullptr : &t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], scratch.ptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// The tensors of a sequence; `gaps`: None stands for a tensor that there is not, which has no memory.
+bool describe_all(PyObject* sequence, std::vector<lb_tensor>& out, Here& here, bool gaps) {
+    PyObject* all = PySequence_Fast(sequence, "expected a sequence of tensors");
+    if (!all) return false;
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(all);
+    bool ok = count <= INT32_MAX;
+    if (!ok) PyErr_SetString(PyExc_ValueError, "too many tensors");
+    try {
+        if (ok) out.resize((size_t)count);
+    } catch (const std::bad_alloc&) {
+        Py_DECREF(all);
+        PyErr_NoMemory();
+        return false;
+    }
+    for (Py_ssize_t i = 0; ok && i < count; i++) {
+        PyObject* t = PySequence_Fast_GET_ITEM(all, i);
+        if (gaps && t == Py_None) out[i] = lb_tensor{};
+        else ok = describe_here(t, &out[i], here);
+    }
+    Py_DECREF(all);
+    return ok;
+}
+
 // clip_grad_norm(tensors, outputs or None (in place), max_norm or None (the norm alone), norm, take, stream); sequences of tensors
 PyObject* clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!wants(n, 6)) return nullptr;
@@ -402,23 +467,8 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     std::vector<lb_tensor> t[2];
     lb_tensor norm;
     Here here;
-    for (int k = 0; k < 2; k++) {
-        if (a[k] == Py_None) continue;
-        PyObject* all = PySequence_Fast(a[k], "expected a sequence of tensors");
-        if (!all) return nullptr;
-        const Py_ssize_t count = PySequence_Fast_GET_SIZE(all);
-        bool ok = count <= INT32_MAX;
-        if (!ok) PyErr_SetString(PyExc_ValueError, "too many tensors");
-        try {
-            if (ok) t[k].resize((size_t)count);
-        } catch (const std::bad_alloc&) {
-            Py_DECREF(all);
-            return PyErr_NoMemory();
-        }
-        for (Py_ssize_t i = 0; ok && i < count; i++) ok = describe_here(PySequence_Fast_GET_ITEM(all, i), &t[k][i], here);
-        Py_DECREF(all);
-        if (!ok) return nullptr;
-    }
+    for (int k = 0; k < 2; k++)
+        if (a[k] != Py_None && !describe_all(a[k], t[k], here, false)) return nullptr;
     if (a[1] != Py_None && t[0].size() != t[1].size()) {
         PyErr_Format(PyExc_ValueError, "%zu tensors and %zu results", t[0].size(), t[1].size());
         return nullptr;
@@ -432,6 +482,40 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_BEGIN_ALLOW_THREADS
     rc = clips ? lb_clip_grad_norm(t[0].data(), a[1] == Py_None ? t[0].data() : t[1].data(), count, most, &norm, scratch.ptr, bytes, stream)
                : lb_grad_norm(t[0].data(), count, &norm, scratch.ptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return finish(rc);
+}
+
+// adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, masters (these three: sequences or None), step, lr (numbers or tensors),
+//            beta1, beta2, eps, weight_decay, norm or None, max_norm, stream)
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!wants(n, 16)) return nullptr;
+    lb_adamw_desc d = {};
+    const bool counted = PyLong_Check(a[7]), fixed = PyFloat_Check(a[8]) || PyLong_Check(a[8]);
+    if (counted) d.step = PyLong_AsLongLong(a[7]);
+    if (fixed) d.lr = PyFloat_AsDouble(a[8]);
+    d.beta1 = PyFloat_AsDouble(a[9]), d.beta2 = PyFloat_AsDouble(a[10]), d.eps = PyFloat_AsDouble(a[11]), d.weight_decay = PyFloat_AsDouble(a[12]);
+    d.max_norm = a[13] == Py_None ? 0.0 : PyFloat_AsDouble(a[14]);
+    void* stream = PyLong_AsVoidPtr(a[15]);
+    if (PyErr_Occurred()) return nullptr;
+    std::vector<lb_tensor> t[7];
+    Here here;
+    for (int k = 0; k < 7; k++) {
+        if (k >= 4 && a[k] == Py_None) continue;
+        if (!describe_all(a[k], t[k], here, k == 6)) return nullptr;
+        if (t[k].size() != t[0].size()) {
+            static const char* const what[] = {"", "gradients", "first moments", "second moments", "scales of first moments", "scales of second moments", "float32 copies"};
+            PyErr_Format(PyExc_ValueError, "%zu parameters and %zu %s", t[0].size(), t[k].size(), what[k]);
+            return nullptr;
+        }
+    }
+    lb_tensor step, lr, norm;
+    if ((!counted && !describe_here(a[7], &step, here)) || (!fixed && !describe_here(a[8], &lr, here)) || (a[13] != Py_None && !describe_here(a[13], &norm, here))) return nullptr;
+    auto list = [&](int k) { return a[k] == Py_None ? nullptr : t[k].data(); };
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lb_adamw_step(&d, t[0].data(), t[1].data(), t[2].data(), t[3].data(), list(4), list(5), list(6), (int)t[0].size(), counted ? nullptr : &step,
+                       fixed ? nullptr : &lr, a[13] == Py_None ? nullptr : &norm, stream);
     Py_END_ALLOW_THREADS
     return finish(rc);
 }
@@ -699,6 +783,9 @@ PyMethodDef methods[] = {
     {"qk_norm_rope_bwd", (PyCFunction)(void (*)(void))qk_norm_rope_bwd, METH_FASTCALL, "lb_qk_norm_rope_bwd on tensors"},
     {"gated_mlp_fwd", (PyCFunction)(void (*)(void))gated_mlp_fwd, METH_FASTCALL, "lb_gated_mlp_fwd on tensors"},
     {"gated_mlp_bwd", (PyCFunction)(void (*)(void))gated_mlp_bwd, METH_FASTCALL, "lb_gated_mlp_bwd on tensors"},
+    {"linear_cross_entropy", (PyCFunction)(void (*)(void))linear_cross_entropy, METH_FASTCALL, "lb_linear_cross_entropy on tensors"},
+    {"linear_cross_entropy_bwd", (PyCFunction)(void (*)(void))linear_cross_entropy_bwd, METH_FASTCALL, "lb_linear_cross_entropy_bwd on tensors"},
+    {"adamw_step", (PyCFunction)(void (*)(void))adamw_step, METH_FASTCALL, "lb_adamw_step on sequences of tensors"},
     {"clip_grad_norm", (PyCFunction)(void (*)(void))clip_grad_norm, METH_FASTCALL, "lb_grad_norm / lb_clip_grad_norm on sequences of tensors"},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1,0 +1,498 @@
+// Softmax cross entropy of a projection to a vocabulary, straight from hidden states x [T, D] and weights W [V, D]: z = x W^T,
+// lse_t = log sum_v exp(z_tv), loss_t = lse_t - z_t,target(t); backward with g_t the gradient of loss_t: dz_tv = (exp(z_tv - lse_t) - [v = target(t)]) g_t,
+// dx = dz W, dW = dz^T x. Rows that do not count have loss and dz of zero. The logits are never kept: forward, each span of the vocabulary leaves
+// its largest logit and the sum of exponentials below it, and what follows joins the spans' pairs; backward, they are computed anew for one piece of
+// the vocabulary at a time, whose dz (rounded to the operands' type, as an operand of the tensor cores has to be) is what the two products read.
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+
+#include "convert.cuh"
+#include "gemm.h"
+#include "launch.cuh"
+#include "linear_loss.h"
+#include "overlap.h"
+
+namespace lb {
+bool gemm(const lb_tensor& a, const lb_tensor& b, const lb_tensor& d, int epilogue, int kernel_choice, void* stream, void* scratch, size_t scratch_bytes,
+          const lb_tensor* aux, const GemmTuning* tuning, SimtProblem* held = nullptr);
+
+namespace {
+
+[[noreturn]] void refuse(const std::string& why) { fail(LB_ERR_INVALID, "linear_cross_entropy: " + why); }
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+
+constexpr int kRowThreads = 128;
+
+// Sums over the threads of a block, to all of them.
+__device__ __forceinline__ SpanSum block_join(SpanSum v, SpanSum* held) {
+    for (int d = 16; d; d >>= 1) v = join(v, SpanSum{__shfl_xor_sync(0xffffffffu, v.most, d), __shfl_xor_sync(0xffffffffu, v.sum, d)});
+    if ((threadIdx.x & 31) == 0) held[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = held[0];
+    for (int k = 1; k < (int)blockDim.x / 32; k++) v = join(v, held[k]);
+    __syncthreads();
+    return v;
+}
+
+// The span sums of logits that lie in memory, float32 [rows, cols], columns `first` and on of the vocabulary; and the target's logit where it is among them.
+__global__ void __launch_bounds__(kRowThreads) span_kernel(const float* logits, long long ld, long long rows, int first, int cols, Targets targets, SpanSum* spans, float* hit) {
+    __shared__ SpanSum held[kRowThreads / 32];
+    grid_wait();
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float* z = logits + row * ld;
+        SpanSum v{-INFINITY, 0.0f};
+        for (int c = threadIdx.x; c < cols; c += kRowThreads) v = join(v, SpanSum{z[c], 1.0f});
+        v = block_join(v, held);
+        if (threadIdx.x == 0) {
+            spans[row] = v;
+            const int target = targets.of(row) - first;
+            if (target >= 0 && target < cols) hit[row] = z[target];
+        }
+    }
+}
+
+// What a block of rows adds to the loss.
+struct LossSum {
+    double sum;
+    long long counted;
+};
+__device__ __forceinline__ LossSum block_sum(LossSum v, LossSum* held) {
+    for (int d = 16; d; d >>= 1) v.sum += __shfl_xor_sync(0xffffffffu, v.sum, d), v.counted += __shfl_xor_sync(0xffffffffu, v.counted, d);
+    if ((threadIdx.x & 31) == 0) held[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = held[0];
+    for (int k = 1; k < (int)blockDim.x / 32; k++) v.sum += held[k].sum, v.counted += held[k].counted;
+    __syncthreads();
+    return v;
+}
+
+// Joins the spans of each row ([span][row]), R rows a block and 256 / R threads a row, in an order of their own: the same bits every time.
+template <int R>
+__global__ void __launch_bounds__(256) rows_kernel(const SpanSum* spans, int n_spans, long long rows, const float* hit, Targets targets, float* lse, float* losses, LossSum* sums) {
+    __shared__ SpanSum held[256];
+    __shared__ LossSum total[8];
+    grid_wait();
+    constexpr int G = 256 / R;
+    const int r = threadIdx.x % R, group = threadIdx.x / R;
+    const long long row = (long long)blockIdx.x * R + r;
+    SpanSum v{-INFINITY, 0.0f};
+    if (row < rows)
+        for (int k = group; k < n_spans; k += G) v = join(v, spans[k * rows + row]);
+    held[threadIdx.x] = v;
+    for (int half = G / 2; half; half /= 2) {
+        __syncthreads();
+        if (group < half) held[threadIdx.x] = join(held[threadIdx.x], held[threadIdx.x + half * R]);
+    }
+    LossSum mine{0.0, 0};
+    if (group == 0 && row < rows) {
+        v = held[threadIdx.x];
+        const float all = v.most + logf(v.sum);
+        lse[row] = all;
+        const bool counts = targets.of(row) >= 0;
+        const float loss = counts ? all - hit[row] : 0.0f;
+        if (losses) losses[row] = loss;
+        mine = {loss, counts};
+    }
+    if (!sums) return;
+    mine = block_sum(mine, total);
+    if (threadIdx.x == 0) sums[blockIdx.x] = mine;
+}
+__global__ void __launch_bounds__(256) loss_kernel(const LossSum* sums, long long n, bool mean, float* loss) {
+    __shared__ LossSum total[8];
+    grid_wait();
+    LossSum v{0.0, 0};
+    for (long long k = threadIdx.x; k < n; k += 256) v.sum += sums[k].sum, v.counted += sums[k].counted;
+    v = block_sum(v, total);
+    if (threadIdx.x == 0) *loss = (float)(mean ? v.sum / (double)max(v.counted, 1LL) : v.sum);
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------
+
+// Rows that count, and the largest |d_loss| of them.
+struct RowCount {
+    long long counted;
+    float most;
+};
+__device__ __forceinline__ RowCount block_count(RowCount v, RowCount* held) {
+    for (int d = 16; d; d >>= 1) v.counted += __shfl_xor_sync(0xffffffffu, v.counted, d), v.most = fmaxf(v.most, __shfl_xor_sync(0xffffffffu, v.most, d));
+    if ((threadIdx.x & 31) == 0) held[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = held[0];
+    for (int k = 1; k < (int)blockDim.x / 32; k++) v.counted += held[k].counted, v.most = fmaxf(v.most, held[k].most);
+    __syncthreads();
+    return v;
+}
+struct LossGrad {
+    const float* at;  // null: one
+    long long step;
+    __device__ __forceinline__ float of(long long row) const { return at ? at[row * step] : 1.0f; }
+};
+__global__ void __launch_bounds__(256) count_kernel(Targets targets, LossGrad grad, long long rows, RowCount* counts) {
+    __shared__ RowCount held[8];
+    grid_wait();
+    RowCount v{0, 0.0f};
+    for (long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < rows; row += (long long)gridDim.x * 256)
+        if (targets.of(row) >= 0) v.counted++, v.most = fmaxf(v.most, fabsf(grad.of(row)));
+    v = block_count(v, held);
+    if (threadIdx.x == 0) counts[blockIdx.x] = v;
+}
+
+// Of each row: the gradient of its logits' scale g (zero where it does not count), its class, and a copy of x whose rows that do not count are zero, so that
+// what stands there (padding may hold infinities or NaN) does not get into dW. float16: g times a power of two that puts the largest near 2^13, since most
+// of dz is far below float16's smallest values; `undo` is what takes it away again.
+template <class T>
+__global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGrad grad, long long rows, const RowCount* counts, int n_counts, bool mean, const T* x, long long ld_x,
+                                                        long long x_col, int D, T* x_out, float* g, int* classes, float* undo) {
+    __shared__ RowCount held[8];
+    grid_wait();
+    RowCount all{0, 0.0f};
+    for (int k = threadIdx.x; k < n_counts; k += 256) all.counted += counts[k].counted, all.most = fmaxf(all.most, counts[k].most);
+    all = block_count(all, held);
+    const float counted = mean ? (float)max(all.counted, 1LL) : 1.0f;
+    float scale = 1.0f;
+    if (sizeof(T) == 2 && undo && all.most > 0.0f && all.most < INFINITY) scale = exp2f((float)max(-120, min(120, 13 - ilogbf(all.most / counted))));
+    if (undo && blockIdx.x == 0 && threadIdx.x == 0) *undo = 1.0f / scale;
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int target = targets.of(row);
+        if (threadIdx.x == 0) g[row] = target < 0 ? 0.0f : grad.of(row) / counted * scale, classes[row] = target;
+        for (int c = threadIdx.x; c < D; c += 256) x_out[row * D + c] = target < 0 ? from_float<T>(0.0f) : x[row * ld_x + c * x_col];
+    }
+}
+
+// dz of logits that lie in memory; may take their place.
+template <class T>
+__global__ void __launch_bounds__(kRowThreads) slope_kernel(const float* logits, long long ld, long long rows, int first, int cols, const float* lse, long long lse_step,
+                                                            const float* g, const int* classes, T* out, long long ld_out) {
+    grid_wait();
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float all = lse[row * lse_step], scale = g[row];
+        const int at = classes[row], target = at - first;
+        for (int c = threadIdx.x; c < cols; c += kRowThreads)
+            out[row * ld_out + c] = from_float<T>(at < 0 ? 0.0f : (expf(logits[row * ld + c] - all) - (c == target ? 1.0f : 0.0f)) * scale);
+    }
+}
+
+// sum = (first piece: 0, else sum) + product; the last piece's is rounded into `out` instead, times `undo` where there is one.
+template <class T>
+__global__ void __launch_bounds__(256) fold_kernel(const float* product, long long rows, int D, float* sum, bool begins, T* out, long long ld_out, const float* undo) {
+    grid_wait();
+    const float scale = undo ? *undo : 1.0f;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * D; i += (long long)gridDim.x * 256) {
+        const float v = begins ? product[i] : sum[i] + product[i];
+        if (out) out[i / D * ld_out + i % D] = from_float<T>(v * scale);
+        else sum[i] = v;
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+lb_tensor matrix(void* ptr, int dtype, long long rows, long long cols, long long ld) {
+    lb_tensor t{};
+    t.ptr = ptr, t.dtype = dtype, t.rank = 2, t.shape[0] = rows, t.shape[1] = cols, t.stride[0] = ld, t.stride[1] = 1;
+    return t;
+}
+lb_tensor transposed(const lb_tensor& t) {
+    lb_tensor u = t;
+    std::swap(u.shape[0], u.shape[1]), std::swap(u.stride[0], u.stride[1]);
+    return u;
+}
+// The dimensions of a tensor but the last `keep` as one, which have to be evenly spaced: [rows, last] or [rows].
+lb_tensor as_rows(const lb_tensor* t, int keep, const char* what) {
+    if (!t) refuse(format("%s is missing", what));
+    if (t->rank < keep || t->rank > LB_MAX_RANK) refuse(format("%s must have rank %d or more", what, keep));
+    for (int d = 0; d < t->rank; d++)
+        if (t->shape[d] < 0) refuse(format("%s has a negative size", what));
+    const int lead = t->rank - keep;
+    long long rows = 1, step = 0;
+    for (int d = 0; d < lead; d++)
+        if (t->shape[d] == 0) rows = 0;  // no rows: nothing about their spacing
+    for (int d = lead - 1; d >= 0 && rows; d--) {
+        if (t->shape[d] == 1) continue;
+        if (rows != 1 && t->stride[d] != step * rows) fail(LB_ERR_UNSUPPORTED, format("linear_cross_entropy: the rows of %s are not evenly spaced", what));
+        if (rows == 1) step = t->stride[d];
+        rows *= t->shape[d];
+    }
+    lb_tensor m{};
+    m.ptr = t->ptr, m.dtype = t->dtype, m.rank = 1 + keep, m.shape[0] = rows, m.stride[0] = step;
+    if (keep) {
+        m.shape[1] = t->shape[lead], m.stride[1] = t->stride[lead];
+        if (rows <= 1) m.stride[0] = m.stride[1] == 1 ? m.shape[1] : 1;
+    }
+    return m;
+}
+void in_memory(const lb_tensor& t, const char* what) {
+    long long n = 1;
+    for (int d = 0; d < t.rank; d++) n *= t.shape[d];
+    if (n && (!t.ptr || (uintptr_t)t.ptr % dtype_size(t.dtype))) refuse(format("%s has no memory or is not aligned to its elements", what));
+}
+void written(const lb_tensor& t, const char* what) {
+    if (t.shape[1] > 1 && t.stride[1] != 1) fail(LB_ERR_UNSUPPORTED, format("linear_cross_entropy: %s must be row-major", what));
+    if (t.shape[0] > 1 && t.stride[0] < t.shape[1]) refuse(format("the rows of %s overlap", what));
+}
+// What is written shares no memory with what is read, or written.
+void keep_apart(std::initializer_list<const lb_tensor*> results, std::initializer_list<const lb_tensor*> operands) {
+    for (auto out = results.begin(); out != results.end(); ++out) {
+        for (const lb_tensor* o : operands)
+            if (share_memory(**out, *o)) refuse("a result shares memory with an operand");
+        for (auto other = results.begin(); other != out; ++other)
+            if (share_memory(**out, **other)) refuse("two results share memory");
+    }
+}
+
+size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
+long long up(long long n, long long to) { return (n + to - 1) / to * to; }
+
+constexpr long long kPieceBytes = 256LL << 20;  // of a piece's logits or their gradients
+
+struct Loss {
+    int reduction, dtype;
+    long long T, D, V;
+    lb_tensor x, w, t;
+    Targets targets;
+    char* scratch = nullptr;
+    size_t held = 0;  // bytes of scratch given out
+
+    Loss(const lb_loss_desc* desc, const lb_tensor* x_t, const lb_tensor* w_t, const lb_tensor* targets_t) {
+        if (!desc) refuse("null argument");
+        reduction = desc->reduction;
+        if (reduction < LB_REDUCTION_NONE || reduction > LB_REDUCTION_MEAN) refuse("unknown reduction");
+        x = as_rows(x_t, 1, "x");
+        if (!w_t || w_t->rank != 2) refuse("the weights must be [classes, width]");
+        w = as_rows(w_t, 1, "weight"), t = as_rows(targets_t, 0, "targets");
+        dtype = x.dtype;
+        if (dtype != LB_F32 && dtype != LB_BF16 && dtype != LB_F16) refuse("float16, bfloat16 or float32 operands");
+        T = x.shape[0], D = x.shape[1], V = w.shape[0];
+        if (w.dtype != dtype || w.shape[1] != D) refuse(format("weight must be [classes, %lld] of x's dtype, got %s[%lld, %lld]", D, dtype_name(w.dtype), V, (long long)w.shape[1]));
+        if (targets_t->rank != x_t->rank - 1) refuse("targets must have the shape of x without its last dimension");
+        for (int d = 0; d < targets_t->rank; d++)
+            if (targets_t->shape[d] != x_t->shape[d]) refuse("targets must have the shape of x without its last dimension");
+        if (t.dtype != LB_I32 && t.dtype != LB_I64) refuse("targets must be int32 or int64");
+        if (D < 1 || V < 1) refuse("a width or vocabulary of zero");
+        if (T > INT32_MAX || D > INT32_MAX || V > INT32_MAX) fail(LB_ERR_UNSUPPORTED, "linear_cross_entropy: sizes of at most 2^31 - 1");
+        in_memory(x, "x"), in_memory(w, "weight"), in_memory(t, "targets");
+        targets = {t.ptr, t.stride[0], desc->ignore_index, t.dtype == LB_I64, (int)V};
+    }
+    template <class U>
+    U* take(size_t count) {  // memory of the call's scratch; counted alone where there is none
+        U* at = (U*)(scratch + held);
+        held += up(count * sizeof(U));
+        return scratch ? at : nullptr;
+    }
+    // A row value of each row: float32, [rows] in any even spacing.
+    lb_tensor row_values(const lb_tensor* v, const lb_tensor* like, const char* what) const {
+        lb_tensor r = as_rows(v, 0, what);
+        if (r.dtype != LB_F32 || v->rank != like->rank) refuse(format("%s must be float32 of the targets' shape", what));
+        for (int d = 0; d < v->rank; d++)
+            if (v->shape[d] != like->shape[d]) refuse(format("%s must be float32 of the targets' shape", what));
+        in_memory(r, what);
+        return r;
+    }
+    // The vocabulary in pieces whose [T, piece] of `item` bytes an element takes about kPieceBytes.
+    long long piece_of(int item) const {
+        const long long most = std::max(256LL, kPieceBytes / item / std::max(1LL, T) / 256 * 256);
+        return std::min(V, most);
+    }
+};
+
+size_t product_scratch(const lb_tensor& a, const lb_tensor& b) { return lb_gemm_operands_scratch_bytes(&a, &b); }
+lb_tensor rows_of(const lb_tensor& m, long long first, long long count) {
+    lb_tensor r = m;
+    r.ptr = (char*)m.ptr + first * m.stride[0] * dtype_size(m.dtype), r.shape[0] = count;
+    return r;
+}
+template <class F>
+void by_type(int dtype, F f) {
+    if (dtype == LB_F32) f((float*)nullptr);
+    else if (dtype == LB_BF16) f((__nv_bfloat16*)nullptr);
+    else f((__half*)nullptr);
+}
+unsigned row_blocks(long long rows) { return (unsigned)std::min<long long>(std::max(1LL, rows), (long long)sm_count_hint() * 16); }
+
+struct Forward : Loss {
+    using Loss::Loss;
+    lb_tensor loss, lse;
+
+    void results(const lb_tensor* loss_t, const lb_tensor* lse_t, const lb_tensor* targets_t) {
+        lse = row_values(lse_t, targets_t, "lse");
+        if (T > 1 && lse.stride[0] != 1) refuse("lse must be dense");
+        if (reduction == LB_REDUCTION_NONE) {
+            loss = row_values(loss_t, targets_t, "loss");
+            if (T > 1 && loss.stride[0] != 1) refuse("loss must be dense");
+            return;
+        }
+        loss = as_rows(loss_t, 0, "loss");
+        if (loss.dtype != LB_F32 || loss.shape[0] != 1) refuse("the loss is one float32 value");
+        in_memory(loss, "loss");
+    }
+    void run(cudaStream_t s, bool only_count) {
+        held = 0;
+        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece;
+        const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
+        const long long blocks = (T + R - 1) / R;
+        SpanSum* spans = take<SpanSum>(pieces * T);
+        float* hit = take<float>(T);
+        LossSum* sums = reduction == LB_REDUCTION_NONE ? nullptr : take<LossSum>(blocks);
+        const long long ld = up(piece, 8);
+        float* logits = take<float>(T * ld);
+        const lb_tensor z = matrix(logits, LB_F32, T, piece, ld);
+        const size_t more = T ? product_scratch(x, transposed(rows_of(w, 0, piece))) : 0;
+        void* product = take<char>(more);
+        if (only_count) return;
+        if (T) {
+            for (long long k = 0; k < pieces; k++) {
+                const long long first = k * piece, cols = std::min(piece, V - first);
+                lb_tensor out = z;
+                out.shape[1] = cols;
+                gemm(x, transposed(rows_of(w, first, cols)), out, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+                launch_overlapped(span_kernel, dim3(row_blocks(T)), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, targets, spans + k * T, hit);
+            }
+            auto join_rows = [&](auto kernel) {
+                launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, s, 0, (const SpanSum*)spans, (int)pieces, T, (const float*)hit, targets, (float*)lse.ptr,
+                                  sums ? nullptr : (float*)loss.ptr, sums);
+            };
+            R == 32 ? join_rows(rows_kernel<32>) : R == 8 ? join_rows(rows_kernel<8>) : join_rows(rows_kernel<1>);
+        }
+        if (sums || reduction != LB_REDUCTION_NONE)
+            launch_overlapped(loss_kernel, dim3(1), dim3(256), 0, s, 0, (const LossSum*)sums, T ? blocks : 0LL, reduction == LB_REDUCTION_MEAN, (float*)loss.ptr);
+    }
+};
+
+struct Backward : Loss {
+    using Loss::Loss;
+    lb_tensor grad{}, lse, dx, dw;
+
+    void results(const lb_tensor* dx_t, const lb_tensor* dw_t) {
+        dx = as_rows(dx_t, 1, "d_x"), dw = as_rows(dw_t, 1, "d_weight");
+        if (dx.dtype != dtype || dx.shape[0] != T || dx.shape[1] != D) refuse("d_x must have the shape and dtype of x");
+        if (dw.dtype != dtype || dw_t->rank != 2 || dw.shape[0] != V || dw.shape[1] != D) refuse("d_weight must have the shape and dtype of the weights");
+        in_memory(dx, "d_x"), in_memory(dw, "d_weight"), written(dx, "d_x"), written(dw, "d_weight");
+    }
+    void operands(const lb_tensor* grad_t, const lb_tensor* lse_t, const lb_tensor* targets_t) {
+        lse = row_values(lse_t, targets_t, "lse");
+        if (!grad_t) return;
+        if (reduction == LB_REDUCTION_NONE) {
+            grad = row_values(grad_t, targets_t, "d_loss");
+            return;
+        }
+        grad = as_rows(grad_t, 0, "d_loss");
+        if (grad.dtype != LB_F32 || grad.shape[0] != 1) refuse("the gradient of the loss is one float32 value");
+        grad.stride[0] = 0;
+        in_memory(grad, "d_loss");
+    }
+    void run(cudaStream_t s, bool only_count) {
+        held = 0;
+        const int item = dtype_size(dtype);
+        const bool half = dtype == LB_F16;
+        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, ld = up(piece, 8);
+        const int n_counts = (int)std::min<long long>(64, (T + 255) / 256);
+        RowCount* counts = take<RowCount>(n_counts);
+        float *g = take<float>(T), *undo = take<float>(1);
+        int* classes = take<int>(T);
+        char* x_kept = take<char>(T * D * item);
+        float* logits = take<float>(T * ld);
+        char* slopes = dtype == LB_F32 ? (char*)logits : take<char>(T * ld * item);
+        const bool folds = pieces > 1 || half;
+        float *dx_piece = folds ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr, *dw_piece = half ? take<float>(piece * D) : nullptr;
+        const lb_tensor kept = matrix(x_kept, dtype, T, D, D), dz = matrix(slopes, dtype, T, piece, ld);
+        size_t more = 0;
+        if (T) more = std::max({product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
+        void* product = take<char>(more);
+        if (only_count) return;
+        if (T == 0) {
+            LB_CUDA(cudaMemset2DAsync(dw.ptr, (size_t)(V > 1 ? dw.stride[0] : D) * item, 0, (size_t)D * item, (size_t)V, s));
+            return;
+        }
+        const LossGrad d_loss{(const float*)grad.ptr, grad.stride[0]};
+        launch_overlapped(count_kernel, dim3((unsigned)n_counts), dim3(256), 0, s, 0, targets, d_loss, T, counts);
+        by_type(dtype, [&](auto* type) {
+            using E = std::remove_pointer_t<decltype(type)>;
+            launch_overlapped(row_grads_kernel<E>, dim3(row_blocks(T)), dim3(256), 0, s, 0, targets, d_loss, T, (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
+                              (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], (int)D, (E*)x_kept, g, classes, half ? undo : nullptr);
+        });
+        for (long long k = 0; k < pieces; k++) {
+            const long long first = k * piece, cols = std::min(piece, V - first);
+            const lb_tensor rows = rows_of(w, first, cols);
+            lb_tensor z = matrix(logits, LB_F32, T, cols, ld), d = dz, dw_rows = rows_of(dw, first, cols);
+            d.shape[1] = cols;
+            gemm(x, transposed(rows), z, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+            by_type(dtype, [&](auto* type) {
+                using E = std::remove_pointer_t<decltype(type)>;
+                launch_overlapped(slope_kernel<E>, dim3(row_blocks(T)), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, (const float*)lse.ptr,
+                                  (long long)lse.stride[0], (const float*)g, (const int*)classes, (E*)slopes, ld);
+            });
+            auto fold = [&](const float* from, const lb_tensor& to, float* sum, bool begins, bool ends) {
+                by_type(dtype, [&](auto* type) {
+                    using E = std::remove_pointer_t<decltype(type)>;
+                    const long long n = to.shape[0] * D;
+                    launch_overlapped(fold_kernel<E>, dim3((unsigned)std::min<long long>((n + 255) / 256, device_info().sms * 8LL)), dim3(256), 0, s, 0, from, (long long)to.shape[0], (int)D,
+                                      sum, begins, ends ? (E*)to.ptr : (E*)nullptr, (long long)to.stride[0], half ? (const float*)undo : (const float*)nullptr);
+                });
+            };
+            const lb_tensor dw_out = half ? matrix(dw_piece, LB_F32, cols, D, D) : dw_rows;
+            gemm(transposed(d), kept, dw_out, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+            if (half) fold(dw_piece, dw_rows, nullptr, true, true);
+            gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+            if (folds) fold(dx_piece, dx, dx_sum, k == 0, k == pieces - 1);
+        }
+    }
+};
+
+void give_scratch(Loss& l, size_t need, void* scratch, size_t bytes) {
+    if (need && (!scratch || bytes < need || (uintptr_t)scratch % 16)) refuse(format("%zu bytes of scratch are needed, 16-byte aligned", need));
+    l.scratch = (char*)scratch;
+}
+
+}  // namespace
+}  // namespace lb
+
+extern "C" {
+
+int lb_linear_cross_entropy_scratch_bytes(const lb_loss_desc* desc, const lb_tensor* x, const lb_tensor* weight, const lb_tensor* targets, size_t* bytes) {
+    return lb::guarded([&] {
+        if (!bytes) lb::refuse("null argument");
+        lb::Forward f(desc, x, weight, targets);
+        f.run(nullptr, true);
+        *bytes = f.held;
+    });
+}
+
+int lb_linear_cross_entropy(const lb_loss_desc* desc, const lb_tensor* x, const lb_tensor* weight, const lb_tensor* targets, const lb_tensor* loss, const lb_tensor* lse,
+                            void* scratch, size_t scratch_bytes, void* stream) {
+    return lb::guarded([&] {
+        lb::Forward f(desc, x, weight, targets);
+        f.results(loss, lse, targets);
+        lb::keep_apart({&f.loss, &f.lse}, {&f.x, &f.w, &f.t});
+        f.run(nullptr, true);
+        lb::give_scratch(f, f.held, scratch, scratch_bytes);
+        lb::driver();
+        f.run((cudaStream_t)stream, false);
+    });
+}
+
+int lb_linear_cross_entropy_bwd_scratch_bytes(const lb_loss_desc* desc, const lb_tensor* x, const lb_tensor* weight, const lb_tensor* targets, const lb_tensor* d_x,
+                                              const lb_tensor* d_weight, size_t* bytes) {
+    return lb::guarded([&] {
+        if (!bytes) lb::refuse("null argument");
+        lb::Backward b(desc, x, weight, targets);
+        b.results(d_x, d_weight);
+        b.run(nullptr, true);
+        *bytes = b.held;
+    });
+}
+
+int lb_linear_cross_entropy_bwd(const lb_loss_desc* desc, const lb_tensor* d_loss, const lb_tensor* x, const lb_tensor* weight, const lb_tensor* targets, const lb_tensor* lse,
+                                const lb_tensor* d_x, const lb_tensor* d_weight, void* scratch, size_t scratch_bytes, void* stream) {
+    return lb::guarded([&] {
+        lb::Backward b(desc, x, weight, targets);
+        b.results(d_x, d_weight), b.operands(d_loss, lse, targets);
+        const lb_tensor& g = d_loss ? b.grad : b.lse;
+        lb::keep_apart({&b.dx, &b.dw}, {&b.x, &b.w, &b.t, &b.lse, &g});
+        b.run(nullptr, true);
+        lb::give_scratch(b, b.held, scratch, scratch_bytes);
+        lb::driver();
+        b.run((cudaStream_t)stream, false);
+    });
+}
+}

@@ -488,3 +488,98 @@ def clip_grad_norm(tensors, max_norm, out=None, like=None, stream=None):
     clipping (0-d float32, on the device); nothing waits for it. In place, tensors of a norm within the bound are read once and left alone. An infinite or NaN norm makes every tensor 0 or NaN, as
     the quotient says."""
     return _norm(tensors, out, float(max_norm), like, stream)
+
+
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _reduction(name) -> int:
+    if name not in REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(REDUCTIONS)}, got {name!r}")
+    return REDUCTIONS[name]
+
+
+def linear_cross_entropy(x, weight, targets, reduction="mean", ignore_index=-100, stream=None):
+    """Softmax cross entropy of the projection `x @ weight^T` through `lb_linear_cross_entropy`, without the logits ever being in memory as a whole: `x`
+    `[.., D]` (hidden states), `weight` `[V, D]` (an output head), `targets` `[..]` int32 or int64. Returns `(loss, lse)`: the loss of each row, or its
+    sum or mean over the rows that count (0 where none does), and each row's log-sum-exp, which the backward pass reads; both float32. A row whose target
+    is `ignore_index` does not count; other targets are clamped into the vocabulary. float16, bfloat16 or float32. Bit-identical from call to call; the
+    same rows among others may differ by a rounding."""
+    require_cuda()
+    code, shape = _reduction(reduction), tuple(targets.shape)
+    (loss, lse), handle = _outputs(x, stream, (() if code else shape, "float32"), (shape, "float32"))
+    _lib.host().linear_cross_entropy(code, ignore_index, x, weight, targets, loss, lse, _scratch(x, stream), handle)
+    return loss, lse
+
+
+def linear_cross_entropy_backward(d_loss, x, weight, targets, lse, reduction="mean", ignore_index=-100, stream=None):
+    """The backward pass of `linear_cross_entropy` on the same operands, through `lb_linear_cross_entropy_bwd`: returns `(d_x, d_weight)` of the
+    operands' shapes and dtype. `d_loss` is the gradient of the loss, float32 of its shape (None: ones). The logits are computed anew, a piece of the
+    vocabulary at a time. Rows that do not count have a gradient of zero and no part in `d_weight`, whatever stands in them. Bit-identical from call to
+    call."""
+    require_cuda()
+    code = _reduction(reduction)
+    (d_x, d_weight), handle = _results_like((x, weight), None, stream)
+    _lib.host().linear_cross_entropy_bwd(code, ignore_index, d_loss, x, weight, targets, lse, d_x, d_weight, _scratch(x, stream), handle)
+    return d_x, d_weight
+
+
+ADAMW_BLOCK = 256  # elements that share a scale where moments are held in 8 bits
+
+
+def adamw_state(params, bits=32):
+    """The moments of a first `adamw_step` on `params`: `(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale)`, lists of zeros. With `bits=32` the
+    moments are float32 tensors shaped like the parameters and there are no scales (None); with `bits=8` they are uint8 tensors of e4m3 codes, with a
+    float32 scale for each 256 elements."""
+    if bits not in (8, 32):
+        raise ValueError(f"bits must be 8 or 32, got {bits!r}")
+    params = list(params)
+
+    def zeros(dtype, shape=None):
+        return [_zeros_like_input(t, None if shape is None else shape(t), dtype) for t in params]
+
+    if bits == 32:
+        return zeros("float32"), zeros("float32"), None, None
+
+    def blocks(t):
+        return (-(-math.prod(t.shape) // ADAMW_BLOCK),)
+
+    return zeros("uint8"), zeros("uint8"), zeros("float32", blocks), zeros("float32", blocks)
+
+
+def _zeros_like_input(like, shape, dtype: str):
+    """Zeros in the framework `like` comes from, of its shape and layout unless `shape` is given."""
+    if type(like).__module__.startswith("torch"):
+        torch = sys.modules["torch"]
+        like = like.detach()
+        return torch.zeros_like(like, dtype=TORCH_DTYPES[dtype]) if shape is None else torch.zeros(shape, dtype=TORCH_DTYPES[dtype], device=like.device)
+    out = _empty_like_input(like, tuple(like.shape) if shape is None else shape, dtype)
+    _lib.check(out.lib.lb_fill_bytes(out.ptr, 0, out.nbytes, current_stream()))
+    return out
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, exp_avg_scale=None, exp_avg_sq_scale=None,
+               masters=None, norm=None, max_norm=None, stream=None):
+    """One AdamW step over a list of parameters through `lb_adamw_step`, in place: with `m` and `v` the moments of the gradient and of its square,
+    `w (1 - lr weight_decay) - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps)` in float32, rounded once to the parameter's type. Parameters of
+    float16, bfloat16 and float32 in any mix, dense in any order of their dimensions; gradients of the same type or float32. `exp_avg` and `exp_avg_sq` are
+    float32 tensors of the parameters' layout, or, with their scales, moments in 8 bits (`adamw_state` makes both). `masters`: float32 copies of 16-bit
+    parameters, on which the step is then taken (None in the place of a parameter that has none). `step` counts from 1; it and `lr` are numbers or one-element
+    tensors on the device (int32, int64 or float32; float32), which a captured graph reads anew in every replay. With `norm` (what `grad_norm` gives) and
+    `max_norm` the gradients are taken times `min(1, max_norm / (norm + 1e-6))`, as `clip_grad_norm` would leave them, and stay as they are. Nothing waits
+    for the device. The same bits from call to call."""
+    require_cuda()
+    params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, masters = (
+        t if t is None or type(t) in (list, tuple) else list(t) for t in (params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, masters))  # fmt: skip
+    if (norm is None) != (max_norm is None):
+        raise ValueError("clipping needs both the norm and max_norm")
+    if not len(params):
+        return
+    handle = _Torch.stream() if _Torch.takes(params[0], stream) else _stream(stream)
+    _lib.host().adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, masters, step, lr, *betas, eps, weight_decay, norm,
+                           0.0 if max_norm is None else max_norm, handle)  # fmt: skip
+    for tensors in (params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
+        if tensors:
+            _written(tensors)
+    if masters:
+        _written([t for t in masters if t is not None])
