@@ -59,7 +59,7 @@ struct GemmArgs {
 // What the kernel for CTA pairs does with a tile: the epilogues of lb_gemm, or one half of the gated feed-forward block. In its forward products
 // the leader's half of the B columns are rows of one weight and the other CTA's the same rows of another, so that each CTA's accumulator holds both
 // projections of 128 columns side by side; in its backward product the epilogue reads what the forward pass has kept.
-enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED, PAIR_GROUP };
+enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED, PAIR_GROUP, PAIR_SPANS, PAIR_LOSS_SLOPES };
 struct PlainArgs : GemmArgs {
     static constexpr int mode = PAIR_PLAIN;
 };
@@ -74,6 +74,20 @@ struct alignas(64) SlopedArgs : GemmArgs {
     static constexpr int mode = PAIR_SLOPED;
     CUtensorMap map_gate, map_up, map_d_gate, map_d_up;  // both projections as kept, and their gradients: pieces of 32 rows of 64
     int act;
+};
+// The linear cross entropy's forward and backward products.
+struct SpansArgs : GemmArgs {
+    static constexpr int mode = PAIR_SPANS;
+    Targets targets;
+    SpanSum* spans;  // [2 * tiles_n][M]
+    float* hit;
+};
+struct LossSlopesArgs : GemmArgs {
+    static constexpr int mode = PAIR_LOSS_SLOPES;
+    const float *lse, *g;
+    const int* classes;
+    long long lse_step;
+    int first;
 };
 
 // Up to three products of one launch, one after another in the grid, each without an epilogue and its K whole.
@@ -454,6 +468,85 @@ __device__ __forceinline__ void sloped_way_out(const Args& p, uint8_t* pieces, u
         }
     }
     if (half == 0 && lane == 0) bulk_wait();
+}
+
+// ---- the linear cross entropy's tiles -------------------------------------------------------------------------------
+// A row's 128 logits of the tile, not stored: their largest and the sum of exponentials, 64 columns at a time, and the target's where it is among them
+// (`target`: its column here).
+template <class Release>
+__device__ __forceinline__ SpanSum drain_span(uint32_t tbase, int width, int target, float* hit, Release release) {
+    SpanSum all{-INFINITY, 0.0f};
+#pragma unroll 1
+    for (int c2 = 0; c2 < BN / 2 / 64; c2++) {
+        uint32_t v[64];
+        tmem_ld_32x32(tbase + c2 * 64, v);
+        tmem_ld_32x32(tbase + c2 * 64 + 32, v + 32);
+        tmem_ld_wait();
+        if (c2 == BN / 2 / 64 - 1) release();
+        const int span = width - c2 * 64, at = target - c2 * 64;  // span: warp-uniform
+        if (LB_RARELY(span <= 0)) continue;
+        if (LB_RARELY(span < 64)) {
+#pragma unroll
+            for (int j = 0; j < 64; j++)
+                if (j >= span) v[j] = 0xff800000u;
+        }
+        if (LB_RARELY(__any_sync(0xffffffffu, (unsigned)at < 64u))) {
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 64; j++)
+                if (j == at) z = __uint_as_float(v[j]);
+            if ((unsigned)at < 64u) *hit = z;
+        }
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 64; j++) most[j & 3] = fmaxf(most[j & 3], __uint_as_float(v[j]));
+        const float top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), all.most), base = (top == -INFINITY ? 0.0f : top) * -kLog2e;
+        const Pair scale = both(kLog2e, kLog2e), shift = both(base, base);
+        Pair sum[2] = {both(0.0f, 0.0f), both(0.0f, 0.0f)};
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const float2 e = apart(fma2(columns(v, j), scale, shift));
+            sum[j & 1] = sum[j & 1] + both(fast_exp2(e.x), fast_exp2(e.y));
+        }
+        const float2 s = apart(sum[0] + sum[1]);
+        all = {top, all.sum * fast_exp2(fmaf(all.most, kLog2e, base)) + (s.x + s.y)};
+    }
+    return all;
+}
+
+// A row's 128 columns of dz: (exp(z - lse) - [class]) g, rounded once. `target`: the class's column here; a row that does not count is zero whatever
+// its logits are.
+template <bool F16, class Release>
+__device__ __forceinline__ void drain_slopes(const GemmArgs& p, uint32_t tbase, int row, int col_base, float lse, float g, bool counts, int target, uint4* stage, int lane,
+                                             Release release) {
+    const Pair scale = both(kLog2e, kLog2e), shift = both(lse * -kLog2e, lse * -kLog2e), weight = both(g, g);
+    const uint32_t keep = counts ? 0xffffffffu : 0u;
+    const int rows = p.M - (row - lane);
+#pragma unroll 1
+    for (int c2 = 0; c2 < BN / 2 / 64; c2++) {
+        const int col0 = col_base + c2 * 64, span = p.N - col0, at = target - c2 * 64;
+        uint32_t v[64];
+        tmem_ld_32x32(tbase + c2 * 64, v);
+        tmem_ld_32x32(tbase + c2 * 64 + 32, v + 32);
+        tmem_ld_wait();
+        if (c2 == BN / 2 / 64 - 1) release();
+        if (LB_RARELY(span <= 0)) continue;
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const float2 e = apart(fma2(columns(v, j), scale, shift));
+            v[2 * j] = __float_as_uint(fast_exp2(e.x)), v[2 * j + 1] = __float_as_uint(fast_exp2(e.y));
+        }
+        if (LB_RARELY(__any_sync(0xffffffffu, (unsigned)at < 64u))) {
+#pragma unroll
+            for (int j = 0; j < 64; j++)
+                if (j == at) v[j] = __float_as_uint(__uint_as_float(v[j]) - 1.0f);
+        }
+        uint4 packed[8];
+        uint32_t* w = (uint32_t*)packed;
+#pragma unroll
+        for (int j = 0; j < 32; j++) w[j] = narrow<F16>(columns(v, j) * weight) & keep;
+        store_rows_coalesced<8>(stage, packed, (uint8_t*)((uint16_t*)p.d + (long long)(row - lane) * p.ldd + col0), p.ldd * 2, rows, lane, (span + 7) / 8);
+    }
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -837,6 +930,26 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else if (p.act == ACT_SILU) drain_gated<ACT_SILU, true>(p, tbase, row, col0, stage, lane, release);
                 else if (p.act == ACT_GELU) drain_gated<ACT_GELU, true>(p, tbase, row, col0, stage, lane, release);
                 else drain_gated<ACT_RELU, true>(p, tbase, row, col0, stage, lane, release);
+            } else if constexpr (Args::mode == PAIR_SPANS) {
+                const int col_base = n_blk * BN + col_half * (BN / 2), target = row < p.M ? p.targets.of(row) - col_base : -1;
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                const SpanSum sum = drain_span(tbase, p.N - col_base, target, p.hit + row, release);
+                if (row < p.M) p.spans[(long long)(2 * n_blk + col_half) * p.M + row] = sum;
+            } else if constexpr (Args::mode == PAIR_LOSS_SLOPES) {
+                const int col_base = n_blk * BN + col_half * (BN / 2);
+                float lse = 0.0f, g = 0.0f;
+                int target = -1;
+                if (row < p.M) lse = p.lse[row * p.lse_step], g = p.g[row], target = p.classes[row];
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                const bool counts = target >= 0;
+                if (p.d_f16) drain_slopes<true>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
+                else drain_slopes<false>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_GROUP) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
@@ -1421,6 +1534,35 @@ void gemm_sloped(const lb_tensor& dy_t, const lb_tensor& w_t, const lb_tensor& k
     p.map_gate = half(kept, 0), p.map_up = half(kept, 1), p.map_d_gate = half(d, 0), p.map_d_up = half(d, 1);
     launch_pairs(p.a_mn_major ? make_map(dy, false, 64, BK) : make_map(dy, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p,
                  tiles, stream);
+}
+
+bool gemm_loss_takes(const lb_tensor& x, const lb_tensor& w) {
+    bool x_cols, w_rows;
+    return tensor_core_operands(view3(x, "x"), turned(view3(w, "w")), x_cols, w_rows);
+}
+int gemm_spans(long long N) { return (int)((N + BN - 1) / BN * 2); }
+template <class Args>
+static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, void* stream) {
+    driver();
+    const View3 x = view3(x_t, "x"), w = view3(w_t, "w");
+    bool x_cols, w_rows;
+    tensor_core_operands(x, turned(w), x_cols, w_rows);
+    long long tiles;
+    pair_args(p, x, w, x_cols, !w_rows, BN, tiles);
+    launch_pairs(p.a_mn_major ? make_map(x, false, 64, BK) : make_map(x, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p, tiles,
+                 stream);
+}
+void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, void* stream) {
+    SpansArgs p{};
+    p.targets = targets, p.spans = spans, p.hit = hit;
+    launch_loss(p, x, w, stream);
+}
+void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,
+                      void* stream) {
+    LossSlopesArgs p{};
+    p.lse = lse, p.lse_step = lse_step, p.g = g, p.classes = classes, p.first = first;
+    p.d = dz.ptr, p.ldd = dz.stride[0];
+    launch_loss(p, x, w, stream);
 }
 
 }  // namespace lb

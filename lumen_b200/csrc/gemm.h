@@ -7,6 +7,7 @@
 #endif
 
 #include "device.h"
+#include "linear_loss.h"
 
 namespace lb {
 
@@ -88,6 +89,15 @@ void gemm_sloped(const lb_tensor& dy, const lb_tensor& w, const lb_tensor& kept,
 // d[k] = a[k] b[k] for up to three products of 16-bit operands that do not depend on one another, in one launch; `_pays`: whether they can and gain by it.
 bool gemm_group_pays(const lb_tensor* a, const lb_tensor* b, int n);
 void gemm_group(const lb_tensor* a, const lb_tensor* b, const lb_tensor* d, int n, void* stream);
+
+// The linear cross entropy's products z = x w^T with their epilogues, 16-bit operands on CTA pairs: x [M, K], w [N, K]. Forward: each row's span sums, `spans`
+// [gemm_spans(N)][M], and its target's logit. Backward: dz [M, N] = (exp(z - lse) - [class]) g, where `w` holds the classes from `first` on; a row of class -1 is
+// zero, and columns up to the next multiple of eight may be written. `_takes`: whether the operands' layouts are theirs.
+bool gemm_loss_takes(const lb_tensor& x, const lb_tensor& w);
+int gemm_spans(long long N);
+void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, void* stream);
+void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,
+                      void* stream);
 
 // A few tokens (gemm_skinny.cu): out [M, N] = x [M, K] w^T with w [N, K], plus `add` [M, N] once rounded (null: nothing); h and kept as in gemm_gated.
 bool skinny_takes(const lb_tensor& x, const lb_tensor& w);

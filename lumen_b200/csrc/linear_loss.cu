@@ -328,20 +328,22 @@ struct Forward : Loss {
     }
     void run(cudaStream_t s, bool only_count) {
         held = 0;
-        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece;
+        const bool fused = T && gemm_loss_takes(x, w);
+        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, n_spans = fused ? gemm_spans(V) : pieces;
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
         const long long blocks = (T + R - 1) / R;
-        SpanSum* spans = take<SpanSum>(pieces * T);
+        SpanSum* spans = take<SpanSum>(n_spans * T);
         float* hit = take<float>(T);
         LossSum* sums = reduction == LB_REDUCTION_NONE ? nullptr : take<LossSum>(blocks);
         const long long ld = up(piece, 8);
-        float* logits = take<float>(T * ld);
+        float* logits = take<float>(fused ? 0 : T * ld);
         const lb_tensor z = matrix(logits, LB_F32, T, piece, ld);
-        const size_t more = T ? product_scratch(x, transposed(rows_of(w, 0, piece))) : 0;
+        const size_t more = T && !fused ? product_scratch(x, transposed(rows_of(w, 0, piece))) : 0;
         void* product = take<char>(more);
         if (only_count) return;
         if (T) {
-            for (long long k = 0; k < pieces; k++) {
+            if (fused) gemm_loss(x, w, targets, spans, hit, s);
+            for (long long k = 0; k < pieces && !fused; k++) {
                 const long long first = k * piece, cols = std::min(piece, V - first);
                 lb_tensor out = z;
                 out.shape[1] = cols;
@@ -349,7 +351,7 @@ struct Forward : Loss {
                 launch_overlapped(span_kernel, dim3(row_blocks(T)), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, targets, spans + k * T, hit);
             }
             auto join_rows = [&](auto kernel) {
-                launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, s, 0, (const SpanSum*)spans, (int)pieces, T, (const float*)hit, targets, (float*)lse.ptr,
+                launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, s, 0, (const SpanSum*)spans, (int)n_spans, T, (const float*)hit, targets, (float*)lse.ptr,
                                   sums ? nullptr : (float*)loss.ptr, sums);
             };
             R == 32 ? join_rows(rows_kernel<32>) : R == 8 ? join_rows(rows_kernel<8>) : join_rows(rows_kernel<1>);
@@ -385,19 +387,20 @@ struct Backward : Loss {
         held = 0;
         const int item = dtype_size(dtype);
         const bool half = dtype == LB_F16;
-        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, ld = up(piece, 8);
+        const bool fused = T && gemm_loss_takes(x, w);
+        const long long piece = piece_of(fused ? 2 : 4), pieces = (V + piece - 1) / piece, ld = up(piece, 8);
         const int n_counts = (int)std::min<long long>(64, (T + 255) / 256);
         RowCount* counts = take<RowCount>(n_counts);
         float *g = take<float>(T), *undo = take<float>(1);
         int* classes = take<int>(T);
         char* x_kept = take<char>(T * D * item);
-        float* logits = take<float>(T * ld);
+        float* logits = take<float>(fused ? 0 : T * ld);
         char* slopes = dtype == LB_F32 ? (char*)logits : take<char>(T * ld * item);
         const bool folds = pieces > 1 || half;
         float *dx_piece = folds ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr, *dw_piece = half ? take<float>(piece * D) : nullptr;
         const lb_tensor kept = matrix(x_kept, dtype, T, D, D), dz = matrix(slopes, dtype, T, piece, ld);
         size_t more = 0;
-        if (T) more = std::max({product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
+        if (T) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
         void* product = take<char>(more);
         if (only_count) return;
         if (T == 0) {
@@ -416,8 +419,9 @@ struct Backward : Loss {
             const lb_tensor rows = rows_of(w, first, cols);
             lb_tensor z = matrix(logits, LB_F32, T, cols, ld), d = dz, dw_rows = rows_of(dw, first, cols);
             d.shape[1] = cols;
-            gemm(x, transposed(rows), z, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-            by_type(dtype, [&](auto* type) {
+            if (fused) gemm_loss_slopes(x, rows, (const float*)lse.ptr, lse.stride[0], g, classes, (int)first, d, s);
+            else gemm(x, transposed(rows), z, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+            if (!fused) by_type(dtype, [&](auto* type) {
                 using E = std::remove_pointer_t<decltype(type)>;
                 launch_overlapped(slope_kernel<E>, dim3(row_blocks(T)), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, (const float*)lse.ptr,
                                   (long long)lse.stride[0], (const float*)g, (const int*)classes, (E*)slopes, ld);
