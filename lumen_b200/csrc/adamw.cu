@@ -11,6 +11,7 @@
 // thousandth a step are far below half a step of e4m3 (a sixteenth); simulated over 3000 steps of normal gradients, the mean ratio of these
 // denominators to exact ones is 1.04 (standard deviation 0.2) with b2 = 0.999 and 1.01 (0.08) with 0.95, where scales that are powers of two freeze at 0.4 and 2.1.
 #include <cmath>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -19,6 +20,7 @@
 #include "convert.cuh"
 #include "dense_lists.h"
 #include "launch.cuh"
+#include "pair.cuh"
 
 namespace lb {
 namespace {
@@ -34,7 +36,7 @@ struct AdamwTable {
     long long n[kMost];
     int first[kMost + 1];   // first chunk of each tensor
     uint8_t dtype[kMost], grad[kMost];
-    int8_t head[kMost];     // elements in front of the first one that groups of eight are aligned from; -1: they are nowhere
+    int8_t head[kMost];     // elements in front of the first one that vectors are aligned from; -1: they are nowhere
     int count;
     // the step
     float b1, b1_rest, b2, b2_rest, eps;
@@ -47,7 +49,7 @@ static_assert(sizeof(AdamwTable) <= 32000, "kernel parameters");
 
 // What every element's step needs.
 struct Step {
-    float b1, b1_rest, b2, b2_rest, eps, factor, keep, rate, c2;  // keep: 1 - lr decay; rate: lr / (1 - b1^t); c2: 1 / (1 - b2^t)
+    float b1, b1_rest, b2, b2_rest, eps, factor, keep, rate, root_c2;  // keep: 1 - lr decay; rate: lr / (1 - b1^t); root_c2: 1 / sqrt(1 - b2^t)
 };
 __device__ Step this_step(const AdamwTable& t, Step* shared) {
     if (threadIdx.x == 0) {
@@ -57,7 +59,7 @@ __device__ Step this_step(const AdamwTable& t, Step* shared) {
         Step s{t.b1, t.b1_rest, t.b2, t.b2_rest, t.eps};
         s.keep = (float)(1.0 - lr * t.decay);
         s.rate = (float)(lr / -expm1(step * t.log_b1));
-        s.c2 = (float)(1.0 / -expm1(step * t.log_b2));
+        s.root_c2 = (float)(1.0 / sqrt(-expm1(step * t.log_b2)));
         s.factor = 1.0f;
         if (t.norm_at) {
             const double quotient = t.max_norm / ((double)*t.norm_at + 1e-6);
@@ -73,123 +75,232 @@ __device__ __forceinline__ void moments(const Step& s, float g, float& m, float&
     m = __fadd_rn(__fmul_rn(m, s.b1), __fmul_rn(g, s.b1_rest));
     v = __fadd_rn(__fmul_rn(v, s.b2), __fmul_rn(__fmul_rn(g, g), s.b2_rest));
 }
-__device__ __forceinline__ float moved(const Step& s, float w, float m, float v) { return w * s.keep - m * s.rate / (__fsqrt_rn(v * s.c2) + s.eps); }
-
-// Eight elements, aligned to as many.
-__device__ __forceinline__ void load8(const float* p, float* x) {
-    const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-__device__ __forceinline__ void store8(float* p, const float* x) {
-    ((float4*)p)[0] = make_float4(x[0], x[1], x[2], x[3]), ((float4*)p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float* x) {
-    const uint4 w = *(const uint4*)p;
-    const T* e = (const T*)&w;
-#pragma unroll
-    for (int k = 0; k < 8; k++) x[k] = to_float(e[k]);
-}
-template <class T>
-__device__ __forceinline__ void store8(T* p, const float* x) {
-    uint4 w;
-    T* e = (T*)&w;
-#pragma unroll
-    for (int k = 0; k < 8; k++) e[k] = from_float<T>(x[k]);
-    *(uint4*)p = w;
+// w keep - m rate / (sqrt(v) sqrt(c2) + eps), with the hardware's root and quotient: a few units in the last place of float32 of a step that is small beside the weight.
+__device__ __forceinline__ float moved(const Step& s, float w, float m, float root) { return w * s.keep - __fdividef(m * s.rate, fmaf(root, s.root_c2, s.eps)); }
+__device__ __forceinline__ float root_of(float v) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
 
+// 32 bytes, aligned to as many; moments and gradients are not read again before the next step.
+template <class T>
+__device__ __forceinline__ void load_wide(const T* p, uint32_t* w) {
+    asm volatile("ld.global.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(__cvta_generic_to_global(p)) : "memory");
+}
+template <class T>
+__device__ __forceinline__ void store_wide(T* p, const uint32_t* w) {
+    asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(p)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// N elements as they lie in memory, on a boundary of N of them or 32 bytes.
+template <class T, int N>
+struct Some {
+    static constexpr int words = N * (int)sizeof(T) / 4;
+    static_assert(words == 4 || words % 8 == 0, "whole vectors");
+    uint32_t w[words];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (words == 4) {
+            const uint4 a = *(const uint4*)p;
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < words; k += 8) load_wide((const uint32_t*)p + k, w + k);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (words == 4) {
+            *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < words; k += 8) store_wide((uint32_t*)p + k, w + k);
+        }
+    }
+    __device__ __forceinline__ void widen(float* x) const {
+#pragma unroll
+        for (int k = 0; k < words; k++) {
+            if constexpr (sizeof(T) == 4) {
+                x[k] = __uint_as_float(w[k]);
+            } else if constexpr (std::is_same_v<T, __half>) {
+                const float2 f = __half22float2(*(const __half2*)&w[k]);
+                x[2 * k] = f.x, x[2 * k + 1] = f.y;
+            } else {
+                x[2 * k] = __uint_as_float(w[k] << 16), x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+            }
+        }
+    }
+    __device__ __forceinline__ void narrow(const float* x) {
+#pragma unroll
+        for (int k = 0; k < words; k++) {
+            if constexpr (sizeof(T) == 4) {
+                w[k] = __float_as_uint(x[k]);
+            } else if constexpr (std::is_same_v<T, __half>) {
+                const __half2 h = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+                w[k] = *(const uint32_t*)&h;
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+                w[k] = *(const uint32_t*)&h;
+            }
+        }
+    }
+};
+
+constexpr int kEach = 16;  // elements of a thread
+// All loads of a thread's elements are on their way at a time.
 template <class P, class G, bool MASTER>
 __device__ __forceinline__ void chunk_step(const AdamwTable& t, int k, long long at, int n, const Step& s) {
     P* p = (P*)t.p[k] + at;
     const G* g = (const G*)t.g[k] + at;
     float *m = (float*)t.m[k] + at, *v = (float*)t.v[k] + at, *master = MASTER ? t.master[k] + at : nullptr;
-    const int head = t.head[k] < 0 ? n : min(n, (int)t.head[k]), eights = (n - head) / 8;
-    for (int i = threadIdx.x; i < eights; i += kThreads) {
-        const int e = head + 8 * i;
-        float w[8], gg[8], mm[8], vv[8];
-        load8(g + e, gg), load8(m + e, mm), load8(v + e, vv);
-        if (MASTER) load8(master + e, w);
-        else load8(p + e, w);
+    const int head = t.head[k] < 0 ? n : min(n, (int)t.head[k]), groups = (n - head) / kEach;
+    using W = std::conditional_t<MASTER, float, P>;
+    W* from = MASTER ? (W*)master : (W*)p;
+    static_assert(chunk_elements(32) == kThreads * kEach, "one group a thread");
+    if ((int)threadIdx.x < groups) {
+        const int e = head + kEach * threadIdx.x;
+        Some<W, kEach> w;
+        Some<G, kEach> gg;
+        Some<float, kEach> mm, vv;
+        gg.load(g + e), mm.load(m + e), vv.load(v + e), w.load(from + e);
+        float x[kEach], y[kEach], m1[kEach], v1[kEach];
+        w.widen(x), gg.widen(y), mm.widen(m1), vv.widen(v1);
 #pragma unroll
-        for (int j = 0; j < 8; j++) moments(s, gg[j], mm[j], vv[j]), w[j] = moved(s, w[j], mm[j], vv[j]);
-        store8(p + e, w), store8(m + e, mm), store8(v + e, vv);
-        if (MASTER) store8(master + e, w);
+        for (int j = 0; j < kEach; j++) moments(s, y[j], m1[j], v1[j]), x[j] = moved(s, x[j], m1[j], root_of(v1[j]));
+        mm.narrow(m1), vv.narrow(v1), w.narrow(x);
+        mm.store(m + e), vv.store(v + e), w.store(from + e);
+        if constexpr (MASTER) {
+            Some<P, kEach> out;
+            out.narrow(x), out.store(p + e);
+        }
     }
-    for (int i = threadIdx.x; i < n - eights * 8; i += kThreads) {
-        const int e = i < head ? i : eights * 8 + i;
+    for (int i = threadIdx.x; i < n - groups * kEach; i += kThreads) {
+        const int e = i < head ? i : groups * kEach + i;
         float mm = m[e], vv = v[e];
         moments(s, to_float(g[e]), mm, vv);
-        const float w = moved(s, MASTER ? master[e] : to_float(p[e]), mm, vv);
+        const float w = moved(s, MASTER ? master[e] : to_float(p[e]), mm, root_of(vv));
         p[e] = from_float<P>(w), m[e] = mm, v[e] = vv;
         if (MASTER) master[e] = w;
     }
 }
 
-__device__ __forceinline__ float from_e4m3(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
+// ---- moments in 8 bits: one warp's block of 256 elements, eight in a row to a lane ------------------------------------
 
-// One warp's block of 256 elements, eight in a row to a lane.
-template <class P, class G, bool MASTER>
-__device__ __forceinline__ void block_step(P* p, const G* g, uint8_t* m, uint8_t* v, float* master, float* m_scale, float* v_scale, int n, bool whole, const Step& s) {
-    const int lane = threadIdx.x & 31, e = lane * 8, count = max(0, min(8, n - e));
-    const float sm = *m_scale, sv = *v_scale;
-    float w[8], gg[8], mm[8], vv[8];
-    uint8_t cm[8], cv[8];
-    if (whole) {
-        *(uint2*)cm = *(const uint2*)(m + e), *(uint2*)cv = *(const uint2*)(v + e);
-        load8(g + e, gg);
-        if (MASTER) load8(master + e, w);
-        else load8(p + e, w);
-    } else {
+// Codes of two elements and their values.
+__device__ __forceinline__ Pair from_e4m3(uint32_t two) {
+    const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3));
+    const float2 f = __half22float2(h);
+    return both(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t to_e4m3(float2 x) { return (uint32_t)__nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3); }
+// The largest magnitude of a warp's values; NaN is above all.
+__device__ __forceinline__ float warp_most(float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x) & 0x7fffffffu)); }
+__device__ __forceinline__ float more(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Codes `m` and `v`, weights and gradients of a lane's eight elements after a step; the block's scales in `sm` and `sv`. What is held comes of roots, products and
+// quotients that are each rounded to nearest.
+__device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, float& sm, float& sv, float* w, const float* g) {
+    uint32_t cm[4] = {m.x & 0xffff, m.x >> 16, m.y & 0xffff, m.y >> 16}, cv[4] = {v.x & 0xffff, v.x >> 16, v.y & 0xffff, v.y >> 16};
+    const Pair scale_m = both(sm, sm), scale_v = both(sv, sv);
+    float2 mm[4], root[4];
+    float top_m = 0.0f, top_v = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const bool in = j < count;
-            cm[j] = in ? m[e + j] : 0, cv[j] = in ? v[e + j] : 0, gg[j] = in ? to_float(g[e + j]) : 0.0f;
-            w[j] = !in ? 0.0f : MASTER ? master[e + j] : to_float(p[e + j]);
-        }
+    for (int j = 0; j < 4; j++) {
+        mm[j] = apart(from_e4m3(cm[j]) * scale_m);
+        const Pair r = from_e4m3(cv[j]) * scale_v;
+        float2 vv = apart(r * r);
+        moments(s, g[2 * j], mm[j].x, vv.x), moments(s, g[2 * j + 1], mm[j].y, vv.y);
+        root[j] = make_float2(__fsqrt_rn(vv.x), __fsqrt_rn(vv.y));
+        w[2 * j] = moved(s, w[2 * j], mm[j].x, root[j].x), w[2 * j + 1] = moved(s, w[2 * j + 1], mm[j].y, root[j].y);
+        top_m = more(more(top_m, fabsf(mm[j].x)), fabsf(mm[j].y)), top_v = more(more(top_v, root[j].x), root[j].y);
     }
-    uint32_t top_m = 0, top_v = 0;  // as bits: what is not negative is ordered alike, NaN above all
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        mm[j] = __fmul_rn(from_e4m3(cm[j]), sm);
-        const float root = __fmul_rn(from_e4m3(cv[j]), sv);
-        vv[j] = __fmul_rn(root, root);
-        moments(s, gg[j], mm[j], vv[j]);
-        w[j] = moved(s, w[j], mm[j], vv[j]);
-        vv[j] = __fsqrt_rn(vv[j]);
-        top_m = max(top_m, __float_as_uint(mm[j]) & 0x7fffffffu), top_v = max(top_v, __float_as_uint(vv[j]) & 0x7fffffffu);
-    }
-    const float most_m = __uint_as_float(__reduce_max_sync(0xffffffffu, top_m)), most_v = __uint_as_float(__reduce_max_sync(0xffffffffu, top_v));
+    const float most_m = warp_most(top_m), most_v = warp_most(top_v);
     const bool no_m = most_m < 0x1p-100f, no_v = most_v < 0x1p-100f;
     const float inv_m = no_m ? 0.0f : __fdiv_rn(448.0f, most_m), inv_v = no_v ? 0.0f : __fdiv_rn(448.0f, most_v);
+    sm = no_m ? 0.0f : __fdiv_rn(most_m, 448.0f), sv = no_v ? 0.0f : __fdiv_rn(most_v, 448.0f);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float2 x = apart(both(root[j].x, root[j].y) * both(inv_v, inv_v));
+        if (x.x < 0x1p-9f && root[j].x > 0.0f) x.x = 0x1p-9f;
+        if (x.y < 0x1p-9f && root[j].y > 0.0f) x.y = 0x1p-9f;
+        cv[j] = to_e4m3(x), cm[j] = to_e4m3(apart(both(mm[j].x, mm[j].y) * both(inv_m, inv_m)));
+    }
+    m = make_uint2(cm[0] | cm[1] << 16, cm[2] | cm[3] << 16), v = make_uint2(cv[0] | cv[1] << 16, cv[2] | cv[3] << 16);
+}
+
+// A block that is short, or whose memory vectors do not fit.
+template <class P, class G, bool MASTER>
+__device__ __forceinline__ void odd_block(P* p, const G* g, uint8_t* m, uint8_t* v, float* master, float* m_scale, float* v_scale, int n, const Step& s) {
+    const int lane = threadIdx.x & 31, e = lane * 8, count = max(0, min(8, n - e));
+    float sm = *m_scale, sv = *v_scale, w[8], gg[8];
+    union {
+        uint2 all;
+        uint8_t one[8];
+    } cm, cv;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        float x = __fmul_rn(vv[j], inv_v);
-        if (x < 0x1p-9f && vv[j] > 0.0f) x = 0x1p-9f;
-        cm[j] = __nv_cvt_float_to_fp8(__fmul_rn(mm[j], inv_m), __NV_SATFINITE, __NV_E4M3), cv[j] = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+        const bool in = j < count;
+        cm.one[j] = in ? m[e + j] : 0, cv.one[j] = in ? v[e + j] : 0, gg[j] = in ? to_float(g[e + j]) : 0.0f;
+        w[j] = !in ? 0.0f : MASTER ? master[e + j] : to_float(p[e + j]);
     }
+    eight_step(s, cm.all, cv.all, sm, sv, w, gg);
     __syncwarp();  // every lane has read the scales
-    if (lane == 0) *m_scale = no_m ? 0.0f : __fdiv_rn(most_m, 448.0f), *v_scale = no_v ? 0.0f : __fdiv_rn(most_v, 448.0f);
-    if (whole) {
-        *(uint2*)(m + e) = *(uint2*)cm, *(uint2*)(v + e) = *(uint2*)cv;
-        store8(p + e, w);
-        if (MASTER) store8(master + e, w);
-    } else {
+    if (lane == 0) *m_scale = sm, *v_scale = sv;
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < count) {
-                m[e + j] = cm[j], v[e + j] = cv[j], p[e + j] = from_float<P>(w[j]);
-                if (MASTER) master[e + j] = w[j];
-            }
-    }
+    for (int j = 0; j < 8; j++)
+        if (j < count) {
+            m[e + j] = cm.one[j], v[e + j] = cv.one[j], p[e + j] = from_float<P>(w[j]);
+            if (MASTER) master[e + j] = w[j];
+        }
 }
+// The next block's loads are on their way while a block is worked on.
 template <class P, class G, bool MASTER>
 __device__ __forceinline__ void chunk_step_8bit(const AdamwTable& t, int k, long long at, int n, const Step& s) {
-    for (int b = threadIdx.x / 32; b * kBlock < n; b += kThreads / 32) {
-        const long long e = at + (long long)b * kBlock, i = e / kBlock;
-        const int count = min(kBlock, n - b * kBlock);
-        block_step<P, G, MASTER>((P*)t.p[k] + e, (const G*)t.g[k] + e, (uint8_t*)t.m[k] + e, (uint8_t*)t.v[k] + e, MASTER ? t.master[k] + e : nullptr, t.m_scale[k] + i,
-                                 t.v_scale[k] + i, count, count == kBlock && t.head[k] == 0, s);
+    P* p = (P*)t.p[k] + at;
+    const G* g = (const G*)t.g[k] + at;
+    uint8_t *m = (uint8_t*)t.m[k] + at, *v = (uint8_t*)t.v[k] + at;
+    float *master = MASTER ? t.master[k] + at : nullptr, *m_scale = t.m_scale[k] + at / kBlock, *v_scale = t.v_scale[k] + at / kBlock;
+    using W = std::conditional_t<MASTER, float, P>;
+    W* from = MASTER ? (W*)master : (W*)p;
+    constexpr int warps = kThreads / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, whole = t.head[k] == 0 ? n / kBlock : 0;
+    struct {
+        Some<W, 8> w;
+        Some<G, 8> g;
+        uint2 m, v;
+        float sm, sv;
+    } next;
+    auto fetch = [&](int b) {
+        const int e = b * kBlock + lane * 8;
+        next.w.load(from + e), next.g.load(g + e);
+        next.m = *(const uint2*)(m + e), next.v = *(const uint2*)(v + e), next.sm = m_scale[b], next.sv = v_scale[b];
+    };
+    if (warp < whole) fetch(warp);
+    for (int b = warp; b < whole; b += warps) {
+        auto now = next;
+        if (b + warps < whole) fetch(b + warps);
+        const int e = b * kBlock + lane * 8;
+        float w[8], gg[8];
+        now.w.widen(w), now.g.widen(gg);
+        eight_step(s, now.m, now.v, now.sm, now.sv, w, gg);
+        now.w.narrow(w), now.w.store(from + e);
+        *(uint2*)(m + e) = now.m, *(uint2*)(v + e) = now.v;
+        if (lane == 0) m_scale[b] = now.sm, v_scale[b] = now.sv;
+        if (MASTER) {
+            Some<P, 8> out;
+            out.narrow(w), out.store(p + e);
+        }
+    }
+    for (int b = whole + warp; b * kBlock < n; b += warps) {
+        const int e = b * kBlock;
+        odd_block<P, G, MASTER>(p + e, g + e, m + e, v + e, MASTER ? master + e : nullptr, m_scale + b, v_scale + b, min(kBlock, n - e), s);
     }
 }
 
@@ -214,8 +325,9 @@ __global__ void __launch_bounds__(kThreads, 2) adamw_kernel(const __grid_constan
     __shared__ Step shared;
     grid_wait();
     const Step s = this_step(t, &shared);
+    int k = tensor_of(t, blockIdx.x);
     for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const int k = tensor_of(t, c);
+        while (t.first[k + 1] <= c) k++;
         const long long at = (long long)(c - t.first[k]) * chunk_elements(BITS);
         const int n = (int)min((long long)chunk_elements(BITS), t.n[k] - at);
         if (t.dtype[k] == LB_F32) chunk_of<BITS, float, float, false>(t, k, at, n, s);
@@ -309,10 +421,10 @@ void run_adamw(const lb_adamw_desc* desc, const lb_tensor* params, const lb_tens
             t.master[i] = masters ? (float*)masters[k].ptr : nullptr;
             t.m_scale[i] = m_scales ? (float*)m_scales[k].ptr : nullptr, t.v_scale[i] = v_scales ? (float*)v_scales[k].ptr : nullptr;
             t.dtype[i] = (uint8_t)params[k].dtype, t.grad[i] = (uint8_t)grads[k].dtype;
-            // vectors are 16 bytes of all tensors' types but codes, which take 8
+            // vectors are 32 bytes, but for moments in 8 bits, whose eight elements are 8 bytes of codes and 16 of 16-bit values
             int head = -1;
-            for (int h = 0; h < 8 && head < 0; h++) {
-                auto fits = [&](const void* ptr, int dtype) { return !ptr || ((uintptr_t)ptr + (size_t)h * dtype_size(dtype)) % std::min(16, 8 * dtype_size(dtype)) == 0; };
+            for (int h = 0; h < 16 && head < 0; h++) {
+                auto fits = [&](const void* ptr, int dtype) { return !ptr || ((uintptr_t)ptr + (size_t)h * dtype_size(dtype)) % (bits == 8 ? 8 * dtype_size(dtype) : 32) == 0; };
                 if (fits(t.p[i], params[k].dtype) && fits(t.g[i], grads[k].dtype) && fits(t.m[i], ms[k].dtype) && fits(t.v[i], vs[k].dtype) && fits(t.master[i], LB_F32)) head = h;
             }
             t.head[i] = (int8_t)head, t.first[i] = (int)first;
