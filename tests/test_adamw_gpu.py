@@ -43,6 +43,24 @@ def held(x, lowest):
     return q.to(torch.float8_e4m3fn).view(torch.uint8).view(-1)[: x.numel()], scale.view(-1)
 
 
+def rounds_to(codes, scale, x, off, lowest, what):
+    """Whether codes and scales hold `x` (64 bits, known up to `off`): the scale is the block's largest value over 448, with three roundings, and each code the
+    nearest e4m3 value to x / scale, up to what x is off by and as many roundings."""
+    rows, off = blocks(x), blocks(off)
+    most = rows.abs().amax(-1)
+    assert bool(((scale.double() - most / 448).abs() <= off.amax(-1) / 448 + 2.0**-21 * most / 448 + 1e-30).all()), f"{what}: scales"
+    unit = scale.double()[:, None].clamp(min=1e-300)
+    q, want = e4m3(blocks(codes)).double(), rows / unit
+    _, exponent = torch.frexp(want)
+    half_step = torch.exp2((exponent - 5).clamp(min=-10).double())  # what lies between two powers of two is a sixteenth of the lower one from its neighbours' middle
+    near = (q - want).abs() <= half_step + off / unit + 2.0**-20 * want.abs()
+    if lowest:
+        near |= (q == 2.0**-9) & (want < 2.0**-9) & (rows > 0)
+        assert bool((q > 0)[rows > 1e-18].all()), f"{what}: something became zero"
+    near |= (scale == 0)[:, None] & (q == 0)
+    assert bool(near.view(-1)[: x.numel()].all()) and not bool(q.view(-1)[x.numel() :].any()), f"{what}: codes"
+
+
 def values(codes, scale):
     return (e4m3(blocks(codes)) * scale[:, None]).view(-1)[: codes.numel()]
 
@@ -97,11 +115,13 @@ class Model:
             m, v = (values(ms[k], mss[k]), values(vs[k], vss[k]).square()) if self.bits == 8 else (ms[k], vs[k])
             m32, v32 = m * b1 + g * (1 - b1), v * b2 + g * g * (1 - b2)
             for got, scale, want, lowest in ((self.m[k], self.ms and self.ms[k], m32, False), (self.v[k], self.vs and self.vs[k], v32, True)):
-                if self.bits == 8:
-                    codes, s = held(torch.sqrt(want) if lowest else want, lowest)
-                    assert torch.equal(scale, s) and torch.equal(got, codes), f"tensor {k}: a moment in 8 bits"
-                else:
+                if self.bits == 32:
                     assert torch.equal(got, want), f"tensor {k}: a moment"
+                    continue
+                # roots and products of a few roundings each, 2^-21 of what is added up
+                size = (m.double() * b1).abs() + (g.double() * (1 - b1)).abs()
+                exact = torch.sqrt(v.double() * b2 + g.double() ** 2 * (1 - b2)) if lowest else m.double() * b1 + g.double() * (1 - b1)
+                rounds_to(got, scale, exact, 2.0**-21 * (exact if lowest else size), lowest, f"tensor {k}")
             m64, v64 = m.double() * b1 + g.double() * (1 - b1), v.double() * b2 + g.double() ** 2 * (1 - b2)
             c1, c2 = 1 / (1 - b1**step), 1 / (1 - b2**step)
             start = masters[k] if masters and masters[k] is not None else p
