@@ -59,7 +59,7 @@ struct GemmArgs {
 // What the kernel for CTA pairs does with a tile: the epilogues of lb_gemm, or one half of the gated feed-forward block. In its forward products
 // the leader's half of the B columns are rows of one weight and the other CTA's the same rows of another, so that each CTA's accumulator holds both
 // projections of 128 columns side by side; in its backward product the epilogue reads what the forward pass has kept.
-enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED, PAIR_GROUP, PAIR_SPANS, PAIR_LOSS_SLOPES };
+enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED, PAIR_GROUP, PAIR_SPANS, PAIR_LOSS_SLOPES, PAIR_SUM };
 struct PlainArgs : GemmArgs {
     static constexpr int mode = PAIR_PLAIN;
 };
@@ -88,6 +88,13 @@ struct LossSlopesArgs : GemmArgs {
     const int* classes;
     long long lse_step;
     int first;
+};
+// A product that is added to a float32 sum, dense [M][N]; the last one's result leaves rounded.
+struct SumArgs : GemmArgs {
+    static constexpr int mode = PAIR_SUM;
+    float* sum;
+    const float* undo;  // what the rounded result is multiplied by; null: nothing
+    int begins, ends;
 };
 
 // Up to three products of one launch, one after another in the grid, each without an epilogue and its K whole.
@@ -549,6 +556,44 @@ __device__ __forceinline__ void drain_slopes(const GemmArgs& p, uint32_t tbase, 
     }
 }
 
+// A row's 128 columns of a product and of the sum that it is added to. N is a multiple of eight, rows of the result are 16-byte aligned.
+template <bool F16, class Release>
+__device__ __forceinline__ void drain_sum(const SumArgs& p, uint32_t tbase, int row, int col_base, uint4* stage, int lane, Release release) {
+    const int rows = p.M - (row - lane);
+    const float scale = p.undo ? *p.undo : 1.0f;
+    float* sum0 = p.sum + (long long)(row - lane) * p.N;  // the warp's first row
+#pragma unroll 1
+    for (int c2 = 0; c2 < BN / 2 / 64; c2++) {
+        const int col0 = col_base + c2 * 64, span = p.N - col0;
+        uint32_t v[64];
+        tmem_ld_32x32(tbase + c2 * 64, v);
+        tmem_ld_32x32(tbase + c2 * 64 + 32, v + 32);
+        tmem_ld_wait();
+        if (c2 == BN / 2 / 64 - 1) release();
+        if (LB_RARELY(span <= 0)) continue;
+        if (!p.begins) {
+            const float4* held = (const float4*)(sum0 + (long long)lane * p.N + col0);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float4 h = row < p.M && 4 * j < span ? held[j] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + h.x), v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + h.y);
+                v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + h.z), v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + h.w);
+            }
+        }
+        if (p.ends) {
+            uint4 packed[8];
+            uint32_t* w = (uint32_t*)packed;
+#pragma unroll
+            for (int j = 0; j < 32; j++) w[j] = narrow<F16>(columns(v, j) * both(scale, scale));
+            store_rows_coalesced<8>(stage, packed, (uint8_t*)((uint16_t*)p.d + (long long)(row - lane) * p.ldd + col0), p.ldd * 2, rows, lane, span / 8);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                store_rows_coalesced<8>(stage, (const uint4*)(v + h * 32), (uint8_t*)(sum0 + col0 + h * 32), (long long)p.N * 4, rows, lane, (span - h * 32) / 4);
+        }
+    }
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
     extern __shared__ uint8_t smem_raw[];
@@ -950,6 +995,14 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 const bool counts = target >= 0;
                 if (p.d_f16) drain_slopes<true>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
                 else drain_slopes<false>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
+            } else if constexpr (Args::mode == PAIR_SUM) {
+                const int col_base = n_blk * BN + col_half * (BN / 2);
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                if (p.d_f16) drain_sum<true>(p, tbase, row, col_base, stage, lane, release);
+                else drain_sum<false>(p, tbase, row, col_base, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_GROUP) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
@@ -1541,6 +1594,25 @@ bool gemm_loss_takes(const lb_tensor& x, const lb_tensor& w) {
     return tensor_core_operands(view3(x, "x"), turned(view3(w, "w")), x_cols, w_rows);
 }
 int gemm_spans(long long N) { return (int)((N + BN - 1) / BN * 2); }
+bool gemm_sum_takes(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& out) {
+    const View3 a = view3(a_t, "a"), b = view3(b_t, "b");
+    bool a_cols, b_cols;
+    if (a.rows <= BM || b.cols % 8 || !tensor_core_operands(a, b, a_cols, b_cols) || !in_pieces(out)) return false;
+    const GemmRoute route = gemm_route(a.rows, b.cols, a.cols, 1, sm_count_hint(), 0, gemm_scratch_bytes(a.rows, b.cols, a.cols, 1), nullptr);
+    return route.ranges == 0 && route.splits == 1;
+}
+void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream) {
+    driver();
+    const View3 a = view3(a_t, "a"), b = view3(b_t, "b"), w = turned(b);
+    bool a_cols, b_cols;
+    tensor_core_operands(a, b, a_cols, b_cols);
+    SumArgs p{};
+    long long tiles;
+    pair_args(p, a, w, a_cols, !b_cols, BN, tiles);
+    p.sum = sum, p.undo = undo, p.begins = begins, p.ends = out != nullptr;
+    if (out) p.d = out->ptr, p.ldd = out->stride[0];
+    launch_pairs(p.a_mn_major ? make_map(a, false, 64, BK) : make_map(a, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p, tiles, stream);
+}
 template <class Args>
 static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, void* stream) {
     driver();

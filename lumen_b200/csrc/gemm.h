@@ -99,9 +99,17 @@ void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, S
 void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,
                       void* stream);
 
+// sum + a b on CTA pairs, `sum` dense float32 [M, N] (nothing where it `begins`): rounded into `out`, times *undo unless that is null, or, with a null `out`, into sum.
+// `_takes`: whether layouts are theirs (`out` stands for all rows of the result) and lb_gemm would take whole K on pairs.
+bool gemm_sum_takes(const lb_tensor& a, const lb_tensor& b, const lb_tensor& out);
+void gemm_sum(const lb_tensor& a, const lb_tensor& b, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream);
+
 // A few tokens (gemm_skinny.cu): out [M, N] = x [M, K] w^T with w [N, K], plus `add` [M, N] once rounded (null: nothing); h and kept as in gemm_gated.
 bool skinny_takes(const lb_tensor& x, const lb_tensor& w);
 void skinny_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept, int act, void* stream);
+// The span sums of gemm_loss for them, [skinny_spans(N)][M].
+int skinny_spans(long long N);
+void skinny_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, void* stream);
 void skinny_product(const lb_tensor& x, const lb_tensor& w, const lb_tensor& out, const lb_tensor* add, void* stream);
 
 }  // namespace lb

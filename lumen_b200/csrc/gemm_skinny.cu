@@ -70,9 +70,19 @@ __device__ __forceinline__ float widen16(uint16_t x) {
     return F16 ? __half2float(__ushort_as_half(x)) : __uint_as_float((uint32_t)x << 16);
 }
 
+struct SkinnyLossArgs : SkinnyArgs {
+    Targets targets;
+    SpanSum* spans;  // [block][M]
+    float* hit;
+};
+
+// PLAIN, GATED, LOSS: a product; the gated block's; the linear cross entropy's span sums.
+enum SkinnyKind : int { SKINNY_PLAIN, SKINNY_GATED, SKINNY_LOSS };
+
 // GATED: rows 0..7 of a tile are the gate's, 8..15 the other projection's. ROWS: 16, or 8 with the tile's second half empty. TOKENS: 8, 16 or 32.
-template <bool GATED, bool F16, int ROWS, int TOKENS>
-__global__ void __launch_bounds__(kMaxWarps * 32, 1) skinny_kernel(const SkinnyArgs p) {
+template <SkinnyKind KIND, bool F16, int ROWS, int TOKENS, class Args>
+__global__ void __launch_bounds__(kMaxWarps * 32, 1) skinny_kernel(const Args p) {
+    constexpr bool GATED = KIND == SKINNY_GATED;
     __shared__ float sums[kMaxWarps][16][TOKENS + 1];
     grid_wait();
     constexpr int TILES = TOKENS / 8;
@@ -118,6 +128,23 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) skinny_kernel(const SkinnyA
     constexpr int COLS = GATED ? 8 : ROWS;
     for (int i = threadIdx.x; i < COLS * TOKENS; i += blockDim.x) {
         const int c = i % COLS, m = i / COLS;
+        if constexpr (KIND == SKINNY_LOSS) {  // COLS lanes a token
+            float z = 0.0f;
+            for (int k = 0; k < p.warps; k++) z += sums[k][c][m];
+            const bool in = row0 + c < p.N;
+            float most = in ? z : -INFINITY;
+#pragma unroll
+            for (int d = COLS / 2; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            const float base = most == -INFINITY ? 0.0f : most;
+            float sum = in ? exp2_approx((z - base) * kLog2e) : 0.0f;
+#pragma unroll
+            for (int d = COLS / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (m < p.M) {
+                if (c == 0) p.spans[(long long)blockIdx.x * p.M + m] = SpanSum{most, sum};
+                if (in && p.targets.of(m) == row0 + c) p.hit[m] = z;
+            }
+            continue;
+        }
         if (m >= p.M || row0 + c >= p.N) continue;
         float a = 0.0f, b = 0.0f;
         for (int k = 0; k < p.warps; k++) {
@@ -140,26 +167,29 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) skinny_kernel(const SkinnyA
     }
 }
 
-template <bool GATED, bool F16>
-void launch_skinny(SkinnyArgs& p, int sms, cudaStream_t s) {
+// Rows of a block's tile: 16 where three quarters of the SMs get one, else 8. us of a gated block of 1 and 8 tokens in a graph, 8 -> 16: 512 columns 3.7, 4.1 -> 4.1,
+// 4.5; 1024 5.2, 6.2 -> 5.8, 6.9; 2048 21.6, 23.1 -> 20.0, 21.1; 2400 26.2, 25.3 -> 25.8, 24.5; 4096 72.2, 74.2 -> 67.3, 66.7
+int skinny_rows(long long N, int sms) { return (N + 15) / 16 * 4 >= 3 * sms ? 16 : 8; }
+
+template <SkinnyKind KIND, bool F16, class Args>
+void launch_skinny(Args& p, int sms, cudaStream_t s) {
+    constexpr bool GATED = KIND == SKINNY_GATED;
     const int blocks = (p.K + 31) / 32;
     // a warp takes some blocks of K at a time, all of them in flight: as many warps as that needs
     const int at_once = ahead(p.M <= 8 ? 8 : p.M <= 16 ? 16 : 32);
     p.warps = std::min(kMaxWarps, (blocks + at_once - 1) / at_once);
     p.per_warp = (blocks + p.warps - 1) / p.warps;
-    // rows of a block: 16 where three quarters of the SMs get one, else 8. us of a gated block of 1 and 8 tokens in a graph, 8 -> 16: 512 columns 3.7, 4.1 -> 4.1,
-    // 4.5; 1024 5.2, 6.2 -> 5.8, 6.9; 2048 21.6, 23.1 -> 20.0, 21.1; 2400 26.2, 25.3 -> 25.8, 24.5; 4096 72.2, 74.2 -> 67.3, 66.7
-    const int rows = GATED ? 8 : (p.N + 15) / 16 * 4 >= 3 * sms ? 16 : 8;
+    const int rows = GATED ? 8 : skinny_rows(p.N, sms);
     const dim3 grid((unsigned)((p.N + rows - 1) / rows)), block((unsigned)p.warps * 32);
     auto go = [&](auto kernel) { launch_overlapped(kernel, grid, block, 0, s, 0, p); };
     if (GATED || rows == 16) {
-        if (p.M <= 8) go(skinny_kernel<GATED, F16, 16, 8>);
-        else if (p.M <= 16) go(skinny_kernel<GATED, F16, 16, 16>);
-        else go(skinny_kernel<GATED, F16, 16, 32>);
-    } else {
-        if (p.M <= 8) go(skinny_kernel<false, F16, 8, 8>);
-        else if (p.M <= 16) go(skinny_kernel<false, F16, 8, 16>);
-        else go(skinny_kernel<false, F16, 8, 32>);
+        if (p.M <= 8) go(skinny_kernel<KIND, F16, 16, 8, Args>);
+        else if (p.M <= 16) go(skinny_kernel<KIND, F16, 16, 16, Args>);
+        else go(skinny_kernel<KIND, F16, 16, 32, Args>);
+    } else if constexpr (!GATED) {
+        if (p.M <= 8) go(skinny_kernel<KIND, F16, 8, 8, Args>);
+        else if (p.M <= 16) go(skinny_kernel<KIND, F16, 8, 16, Args>);
+        else go(skinny_kernel<KIND, F16, 8, 32, Args>);
     }
 }
 
@@ -188,15 +218,28 @@ void skinny_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, co
     SkinnyArgs p = skinny_args(x, w, h);
     p.act = act;
     if (kept) p.kept = kept->ptr, p.ld_kept = kept->stride[0];
-    if (x.dtype == LB_F16) launch_skinny<true, true>(p, device_info().sms, (cudaStream_t)stream);
-    else launch_skinny<true, false>(p, device_info().sms, (cudaStream_t)stream);
+    if (x.dtype == LB_F16) launch_skinny<SKINNY_GATED, true>(p, device_info().sms, (cudaStream_t)stream);
+    else launch_skinny<SKINNY_GATED, false>(p, device_info().sms, (cudaStream_t)stream);
 }
 void skinny_product(const lb_tensor& x, const lb_tensor& w, const lb_tensor& out, const lb_tensor* add, void* stream) {
     driver();
     SkinnyArgs p = skinny_args(x, w, out);
     if (add) p.add = add->ptr, p.ld_add = add->stride[0];
-    if (x.dtype == LB_F16) launch_skinny<false, true>(p, device_info().sms, (cudaStream_t)stream);
-    else launch_skinny<false, false>(p, device_info().sms, (cudaStream_t)stream);
+    if (x.dtype == LB_F16) launch_skinny<SKINNY_PLAIN, true>(p, device_info().sms, (cudaStream_t)stream);
+    else launch_skinny<SKINNY_PLAIN, false>(p, device_info().sms, (cudaStream_t)stream);
+}
+
+int skinny_spans(long long N) {
+    const int rows = skinny_rows(N, sm_count_hint());
+    return (int)((N + rows - 1) / rows);
+}
+void skinny_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, void* stream) {
+    driver();
+    SkinnyLossArgs p{};
+    (SkinnyArgs&)p = skinny_args(x, w, w);
+    p.N = (int)w.shape[0], p.out = nullptr, p.targets = targets, p.spans = spans, p.hit = hit;
+    if (x.dtype == LB_F16) launch_skinny<SKINNY_LOSS, true>(p, sm_count_hint(), (cudaStream_t)stream);
+    else launch_skinny<SKINNY_LOSS, false>(p, sm_count_hint(), (cudaStream_t)stream);
 }
 
 }  // namespace lb

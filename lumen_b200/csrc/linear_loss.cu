@@ -154,10 +154,20 @@ __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGra
     float scale = 1.0f;
     if (sizeof(T) == 2 && undo && all.most > 0.0f && all.most < INFINITY) scale = exp2f((float)max(-120, min(120, 13 - ilogbf(all.most / counted))));
     if (undo && blockIdx.x == 0 && threadIdx.x == 0) *undo = 1.0f / scale;
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vectors = x_col == 1 && D % V == 0 && ld_x % V == 0 && (uintptr_t)x % 16 == 0;
+    const int lane = threadIdx.x & 31;
+    for (long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32; row < rows; row += (long long)gridDim.x * 8) {  // a warp a row
         const int target = targets.of(row);
-        if (threadIdx.x == 0) g[row] = target < 0 ? 0.0f : grad.of(row) / counted * scale, classes[row] = target;
-        for (int c = threadIdx.x; c < D; c += 256) x_out[row * D + c] = target < 0 ? from_float<T>(0.0f) : x[row * ld_x + c * x_col];
+        if (lane == 0) g[row] = target < 0 ? 0.0f : grad.of(row) / counted * scale, classes[row] = target;
+        const T* from = x + row * ld_x;
+        T* to = x_out + row * D;
+        if (vectors) {
+#pragma unroll 4
+            for (int c = lane; c < D / V; c += 32) ((uint4*)to)[c] = target < 0 ? make_uint4(0u, 0u, 0u, 0u) : ((const uint4*)from)[c];
+        } else {
+            for (int c = lane; c < D; c += 32) to[c] = target < 0 ? from_float<T>(0.0f) : from[c * x_col];
+        }
     }
 }
 
@@ -328,8 +338,8 @@ struct Forward : Loss {
     }
     void run(cudaStream_t s, bool only_count) {
         held = 0;
-        const bool fused = T && gemm_loss_takes(x, w);
-        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, n_spans = fused ? gemm_spans(V) : pieces;
+        const bool few = T && skinny_takes(x, w), fused = few || (T && gemm_loss_takes(x, w));
+        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, n_spans = few ? skinny_spans(V) : fused ? gemm_spans(V) : pieces;
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
         const long long blocks = (T + R - 1) / R;
         SpanSum* spans = take<SpanSum>(n_spans * T);
@@ -342,7 +352,8 @@ struct Forward : Loss {
         void* product = take<char>(more);
         if (only_count) return;
         if (T) {
-            if (fused) gemm_loss(x, w, targets, spans, hit, s);
+            if (few) skinny_loss(x, w, targets, spans, hit, s);
+            else if (fused) gemm_loss(x, w, targets, spans, hit, s);
             for (long long k = 0; k < pieces && !fused; k++) {
                 const long long first = k * piece, cols = std::min(piece, V - first);
                 lb_tensor out = z;
@@ -396,9 +407,11 @@ struct Backward : Loss {
         char* x_kept = take<char>(T * D * item);
         float* logits = take<float>(fused ? 0 : T * ld);
         char* slopes = dtype == LB_F32 ? (char*)logits : take<char>(T * ld * item);
-        const bool folds = pieces > 1 || half;
-        float *dx_piece = folds ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr, *dw_piece = half ? take<float>(piece * D) : nullptr;
         const lb_tensor kept = matrix(x_kept, dtype, T, D, D), dz = matrix(slopes, dtype, T, piece, ld);
+        // sums over pieces, and what takes float16's scale away: in the products' epilogue where they run on whole tiles, else behind them
+        const bool folds = pieces > 1 || half, dx_tiles = folds && T && gemm_sum_takes(dz, rows_of(w, 0, piece), dx), dw_tiles = half && T && gemm_sum_takes(transposed(dz), kept, dw);
+        float *dx_piece = folds && !dx_tiles ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
+        float* dw_piece = half && !dw_tiles ? take<float>(piece * D) : nullptr;
         size_t more = 0;
         if (T) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
         void* product = take<char>(more);
@@ -411,7 +424,7 @@ struct Backward : Loss {
         launch_overlapped(count_kernel, dim3((unsigned)n_counts), dim3(256), 0, s, 0, targets, d_loss, T, counts);
         by_type(dtype, [&](auto* type) {
             using E = std::remove_pointer_t<decltype(type)>;
-            launch_overlapped(row_grads_kernel<E>, dim3(row_blocks(T)), dim3(256), 0, s, 0, targets, d_loss, T, (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
+            launch_overlapped(row_grads_kernel<E>, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
                               (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], (int)D, (E*)x_kept, g, classes, half ? undo : nullptr);
         });
         for (long long k = 0; k < pieces; k++) {
@@ -434,11 +447,19 @@ struct Backward : Loss {
                                       sum, begins, ends ? (E*)to.ptr : (E*)nullptr, (long long)to.stride[0], half ? (const float*)undo : (const float*)nullptr);
                 });
             };
-            const lb_tensor dw_out = half ? matrix(dw_piece, LB_F32, cols, D, D) : dw_rows;
-            gemm(transposed(d), kept, dw_out, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-            if (half) fold(dw_piece, dw_rows, nullptr, true, true);
-            gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-            if (folds) fold(dx_piece, dx, dx_sum, k == 0, k == pieces - 1);
+            const bool begins = k == 0, ends = k == pieces - 1;
+            if (dw_tiles) {
+                gemm_sum(transposed(d), kept, nullptr, true, &dw_rows, undo, s);
+            } else {
+                gemm(transposed(d), kept, half ? matrix(dw_piece, LB_F32, cols, D, D) : dw_rows, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+                if (half) fold(dw_piece, dw_rows, nullptr, true, true);
+            }
+            if (dx_tiles) {
+                gemm_sum(d, rows, dx_sum, begins, ends ? &dx : nullptr, half ? undo : nullptr, s);
+            } else {
+                gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+                if (folds) fold(dx_piece, dx, dx_sum, begins, ends);
+            }
         }
     }
 };
