@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <queue>
 #include <vector>
 
 #include "divide.cuh"
@@ -59,7 +60,7 @@ struct GemmArgs {
 // What the kernel for CTA pairs does with a tile: the epilogues of lb_gemm, or one half of the gated feed-forward block. In its forward products
 // the leader's half of the B columns are rows of one weight and the other CTA's the same rows of another, so that each CTA's accumulator holds both
 // projections of 128 columns side by side; in its backward product the epilogue reads what the forward pass has kept.
-enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED, PAIR_GROUP, PAIR_SPANS, PAIR_LOSS_SLOPES, PAIR_SUM };
+enum PairMode : int { PAIR_PLAIN, PAIR_GATED, PAIR_SLOPED, PAIR_GROUP, PAIR_SPANS, PAIR_LOSS_SLOPES, PAIR_SUM, PAIR_LISTED };
 struct PlainArgs : GemmArgs {
     static constexpr int mode = PAIR_PLAIN;
 };
@@ -82,8 +83,9 @@ struct SpansArgs : GemmArgs {
     SpanSum* spans;  // [2 * tiles_n][M]
     float* hit;
 };
-struct LossSlopesArgs : GemmArgs {
+struct alignas(64) LossSlopesArgs : GemmArgs {
     static constexpr int mode = PAIR_LOSS_SLOPES;
+    CUtensorMap map_d;  // pieces of 32 rows of 64
     const float *lse, *g;
     const int* classes;
     long long lse_step;
@@ -106,9 +108,22 @@ struct alignas(64) GroupArgs : GemmArgs {
     int first[kGroup];  // first unit of each, those that there are not beginning at the end
     int units;
 };
+// Two such products as PAIR_SUM takes them, whose units each pair takes from a list of its own: entry `unit` of the table is what the grid's unit `unit` is, kNone where a
+// pair has no more.
+constexpr int kListed = 8192, kNone = 0xffff;
+struct alignas(64) ListedArgs : GemmArgs {
+    static constexpr int mode = PAIR_LISTED;
+    CUtensorMap map_a[2], map_b[2];
+    SumArgs product[2];
+    int second;  // first unit of the second product
+    int units;   // entries of the table
+    uint16_t unit_of[kListed];
+};
+static_assert(sizeof(ListedArgs) <= 30000, "kernel parameters");
+
 // The product that a unit belongs to; `unit` becomes its number in it.
 template <class Args>
-__device__ __forceinline__ const GemmArgs& product_of(const Args& p, int& unit, int& which) {
+__device__ __forceinline__ const auto& product_of(const Args& p, int& unit, int& which) {
     which = 0;
     if constexpr (Args::mode == PAIR_GROUP) {
 #pragma unroll
@@ -116,10 +131,22 @@ __device__ __forceinline__ const GemmArgs& product_of(const Args& p, int& unit, 
             if (unit >= p.first[k]) which = k;
         unit -= p.first[which];
         return p.product[which];
+    } else if constexpr (Args::mode == PAIR_LISTED) {
+        which = unit >= p.second;
+        if (which) unit -= p.second;
+        return p.product[which];
     } else {
         return p;
     }
 }
+// What the grid's unit `unit` is; kNone: nothing, nor is any behind it.
+template <class Args>
+__device__ __forceinline__ int listed(const Args& p, int unit) {
+    if constexpr (Args::mode == PAIR_LISTED) return p.unit_of[unit];
+    else return unit;
+}
+template <class Args>
+constexpr bool many_products() { return Args::mode == PAIR_GROUP || Args::mode == PAIR_LISTED; }
 
 // Unit `unit` of the grid: split * tiles + tile, neighbours share a K range.
 __device__ __forceinline__ int tile_coords(const GemmArgs& p, int unit, int& b, int& m_blk, int& n_blk) {
@@ -522,13 +549,12 @@ __device__ __forceinline__ SpanSum drain_span(uint32_t tbase, int width, int tar
 }
 
 // A row's 128 columns of dz: (exp(z - lse) - [class]) g, rounded once. `target`: the class's column here; a row that does not count is zero whatever
-// its logits are.
+// its logits are. 32 rows of 64 columns leave by TMA at a time, from a place of the warp's own, which the next ones' exponentials leave time to be read out.
 template <bool F16, class Release>
-__device__ __forceinline__ void drain_slopes(const GemmArgs& p, uint32_t tbase, int row, int col_base, float lse, float g, bool counts, int target, uint4* stage, int lane,
+__device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t tbase, int row, int col_base, float lse, float g, bool counts, int target, uint4* stage, int lane,
                                              Release release) {
     const Pair scale = both(kLog2e, kLog2e), shift = both(lse * -kLog2e, lse * -kLog2e), weight = both(g, g);
-    const uint32_t keep = counts ? 0xffffffffu : 0u;
-    const int rows = p.M - (row - lane);
+    const uint32_t keep = counts ? 0xffffffffu : 0u, area = smem_u32(stage) + lane * 128;
 #pragma unroll 1
     for (int c2 = 0; c2 < BN / 2 / 64; c2++) {
         const int col0 = col_base + c2 * 64, span = p.N - col0, at = target - c2 * 64;
@@ -548,11 +574,16 @@ __device__ __forceinline__ void drain_slopes(const GemmArgs& p, uint32_t tbase, 
             for (int j = 0; j < 64; j++)
                 if (j == at) v[j] = __float_as_uint(__uint_as_float(v[j]) - 1.0f);
         }
-        uint4 packed[8];
-        uint32_t* w = (uint32_t*)packed;
+        uint32_t w[32];
 #pragma unroll
         for (int j = 0; j < 32; j++) w[j] = narrow<F16>(columns(v, j) * weight) & keep;
-        store_rows_coalesced<8>(stage, packed, (uint8_t*)((uint16_t*)p.d + (long long)(row - lane) * p.ldd + col0), p.ldd * 2, rows, lane, (span + 7) / 8);
+        if (lane == 0) bulk_wait_read();  // the place has been read out
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; q++) st_shared(area + ((q ^ (lane & 7)) << 4), make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]));
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && row < p.M) tma_store_3d(&p.map_d, stage, col0, row, 0), bulk_commit();  // (lane 0's is the warp's first row)
     }
 }
 
@@ -794,6 +825,10 @@ constexpr int pair_smem(int mode) {
 }
 static_assert(pair_smem(PAIR_SLOPED) <= 227 * 1024, "shared memory");
 
+// What leaves by TMA lies between the ring and the barriers, at a multiple of 1024 bytes.
+constexpr int pair_places(int mode) { return mode == PAIR_SLOPED ? 4 * kPieces * kPieceBytes : mode == PAIR_LOSS_SLOPES ? kEpilogueStageBytes : 0; }
+static_assert(PSTAGES * (kPairStageBytesA + kPairStageBytesB) % 1024 == 0, "swizzled places");
+
 template <class Args>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Args p) {
@@ -802,7 +837,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     uint8_t* smem = align_1024(smem_raw);
     uint8_t* smem_a = smem;
     uint8_t* smem_b = smem + STAGES_ * kPairStageBytesA;
-    uint64_t* full = (uint64_t*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + (Args::mode == PAIR_SLOPED ? 4 * kPieces * kPieceBytes : 0));
+    uint64_t* full = (uint64_t*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + pair_places(Args::mode));
     uint64_t* empty = full + STAGES_;
     uint64_t* tmem_full = empty + STAGES_;
     uint64_t* tmem_empty = tmem_full + 2;
@@ -814,7 +849,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const uint32_t rank = cluster_ctarank();
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
     int num_units;  // tiles_m counts 256-row pair tiles here
-    if constexpr (Args::mode == PAIR_GROUP) num_units = p.units;
+    if constexpr (many_products<Args>()) num_units = p.units;
     else num_units = p.tiles_m * p.tiles_n * p.batch * p.splits;
 
     if (threadIdx.x == 0) {
@@ -830,7 +865,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             for (int s = 0; s < 4 * kPieces; s++) mbar_init(&landed[s], 1);
         *abort_flag = 0;
         fence_barrier_init();
-        if constexpr (Args::mode != PAIR_GROUP) tma_prefetch_desc(&map_a), tma_prefetch_desc(&map_b);
+        if constexpr (!many_products<Args>()) tma_prefetch_desc(&map_a), tma_prefetch_desc(&map_b);
         if constexpr (Args::mode == PAIR_GATED) tma_prefetch_desc(&p.map_up);
     }
     if (warp == 1) {
@@ -851,13 +886,14 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             uint32_t phase = 0;
             bool ok = true;
             for (int unit = pair; unit < num_units && ok; unit += num_pairs) {
-                int at = unit, which, b, m_blk, n_blk;
+                int at = listed(p, unit), which, b, m_blk, n_blk;
+                if (Args::mode == PAIR_LISTED && at == kNone) break;
                 const GemmArgs& q = product_of(p, at, which);
                 const int total_kb = (q.K + BK - 1) / BK, kb0 = tile_coords(q, at, b, m_blk, n_blk) * q.kb_per_split;
                 const int row0 = m_blk * 2 * BM + (int)rank * BM;
                 int col0 = n_blk * BN + (int)rank * (BN / 2);
                 const CUtensorMap *operand_a = &map_a, *operand_b = &map_b;
-                if constexpr (Args::mode == PAIR_GROUP) operand_a = &p.map_a[which], operand_b = &p.map_b[which];
+                if constexpr (many_products<Args>()) operand_a = &p.map_a[which], operand_b = &p.map_b[which];
                 if constexpr (Args::mode == PAIR_GATED) {
                     col0 = n_blk * (BN / 2);
                     if (rank) operand_b = &p.map_up;
@@ -900,7 +936,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 db0 = q.b_mn_major ? make_smem_desc(smem_u32(smem_b), 64 * BK * 2, 1024) : make_smem_desc(smem_u32(smem_b), 16, 1024);
                 a_step = q.a_mn_major ? 2048u : 32u, b_step = q.b_mn_major ? 2048u : 32u;
             };
-            if constexpr (Args::mode != PAIR_GROUP) operands(p);
+            if constexpr (!many_products<Args>()) operands(p);
             int stage = 0;
             uint32_t phase = 0;
             int local = 0;
@@ -908,12 +944,13 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             for (int unit = pair; unit < num_units && ok; unit += num_pairs, local++) {
                 const int buf = local & 1;
                 const uint32_t use = (uint32_t)(local >> 1);
+                int at = listed(p, unit), which;
+                if (Args::mode == PAIR_LISTED && at == kNone) break;
                 if (!(ok = mbar_wait_cluster_warp(&tmem_empty[buf], (use & 1) ^ 1, abort_flag))) break;
                 tc_fence_after();
                 const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
-                int at = unit, which;
                 const GemmArgs& q = product_of(p, at, which);
-                if constexpr (Args::mode == PAIR_GROUP) operands(q);
+                if constexpr (many_products<Args>()) operands(q);
                 const int total_kb = (q.K + BK - 1) / BK, kb0 = (int)q.by_tiles.div(at) * q.kb_per_split;
                 const int num_kb = min(total_kb, kb0 + q.kb_per_split) - kb0;
                 for (int kb = 0; kb < num_kb; kb++) {
@@ -942,7 +979,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         // ---- epilogue: warps 2..9 of both CTAs, each CTA on its own 128 rows ----
         const int quarter = warp & 3;
         const int col_half = (warp - 2) >> 2;
-        uint4* stage = (uint4*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + 256) + (warp - 2) * (kStageBytesPerWarp / 16);
+        uint4* stage = (uint4*)(smem + STAGES_ * (kPairStageBytesA + kPairStageBytesB) + (Args::mode == PAIR_LOSS_SLOPES ? 0 : 256)) + (warp - 2) * (kStageBytesPerWarp / 16);
         int local = 0;
         bool ok = true;
         auto in_vectors = [](const GemmArgs& q) {
@@ -954,8 +991,9 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         for (int unit = pair; unit < num_units && ok; unit += num_pairs, local++) {
             const int buf = local & 1;
             const uint32_t use = (uint32_t)(local >> 1);
-            int at = unit, which, b, m_blk, n_blk;
-            const GemmArgs& q = product_of(p, at, which);
+            int at = listed(p, unit), which, b, m_blk, n_blk;
+            if (Args::mode == PAIR_LISTED && at == kNone) break;
+            const auto& q = product_of(p, at, which);
             const int split = tile_coords(q, at, b, m_blk, n_blk);
             const int row = m_blk * 2 * BM + (int)rank * BM + quarter * 32 + lane;
             auto release = [&] {
@@ -995,14 +1033,14 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 const bool counts = target >= 0;
                 if (p.d_f16) drain_slopes<true>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
                 else drain_slopes<false>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
-            } else if constexpr (Args::mode == PAIR_SUM) {
+            } else if constexpr (Args::mode == PAIR_SUM || Args::mode == PAIR_LISTED) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                if (p.d_f16) drain_sum<true>(p, tbase, row, col_base, stage, lane, release);
-                else drain_sum<false>(p, tbase, row, col_base, stage, lane, release);
+                if (q.d_f16) drain_sum<true>(q, tbase, row, col_base, stage, lane, release);
+                else drain_sum<false>(q, tbase, row, col_base, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_GROUP) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
@@ -1027,6 +1065,9 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     }
+
+    if constexpr (Args::mode == PAIR_LOSS_SLOPES)
+        if (warp >= 2 && lane == 0) bulk_wait();  // what leaves by TMA has left
 
     // ---- teardown: every role of both CTAs leaves its loop (normally, or because an abort flag was raised) ----
     tc_fence_before();
@@ -1123,7 +1164,7 @@ CUtensorMap make_map(const View3& v, bool contiguous_is_cols, int box_inner, int
     long long inner = contiguous_is_cols ? v.cols : v.rows, outer = contiguous_is_cols ? v.rows : v.cols;
     long long outer_stride = contiguous_is_cols ? v.sr : v.sc;
     cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)v.batch};
-    if (outer == 1) outer_stride = inner;
+    if (outer == 1) outer_stride = (inner + 7) / 8 * 8;
     cuuint64_t strides[2] = {(cuuint64_t)outer_stride * 2, (cuuint64_t)(v.batch > 1 ? v.sb : outer_stride * outer) * 2};
     cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer, 1};
     cuuint32_t elem[3] = {1, 1, 1};
@@ -1613,6 +1654,86 @@ void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begin
     if (out) p.d = out->ptr, p.ldd = out->stride[0];
     launch_pairs(p.a_mn_major ? make_map(a, false, 64, BK) : make_map(a, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p, tiles, stream);
 }
+// The units of two products in the order of the longer K, each to the pair that has least to do so far: us as in pairs_us. False where the table does not hold them.
+static bool list_units(const long long* tiles, const long long* blocks, int pairs, std::vector<std::vector<uint16_t>>& of, double& us) {
+    if (tiles[0] + tiles[1] >= kListed - pairs || tiles[0] + tiles[1] >= kNone) return false;
+    typedef std::pair<double, int> Load;
+    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
+    for (int k = 0; k < pairs; k++) least.push({0.0, k});
+    of.assign((size_t)pairs, {});
+    us = 0.0;
+    size_t most = 0;
+    int unit = 0;
+    for (int k = 0; k < 2; k++)
+        for (long long i = 0; i < tiles[k]; i++, unit++) {
+            Load l = least.top();
+            least.pop();
+            l.first += 0.3 * (double)blocks[k] + 2.0;
+            of[(size_t)l.second].push_back((uint16_t)unit);
+            most = std::max(most, of[(size_t)l.second].size()), us = std::max(us, l.first);
+            least.push(l);
+        }
+    us += 3.0 + 0.1 * (double)(tiles[0] * blocks[0] + tiles[1] * blocks[1]) / pairs;
+    return most * (size_t)pairs <= kListed;
+}
+static void listed_sizes(const lb_tensor* a, const lb_tensor* b, int* order, long long* tiles, long long* blocks) {
+    order[0] = a[0].shape[1] < a[1].shape[1], order[1] = 1 - order[0];
+    for (int k = 0; k < 2; k++) {
+        const lb_tensor &x = a[order[k]], &y = b[order[k]];
+        tiles[k] = (x.shape[0] + 2 * BM - 1) / (2 * BM) * ((y.shape[1] + BN - 1) / BN), blocks[k] = (x.shape[1] + BK - 1) / BK;
+    }
+}
+bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out) {
+    const int sms = sm_count_hint(), pairs = sms / 2;
+    double alone = 0.0, shared;
+    int order[2];
+    long long tiles[2], blocks[2];
+    listed_sizes(a, b, order, tiles, blocks);
+    for (int k = 0; k < 2; k++) {
+        const View3 x = view3(a[k], "a"), y = view3(b[k], "b");
+        bool a_cols, b_cols;
+        if (x.rows <= BM || y.cols % 8 || !tensor_core_operands(x, y, a_cols, b_cols) || !in_pieces(out[k])) return false;
+        const int split = gemm_splits(x.rows, y.cols, x.cols, 1, sms);
+        if (gemm_route(x.rows, y.cols, x.cols, 1, sms, 0, split > 1 ? gemm_scratch_bytes(x.rows, y.cols, x.cols, 1) : 0, nullptr).ranges) return false;
+        alone += pairs_us(k == order[0] ? tiles[0] : tiles[1], k == order[0] ? blocks[0] : blocks[1], split, pairs, (double)(x.rows * y.cols) * 1e-6);
+    }
+    std::vector<std::vector<uint16_t>> of;
+    return list_units(tiles, blocks, pairs, of, shared) && shared < alone;
+}
+void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, const bool* begins, const lb_tensor* const* out, const float* undo, void* stream) {
+    driver();
+    const DeviceInfo& dev = device_info();
+    ListedArgs p{};
+    int order[2];
+    long long tiles[2], blocks[2];
+    listed_sizes(a_t, b_t, order, tiles, blocks);
+    for (int k = 0; k < 2; k++) {
+        const int i = order[k];
+        const View3 a = view3(a_t[i], "a"), b = view3(b_t[i], "b"), w = turned(b);
+        bool a_cols, b_cols;
+        tensor_core_operands(a, b, a_cols, b_cols);
+        SumArgs& q = p.product[k];
+        pair_args(q, a, w, a_cols, !b_cols, BN, tiles[k]);
+        q.sum = sum[i], q.undo = undo, q.begins = begins[i], q.ends = out[i] != nullptr;
+        if (out[i]) q.d = out[i]->ptr, q.ldd = out[i]->stride[0];
+        p.map_a[k] = q.a_mn_major ? make_map(a, false, 64, BK) : make_map(a, true, BK, BM);
+        p.map_b[k] = q.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2);
+    }
+    p.second = (int)tiles[0], p.status = status_word();
+    first_use_on_device((const void*)gemm_tcgen05_pair<ListedArgs>, [] {
+        LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<ListedArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(PAIR_LISTED)));
+    });
+    const int resident = resident_pairs(dev), pairs = (int)std::min<long long>(tiles[0] + tiles[1], resident > 0 ? resident : dev.sms / 2);
+    std::vector<std::vector<uint16_t>> of;
+    double us;
+    if (!list_units(tiles, blocks, pairs, of, us)) fail(LB_ERR_UNSUPPORTED, "gemm: too many output tiles for one launch");
+    size_t most = 0;
+    for (const auto& list : of) most = std::max(most, list.size());
+    for (size_t slot = 0; slot < most; slot++)
+        for (int k = 0; k < pairs; k++) p.unit_of[slot * pairs + k] = slot < of[(size_t)k].size() ? of[(size_t)k][slot] : (uint16_t)kNone;
+    p.units = (int)most * pairs;
+    launch_overlapped(gemm_tcgen05_pair<ListedArgs>, dim3((unsigned)(2 * pairs)), dim3(kThreads), pair_smem(PAIR_LISTED), (cudaStream_t)stream, 0, p.map_a[0], p.map_b[0], p);
+}
 template <class Args>
 static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, void* stream) {
     driver();
@@ -1633,7 +1754,7 @@ void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, 
                       void* stream) {
     LossSlopesArgs p{};
     p.lse = lse, p.lse_step = lse_step, p.g = g, p.classes = classes, p.first = first;
-    p.d = dz.ptr, p.ldd = dz.stride[0];
+    p.map_d = make_map(view3(dz, "dz"), true, 64, 32);
     launch_loss(p, x, w, stream);
 }
 

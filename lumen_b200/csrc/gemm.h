@@ -104,6 +104,10 @@ void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, 
 bool gemm_sum_takes(const lb_tensor& a, const lb_tensor& b, const lb_tensor& out);
 void gemm_sum(const lb_tensor& a, const lb_tensor& b, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream);
 
+// Two of them that do not depend on one another in one launch; `_pay`: whether layouts are theirs and the model of pairs says that they gain by it.
+bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out);
+void gemm_sums(const lb_tensor* a, const lb_tensor* b, float* const* sum, const bool* begins, const lb_tensor* const* out, const float* undo, void* stream);
+
 // A few tokens (gemm_skinny.cu): out [M, N] = x [M, K] w^T with w [N, K], plus `add` [M, N] once rounded (null: nothing); h and kept as in gemm_gated.
 bool skinny_takes(const lb_tensor& x, const lb_tensor& w);
 void skinny_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, const lb_tensor* kept, int act, void* stream);

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(256) count_kernel(Targets targets, LossGrad gr
 // of dz is far below float16's smallest values; `undo` is what takes it away again.
 template <class T>
 __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGrad grad, long long rows, const RowCount* counts, int n_counts, bool mean, const T* x, long long ld_x,
-                                                        long long x_col, int D, T* x_out, float* g, int* classes, float* undo) {
+                                                        long long x_col, int D, T* x_out, long long ld_out, float* g, int* classes, float* undo) {
     __shared__ RowCount held[8];
     grid_wait();
     RowCount all{0, 0.0f};
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGra
         const int target = targets.of(row);
         if (lane == 0) g[row] = target < 0 ? 0.0f : grad.of(row) / counted * scale, classes[row] = target;
         const T* from = x + row * ld_x;
-        T* to = x_out + row * D;
+        T* to = x_out + row * ld_out;
         if (vectors) {
 #pragma unroll 4
             for (int c = lane; c < D / V; c += 32) ((uint4*)to)[c] = target < 0 ? make_uint4(0u, 0u, 0u, 0u) : ((const uint4*)from)[c];
@@ -399,17 +399,20 @@ struct Backward : Loss {
         const int item = dtype_size(dtype);
         const bool half = dtype == LB_F16;
         const bool fused = T && gemm_loss_takes(x, w);
-        const long long piece = piece_of(fused ? 2 : 4), pieces = (V + piece - 1) / piece, ld = up(piece, 8);
+        const long long piece = piece_of(fused ? 2 : 4), pieces = (V + piece - 1) / piece, ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
         const int n_counts = (int)std::min<long long>(64, (T + 255) / 256);
         RowCount* counts = take<RowCount>(n_counts);
         float *g = take<float>(T), *undo = take<float>(1);
         int* classes = take<int>(T);
-        char* x_kept = take<char>(T * D * item);
+        char* x_kept = take<char>(T * ld_kept * item);
         float* logits = take<float>(fused ? 0 : T * ld);
         char* slopes = dtype == LB_F32 ? (char*)logits : take<char>(T * ld * item);
-        const lb_tensor kept = matrix(x_kept, dtype, T, D, D), dz = matrix(slopes, dtype, T, piece, ld);
+        const lb_tensor kept = matrix(x_kept, dtype, T, D, ld_kept), dz = matrix(slopes, dtype, T, piece, ld);
         // sums over pieces, and what takes float16's scale away: in the products' epilogue where they run on whole tiles, else behind them
-        const bool folds = pieces > 1 || half, dx_tiles = folds && T && gemm_sum_takes(dz, rows_of(w, 0, piece), dx), dw_tiles = half && T && gemm_sum_takes(transposed(dz), kept, dw);
+        // (both in one launch where that fills the GPU better)
+        const lb_tensor sums_a[] = {transposed(dz), dz}, sums_b[] = {kept, rows_of(w, 0, piece)}, sums_out[] = {dw, dx};
+        const bool folds = pieces > 1 || half, both = T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
+                   dw_tiles = both || (half && T && gemm_sum_takes(sums_a[0], sums_b[0], dw));
         float *dx_piece = folds && !dx_tiles ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
         float* dw_piece = half && !dw_tiles ? take<float>(piece * D) : nullptr;
         size_t more = 0;
@@ -425,14 +428,14 @@ struct Backward : Loss {
         by_type(dtype, [&](auto* type) {
             using E = std::remove_pointer_t<decltype(type)>;
             launch_overlapped(row_grads_kernel<E>, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
-                              (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], (int)D, (E*)x_kept, g, classes, half ? undo : nullptr);
+                              (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], (int)D, (E*)x_kept, ld_kept, g, classes, half ? undo : nullptr);
         });
         for (long long k = 0; k < pieces; k++) {
             const long long first = k * piece, cols = std::min(piece, V - first);
             const lb_tensor rows = rows_of(w, first, cols);
             lb_tensor z = matrix(logits, LB_F32, T, cols, ld), d = dz, dw_rows = rows_of(dw, first, cols);
             d.shape[1] = cols;
-            if (fused) gemm_loss_slopes(x, rows, (const float*)lse.ptr, lse.stride[0], g, classes, (int)first, d, s);
+            if (fused) gemm_loss_slopes(kept, rows, (const float*)lse.ptr, lse.stride[0], g, classes, (int)first, d, s);
             else gemm(x, transposed(rows), z, EPI_NONE, 0, s, product, more, nullptr, nullptr);
             if (!fused) by_type(dtype, [&](auto* type) {
                 using E = std::remove_pointer_t<decltype(type)>;
@@ -448,6 +451,14 @@ struct Backward : Loss {
                 });
             };
             const bool begins = k == 0, ends = k == pieces - 1;
+            if (both) {
+                const lb_tensor a[] = {transposed(d), d}, b[] = {kept, rows};
+                float* const sum[] = {nullptr, dx_sum};
+                const bool first_of[] = {true, begins};
+                const lb_tensor* const out[] = {&dw_rows, ends ? &dx : nullptr};
+                gemm_sums(a, b, sum, first_of, out, half ? undo : nullptr, s);
+                continue;
+            }
             if (dw_tiles) {
                 gemm_sum(transposed(d), kept, nullptr, true, &dw_rows, undo, s);
             } else {

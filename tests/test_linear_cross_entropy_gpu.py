@@ -86,7 +86,7 @@ SHAPES = [
     (1, 64, 256), (1, 1024, 5000), (2, 8, 1), (2, 16, 2), (3, 40, 7), (4, 256, 30011), (7, 136, 129), (8, 512, 4096), (9, 64, 1000), (16, 328, 2048), (17, 72, 5003),
     (31, 104, 127), (32, 512, 513), (33, 64, 128), (61, 1024, 4099), (100, 264, 255), (127, 40, 257), (128, 128, 256), (129, 256, 1031), (200, 8, 12000),
     (256, 128, 256), (257, 520, 385), (300, 1120, 3001), (511, 72, 129), (700, 8, 8), (1000, 320, 1160), (1531, 96, 700), (2600, 64, 520), (5000, 16, 40),
-    (20000, 8, 9), (5, 15, 9), (40, 33, 70), (130, 100, 61), (600, 24, 1), (65, 4096, 300),
+    (20000, 8, 9), (5, 15, 9), (40, 33, 70), (130, 100, 61), (600, 24, 1), (65, 4096, 300), (1400, 520, 4001), (2600, 840, 3001), (3000, 264, 10000),
 ]  # fmt: skip
 
 
