@@ -216,6 +216,11 @@ __device__ __forceinline__ float inverse(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// With one step of Newton's iteration, for what a whole block's codes are found by: near the middle of two codes a unit in the last place decides.
+__device__ __forceinline__ float inverse_refined(float x) {
+    const float r = inverse(x);
+    return fmaf(fmaf(-x, r, 1.0f), r, r);
+}
 
 // Codes `m` and `v`, weights and gradients of a lane's eight elements after a step; the block's scales in `sm` and `sv`.
 //
@@ -242,7 +247,7 @@ __device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, fl
     }
     const float most_m = warp_most(top_m), most_v = warp_most(top_v);
     const bool no_m = most_m < 0x1p-100f, no_v = most_v < 0x1p-100f;
-    const float inv_m = no_m ? 0.0f : 448.0f * inverse(most_m), inv_v = no_v ? 0.0f : 448.0f * inverse(most_v);
+    const float inv_m = no_m ? 0.0f : 448.0f * inverse_refined(most_m), inv_v = no_v ? 0.0f : 448.0f * inverse_refined(most_v);
     sm = no_m ? 0.0f : most_m * (1.0f / 448.0f), sv = no_v ? 0.0f : most_v * (1.0f / 448.0f);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -389,15 +394,17 @@ void run_adamw(const lb_adamw_desc* desc, const lb_tensor* params, const lb_tens
     scalar(step, {LB_F32, LB_I32, LB_I64}, "the step count (float32, int32 or int64)");
     scalar(lr, {LB_F32}, "the learning rate (float32)"), scalar(norm, {LB_F32}, "the norm (float32)");
 
+    static const char* const names[] = {"parameter", "gradient", "first moment", "second moment", "float32 copy", "scales", "step count", "learning rate", "norm"};
+    if (n >= 1 << 24) fail(LB_ERR_UNSUPPORTED, "adamw: too many tensors");
     std::vector<Place> places;
     places.reserve((size_t)n * 7 + 3);
     std::vector<long long> count((size_t)n);
-    auto look = [&](const lb_tensor& t, const lb_tensor& like, int dtype, const char* what, int k, bool written) {
-        if (t.rank < 0 || t.rank > LB_MAX_RANK) refuse(format("%s %d has rank %d", what, k, t.rank));
-        if (t.dtype != dtype) refuse(format("%s %d is %s, not %s", what, k, dtype_name(t.dtype), dtype_name(dtype)));
-        if (!same_order(t, like)) refuse(format("%s %d must have its parameter's shape and strides", what, k));
-        if (count[k] && (!t.ptr || (uintptr_t)t.ptr % dtype_size(dtype))) refuse(format("%s %d has no memory or is not aligned to its elements", what, k));
-        places.push_back({(uintptr_t)t.ptr, (uintptr_t)t.ptr + (size_t)count[k] * dtype_size(dtype), what, k, written});
+    auto look = [&](const lb_tensor& t, const lb_tensor& like, int dtype, uint32_t what, int k, bool written) {
+        if (t.rank < 0 || t.rank > LB_MAX_RANK) refuse(format("%s %d has rank %d", names[what], k, t.rank));
+        if (t.dtype != dtype) refuse(format("%s %d is %s, not %s", names[what], k, dtype_name(t.dtype), dtype_name(dtype)));
+        if (!same_order(t, like)) refuse(format("%s %d must have its parameter's shape and strides", names[what], k));
+        if (count[k] && (!t.ptr || (uintptr_t)t.ptr % dtype_size(dtype))) refuse(format("%s %d has no memory or is not aligned to its elements", names[what], k));
+        places.push_back({(uintptr_t)t.ptr, (uintptr_t)t.ptr + (size_t)count[k] * dtype_size(dtype), (uint32_t)k, what, written});
     };
     for (int k = 0; k < n; k++) {
         const lb_tensor& p = params[k];
@@ -406,12 +413,12 @@ void run_adamw(const lb_adamw_desc* desc, const lb_tensor* params, const lb_tens
         count[k] = dense_elements(p);
         if (count[k] < 0) refuse(format("parameter %d is not dense", k));
         if (count[k] / chunk_elements(32) >= INT32_MAX / kMost) fail(LB_ERR_UNSUPPORTED, format("adamw: parameter %d has too many elements", k));
-        look(p, p, p.dtype, "parameter", k, true);
-        look(grads[k], p, grads[k].dtype == LB_F32 ? LB_F32 : p.dtype, "gradient", k, false);
-        look(ms[k], p, bits == 8 ? LB_U8 : LB_F32, "first moment", k, true), look(vs[k], p, bits == 8 ? LB_U8 : LB_F32, "second moment", k, true);
+        look(p, p, p.dtype, 0, k, true);
+        look(grads[k], p, grads[k].dtype == LB_F32 ? LB_F32 : p.dtype, 1, k, false);
+        look(ms[k], p, bits == 8 ? LB_U8 : LB_F32, 2, k, true), look(vs[k], p, bits == 8 ? LB_U8 : LB_F32, 3, k, true);
         if (masters && masters[k].ptr && count[k]) {
             if (p.dtype == LB_F32) refuse(format("parameter %d is float32 itself: it has no float32 copy", k));
-            look(masters[k], p, LB_F32, "float32 copy", k, true);
+            look(masters[k], p, LB_F32, 4, k, true);
         }
         for (const lb_tensor* scales : {m_scales, v_scales}) {
             if (!scales) continue;
@@ -420,13 +427,13 @@ void run_adamw(const lb_adamw_desc* desc, const lb_tensor* params, const lb_tens
             if (t.dtype != LB_F32 || t.rank != 1 || t.shape[0] != blocks || (blocks > 1 && t.stride[0] != 1))
                 refuse(format("the scales of parameter %d must be dense float32 [%lld], one for %d elements", k, blocks, kBlock));
             if (blocks && (!t.ptr || (uintptr_t)t.ptr % 4)) refuse(format("the scales of parameter %d have no memory or are not aligned", k));
-            places.push_back({(uintptr_t)t.ptr, (uintptr_t)t.ptr + (size_t)blocks * 4, "scales", k, true});
+            places.push_back({(uintptr_t)t.ptr, (uintptr_t)t.ptr + (size_t)blocks * 4, (uint32_t)k, 5, true});
         }
     }
     for (const lb_tensor* t : {step, lr, norm})
-        if (t) places.push_back({(uintptr_t)t->ptr, (uintptr_t)t->ptr + dtype_size(t->dtype), t == step ? "step count" : t == lr ? "learning rate" : "norm", 0, false});
+        if (t) places.push_back({(uintptr_t)t->ptr, (uintptr_t)t->ptr + dtype_size(t->dtype), 0, t == step ? 6u : t == lr ? 7u : 8u, false});
     const Place *a, *b;
-    if (meeting(places, a, b)) refuse(format("%s %d and %s %d share memory", a->what, a->index, b->what, b->index));
+    if (meeting(places, a, b)) refuse(format("%s %d and %s %d share memory", names[a->what], (int)a->index, names[b->what], (int)b->index));
     driver();
 
     const int grid = device_info().sms * 2;

@@ -48,12 +48,10 @@ __device__ __forceinline__ int tensor_of(const Table& t, int c) {
 }
 #endif
 
-// The memory of a list's tensors, to find two places that share some of it.
+// The memory of the tensors of a call, to find two places that share some of it: `index` and `what` are the caller's.
 struct Place {
     uintptr_t from, to;
-    const char* what;
-    int index;
-    bool written;
+    uint32_t index : 24, what : 7, written : 1;
 };
 // Two places of which one is written and that share memory; false where there are none. Sorts the places.
 inline bool meeting(std::vector<Place>& places, const Place*& a, const Place*& b) {

@@ -36,19 +36,30 @@ __device__ __forceinline__ SpanSum block_join(SpanSum v, SpanSum* held) {
     return v;
 }
 
-// The span sums of logits that lie in memory, float32 [rows, cols], columns `first` and on of the vocabulary; and the target's logit where it is among them.
+// The span sums of logits that lie in memory, float32 [rows, cols], columns `first` and on of the vocabulary, a span of kSpan columns a block; and the target's
+// logit where it is among them.
+constexpr int kEach = 16, kSpan = kRowThreads * kEach;
 __global__ void __launch_bounds__(kRowThreads) span_kernel(const float* logits, long long ld, long long rows, int first, int cols, Targets targets, SpanSum* spans, float* hit) {
     __shared__ SpanSum held[kRowThreads / 32];
     grid_wait();
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int from = blockIdx.x * kSpan;
+    for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
         const float* z = logits + row * ld;
-        SpanSum v{-INFINITY, 0.0f};
-        for (int c = threadIdx.x; c < cols; c += kRowThreads) v = join(v, SpanSum{z[c], 1.0f});
-        v = block_join(v, held);
+        float v[kEach], most = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kEach; k++) {
+            const int c = from + threadIdx.x + k * kRowThreads;
+            v[k] = c < cols ? z[c] : -INFINITY, most = fmaxf(most, v[k]);
+        }
+        const float base = most == -INFINITY ? 0.0f : most;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kEach; k++) sum += exp2_approx((v[k] - base) * kLog2e);
+        const SpanSum all = block_join({most, sum}, held);
         if (threadIdx.x == 0) {
-            spans[row] = v;
+            spans[blockIdx.x * rows + row] = all;
             const int target = targets.of(row) - first;
-            if (target >= 0 && target < cols) hit[row] = z[target];
+            if (target >= from && target < min(cols, from + kSpan)) hit[row] = z[target];
         }
     }
 }
@@ -148,7 +159,12 @@ __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGra
     __shared__ RowCount held[8];
     grid_wait();
     RowCount all{0, 0.0f};
-    for (int k = threadIdx.x; k < n_counts; k += 256) all.counted += counts[k].counted, all.most = fmaxf(all.most, counts[k].most);
+    if (counts) {
+        for (int k = threadIdx.x; k < n_counts; k += 256) all.counted += counts[k].counted, all.most = fmaxf(all.most, counts[k].most);
+    } else {
+        for (long long row = threadIdx.x; row < rows; row += 256)
+            if (targets.of(row) >= 0) all.counted++, all.most = fmaxf(all.most, fabsf(grad.of(row)));
+    }
     all = block_count(all, held);
     const float counted = mean ? (float)max(all.counted, 1LL) : 1.0f;
     float scale = 1.0f;
@@ -176,10 +192,10 @@ template <class T>
 __global__ void __launch_bounds__(kRowThreads) slope_kernel(const float* logits, long long ld, long long rows, int first, int cols, const float* lse, long long lse_step,
                                                             const float* g, const int* classes, T* out, long long ld_out) {
     grid_wait();
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
         const float all = lse[row * lse_step], scale = g[row];
         const int at = classes[row], target = at - first;
-        for (int c = threadIdx.x; c < cols; c += kRowThreads)
+        for (int c = blockIdx.x * kRowThreads + threadIdx.x; c < cols; c += gridDim.x * kRowThreads)
             out[row * ld_out + c] = from_float<T>(at < 0 ? 0.0f : (expf(logits[row * ld + c] - all) - (c == target ? 1.0f : 0.0f)) * scale);
     }
 }
@@ -189,11 +205,13 @@ template <class T>
 __global__ void __launch_bounds__(256) fold_kernel(const float* product, long long rows, int D, float* sum, bool begins, T* out, long long ld_out, const float* undo) {
     grid_wait();
     const float scale = undo ? *undo : 1.0f;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * D; i += (long long)gridDim.x * 256) {
-        const float v = begins ? product[i] : sum[i] + product[i];
-        if (out) out[i / D * ld_out + i % D] = from_float<T>(v * scale);
-        else sum[i] = v;
-    }
+    for (long long row = blockIdx.y; row < rows; row += gridDim.y)
+        for (int c = blockIdx.x * 256 + threadIdx.x; c < D; c += gridDim.x * 256) {
+            const long long i = row * D + c;
+            const float v = begins ? product[i] : sum[i] + product[i];
+            if (out) out[row * ld_out + c] = from_float<T>(v * scale);
+            else sum[i] = v;
+        }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -318,6 +336,11 @@ void by_type(int dtype, F f) {
     else if (dtype == LB_BF16) f((__nv_bfloat16*)nullptr);
     else f((__half*)nullptr);
 }
+// A grid of rows by columns (`across` a block): whole columns first, rows in turn beyond 16 blocks an SM.
+dim3 by_rows(long long rows, long long cols, int across) {
+    const long long x = std::max(1LL, (cols + across - 1) / across);
+    return dim3((unsigned)x, (unsigned)std::min<long long>(std::max(1LL, rows), std::max(1LL, sm_count_hint() * 16 / x)));
+}
 unsigned row_blocks(long long rows) { return (unsigned)std::min<long long>(std::max(1LL, rows), (long long)sm_count_hint() * 16); }
 
 struct Forward : Loss {
@@ -339,7 +362,8 @@ struct Forward : Loss {
     void run(cudaStream_t s, bool only_count) {
         held = 0;
         const bool few = T && skinny_takes(x, w), fused = few || (T && gemm_loss_takes(x, w));
-        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, n_spans = few ? skinny_spans(V) : fused ? gemm_spans(V) : pieces;
+        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, each = (piece + kSpan - 1) / kSpan, last = (V - (pieces - 1) * piece + kSpan - 1) / kSpan,
+                        n_spans = few ? skinny_spans(V) : fused ? gemm_spans(V) : (pieces - 1) * each + last;
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
         const long long blocks = (T + R - 1) / R;
         SpanSum* spans = take<SpanSum>(n_spans * T);
@@ -359,7 +383,7 @@ struct Forward : Loss {
                 lb_tensor out = z;
                 out.shape[1] = cols;
                 gemm(x, transposed(rows_of(w, first, cols)), out, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-                launch_overlapped(span_kernel, dim3(row_blocks(T)), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, targets, spans + k * T, hit);
+                launch_overlapped(span_kernel, by_rows(T, cols, kSpan), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, targets, spans + k * each * T, hit);
             }
             auto join_rows = [&](auto kernel) {
                 launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, s, 0, (const SpanSum*)spans, (int)n_spans, T, (const float*)hit, targets, (float*)lse.ptr,
@@ -424,10 +448,11 @@ struct Backward : Loss {
             return;
         }
         const LossGrad d_loss{(const float*)grad.ptr, grad.stride[0]};
-        launch_overlapped(count_kernel, dim3((unsigned)n_counts), dim3(256), 0, s, 0, targets, d_loss, T, counts);
+        const bool counts_itself = T <= 1024;  // every block: a launch (2 us) costs more than that
+        if (!counts_itself) launch_overlapped(count_kernel, dim3((unsigned)n_counts), dim3(256), 0, s, 0, targets, d_loss, T, counts);
         by_type(dtype, [&](auto* type) {
             using E = std::remove_pointer_t<decltype(type)>;
-            launch_overlapped(row_grads_kernel<E>, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
+            launch_overlapped(row_grads_kernel<E>, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, counts_itself ? (const RowCount*)nullptr : (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
                               (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], (int)D, (E*)x_kept, ld_kept, g, classes, half ? undo : nullptr);
         });
         for (long long k = 0; k < pieces; k++) {
@@ -439,14 +464,13 @@ struct Backward : Loss {
             else gemm(x, transposed(rows), z, EPI_NONE, 0, s, product, more, nullptr, nullptr);
             if (!fused) by_type(dtype, [&](auto* type) {
                 using E = std::remove_pointer_t<decltype(type)>;
-                launch_overlapped(slope_kernel<E>, dim3(row_blocks(T)), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, (const float*)lse.ptr,
+                launch_overlapped(slope_kernel<E>, by_rows(T, cols, 4 * kRowThreads), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, (const float*)lse.ptr,
                                   (long long)lse.stride[0], (const float*)g, (const int*)classes, (E*)slopes, ld);
             });
             auto fold = [&](const float* from, const lb_tensor& to, float* sum, bool begins, bool ends) {
                 by_type(dtype, [&](auto* type) {
                     using E = std::remove_pointer_t<decltype(type)>;
-                    const long long n = to.shape[0] * D;
-                    launch_overlapped(fold_kernel<E>, dim3((unsigned)std::min<long long>((n + 255) / 256, device_info().sms * 8LL)), dim3(256), 0, s, 0, from, (long long)to.shape[0], (int)D,
+                    launch_overlapped(fold_kernel<E>, by_rows(to.shape[0], D, 256), dim3(256), 0, s, 0, from, (long long)to.shape[0], (int)D,
                                       sum, begins, ends ? (E*)to.ptr : (E*)nullptr, (long long)to.stride[0], half ? (const float*)undo : (const float*)nullptr);
                 });
             };
@@ -457,6 +481,14 @@ struct Backward : Loss {
                 const bool first_of[] = {true, begins};
                 const lb_tensor* const out[] = {&dw_rows, ends ? &dx : nullptr};
                 gemm_sums(a, b, sum, first_of, out, half ? undo : nullptr, s);
+                continue;
+            }
+            if (dtype == LB_F32) {  // what leaves SMs idle by itself shares a launch
+                SimtProblem q[2];
+                gemm(transposed(d), kept, dw_rows, EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, &q[0]);
+                gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, &q[1]);
+                gemm_simt_many(q, 2, device_info().sms, true, s);
+                if (folds) fold(dx_piece, dx, dx_sum, begins, ends);
                 continue;
             }
             if (dw_tiles) {

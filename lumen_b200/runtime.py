@@ -235,6 +235,10 @@ class _Torch:
         return cls.empty_like(t, memory_format=cls.dense)
 
     @classmethod
+    def float32_like(cls, t):
+        return cls.empty_like(t, dtype=cls.float32, memory_format=cls.dense)
+
+    @classmethod
     def stream(cls) -> int:
         return cls.raw_stream(cls.device())
 
@@ -506,8 +510,13 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", ignore_index=-100
     is `ignore_index` does not count; other targets are clamped into the vocabulary. float16, bfloat16 or float32. Bit-identical from call to call; the
     same rows among others may differ by a rounding."""
     require_cuda()
-    code, shape = _reduction(reduction), tuple(targets.shape)
-    (loss, lse), handle = _outputs(x, stream, (() if code else shape, "float32"), (shape, "float32"))
+    code = _reduction(reduction)
+    if _Torch.takes(x, stream) and type(targets) is _Torch.tensor:
+        lse, handle = _Torch.float32_like(targets), _Torch.stream()
+        loss = x.new_empty((), dtype=_Torch.float32) if code else _Torch.float32_like(targets)
+    else:
+        shape = tuple(targets.shape)
+        (loss, lse), handle = _outputs(x, stream, (() if code else shape, "float32"), (shape, "float32"))
     _lib.host().linear_cross_entropy(code, ignore_index, x, weight, targets, loss, lse, _scratch(x, stream), handle)
     return loss, lse
 
@@ -578,8 +587,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     handle = _Torch.stream() if _Torch.takes(params[0], stream) else _stream(stream)
     _lib.host().adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, masters, step, lr, *betas, eps, weight_decay, norm,
                            0.0 if max_norm is None else max_norm, handle)  # fmt: skip
-    for tensors in (params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
-        if tensors:
-            _written(tensors)
+    changed = [*params, *exp_avg, *exp_avg_sq]
+    if exp_avg_scale:
+        changed += [*exp_avg_scale, *exp_avg_sq_scale]
     if masters:
-        _written([t for t in masters if t is not None])
+        changed += [t for t in masters if t is not None]
+    _written(changed)
