@@ -55,7 +55,13 @@ struct GemmArgs {
     // unit writes a float32 partial tile to `partial` [splits][batch][M][N] and splitk_reduce adds them in order
     int splits, kb_per_split;
     float* partial;
+    // float32 operands in three parts of bfloat16 each (the modes that take them): K blocks of a part, 0: none; elements from a part to the next along the
+    // contiguous axis. Six of the nine products of parts are added up, the smallest first.
+    int part_kb, a_part, b_part;
 };
+// Which parts of A and B the products take, two bits each: (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0).
+constexpr int kPartProducts = 6;
+constexpr uint32_t kPartsOfA = 0x052u, kPartsOfB = 0x118u;
 
 // What the kernel for CTA pairs does with a tile: the epilogues of lb_gemm, or one half of the gated feed-forward block. In its forward products
 // the leader's half of the B columns are rows of one weight and the other CTA's the same rows of another, so that each CTA's accumulator holds both
@@ -80,12 +86,14 @@ struct alignas(64) SlopedArgs : GemmArgs {
 struct SpansArgs : GemmArgs {
     static constexpr int mode = PAIR_SPANS;
     Targets targets;
+    int first;       // the class of the first column
     SpanSum* spans;  // [2 * tiles_n][M]
     float* hit;
 };
 struct alignas(64) LossSlopesArgs : GemmArgs {
     static constexpr int mode = PAIR_LOSS_SLOPES;
     CUtensorMap map_d;  // pieces of 32 rows of 64
+    int d_part;         // float32 operands: dz's parts are as far apart
     const float *lse, *g;
     const int* classes;
     long long lse_step;
@@ -96,7 +104,7 @@ struct SumArgs : GemmArgs {
     static constexpr int mode = PAIR_SUM;
     float* sum;
     const float* undo;  // what the rounded result is multiplied by; null: nothing
-    int begins, ends;
+    int begins, ends, d_f32;
 };
 
 // Up to three products of one launch, one after another in the grid, each without an epilogue and its K whole.
@@ -144,6 +152,15 @@ template <class Args>
 __device__ __forceinline__ int listed(const Args& p, int unit) {
     if constexpr (Args::mode == PAIR_LISTED) return p.unit_of[unit];
     else return unit;
+}
+// The modes that take operands in parts, and the K blocks of a product of theirs.
+template <class Args>
+constexpr bool in_parts() { return Args::mode == PAIR_SPANS || Args::mode == PAIR_LOSS_SLOPES || Args::mode == PAIR_SUM || Args::mode == PAIR_LISTED; }
+template <class Args>
+__device__ __forceinline__ int k_blocks(const GemmArgs& q) {
+    const int whole = (q.K + BK - 1) / BK;
+    if constexpr (in_parts<Args>()) return q.part_kb ? kPartProducts * q.part_kb : whole;
+    return whole;
 }
 template <class Args>
 constexpr bool many_products() { return Args::mode == PAIR_GROUP || Args::mode == PAIR_LISTED; }
@@ -550,7 +567,9 @@ __device__ __forceinline__ SpanSum drain_span(uint32_t tbase, int width, int tar
 
 // A row's 128 columns of dz: (exp(z - lse) - [class]) g, rounded once. `target`: the class's column here; a row that does not count is zero whatever
 // its logits are. 32 rows of 64 columns leave by TMA at a time, from a place of the warp's own, which the next ones' exponentials leave time to be read out.
-template <bool F16, class Release>
+// FORM: bfloat16, float16, or float32 in three parts of bfloat16, each what the ones before leave, rounded; columns behind the last are zero there, as K's end is of a product's operand.
+enum SlopeForm { SLOPE_BF16, SLOPE_F16, SLOPE_PARTS };
+template <SlopeForm FORM, class Release>
 __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t tbase, int row, int col_base, float lse, float g, bool counts, int target, uint4* stage, int lane,
                                              Release release) {
     const Pair scale = both(kLog2e, kLog2e), shift = both(lse * -kLog2e, lse * -kLog2e), weight = both(g, g);
@@ -574,16 +593,39 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
             for (int j = 0; j < 64; j++)
                 if (j == at) v[j] = __float_as_uint(__uint_as_float(v[j]) - 1.0f);
         }
-        uint32_t w[32];
+        if (FORM == SLOPE_PARTS) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) w[j] = narrow<F16>(columns(v, j) * weight) & keep;
-        if (lane == 0) bulk_wait_read();  // the place has been read out
-        __syncwarp();
+            for (int j = 0; j < 32; j++) {
+                const float2 d = apart(columns(v, j) * weight);
+                v[2 * j] = __float_as_uint(d.x) & keep, v[2 * j + 1] = __float_as_uint(d.y) & keep;
+            }
+            if (LB_RARELY(span < 64)) {
 #pragma unroll
-        for (int q = 0; q < 8; q++) st_shared(area + ((q ^ (lane & 7)) << 4), make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]));
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0 && row < p.M) tma_store_3d(&p.map_d, stage, col0, row, 0), bulk_commit();  // (lane 0's is the warp's first row)
+                for (int j = 0; j < 64; j++)
+                    if (j >= span) v[j] = 0u;
+            }
+        }
+#pragma unroll 1
+        for (int part = 0; part < (FORM == SLOPE_PARTS ? 3 : 1); part++) {
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                if (FORM == SLOPE_PARTS) {
+                    w[j] = narrow<false>(columns(v, j));
+                    const float2 rest = apart(columns(v, j) + -widen<false>(w[j]));
+                    v[2 * j] = __float_as_uint(rest.x), v[2 * j + 1] = __float_as_uint(rest.y);
+                } else {
+                    w[j] = narrow<FORM == SLOPE_F16>(columns(v, j) * weight) & keep;
+                }
+            }
+            if (lane == 0) bulk_wait_read();  // the place has been read out
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 8; q++) st_shared(area + ((q ^ (lane & 7)) << 4), make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]));
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0 && row < p.M) tma_store_3d(&p.map_d, stage, col0 + part * p.d_part, row, 0), bulk_commit();  // (lane 0's is the warp's first row)
+        }
     }
 }
 
@@ -593,6 +635,8 @@ __device__ __forceinline__ void drain_sum(const SumArgs& p, uint32_t tbase, int 
     const int rows = p.M - (row - lane);
     const float scale = p.undo ? *p.undo : 1.0f;
     float* sum0 = p.sum + (long long)(row - lane) * p.N;  // the warp's first row
+    const long long out_ld = p.ends ? p.ldd : p.N;         // where float32 values go
+    float* out0 = p.ends ? (float*)p.d + (row - lane) * p.ldd : sum0;
 #pragma unroll 1
     for (int c2 = 0; c2 < BN / 2 / 64; c2++) {
         const int col0 = col_base + c2 * 64, span = p.N - col0;
@@ -611,7 +655,7 @@ __device__ __forceinline__ void drain_sum(const SumArgs& p, uint32_t tbase, int 
                 v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + h.z), v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + h.w);
             }
         }
-        if (p.ends) {
+        if (p.ends && !p.d_f32) {
             uint4 packed[8];
             uint32_t* w = (uint32_t*)packed;
 #pragma unroll
@@ -620,7 +664,7 @@ __device__ __forceinline__ void drain_sum(const SumArgs& p, uint32_t tbase, int 
         } else {
 #pragma unroll
             for (int h = 0; h < 2; h++)
-                store_rows_coalesced<8>(stage, (const uint4*)(v + h * 32), (uint8_t*)(sum0 + col0 + h * 32), (long long)p.N * 4, rows, lane, (span - h * 32) / 4);
+                store_rows_coalesced<8>(stage, (const uint4*)(v + h * 32), (uint8_t*)(out0 + col0 + h * 32), out_ld * 4, rows, lane, (span - h * 32) / 4);
         }
     }
 }
@@ -889,7 +933,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 int at = listed(p, unit), which, b, m_blk, n_blk;
                 if (Args::mode == PAIR_LISTED && at == kNone) break;
                 const GemmArgs& q = product_of(p, at, which);
-                const int total_kb = (q.K + BK - 1) / BK, kb0 = tile_coords(q, at, b, m_blk, n_blk) * q.kb_per_split;
+                const int total_kb = k_blocks<Args>(q), kb0 = tile_coords(q, at, b, m_blk, n_blk) * q.kb_per_split;
                 const int row0 = m_blk * 2 * BM + (int)rank * BM;
                 int col0 = n_blk * BN + (int)rank * (BN / 2);
                 const CUtensorMap *operand_a = &map_a, *operand_b = &map_b;
@@ -904,17 +948,24 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     if (rank == 0) mbar_expect_tx(&full[stage], 2 * (kPairStageBytesA + kPairStageBytesB));
                     uint8_t* sa = smem_a + stage * kPairStageBytesA;
                     uint8_t* sb = smem_b + stage * kPairStageBytesB;
+                    int k = kb * BK, in_a = 0, in_b = 0;
+                    if constexpr (in_parts<Args>())
+                        if (q.part_kb) {
+                            const int product = kb / q.part_kb;
+                            k -= product * q.part_kb * BK;
+                            in_a = (int)(kPartsOfA >> 2 * product & 3) * q.a_part, in_b = (int)(kPartsOfB >> 2 * product & 3) * q.b_part;
+                        }
                     if (!q.a_mn_major) {
-                        tma_load_3d_pair(sa, operand_a, &full[stage], kb * BK, row0, b);  // box {64 k, 128 m}
+                        tma_load_3d_pair(sa, operand_a, &full[stage], k + in_a, row0, b);  // box {64 k, 128 m}
                     } else {
                         for (int j = 0; j < BM / 64; j++)  // boxes {64 m, 64 k}
-                            tma_load_3d_pair(sa + j * (64 * BK * 2), operand_a, &full[stage], row0 + j * 64, kb * BK, b);
+                            tma_load_3d_pair(sa + j * (64 * BK * 2), operand_a, &full[stage], row0 + j * 64 + in_a, k, b);
                     }
                     if (!q.b_mn_major) {
-                        tma_load_3d_pair(sb, operand_b, &full[stage], kb * BK, col0, b);  // box {64 k, 128 n}
+                        tma_load_3d_pair(sb, operand_b, &full[stage], k + in_b, col0, b);  // box {64 k, 128 n}
                     } else {
                         for (int j = 0; j < BN / 2 / 64; j++)  // boxes {64 n, 64 k}
-                            tma_load_3d_pair(sb + j * (64 * BK * 2), operand_b, &full[stage], col0 + j * 64, kb * BK, b);
+                            tma_load_3d_pair(sb + j * (64 * BK * 2), operand_b, &full[stage], col0 + j * 64 + in_b, k, b);
                     }
                     if (++stage == STAGES_) {
                         stage = 0;
@@ -951,7 +1002,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
                 const GemmArgs& q = product_of(p, at, which);
                 if constexpr (many_products<Args>()) operands(q);
-                const int total_kb = (q.K + BK - 1) / BK, kb0 = (int)q.by_tiles.div(at) * q.kb_per_split;
+                const int total_kb = k_blocks<Args>(q), kb0 = (int)q.by_tiles.div(at) * q.kb_per_split;
                 const int num_kb = min(total_kb, kb0 + q.kb_per_split) - kb0;
                 for (int kb = 0; kb < num_kb; kb++) {
                     if (!(ok = mbar_wait_warp(&full[stage], phase, abort_flag))) break;
@@ -1014,7 +1065,7 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else if (p.act == ACT_GELU) drain_gated<ACT_GELU, true>(p, tbase, row, col0, stage, lane, release);
                 else drain_gated<ACT_RELU, true>(p, tbase, row, col0, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_SPANS) {
-                const int col_base = n_blk * BN + col_half * (BN / 2), target = row < p.M ? p.targets.of(row) - col_base : -1;
+                const int col_base = n_blk * BN + col_half * (BN / 2), target = row < p.M ? p.targets.of(row) - p.first - col_base : -1;
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
                 __syncwarp();
                 tc_fence_after();
@@ -1031,8 +1082,9 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 tc_fence_after();
                 const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
                 const bool counts = target >= 0;
-                if (p.d_f16) drain_slopes<true>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
-                else drain_slopes<false>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
+                if (p.d_part) drain_slopes<SLOPE_PARTS>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
+                else if (p.d_f16) drain_slopes<SLOPE_F16>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
+                else drain_slopes<SLOPE_BF16>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_SUM || Args::mode == PAIR_LISTED) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
@@ -1635,6 +1687,15 @@ bool gemm_loss_takes(const lb_tensor& x, const lb_tensor& w) {
     return tensor_core_operands(view3(x, "x"), turned(view3(w, "w")), x_cols, w_rows);
 }
 int gemm_spans(long long N) { return (int)((N + BN - 1) / BN * 2); }
+// The map of an operand, its rows along K (k_major) or across it; `part`: the parts of float32 values lie as far apart along the contiguous axis.
+static CUtensorMap operand_map(View3 v, bool k_major, int rows, long long part) {
+    if (part) (k_major ? v.cols : v.rows) = 3 * part;
+    return k_major ? make_map(v, true, BK, rows) : make_map(v, false, 64, BK);
+}
+static void set_parts(GemmArgs& p, const Parts& parts) {
+    if (!parts.a) return;
+    p.part_kb = (p.K + BK - 1) / BK, p.kb_per_split = kPartProducts * p.part_kb, p.a_part = (int)parts.a, p.b_part = (int)parts.b;
+}
 bool gemm_sum_takes(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& out) {
     const View3 a = view3(a_t, "a"), b = view3(b_t, "b");
     bool a_cols, b_cols;
@@ -1642,7 +1703,7 @@ bool gemm_sum_takes(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor&
     const GemmRoute route = gemm_route(a.rows, b.cols, a.cols, 1, sm_count_hint(), 0, gemm_scratch_bytes(a.rows, b.cols, a.cols, 1), nullptr);
     return route.ranges == 0 && route.splits == 1;
 }
-void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream) {
+void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream, Parts parts) {
     driver();
     const View3 a = view3(a_t, "a"), b = view3(b_t, "b"), w = turned(b);
     bool a_cols, b_cols;
@@ -1650,9 +1711,10 @@ void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begin
     SumArgs p{};
     long long tiles;
     pair_args(p, a, w, a_cols, !b_cols, BN, tiles);
+    set_parts(p, parts);
     p.sum = sum, p.undo = undo, p.begins = begins, p.ends = out != nullptr;
-    if (out) p.d = out->ptr, p.ldd = out->stride[0];
-    launch_pairs(p.a_mn_major ? make_map(a, false, 64, BK) : make_map(a, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p, tiles, stream);
+    if (out) p.d = out->ptr, p.ldd = out->stride[0], p.d_f32 = out->dtype == LB_F32;
+    launch_pairs(operand_map(a, a_cols, BM, parts.a), operand_map(w, !b_cols, BN / 2, parts.b), p, tiles, stream);
 }
 // The units of two products in the order of the longer K, each to the pair that has least to do so far: us as in pairs_us. False where the table does not hold them.
 static bool list_units(const long long* tiles, const long long* blocks, int pairs, std::vector<std::vector<uint16_t>>& of, double& us) {
@@ -1676,11 +1738,11 @@ static bool list_units(const long long* tiles, const long long* blocks, int pair
     us += 3.0 + 0.1 * (double)(tiles[0] * blocks[0] + tiles[1] * blocks[1]) / pairs;
     return most * (size_t)pairs <= kListed;
 }
-static void listed_sizes(const lb_tensor* a, const lb_tensor* b, int* order, long long* tiles, long long* blocks) {
+static void listed_sizes(const lb_tensor* a, const lb_tensor* b, int* order, long long* tiles, long long* blocks, bool parts) {
     order[0] = a[0].shape[1] < a[1].shape[1], order[1] = 1 - order[0];
     for (int k = 0; k < 2; k++) {
         const lb_tensor &x = a[order[k]], &y = b[order[k]];
-        tiles[k] = (x.shape[0] + 2 * BM - 1) / (2 * BM) * ((y.shape[1] + BN - 1) / BN), blocks[k] = (x.shape[1] + BK - 1) / BK;
+        tiles[k] = (x.shape[0] + 2 * BM - 1) / (2 * BM) * ((y.shape[1] + BN - 1) / BN), blocks[k] = (x.shape[1] + BK - 1) / BK * (parts ? kPartProducts : 1);
     }
 }
 bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out) {
@@ -1688,7 +1750,7 @@ bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out)
     double alone = 0.0, shared;
     int order[2];
     long long tiles[2], blocks[2];
-    listed_sizes(a, b, order, tiles, blocks);
+    listed_sizes(a, b, order, tiles, blocks, false);
     for (int k = 0; k < 2; k++) {
         const View3 x = view3(a[k], "a"), y = view3(b[k], "b");
         bool a_cols, b_cols;
@@ -1700,13 +1762,22 @@ bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out)
     std::vector<std::vector<uint16_t>> of;
     return list_units(tiles, blocks, pairs, of, shared) && shared < alone;
 }
-void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, const bool* begins, const lb_tensor* const* out, const float* undo, void* stream) {
+bool gemm_sums_fit(const lb_tensor* a, const lb_tensor* b) {
+    int order[2];
+    long long tiles[2], blocks[2];
+    listed_sizes(a, b, order, tiles, blocks, true);
+    std::vector<std::vector<uint16_t>> of;
+    double us;
+    return list_units(tiles, blocks, sm_count_hint() / 2, of, us);
+}
+void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, const bool* begins, const lb_tensor* const* out, const float* undo, void* stream,
+               const Parts* parts) {
     driver();
     const DeviceInfo& dev = device_info();
     ListedArgs p{};
     int order[2];
     long long tiles[2], blocks[2];
-    listed_sizes(a_t, b_t, order, tiles, blocks);
+    listed_sizes(a_t, b_t, order, tiles, blocks, parts != nullptr);
     for (int k = 0; k < 2; k++) {
         const int i = order[k];
         const View3 a = view3(a_t[i], "a"), b = view3(b_t[i], "b"), w = turned(b);
@@ -1714,10 +1785,11 @@ void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, co
         tensor_core_operands(a, b, a_cols, b_cols);
         SumArgs& q = p.product[k];
         pair_args(q, a, w, a_cols, !b_cols, BN, tiles[k]);
+        const Parts part = parts ? parts[i] : Parts{};
+        set_parts(q, part);
         q.sum = sum[i], q.undo = undo, q.begins = begins[i], q.ends = out[i] != nullptr;
-        if (out[i]) q.d = out[i]->ptr, q.ldd = out[i]->stride[0];
-        p.map_a[k] = q.a_mn_major ? make_map(a, false, 64, BK) : make_map(a, true, BK, BM);
-        p.map_b[k] = q.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2);
+        if (out[i]) q.d = out[i]->ptr, q.ldd = out[i]->stride[0], q.d_f32 = out[i]->dtype == LB_F32;
+        p.map_a[k] = operand_map(a, a_cols, BM, part.a), p.map_b[k] = operand_map(w, !b_cols, BN / 2, part.b);
     }
     p.second = (int)tiles[0], p.status = status_word();
     first_use_on_device((const void*)gemm_tcgen05_pair<ListedArgs>, [] {
@@ -1735,27 +1807,29 @@ void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, co
     launch_overlapped(gemm_tcgen05_pair<ListedArgs>, dim3((unsigned)(2 * pairs)), dim3(kThreads), pair_smem(PAIR_LISTED), (cudaStream_t)stream, 0, p.map_a[0], p.map_b[0], p);
 }
 template <class Args>
-static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, void* stream) {
+static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, const Parts& parts, void* stream) {
     driver();
     const View3 x = view3(x_t, "x"), w = view3(w_t, "w");
     bool x_cols, w_rows;
     tensor_core_operands(x, turned(w), x_cols, w_rows);
     long long tiles;
     pair_args(p, x, w, x_cols, !w_rows, BN, tiles);
-    launch_pairs(p.a_mn_major ? make_map(x, false, 64, BK) : make_map(x, true, BK, BM), p.b_mn_major ? make_map(w, false, 64, BK) : make_map(w, true, BK, BN / 2), p, tiles,
-                 stream);
+    set_parts(p, parts);
+    launch_pairs(operand_map(x, x_cols, BM, parts.a), operand_map(w, !w_rows, BN / 2, parts.b), p, tiles, stream);
 }
-void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, void* stream) {
+void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, int first, SpanSum* spans, float* hit, void* stream, Parts parts) {
     SpansArgs p{};
-    p.targets = targets, p.spans = spans, p.hit = hit;
-    launch_loss(p, x, w, stream);
+    p.targets = targets, p.first = first, p.spans = spans, p.hit = hit;
+    launch_loss(p, x, w, parts, stream);
 }
 void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,
-                      void* stream) {
+                      void* stream, Parts parts, long long dz_part) {
     LossSlopesArgs p{};
-    p.lse = lse, p.lse_step = lse_step, p.g = g, p.classes = classes, p.first = first;
-    p.map_d = make_map(view3(dz, "dz"), true, 64, 32);
-    launch_loss(p, x, w, stream);
+    p.lse = lse, p.lse_step = lse_step, p.g = g, p.classes = classes, p.first = first, p.d_part = (int)dz_part;
+    View3 d = view3(dz, "dz");
+    if (dz_part) d.cols = 3 * dz_part;
+    p.map_d = make_map(d, true, 64, 32);
+    launch_loss(p, x, w, parts, stream);
 }
 
 }  // namespace lb

@@ -91,22 +91,31 @@ bool gemm_group_pays(const lb_tensor* a, const lb_tensor* b, int n);
 void gemm_group(const lb_tensor* a, const lb_tensor* b, const lb_tensor* d, int n, void* stream);
 
 // The linear cross entropy's products z = x w^T with their epilogues, 16-bit operands on CTA pairs: x [M, K], w [N, K]. Forward: each row's span sums, `spans`
-// [gemm_spans(N)][M], and its target's logit. Backward: dz [M, N] = (exp(z - lse) - [class]) g, where `w` holds the classes from `first` on; a row of class -1 is
+// [gemm_spans(N)][M], and its target's logit; `first`: the class of w's first row. Backward: dz [M, N] = (exp(z - lse) - [class]) g, where `w` holds the classes from `first` on; a row of class -1 is
 // zero, and columns up to the next multiple of eight may be written. `_takes`: whether the operands' layouts are theirs.
+//
+// float32 operands come in three parts of bfloat16: tensors of that type and of the operand's size, whose other parts lie `Parts` elements further along the
+// contiguous axis each (behind the first along K: zeros up to a multiple of 64). A product is then the sum of six of parts, which lacks 2^-23 of it.
+struct Parts {
+    long long a = 0, b = 0;  // 0: 16-bit operands, whole
+};
 bool gemm_loss_takes(const lb_tensor& x, const lb_tensor& w);
 int gemm_spans(long long N);
-void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, void* stream);
+void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, int first, SpanSum* spans, float* hit, void* stream, Parts parts = {});
 void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,
-                      void* stream);
+                      void* stream, Parts parts = {}, long long dz_part = 0);
 
-// sum + a b on CTA pairs, `sum` dense float32 [M, N] (nothing where it `begins`): rounded into `out`, times *undo unless that is null, or, with a null `out`, into sum.
+// sum + a b on CTA pairs, `sum` dense float32 [M, N] (nothing where it `begins`): rounded into `out` (float32 or the operands' type), times *undo unless that is null, or, with a null `out`, into sum.
 // `_takes`: whether layouts are theirs (`out` stands for all rows of the result) and lb_gemm would take whole K on pairs.
 bool gemm_sum_takes(const lb_tensor& a, const lb_tensor& b, const lb_tensor& out);
-void gemm_sum(const lb_tensor& a, const lb_tensor& b, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream);
+void gemm_sum(const lb_tensor& a, const lb_tensor& b, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream, Parts parts = {});
 
 // Two of them that do not depend on one another in one launch; `_pay`: whether layouts are theirs and the model of pairs says that they gain by it.
 bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out);
-void gemm_sums(const lb_tensor* a, const lb_tensor* b, float* const* sum, const bool* begins, const lb_tensor* const* out, const float* undo, void* stream);
+// `_fit`: whether two products of parts are few enough tiles for it.
+bool gemm_sums_fit(const lb_tensor* a, const lb_tensor* b);
+void gemm_sums(const lb_tensor* a, const lb_tensor* b, float* const* sum, const bool* begins, const lb_tensor* const* out, const float* undo, void* stream,
+               const Parts* parts = nullptr);
 
 // A few tokens (gemm_skinny.cu): out [M, N] = x [M, K] w^T with w [N, K], plus `add` [M, N] once rounded (null: nothing); h and kept as in gemm_gated.
 bool skinny_takes(const lb_tensor& x, const lb_tensor& w);

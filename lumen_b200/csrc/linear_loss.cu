@@ -187,6 +187,42 @@ __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGra
     }
 }
 
+// float32 values in three parts of bfloat16, [rows][3][part] with zeros behind the columns: the value rounded, what that leaves rounded, and the rest, 24 bits in all.
+// Infinities become the largest finite values (a product of one with a part that is zero would be NaN); NaN stays. Rows of class -1 are zero.
+__global__ void __launch_bounds__(256) parts_kernel(const float* from, long long row_step, long long col_step, long long rows, int cols, int part, const int* classes,
+                                                    __nv_bfloat16* to) {
+    grid_wait();
+    constexpr float kMost = 3.3895313892515355e38f;  // bfloat16's
+    const bool vectors = col_step == 1 && row_step % 4 == 0 && cols % 4 == 0 && (uintptr_t)from % 16 == 0;
+    for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
+        const bool there = !classes || classes[row] >= 0;
+        const float* x = from + row * row_step;
+        __nv_bfloat16* out = to + row * 3 * part;
+        for (int c = (blockIdx.x * 256 + threadIdx.x) * 4; c < part; c += gridDim.x * 1024) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (there && c < cols) {
+                if (vectors) {
+                    const float4 w = *(const float4*)(x + c);
+                    v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (c + j < cols) v[j] = x[(c + j) * col_step];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (!isnan(v[j])) v[j] = fminf(fmaxf(v[j], -kMost), kMost);
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+                *(uint2*)(out + (long long)k * part + c) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+                v[0] -= __low2float(a), v[1] -= __high2float(a), v[2] -= __low2float(b), v[3] -= __high2float(b);
+            }
+        }
+    }
+}
+
 // dz of logits that lie in memory; may take their place.
 template <class T>
 __global__ void __launch_bounds__(kRowThreads) slope_kernel(const float* logits, long long ld, long long rows, int first, int cols, const float* lse, long long lse_step,
@@ -317,9 +353,12 @@ struct Loss {
         in_memory(r, what);
         return r;
     }
-    // The vocabulary in pieces whose [T, piece] of `item` bytes an element takes about kPieceBytes.
-    long long piece_of(int item) const {
-        const long long most = std::max(256LL, kPieceBytes / item / std::max(1LL, T) / 256 * 256);
+    // Whether float32 operands go to the tensor cores in parts of 16 bits: six products of them take less than one of float32 on the CUDA cores where there are enough rows
+    // for what it takes to split the weights (16 bytes an element in all, 70 rows' products there) and enough to do for two launches more.
+    bool in_parts() const { return dtype == LB_F32 && T > 64 && (double)T * (double)V * (double)D >= 3e8; }
+    // The vocabulary in pieces whose [width, piece] of `item` bytes an element takes about kPieceBytes.
+    long long piece_of(int item, long long width) const {
+        const long long most = std::max(256LL, kPieceBytes / item / std::max(1LL, width) / 256 * 256);
         return std::min(V, most);
     }
 };
@@ -330,6 +369,12 @@ lb_tensor rows_of(const lb_tensor& m, long long first, long long count) {
     r.ptr = (char*)m.ptr + first * m.stride[0] * dtype_size(m.dtype), r.shape[0] = count;
     return r;
 }
+// Rows that a float32 result of the tensor-core kernels is stored to in vectors.
+bool in_vectors(const lb_tensor& t) { return (uintptr_t)t.ptr % 16 == 0 && t.stride[1] == 1 && (t.shape[0] <= 1 || (t.stride[0] % 8 == 0 && t.stride[0] >= t.shape[1])); }
+// float32 values in parts, as a tensor of the first of them.
+lb_tensor parted(void* ptr, long long rows, long long cols, long long part) { return matrix(ptr, LB_BF16, rows, cols, 3 * part); }
+void split(const lb_tensor& t, const int* classes, const lb_tensor& to, cudaStream_t s);
+
 template <class F>
 void by_type(int dtype, F f) {
     if (dtype == LB_F32) f((float*)nullptr);
@@ -342,6 +387,12 @@ dim3 by_rows(long long rows, long long cols, int across) {
     return dim3((unsigned)x, (unsigned)std::min<long long>(std::max(1LL, rows), std::max(1LL, sm_count_hint() * 16 / x)));
 }
 unsigned row_blocks(long long rows) { return (unsigned)std::min<long long>(std::max(1LL, rows), (long long)sm_count_hint() * 16); }
+
+void split(const lb_tensor& t, const int* classes, const lb_tensor& to, cudaStream_t s) {
+    const long long part = to.stride[0] / 3;
+    launch_overlapped(parts_kernel, by_rows(t.shape[0], part, 1024), dim3(256), 0, s, 0, (const float*)t.ptr, (long long)t.stride[0], (long long)t.stride[1], (long long)t.shape[0],
+                      (int)t.shape[1], (int)part, classes, (__nv_bfloat16*)to.ptr);
+}
 
 struct Forward : Loss {
     using Loss::Loss;
@@ -361,25 +412,33 @@ struct Forward : Loss {
     }
     void run(cudaStream_t s, bool only_count) {
         held = 0;
-        const bool few = T && skinny_takes(x, w), fused = few || (T && gemm_loss_takes(x, w));
-        const long long piece = piece_of(4), pieces = (V + piece - 1) / piece, each = (piece + kSpan - 1) / kSpan, last = (V - (pieces - 1) * piece + kSpan - 1) / kSpan,
-                        n_spans = few ? skinny_spans(V) : fused ? gemm_spans(V) : (pieces - 1) * each + last;
+        const bool few = T && skinny_takes(x, w), parts = in_parts(), fused = few || (T && gemm_loss_takes(x, w));
+        const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(4, T), pieces = (V + piece - 1) / piece, each = (piece + kSpan - 1) / kSpan, last = (V - (pieces - 1) * piece + kSpan - 1) / kSpan,
+                        n_spans = few ? skinny_spans(V) : fused ? gemm_spans(V) : parts ? (pieces - 1) * gemm_spans(piece) + gemm_spans(V - (pieces - 1) * piece) : (pieces - 1) * each + last;
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
         const long long blocks = (T + R - 1) / R;
         SpanSum* spans = take<SpanSum>(n_spans * T);
         float* hit = take<float>(T);
         LossSum* sums = reduction == LB_REDUCTION_NONE ? nullptr : take<LossSum>(blocks);
         const long long ld = up(piece, 8);
-        float* logits = take<float>(fused ? 0 : T * ld);
+        float* logits = take<float>(fused || parts ? 0 : T * ld);
+        char *x_parts = take<char>(parts ? T * 6 * part : 0), *w_parts = take<char>(parts ? piece * 6 * part : 0);
         const lb_tensor z = matrix(logits, LB_F32, T, piece, ld);
-        const size_t more = T && !fused ? product_scratch(x, transposed(rows_of(w, 0, piece))) : 0;
+        const size_t more = T && !fused && !parts ? product_scratch(x, transposed(rows_of(w, 0, piece))) : 0;
         void* product = take<char>(more);
         if (only_count) return;
         if (T) {
             if (few) skinny_loss(x, w, targets, spans, hit, s);
-            else if (fused) gemm_loss(x, w, targets, spans, hit, s);
+            else if (fused) gemm_loss(x, w, targets, 0, spans, hit, s);
+            if (parts) split(x, nullptr, parted(x_parts, T, D, part), s);
             for (long long k = 0; k < pieces && !fused; k++) {
                 const long long first = k * piece, cols = std::min(piece, V - first);
+                if (parts) {
+                    const lb_tensor rows = parted(w_parts, cols, D, part);
+                    split(rows_of(w, first, cols), nullptr, rows, s);
+                    gemm_loss(parted(x_parts, T, D, part), rows, targets, (int)first, spans + k * gemm_spans(piece) * T, hit, s, {part, part});
+                    continue;
+                }
                 lb_tensor out = z;
                 out.shape[1] = cols;
                 gemm(x, transposed(rows_of(w, first, cols)), out, EPI_NONE, 0, s, product, more, nullptr, nullptr);
@@ -422,25 +481,25 @@ struct Backward : Loss {
         held = 0;
         const int item = dtype_size(dtype);
         const bool half = dtype == LB_F16;
-        const bool fused = T && gemm_loss_takes(x, w);
-        const long long piece = piece_of(fused ? 2 : 4), pieces = (V + piece - 1) / piece, ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
+        const bool fused = T && gemm_loss_takes(x, w), parts = in_parts() && D % 8 == 0 && in_vectors(dx) && in_vectors(dw);
+        const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(fused ? 2 : 4, T), pieces = (V + piece - 1) / piece, ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
         const int n_counts = (int)std::min<long long>(64, (T + 255) / 256);
         RowCount* counts = take<RowCount>(n_counts);
         float *g = take<float>(T), *undo = take<float>(1);
         int* classes = take<int>(T);
-        char* x_kept = take<char>(T * ld_kept * item);
-        float* logits = take<float>(fused ? 0 : T * ld);
-        char* slopes = dtype == LB_F32 ? (char*)logits : take<char>(T * ld * item);
+        char *x_kept = take<char>(parts ? T * 6 * part : T * ld_kept * item), *w_parts = take<char>(parts ? piece * 6 * part : 0);
+        float* logits = take<float>(fused || parts ? 0 : T * ld);
+        char* slopes = parts ? take<char>(T * 6 * ld) : dtype == LB_F32 ? (char*)logits : take<char>(T * ld * item);
         const lb_tensor kept = matrix(x_kept, dtype, T, D, ld_kept), dz = matrix(slopes, dtype, T, piece, ld);
         // sums over pieces, and what takes float16's scale away: in the products' epilogue where they run on whole tiles, else behind them
         // (both in one launch where that fills the GPU better)
         const lb_tensor sums_a[] = {transposed(dz), dz}, sums_b[] = {kept, rows_of(w, 0, piece)}, sums_out[] = {dw, dx};
-        const bool folds = pieces > 1 || half, both = T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
+        const bool folds = pieces > 1 || half, both = !parts && T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
                    dw_tiles = both || (half && T && gemm_sum_takes(sums_a[0], sums_b[0], dw));
-        float *dx_piece = folds && !dx_tiles ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
+        float *dx_piece = folds && !dx_tiles && !parts ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
         float* dw_piece = half && !dw_tiles ? take<float>(piece * D) : nullptr;
         size_t more = 0;
-        if (T) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
+        if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
         void* product = take<char>(more);
         if (only_count) return;
         if (T == 0) {
@@ -453,11 +512,28 @@ struct Backward : Loss {
         by_type(dtype, [&](auto* type) {
             using E = std::remove_pointer_t<decltype(type)>;
             launch_overlapped(row_grads_kernel<E>, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, counts_itself ? (const RowCount*)nullptr : (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
-                              (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], (int)D, (E*)x_kept, ld_kept, g, classes, half ? undo : nullptr);
+                              (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], parts ? 0 : (int)D, (E*)x_kept, ld_kept, g, classes, half ? undo : nullptr);
         });
+        if (parts) split(x, classes, parted(x_kept, T, D, part), s);
         for (long long k = 0; k < pieces; k++) {
             const long long first = k * piece, cols = std::min(piece, V - first);
             const lb_tensor rows = rows_of(w, first, cols);
+            if (parts) {
+                const lb_tensor xp = parted(x_kept, T, D, part), wp = parted(w_parts, cols, D, part), dp = parted(slopes, T, cols, ld), dw_rows = rows_of(dw, first, cols);
+                split(rows, nullptr, wp, s);
+                gemm_loss_slopes(xp, wp, (const float*)lse.ptr, lse.stride[0], g, classes, (int)first, dp, s, {part, part}, ld);
+                const lb_tensor a[] = {transposed(dp), dp}, b[] = {xp, wp};
+                float* const sum[] = {nullptr, dx_sum};
+                const bool begins[] = {true, k == 0};
+                const lb_tensor* const out[] = {&dw_rows, k == pieces - 1 ? &dx : nullptr};
+                const Parts apart[] = {{ld, part}, {ld, part}};
+                if (gemm_sums_fit(a, b)) {
+                    gemm_sums(a, b, sum, begins, out, nullptr, s, apart);
+                } else {
+                    for (int i = 0; i < 2; i++) gemm_sum(a[i], b[i], sum[i], begins[i], out[i], nullptr, s, apart[i]);
+                }
+                continue;
+            }
             lb_tensor z = matrix(logits, LB_F32, T, cols, ld), d = dz, dw_rows = rows_of(dw, first, cols);
             d.shape[1] = cols;
             if (fused) gemm_loss_slopes(kept, rows, (const float*)lse.ptr, lse.stride[0], g, classes, (int)first, d, s);

@@ -107,7 +107,7 @@ def test_forward_and_backward(cuda, shape, dtype):
     device_status()
 
 
-@pytest.mark.parametrize("dtype, shape", [(torch.bfloat16, (600, 16, 230001)), (torch.float16, (610, 16, 230001)), (torch.float32, (600, 16, 120001)), (torch.bfloat16, (600, 15, 120001)),
+@pytest.mark.parametrize("dtype, shape", [(torch.bfloat16, (600, 16, 230001)), (torch.float16, (610, 16, 230001)), (torch.float32, (600, 16, 120001)), (torch.bfloat16, (600, 15, 120001)), (torch.float32, (60, 8, 1200001)),
                                           (torch.bfloat16, (8192, 1024, 20001)), (torch.float16, (8200, 1000, 20001))])  # fmt: skip
 def test_a_vocabulary_in_several_pieces(cuda, dtype, shape):
     x, w, targets = operands(cuda, *shape, dtype, ignored=0.1)
