@@ -1091,7 +1091,8 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                if (q.d_f16) drain_sum<true>(q, tbase, row, col_base, stage, lane, release);
+                if (LB_RARELY(q.splits > 1)) drain_partial(q, tbase, row, col_base, 0, split, stage, lane, release);
+                else if (q.d_f16) drain_sum<true>(q, tbase, row, col_base, stage, lane, release);
                 else drain_sum<false>(q, tbase, row, col_base, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_GROUP) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
@@ -1702,6 +1703,30 @@ bool gemm_sum_takes(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor&
     if (a.rows <= BM || b.cols % 8 || !tensor_core_operands(a, b, a_cols, b_cols) || !in_pieces(out)) return false;
     const GemmRoute route = gemm_route(a.rows, b.cols, a.cols, 1, sm_count_hint(), 0, gemm_scratch_bytes(a.rows, b.cols, a.cols, 1), nullptr);
     return route.ranges == 0 && route.splits == 1;
+}
+int gemm_part_ranges(long long M, long long N, long long K) {
+    const int pairs = sm_count_hint() / 2;
+    const long long tiles = (M + 2 * BM - 1) / (2 * BM) * ((N + BN - 1) / BN), total_kb = (K + BK - 1) / BK * kPartProducts;
+    if (tiles >= 4LL * pairs || total_kb < 32) return 1;
+    const double millions = (double)(M * N) * 1e-6;
+    int best = 1;
+    double best_us = pairs_us(tiles, total_kb, 1, pairs, millions) * 0.9;
+    for (int s = 2; s <= 64 && total_kb / s >= 16; s++)
+        if (const double us = pairs_us(tiles, total_kb, s, pairs, millions); us < best_us) best = s, best_us = us;
+    const long long kb = (total_kb + best - 1) / best;
+    return (int)((total_kb + kb - 1) / kb);
+}
+void gemm_part_sums(const lb_tensor& a_t, const lb_tensor& b_t, int ranges, float* partial, void* stream, Parts parts) {
+    driver();
+    const View3 a = view3(a_t, "a"), b = view3(b_t, "b"), w = turned(b);
+    bool a_cols, b_cols;
+    tensor_core_operands(a, b, a_cols, b_cols);
+    SumArgs p{};
+    long long tiles;
+    pair_args(p, a, w, a_cols, !b_cols, BN, tiles);
+    set_parts(p, parts);
+    p.splits = ranges, p.kb_per_split = (kPartProducts * p.part_kb + ranges - 1) / ranges, p.partial = partial;
+    launch_pairs(operand_map(a, a_cols, BM, parts.a), operand_map(w, !b_cols, BN / 2, parts.b), p, tiles * ranges, stream);
 }
 void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream, Parts parts) {
     driver();

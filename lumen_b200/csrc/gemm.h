@@ -110,6 +110,9 @@ void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, 
 bool gemm_sum_takes(const lb_tensor& a, const lb_tensor& b, const lb_tensor& out);
 void gemm_sum(const lb_tensor& a, const lb_tensor& b, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream, Parts parts = {});
 
+// The same of operands in parts with K cut into so many ranges (1: better whole), whose sums go to `partial` [ranges][M][N].
+int gemm_part_ranges(long long M, long long N, long long K);
+void gemm_part_sums(const lb_tensor& a, const lb_tensor& b, int ranges, float* partial, void* stream, Parts parts);
 // Two of them that do not depend on one another in one launch; `_pay`: whether layouts are theirs and the model of pairs says that they gain by it.
 bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out);
 // `_fit`: whether two products of parts are few enough tiles for it.

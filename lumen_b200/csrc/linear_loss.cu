@@ -64,6 +64,65 @@ __global__ void __launch_bounds__(kRowThreads) span_kernel(const float* logits, 
     }
 }
 
+// Few rows of float32, straight from the weights, which are read once: a warp takes four classes' rows at a time, its lanes a vector of K each, against all tokens (from
+// the L1), and the lanes' sums are added at the end. A block's 32 classes are a span; with `logits` those are stored instead. Bound by the weights' bytes up to
+// eight tokens, then by the fused multiply-adds and the loads of x, 16 and 4 a warp and vector of four classes.
+constexpr int kFewWarps = 8, kFewRows = 4, kFewSpan = kFewWarps * kFewRows, kFewTokens = 16;
+template <int TOKENS, int VEC>
+__global__ void __launch_bounds__(kFewWarps * 32) few_kernel(const float* x, long long ld_x, const float* w, long long ld_w, int T, int D, int V, Targets targets, SpanSum* spans,
+                                                             float* hit, float* logits, long long ld) {
+    __shared__ float z[TOKENS][kFewSpan];
+    grid_wait();
+    typedef std::conditional_t<VEC == 4, float4, float> Vec;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, row0 = blockIdx.x * kFewSpan + warp * kFewRows;
+    float acc[kFewRows][TOKENS] = {};
+    const float* rows[kFewRows];
+#pragma unroll
+    for (int r = 0; r < kFewRows; r++) rows[r] = w + (long long)min(row0 + r, V - 1) * ld_w;
+    for (int k = lane * VEC; k < D; k += 32 * VEC) {
+        float a[kFewRows][VEC];
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) *(Vec*)a[r] = *(const Vec*)(rows[r] + k);
+#pragma unroll
+        for (int t = 0; t < TOKENS; t++) {
+            float b[VEC];
+            *(Vec*)b = *(const Vec*)(x + (long long)min(t, T - 1) * ld_x + k);
+#pragma unroll
+            for (int r = 0; r < kFewRows; r++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) acc[r][t] = fmaf(a[r][j], b[j], acc[r][t]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kFewRows; r++)
+#pragma unroll
+        for (int t = 0; t < TOKENS; t++) {
+            float v = acc[r][t];
+#pragma unroll
+            for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+            if (lane == 0) z[t][warp * kFewRows + r] = v;
+        }
+    __syncthreads();
+    const int at = blockIdx.x * kFewSpan + lane;
+    for (int t = warp; t < T; t += kFewWarps) {
+        const float v = z[t][lane];
+        const bool in = at < V;
+        if (logits) {
+            if (in) logits[t * ld + at] = v;
+            continue;
+        }
+        float most = in ? v : -INFINITY;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        const float base = most == -INFINITY ? 0.0f : most;
+        float sum = in ? exp2_approx((v - base) * kLog2e) : 0.0f;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) spans[(long long)blockIdx.x * T + t] = {most, sum};
+        if (in && targets.of(t) == at) hit[t] = v;
+    }
+}
+
 // What a block of rows adds to the loss.
 struct LossSum {
     double sum;
@@ -236,15 +295,17 @@ __global__ void __launch_bounds__(kRowThreads) slope_kernel(const float* logits,
     }
 }
 
-// sum = (first piece: 0, else sum) + product; the last piece's is rounded into `out` instead, times `undo` where there is one.
+// sum = (first piece: 0, else sum) + product, which is `ranges` sums to add up in their order; the last piece's is rounded into `out` instead, times `undo` where there is one.
 template <class T>
-__global__ void __launch_bounds__(256) fold_kernel(const float* product, long long rows, int D, float* sum, bool begins, T* out, long long ld_out, const float* undo) {
+__global__ void __launch_bounds__(256) fold_kernel(const float* product, int ranges, long long rows, int D, float* sum, bool begins, T* out, long long ld_out, const float* undo) {
     grid_wait();
     const float scale = undo ? *undo : 1.0f;
     for (long long row = blockIdx.y; row < rows; row += gridDim.y)
         for (int c = blockIdx.x * 256 + threadIdx.x; c < D; c += gridDim.x * 256) {
             const long long i = row * D + c;
-            const float v = begins ? product[i] : sum[i] + product[i];
+            float v = begins ? 0.0f : sum[i];
+#pragma unroll 4
+            for (int k = 0; k < ranges; k++) v += product[(long long)k * rows * D + i];
             if (out) out[row * ld_out + c] = from_float<T>(v * scale);
             else sum[i] = v;
         }
@@ -394,6 +455,21 @@ void split(const lb_tensor& t, const int* classes, const lb_tensor& to, cudaStre
                       (int)t.shape[1], (int)part, classes, (__nv_bfloat16*)to.ptr);
 }
 
+// Whether few_kernel takes the products of x and w; the vectors that both can be read in.
+bool few_float32(const lb_tensor& x, const lb_tensor& w) { return x.dtype == LB_F32 && x.shape[0] <= kFewTokens && x.stride[1] == 1 && w.stride[1] == 1; }
+void run_few(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, float* logits, long long ld, cudaStream_t s) {
+    auto vectors = [](const lb_tensor& t) { return (uintptr_t)t.ptr % 16 == 0 && (t.shape[0] <= 1 || t.stride[0] % 4 == 0); };
+    const int T = (int)x.shape[0], D = (int)x.shape[1], V = (int)w.shape[0];
+    const bool vec = D % 4 == 0 && vectors(x) && vectors(w);
+    auto go = [&](auto kernel) {
+        launch_overlapped(kernel, dim3((unsigned)((V + kFewSpan - 1) / kFewSpan)), dim3(kFewWarps * 32), 0, s, 0, (const float*)x.ptr, (long long)x.stride[0], (const float*)w.ptr,
+                          (long long)w.stride[0], T, D, V, targets, spans, hit, logits, ld);
+    };
+    if (T <= 4) vec ? go(few_kernel<4, 4>) : go(few_kernel<4, 1>);
+    else if (T <= 8) vec ? go(few_kernel<8, 4>) : go(few_kernel<8, 1>);
+    else vec ? go(few_kernel<16, 4>) : go(few_kernel<16, 1>);
+}
+
 struct Forward : Loss {
     using Loss::Loss;
     lb_tensor loss, lse;
@@ -412,9 +488,9 @@ struct Forward : Loss {
     }
     void run(cudaStream_t s, bool only_count) {
         held = 0;
-        const bool few = T && skinny_takes(x, w), parts = in_parts(), fused = few || (T && gemm_loss_takes(x, w));
+        const bool few16 = T && skinny_takes(x, w), few32 = T && few_float32(x, w), few = few16 || few32, parts = in_parts(), fused = few || (T && gemm_loss_takes(x, w));
         const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(4, T), pieces = (V + piece - 1) / piece, each = (piece + kSpan - 1) / kSpan, last = (V - (pieces - 1) * piece + kSpan - 1) / kSpan,
-                        n_spans = few ? skinny_spans(V) : fused ? gemm_spans(V) : parts ? (pieces - 1) * gemm_spans(piece) + gemm_spans(V - (pieces - 1) * piece) : (pieces - 1) * each + last;
+                        n_spans = few32 ? (V + kFewSpan - 1) / kFewSpan : few ? skinny_spans(V) : fused ? gemm_spans(V) : parts ? (pieces - 1) * gemm_spans(piece) + gemm_spans(V - (pieces - 1) * piece) : (pieces - 1) * each + last;
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
         const long long blocks = (T + R - 1) / R;
         SpanSum* spans = take<SpanSum>(n_spans * T);
@@ -428,7 +504,8 @@ struct Forward : Loss {
         void* product = take<char>(more);
         if (only_count) return;
         if (T) {
-            if (few) skinny_loss(x, w, targets, spans, hit, s);
+            if (few32) run_few(x, w, targets, spans, hit, nullptr, 0, s);
+            else if (few16) skinny_loss(x, w, targets, spans, hit, s);
             else if (fused) gemm_loss(x, w, targets, 0, spans, hit, s);
             if (parts) split(x, nullptr, parted(x_parts, T, D, part), s);
             for (long long k = 0; k < pieces && !fused; k++) {
@@ -458,6 +535,12 @@ struct Forward : Loss {
 struct Backward : Loss {
     using Loss::Loss;
     lb_tensor grad{}, lse, dx, dw;
+
+    // Ranges of a long K that d_x is cut into on the CUDA cores, where a sum is one chain: until every SM has four of the blocks of 128 threads that a product of so few rows has.
+    int core_ranges(long long K) const {
+        const long long tiles = (T + 15) / 16 * ((D + 31) / 32);
+        return (int)std::max(1LL, std::min({4LL * sm_count_hint() / tiles, K / 256, 64LL}));
+    }
 
     void results(const lb_tensor* dx_t, const lb_tensor* dw_t) {
         dx = as_rows(dx_t, 1, "d_x"), dw = as_rows(dw_t, 1, "d_weight");
@@ -496,8 +579,9 @@ struct Backward : Loss {
         const lb_tensor sums_a[] = {transposed(dz), dz}, sums_b[] = {kept, rows_of(w, 0, piece)}, sums_out[] = {dw, dx};
         const bool folds = pieces > 1 || half, both = !parts && T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
                    dw_tiles = both || (half && T && gemm_sum_takes(sums_a[0], sums_b[0], dw));
-        float *dx_piece = folds && !dx_tiles && !parts ? take<float>(T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
-        float* dw_piece = half && !dw_tiles ? take<float>(piece * D) : nullptr;
+        const int ranges = dtype != LB_F32 || !T ? 1 : parts ? gemm_part_ranges(T, D, piece) : core_ranges(piece), dw_ranges = parts ? gemm_part_ranges(piece, D, T) : 1;
+        float *dx_piece = ranges > 1 || (folds && !dx_tiles && !parts) ? take<float>((ranges + 1) * T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
+        float* dw_piece = (half && !dw_tiles) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
         size_t more = 0;
         if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
         void* product = take<char>(more);
@@ -518,6 +602,13 @@ struct Backward : Loss {
         for (long long k = 0; k < pieces; k++) {
             const long long first = k * piece, cols = std::min(piece, V - first);
             const lb_tensor rows = rows_of(w, first, cols);
+            auto fold = [&](const float* from, int ranges, const lb_tensor& to, float* sum, bool begins, bool ends) {
+                by_type(dtype, [&](auto* type) {
+                    using E = std::remove_pointer_t<decltype(type)>;
+                    launch_overlapped(fold_kernel<E>, by_rows(to.shape[0], D, 256), dim3(256), 0, s, 0, from, ranges, (long long)to.shape[0], (int)D,
+                                      sum, begins, ends ? (E*)to.ptr : (E*)nullptr, (long long)to.stride[0], half ? (const float*)undo : (const float*)nullptr);
+                });
+            };
             if (parts) {
                 const lb_tensor xp = parted(x_kept, T, D, part), wp = parted(w_parts, cols, D, part), dp = parted(slopes, T, cols, ld), dw_rows = rows_of(dw, first, cols);
                 split(rows, nullptr, wp, s);
@@ -527,29 +618,32 @@ struct Backward : Loss {
                 const bool begins[] = {true, k == 0};
                 const lb_tensor* const out[] = {&dw_rows, k == pieces - 1 ? &dx : nullptr};
                 const Parts apart[] = {{ld, part}, {ld, part}};
-                if (gemm_sums_fit(a, b)) {
+                if (ranges == 1 && dw_ranges == 1 && gemm_sums_fit(a, b)) {
                     gemm_sums(a, b, sum, begins, out, nullptr, s, apart);
-                } else {
-                    for (int i = 0; i < 2; i++) gemm_sum(a[i], b[i], sum[i], begins[i], out[i], nullptr, s, apart[i]);
+                    continue;
+                }
+                for (int i = 0; i < 2; i++) {
+                    const int n = i ? gemm_part_ranges(T, D, cols) : gemm_part_ranges(cols, D, T);
+                    float* partial = i ? dx_piece : dw_piece;
+                    if (n == 1 || n > (i ? ranges : dw_ranges)) {  // (a shorter piece may want more than there is memory for)
+                        gemm_sum(a[i], b[i], sum[i], begins[i], out[i], nullptr, s, apart[i]);
+                    } else {
+                        gemm_part_sums(a[i], b[i], n, partial, s, apart[i]);
+                        fold(partial, n, i ? dx : dw_rows, i ? dx_sum : nullptr, begins[i], out[i] != nullptr);
+                    }
                 }
                 continue;
             }
             lb_tensor z = matrix(logits, LB_F32, T, cols, ld), d = dz, dw_rows = rows_of(dw, first, cols);
             d.shape[1] = cols;
             if (fused) gemm_loss_slopes(kept, rows, (const float*)lse.ptr, lse.stride[0], g, classes, (int)first, d, s);
+            else if (few_float32(x, rows)) run_few(x, rows, targets, nullptr, nullptr, logits, ld, s);
             else gemm(x, transposed(rows), z, EPI_NONE, 0, s, product, more, nullptr, nullptr);
             if (!fused) by_type(dtype, [&](auto* type) {
                 using E = std::remove_pointer_t<decltype(type)>;
                 launch_overlapped(slope_kernel<E>, by_rows(T, cols, 4 * kRowThreads), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, (const float*)lse.ptr,
                                   (long long)lse.stride[0], (const float*)g, (const int*)classes, (E*)slopes, ld);
             });
-            auto fold = [&](const float* from, const lb_tensor& to, float* sum, bool begins, bool ends) {
-                by_type(dtype, [&](auto* type) {
-                    using E = std::remove_pointer_t<decltype(type)>;
-                    launch_overlapped(fold_kernel<E>, by_rows(to.shape[0], D, 256), dim3(256), 0, s, 0, from, (long long)to.shape[0], (int)D,
-                                      sum, begins, ends ? (E*)to.ptr : (E*)nullptr, (long long)to.stride[0], half ? (const float*)undo : (const float*)nullptr);
-                });
-            };
             const bool begins = k == 0, ends = k == pieces - 1;
             if (both) {
                 const lb_tensor a[] = {transposed(d), d}, b[] = {kept, rows};
@@ -562,22 +656,42 @@ struct Backward : Loss {
             if (dtype == LB_F32) {  // what leaves SMs idle by itself shares a launch
                 SimtProblem q[2];
                 gemm(transposed(d), kept, dw_rows, EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, &q[0]);
+                if (ranges > 1) {  // as many products of a batch
+                    const long long each = (cols + ranges - 1) / ranges, whole = cols / each;
+                    lb_tensor a = d, b = rows, out = matrix(dx_piece, LB_F32, T, D, D);
+                    a.rank = b.rank = out.rank = 3;
+                    a.shape[0] = b.shape[0] = out.shape[0] = whole, a.shape[1] = T, a.shape[2] = b.shape[1] = each, b.shape[2] = out.shape[2] = D, out.shape[1] = T;
+                    a.stride[0] = each, a.stride[1] = ld, a.stride[2] = 1, b.stride[0] = each * rows.stride[0], b.stride[1] = rows.stride[0], b.stride[2] = rows.stride[1];
+                    out.stride[0] = T * D, out.stride[1] = D, out.stride[2] = 1;
+                    gemm(a, b, out, EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, nullptr);
+                    const long long at = whole * each;
+                    int count = (int)whole;
+                    if (at < cols) {  // the last one, shorter
+                        lb_tensor a_end = d, b_end = rows_of(rows, at, cols - at);
+                        a_end.ptr = (float*)d.ptr + at, a_end.shape[1] = cols - at;
+                        gemm(a_end, b_end, matrix(dx_piece + whole * T * D, LB_F32, T, D, D), EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, nullptr);
+                        count++;
+                    }
+                    gemm_simt_many(q, 1, device_info().sms, true, s);
+                    fold(dx_piece, count, dx, dx_sum, begins, ends);
+                    continue;
+                }
                 gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, &q[1]);
                 gemm_simt_many(q, 2, device_info().sms, true, s);
-                if (folds) fold(dx_piece, dx, dx_sum, begins, ends);
+                if (folds) fold(dx_piece, 1, dx, dx_sum, begins, ends);
                 continue;
             }
             if (dw_tiles) {
                 gemm_sum(transposed(d), kept, nullptr, true, &dw_rows, undo, s);
             } else {
                 gemm(transposed(d), kept, half ? matrix(dw_piece, LB_F32, cols, D, D) : dw_rows, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-                if (half) fold(dw_piece, dw_rows, nullptr, true, true);
+                if (half) fold(dw_piece, 1, dw_rows, nullptr, true, true);
             }
             if (dx_tiles) {
                 gemm_sum(d, rows, dx_sum, begins, ends ? &dx : nullptr, half ? undo : nullptr, s);
             } else {
                 gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-                if (folds) fold(dx_piece, dx, dx_sum, begins, ends);
+                if (folds) fold(dx_piece, 1, dx, dx_sum, begins, ends);
             }
         }
     }
