@@ -162,6 +162,17 @@ __device__ __forceinline__ int k_blocks(const GemmArgs& q) {
     if constexpr (in_parts<Args>()) return q.part_kb ? kPartProducts * q.part_kb : whole;
     return whole;
 }
+// Where K block `kb` lies: along K, and how much further along each operand's contiguous axis.
+template <class Args>
+__device__ __forceinline__ void k_of(const GemmArgs& q, int kb, int& k, int& in_a, int& in_b) {
+    k = kb * BK, in_a = in_b = 0;
+    if constexpr (in_parts<Args>())
+        if (q.part_kb) {
+            const int product = kb / q.part_kb;
+            k -= product * q.part_kb * BK;
+            in_a = (int)(kPartsOfA >> 2 * product & 3) * q.a_part, in_b = (int)(kPartsOfB >> 2 * product & 3) * q.b_part;
+        }
+}
 template <class Args>
 constexpr bool many_products() { return Args::mode == PAIR_GROUP || Args::mode == PAIR_LISTED; }
 
@@ -629,6 +640,34 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
     }
 }
 
+// What an epilogue of the cross entropy has of its row, fetched ahead of the accumulator.
+struct LossRow {
+    float lse = 0.0f, g = 0.0f;
+    int target = -1;
+};
+template <class Args>
+__device__ __forceinline__ LossRow loss_row(const Args& p, int row) {
+    LossRow r;
+    if (row < p.M) {
+        if constexpr (Args::mode == PAIR_SPANS) r.target = p.targets.of(row);
+        else r.lse = p.lse[row * p.lse_step], r.g = p.g[row], r.target = p.classes[row];
+    }
+    return r;
+}
+template <class Args, class Release>
+__device__ __forceinline__ void drain_loss(const Args& p, uint32_t tbase, int row, int n_blk, int col_half, const LossRow& r, uint4* stage, int lane, Release release) {
+    const int col_base = n_blk * BN + col_half * (BN / 2), target = r.target - p.first - col_base;
+    if constexpr (Args::mode == PAIR_SPANS) {
+        const SpanSum sum = drain_span(tbase, p.N - col_base, r.target < 0 ? -1 : target, p.hit + row, release);
+        if (row < p.M) p.spans[(long long)(2 * n_blk + col_half) * p.M + row] = sum;
+    } else {
+        const bool counts = r.target >= 0;
+        if (p.d_part) drain_slopes<SLOPE_PARTS>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
+        else if (p.d_f16) drain_slopes<SLOPE_F16>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
+        else drain_slopes<SLOPE_BF16>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
+    }
+}
+
 // A row's 128 columns of a product and of the sum that it is added to. N is a multiple of eight, rows of the result are 16-byte aligned.
 template <bool F16, class Release>
 __device__ __forceinline__ void drain_sum(const SumArgs& p, uint32_t tbase, int row, int col_base, uint4* stage, int lane, Release release) {
@@ -669,13 +708,18 @@ __device__ __forceinline__ void drain_sum(const SumArgs& p, uint32_t tbase, int 
     }
 }
 
+// What leaves by TMA lies between the ring and the barriers, at a multiple of 1024 bytes.
+constexpr int pair_places(int mode) { return mode == PAIR_SLOPED ? 4 * kPieces * kPieceBytes : mode == PAIR_LOSS_SLOPES ? kEpilogueStageBytes : 0; }
+static_assert(STAGES * (kStageBytesA + kStageBytesB) % 1024 == 0, "swizzled places");
+
+template <class Args>
 __global__ void __launch_bounds__(kThreads, 1)
-gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
+gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Args p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
     uint8_t* smem_a = smem;
     uint8_t* smem_b = smem + STAGES * kStageBytesA;
-    uint64_t* full = (uint64_t*)(smem + STAGES * (kStageBytesA + kStageBytesB));
+    uint64_t* full = (uint64_t*)(smem + STAGES * (kStageBytesA + kStageBytesB) + pair_places(Args::mode));
     uint64_t* empty = full + STAGES;
     uint64_t* tmem_full = empty + STAGES;
     uint64_t* tmem_empty = tmem_full + 2;
@@ -684,7 +728,7 @@ gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp-uniform for the compiler too
     const int num_tiles = p.tiles_m * p.tiles_n * p.batch;
-    const int total_kb = (p.K + BK - 1) / BK;
+    const int total_kb = k_blocks<Args>(p);
     const int num_units = num_tiles * p.splits;  // unit = split * num_tiles + tile: neighbours share a K range
 
     if (threadIdx.x == 0) {
@@ -725,17 +769,19 @@ gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
                     mbar_expect_tx(&full[stage], kStageBytesA + kStageBytesB);
                     uint8_t* sa = smem_a + stage * kStageBytesA;
                     uint8_t* sb = smem_b + stage * kStageBytesB;
+                    int k, in_a, in_b;
+                    k_of<Args>(p, kb, k, in_a, in_b);
                     if (!p.a_mn_major) {
-                        tma_load_3d(sa, &map_a, &full[stage], kb * BK, m_blk * BM, b);  // box {64 k, 128 m}
+                        tma_load_3d(sa, &map_a, &full[stage], k + in_a, m_blk * BM, b);  // box {64 k, 128 m}
                     } else {
                         for (int j = 0; j < BM / 64; j++)  // boxes {64 m, 64 k}
-                            tma_load_3d(sa + j * (64 * BK * 2), &map_a, &full[stage], m_blk * BM + j * 64, kb * BK, b);
+                            tma_load_3d(sa + j * (64 * BK * 2), &map_a, &full[stage], m_blk * BM + j * 64 + in_a, k, b);
                     }
                     if (!p.b_mn_major) {
-                        tma_load_3d(sb, &map_b, &full[stage], kb * BK, n_blk * BN, b);  // box {64 k, 256 n}
+                        tma_load_3d(sb, &map_b, &full[stage], k + in_b, n_blk * BN, b);  // box {64 k, 256 n}
                     } else {
                         for (int j = 0; j < BN / 64; j++)  // boxes {64 n, 64 k}
-                            tma_load_3d(sb + j * (64 * BK * 2), &map_b, &full[stage], n_blk * BN + j * 64, kb * BK, b);
+                            tma_load_3d(sb + j * (64 * BK * 2), &map_b, &full[stage], n_blk * BN + j * 64 + in_b, k, b);
                     }
                     if (++stage == STAGES) {
                         stage = 0;
@@ -791,7 +837,7 @@ gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         // quarter split the tile's 256 columns between them. ----
         const int quarter = warp & 3;
         const int col_half = (warp - 2) >> 2;
-        uint4* stage = (uint4*)(smem + STAGES * (kStageBytesA + kStageBytesB) + 256) + (warp - 2) * (kStageBytesPerWarp / 16);
+        uint4* stage = (uint4*)(smem + STAGES * (kStageBytesA + kStageBytesB) + (Args::mode == PAIR_LOSS_SLOPES ? 0 : 256)) + (warp - 2) * (kStageBytesPerWarp / 16);
         int local = 0;
         bool ok = true;
         const bool vec_ok = p.d_bf16 || p.d_f16 ? (p.ldd % 8 == 0 && p.d_batch_stride % 8 == 0 && ((uintptr_t)p.d & 15) == 0)
@@ -803,25 +849,42 @@ gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             const int split = tile_coords(p, unit, b, m_blk, n_blk);
             const int row = m_blk * BM + quarter * 32 + lane;
             const int col_base = n_blk * BN + col_half * (BN / 2);
-            const long long row_off = (long long)b * p.d_batch_stride + (long long)row * p.ldd;
-            const bool fast = __all_sync(0xffffffffu, aux_fast_path(p, row, col_base, vec_ok));  // warp-uniform: both drains load tensor memory warp-wide
-            const uint16_t* ax_warp = (const uint16_t*)p.aux + (long long)b * p.aux_batch_stride + (long long)(row - lane) * p.ld_aux + col_base;
-            uint4 raw[4];
-            if (fast) aux_load(ax_warp, p.ld_aux, lane, raw);
-            if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
-            __syncwarp();
-            tc_fence_after();
-            const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-            auto release = [&] {
-                tc_fence_before();
+            if constexpr (Args::mode == PAIR_PLAIN) {
+                const long long row_off = (long long)b * p.d_batch_stride + (long long)row * p.ldd;
+                const bool fast = __all_sync(0xffffffffu, aux_fast_path(p, row, col_base, vec_ok));  // warp-uniform: both drains load tensor memory warp-wide
+                const uint16_t* ax_warp = (const uint16_t*)p.aux + (long long)b * p.aux_batch_stride + (long long)(row - lane) * p.ld_aux + col_base;
+                uint4 raw[4];
+                if (fast) aux_load(ax_warp, p.ld_aux, lane, raw);
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&tmem_empty[buf]);
-            };
-            if (fast) drain_tile_aux(p, tbase, row_off + col_base, ax_warp, raw, stage, lane, release);
-            else if (LB_RARELY(p.splits > 1)) drain_partial(p, tbase, row, col_base, b, split, stage, lane, release);
-            else drain_tile(p, tbase, row, row_off, col_base, b, vec_ok, stage, lane, release);
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                auto release = [&] {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tmem_empty[buf]);
+                };
+                if (fast) drain_tile_aux(p, tbase, row_off + col_base, ax_warp, raw, stage, lane, release);
+                else if (LB_RARELY(p.splits > 1)) drain_partial(p, tbase, row, col_base, b, split, stage, lane, release);
+                else drain_tile(p, tbase, row, row_off, col_base, b, vec_ok, stage, lane, release);
+            } else {
+                const LossRow at = loss_row(p, row);
+                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                auto release = [&] {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tmem_empty[buf]);
+                };
+                drain_loss(p, tbase, row, n_blk, col_half, at, stage, lane, release);
+            }
         }
     }
+
+    if constexpr (Args::mode == PAIR_LOSS_SLOPES)
+        if (warp >= 2 && lane == 0) bulk_wait();  // what leaves by TMA has left
 
     // ---- teardown: every role leaves its loop (normally, or because the abort flag was raised) ----
     tc_fence_before();
@@ -868,10 +931,6 @@ constexpr int pair_smem(int mode) {
     return mode == PAIR_SLOPED ? 4 * (kPairStageBytesA + kPairStageBytesB) + 4 * kPieces * kPieceBytes + 1024 + 512 : kPairSmemBytes;
 }
 static_assert(pair_smem(PAIR_SLOPED) <= 227 * 1024, "shared memory");
-
-// What leaves by TMA lies between the ring and the barriers, at a multiple of 1024 bytes.
-constexpr int pair_places(int mode) { return mode == PAIR_SLOPED ? 4 * kPieces * kPieceBytes : mode == PAIR_LOSS_SLOPES ? kEpilogueStageBytes : 0; }
-static_assert(PSTAGES * (kPairStageBytesA + kPairStageBytesB) % 1024 == 0, "swizzled places");
 
 template <class Args>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -948,13 +1007,8 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     if (rank == 0) mbar_expect_tx(&full[stage], 2 * (kPairStageBytesA + kPairStageBytesB));
                     uint8_t* sa = smem_a + stage * kPairStageBytesA;
                     uint8_t* sb = smem_b + stage * kPairStageBytesB;
-                    int k = kb * BK, in_a = 0, in_b = 0;
-                    if constexpr (in_parts<Args>())
-                        if (q.part_kb) {
-                            const int product = kb / q.part_kb;
-                            k -= product * q.part_kb * BK;
-                            in_a = (int)(kPartsOfA >> 2 * product & 3) * q.a_part, in_b = (int)(kPartsOfB >> 2 * product & 3) * q.b_part;
-                        }
+                    int k, in_a, in_b;
+                    k_of<Args>(q, kb, k, in_a, in_b);
                     if (!q.a_mn_major) {
                         tma_load_3d_pair(sa, operand_a, &full[stage], k + in_a, row0, b);  // box {64 k, 128 m}
                     } else {
@@ -1064,27 +1118,13 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else if (p.act == ACT_SILU) drain_gated<ACT_SILU, true>(p, tbase, row, col0, stage, lane, release);
                 else if (p.act == ACT_GELU) drain_gated<ACT_GELU, true>(p, tbase, row, col0, stage, lane, release);
                 else drain_gated<ACT_RELU, true>(p, tbase, row, col0, stage, lane, release);
-            } else if constexpr (Args::mode == PAIR_SPANS) {
-                const int col_base = n_blk * BN + col_half * (BN / 2), target = row < p.M ? p.targets.of(row) - p.first - col_base : -1;
+            } else if constexpr (Args::mode == PAIR_SPANS || Args::mode == PAIR_LOSS_SLOPES) {
+                const LossRow at_row = loss_row(p, row);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                const SpanSum sum = drain_span(tbase, p.N - col_base, target, p.hit + row, release);
-                if (row < p.M) p.spans[(long long)(2 * n_blk + col_half) * p.M + row] = sum;
-            } else if constexpr (Args::mode == PAIR_LOSS_SLOPES) {
-                const int col_base = n_blk * BN + col_half * (BN / 2);
-                float lse = 0.0f, g = 0.0f;
-                int target = -1;
-                if (row < p.M) lse = p.lse[row * p.lse_step], g = p.g[row], target = p.classes[row];
-                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
-                __syncwarp();
-                tc_fence_after();
-                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                const bool counts = target >= 0;
-                if (p.d_part) drain_slopes<SLOPE_PARTS>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
-                else if (p.d_f16) drain_slopes<SLOPE_F16>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
-                else drain_slopes<SLOPE_BF16>(p, tbase, row, col_base, lse, g, counts, target - p.first - col_base, stage, lane, release);
+                drain_loss(p, tbase, row, n_blk, col_half, at_row, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_SUM || Args::mode == PAIR_LISTED) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
@@ -1478,7 +1518,7 @@ bool gemm(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& d_t, int 
             return false;
         }
         first_use_on_device((const void*)gemm_tcgen05_pair<PlainArgs>, [] {
-            LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+            LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05<PlainArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
             LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<PlainArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
         });
         const int max_pairs = resident_pairs(dev);
@@ -1494,7 +1534,7 @@ bool gemm(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& d_t, int 
             launch_overlapped(gemm_tcgen05_pair<PlainArgs>, dim3((unsigned)grid), dim3(kThreads), kPairSmemBytes, s, 0, map_a, map_b, p);
         } else {
             int grid = (int)std::min<long long>(tiles * p.splits, sms);
-            launch_overlapped(gemm_tcgen05, dim3((unsigned)grid), dim3(kThreads), kSmemBytes, s, 0, map_a, map_b, p);
+            launch_overlapped(gemm_tcgen05<PlainArgs>, dim3((unsigned)grid), dim3(kThreads), kSmemBytes, s, 0, map_a, map_b, p);
         }
         if (p.splits > 1) {
             const size_t quad = d.dtype == LB_F32 ? 16 : 8;  // bytes of four elements
@@ -1840,6 +1880,15 @@ static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, con
     long long tiles;
     pair_args(p, x, w, x_cols, !w_rows, BN, tiles);
     set_parts(p, parts);
+    if (p.M <= BM) {  // one row of tiles: twice as many blocks without a second half of each tile that is empty
+        const DeviceInfo& dev = device_info();
+        first_use_on_device((const void*)gemm_tcgen05<Args>, [] {
+            LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05<Args>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        });
+        launch_overlapped(gemm_tcgen05<Args>, dim3((unsigned)std::min<long long>(tiles, dev.sms)), dim3(kThreads), kSmemBytes, (cudaStream_t)stream, 0, operand_map(x, x_cols, BM, parts.a),
+                          operand_map(w, !w_rows, BN, parts.b), p);
+        return;
+    }
     launch_pairs(operand_map(x, x_cols, BM, parts.a), operand_map(w, !w_rows, BN / 2, parts.b), p, tiles, stream);
 }
 void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, int first, SpanSum* spans, float* hit, void* stream, Parts parts) {

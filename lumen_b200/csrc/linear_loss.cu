@@ -93,15 +93,28 @@ __global__ void __launch_bounds__(kFewWarps * 32) few_kernel(const float* x, lon
                 for (int j = 0; j < VEC; j++) acc[r][t] = fmaf(a[r][j], b[j], acc[r][t]);
         }
     }
+    // the lanes' sums: at each step a lane hands the half of the values over that the other one keeps
+    float* v = &acc[0][0];
+    int first = 0;
+    constexpr int ALL = kFewRows * TOKENS;
 #pragma unroll
-    for (int r = 0; r < kFewRows; r++)
+    for (int d = 16, n = ALL; d; d >>= 1) {
+        if (n > 1) {
+            n /= 2;
+            const bool upper = lane & d;
 #pragma unroll
-        for (int t = 0; t < TOKENS; t++) {
-            float v = acc[r][t];
-#pragma unroll
-            for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-            if (lane == 0) z[t][warp * kFewRows + r] = v;
+            for (int i = 0; i < ALL / 2; i++) {
+                if (i >= n) continue;
+                const float give = upper ? v[i] : v[i + n], keep = upper ? v[i + n] : v[i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+            }
+            if (upper) first += n;
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < (ALL > 32 ? ALL / 32 : 1); i++) z[(first + i) % TOKENS][warp * kFewRows + (first + i) / TOKENS] = v[i];
     __syncthreads();
     const int at = blockIdx.x * kFewSpan + lane;
     for (int t = warp; t < T; t += kFewWarps) {
@@ -414,9 +427,11 @@ struct Loss {
         in_memory(r, what);
         return r;
     }
-    // Whether float32 operands go to the tensor cores in parts of 16 bits: six products of them take less than one of float32 on the CUDA cores where there are enough rows
-    // for what it takes to split the weights (16 bytes an element in all, 70 rows' products there) and enough to do for two launches more.
-    bool in_parts() const { return dtype == LB_F32 && T > 64 && (double)T * (double)V * (double)D >= 3e8; }
+    // Whether float32 operands go to the tensor cores in parts of 16 bits: six products of them take less than one of float32 on the CUDA cores, but there are 16 bytes
+    // an element of the weights to be moved for it, and three launches. us in a graph, CUDA cores -> parts, forward and backward: 33 x 344 x 116035 228 -> 240 and 855 -> 415, 53 of
+    // it 231 -> 222 and 956 -> 402, 64 x 2048 x 32768 392 -> 321 and 1248 -> 539, 300 x 64 x 5000 (9.6e7) 20.6 -> 17.4 and 59.7 -> 49.4, 1000 x 128 x 2000 36 -> 18 and 107 -> 50,
+    // 2000 x 1024 x 8000 1300 -> 151 and 4055 -> 476. Up to 16 rows few_kernel reads the weights once.
+    bool in_parts() const { return dtype == LB_F32 && T > kFewTokens && (double)T * (double)V * (double)D >= 3e7; }
     // The vocabulary in pieces whose [width, piece] of `item` bytes an element takes about kPieceBytes.
     long long piece_of(int item, long long width) const {
         const long long most = std::max(256LL, kPieceBytes / item / std::max(1LL, width) / 256 * 256);
@@ -657,7 +672,7 @@ struct Backward : Loss {
                 SimtProblem q[2];
                 gemm(transposed(d), kept, dw_rows, EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, &q[0]);
                 if (ranges > 1) {  // as many products of a batch
-                    const long long each = (cols + ranges - 1) / ranges, whole = cols / each;
+                    const long long whole = std::min<long long>(ranges, cols), each = cols / whole;
                     lb_tensor a = d, b = rows, out = matrix(dx_piece, LB_F32, T, D, D);
                     a.rank = b.rank = out.rank = 3;
                     a.shape[0] = b.shape[0] = out.shape[0] = whole, a.shape[1] = T, a.shape[2] = b.shape[1] = each, b.shape[2] = out.shape[2] = D, out.shape[1] = T;
@@ -666,7 +681,7 @@ struct Backward : Loss {
                     gemm(a, b, out, EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, nullptr);
                     const long long at = whole * each;
                     int count = (int)whole;
-                    if (at < cols) {  // the last one, shorter
+                    if (at < cols) {  // what is left, fewer than there are ranges
                         lb_tensor a_end = d, b_end = rows_of(rows, at, cols - at);
                         a_end.ptr = (float*)d.ptr + at, a_end.shape[1] = cols - at;
                         gemm(a_end, b_end, matrix(dx_piece + whole * T * D, LB_F32, T, D, D), EPI_NONE, 0, s, nullptr, 0, nullptr, nullptr, nullptr);
