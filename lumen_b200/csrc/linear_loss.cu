@@ -551,6 +551,13 @@ struct Backward : Loss {
     using Loss::Loss;
     lb_tensor grad{}, lse, dx, dw;
 
+    // Ranges of K, the vocabulary, that d_x of up to 128 rows of 16 bits is cut into on the one-CTA tiles: an SM each, where the eight that lb_gemm's narrow tiles are cut into at
+    // most would walk 48 K blocks and there are more than twice as many here. (0: lb_gemm's own choice.) us of the backward pass in a graph, that -> these: 16 x 1024 x 32768
+    // 72.7 -> 61.2, 33 of it 75.1 -> 62.8, 128 76.0 -> 66.2; where these are not taken: 5 x 496 x 18250 38 -> 40, 16 x 512 x 8000 24.3 -> 26.3, 128 x 4096 x 32768 (nine ranges) 179 -> 182.
+    int few_ranges(long long K) const {
+        const long long blocks = (K + 63) / 64, tiles = (D + 255) / 256, ranges = sm_count_hint() / tiles;
+        return dtype == LB_F32 || T > 128 || blocks < 384 || ranges <= 16 ? 0 : (int)std::min(ranges, blocks / 8);
+    }
     // Ranges of a long K that d_x is cut into on the CUDA cores, where a sum is one chain: until every SM has four of the blocks of 128 threads that a product of so few rows has.
     int core_ranges(long long K) const {
         const long long tiles = (T + 15) / 16 * ((D + 31) / 32);
@@ -599,6 +606,8 @@ struct Backward : Loss {
         float* dw_piece = (half && !dw_tiles) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
         size_t more = 0;
         if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
+        const GemmTuning few{T ? few_ranges(piece) : 0, 0};
+        if (few.splits > 1) more = std::max<size_t>(more, (size_t)few.splits * T * D * 4);
         void* product = take<char>(more);
         if (only_count) return;
         if (T == 0) {
@@ -705,7 +714,9 @@ struct Backward : Loss {
             if (dx_tiles) {
                 gemm_sum(d, rows, dx_sum, begins, ends ? &dx : nullptr, half ? undo : nullptr, s);
             } else {
-                gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, 0, s, product, more, nullptr, nullptr);
+                const GemmTuning ranges_of{few_ranges(cols), 0};
+                const bool cut = ranges_of.splits > 1;
+                gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, cut ? 3 : 0, s, product, more, nullptr, cut ? &ranges_of : nullptr);
                 if (folds) fold(dx_piece, 1, dx, dx_sum, begins, ends);
             }
         }
