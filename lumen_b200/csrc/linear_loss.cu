@@ -504,46 +504,51 @@ struct Forward : Loss {
     void run(cudaStream_t s, bool only_count) {
         held = 0;
         const bool few16 = T && skinny_takes(x, w), few32 = T && few_float32(x, w), few = few16 || few32, parts = in_parts(), fused = few || (T && gemm_loss_takes(x, w));
-        const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(4, T), pieces = (V + piece - 1) / piece, each = (piece + kSpan - 1) / kSpan, last = (V - (pieces - 1) * piece + kSpan - 1) / kSpan,
-                        n_spans = few32 ? (V + kFewSpan - 1) / kFewSpan : few ? skinny_spans(V) : fused ? gemm_spans(V) : parts ? (pieces - 1) * gemm_spans(piece) + gemm_spans(V - (pieces - 1) * piece) : (pieces - 1) * each + last;
+        // some rows at a time, whose spans (or copies) stay small whatever the number of rows
+        const long long part = up(D, 64), at_once = few ? T : std::min(T, fused ? std::max(4096LL, kPieceBytes / 8 / gemm_spans(V) / 1024 * 1024) : 65536LL);
+        const long long piece = parts ? piece_of(6, std::max(at_once, part)) : piece_of(4, at_once), pieces = (V + piece - 1) / piece, last = V - (pieces - 1) * piece;
+        auto spans_of = [&](long long cols) { return parts ? (long long)gemm_spans(cols) : (cols + kSpan - 1) / kSpan; };
+        const long long n_spans = few32 ? (V + kFewSpan - 1) / kFewSpan : few ? skinny_spans(V) : fused ? gemm_spans(V) : (pieces - 1) * spans_of(piece) + spans_of(last);
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
-        const long long blocks = (T + R - 1) / R;
-        SpanSum* spans = take<SpanSum>(n_spans * T);
-        float* hit = take<float>(T);
-        LossSum* sums = reduction == LB_REDUCTION_NONE ? nullptr : take<LossSum>(blocks);
+        const long long blocks = (at_once + R - 1) / R, rounds = T ? (T + at_once - 1) / at_once : 0, all_blocks = rounds ? (rounds - 1) * blocks + (T - (rounds - 1) * at_once + R - 1) / R : 0;
+        SpanSum* spans = take<SpanSum>(n_spans * at_once);
+        float* hit = take<float>(at_once);
+        LossSum* sums = reduction == LB_REDUCTION_NONE ? nullptr : take<LossSum>(all_blocks);
         const long long ld = up(piece, 8);
-        float* logits = take<float>(fused || parts ? 0 : T * ld);
-        char *x_parts = take<char>(parts ? T * 6 * part : 0), *w_parts = take<char>(parts ? piece * 6 * part : 0);
-        const lb_tensor z = matrix(logits, LB_F32, T, piece, ld);
-        const size_t more = T && !fused && !parts ? product_scratch(x, transposed(rows_of(w, 0, piece))) : 0;
+        float* logits = take<float>(fused || parts ? 0 : at_once * ld);
+        char *x_parts = take<char>(parts ? at_once * 6 * part : 0), *w_parts = take<char>(parts ? piece * 6 * part : 0);
+        const size_t more = T && !fused && !parts ? product_scratch(rows_of(x, 0, at_once), transposed(rows_of(w, 0, piece))) : 0;
         void* product = take<char>(more);
         if (only_count) return;
-        if (T) {
-            if (few32) run_few(x, w, targets, spans, hit, nullptr, 0, s);
-            else if (few16) skinny_loss(x, w, targets, spans, hit, s);
-            else if (fused) gemm_loss(x, w, targets, 0, spans, hit, s);
-            if (parts) split(x, nullptr, parted(x_parts, T, D, part), s);
+        for (long long round = 0; round < rounds; round++) {
+            const long long t0 = round * at_once, n = std::min(at_once, T - t0);
+            const lb_tensor rows = rows_of(x, t0, n), copies = parted(x_parts, n, D, part);
+            Targets classes = targets;
+            classes.at = (const char*)targets.at + t0 * targets.step * (targets.wide ? 8 : 4);
+            if (few32) run_few(rows, w, classes, spans, hit, nullptr, 0, s);
+            else if (few16) skinny_loss(rows, w, classes, spans, hit, s);
+            else if (fused) gemm_loss(rows, w, classes, 0, spans, hit, s);
+            if (parts) split(rows, nullptr, copies, s);
             for (long long k = 0; k < pieces && !fused; k++) {
                 const long long first = k * piece, cols = std::min(piece, V - first);
+                SpanSum* to = spans + k * spans_of(piece) * n;
                 if (parts) {
-                    const lb_tensor rows = parted(w_parts, cols, D, part);
-                    split(rows_of(w, first, cols), nullptr, rows, s);
-                    gemm_loss(parted(x_parts, T, D, part), rows, targets, (int)first, spans + k * gemm_spans(piece) * T, hit, s, {part, part});
-                    continue;
+                    const lb_tensor weights = parted(w_parts, cols, D, part);
+                    if (pieces > 1 || round == 0) split(rows_of(w, first, cols), nullptr, weights, s);
+                    gemm_loss(copies, weights, classes, (int)first, to, hit, s, {part, part});
+                } else {
+                    gemm(rows, transposed(rows_of(w, first, cols)), matrix(logits, LB_F32, n, cols, ld), EPI_NONE, 0, s, product, more, nullptr, nullptr);
+                    launch_overlapped(span_kernel, by_rows(n, cols, kSpan), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, n, (int)first, (int)cols, classes, to, hit);
                 }
-                lb_tensor out = z;
-                out.shape[1] = cols;
-                gemm(x, transposed(rows_of(w, first, cols)), out, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-                launch_overlapped(span_kernel, by_rows(T, cols, kSpan), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, targets, spans + k * each * T, hit);
             }
             auto join_rows = [&](auto kernel) {
-                launch_overlapped(kernel, dim3((unsigned)blocks), dim3(256), 0, s, 0, (const SpanSum*)spans, (int)n_spans, T, (const float*)hit, targets, (float*)lse.ptr,
-                                  sums ? nullptr : (float*)loss.ptr, sums);
+                launch_overlapped(kernel, dim3((unsigned)((n + R - 1) / R)), dim3(256), 0, s, 0, (const SpanSum*)spans, (int)n_spans, n, (const float*)hit, classes, (float*)lse.ptr + t0,
+                                  sums ? nullptr : (float*)loss.ptr + t0, sums ? sums + round * blocks : nullptr);
             };
             R == 32 ? join_rows(rows_kernel<32>) : R == 8 ? join_rows(rows_kernel<8>) : join_rows(rows_kernel<1>);
         }
-        if (sums || reduction != LB_REDUCTION_NONE)
-            launch_overlapped(loss_kernel, dim3(1), dim3(256), 0, s, 0, (const LossSum*)sums, T ? blocks : 0LL, reduction == LB_REDUCTION_MEAN, (float*)loss.ptr);
+        if (reduction != LB_REDUCTION_NONE)
+            launch_overlapped(loss_kernel, dim3(1), dim3(256), 0, s, 0, (const LossSum*)sums, all_blocks, reduction == LB_REDUCTION_MEAN, (float*)loss.ptr);
     }
 };
 

@@ -118,6 +118,20 @@ def test_a_vocabulary_in_several_pieces(cuda, dtype, shape):
     device_status()
 
 
+@pytest.mark.parametrize("dtype, shape", [(torch.bfloat16, (300001, 8, 16385)), (torch.float32, (70001, 8, 300)), (torch.float16, (66001, 7, 40))])
+def test_rows_in_several_rounds(cuda, dtype, shape):
+    x, w, targets = operands(cuda, *shape, dtype, ignored=0.1)
+    mean, lse = linear_cross_entropy(x, w, targets)
+    losses, again = linear_cross_entropy(x, w, targets, reduction="none")
+    assert torch.equal(lse, again)
+    some = torch.cat((torch.arange(0, shape[0], shape[0] // 999, device=cuda), torch.arange(shape[0] - 300, shape[0], device=cuda)))
+    check_forward(x[some], w, targets[some], "none", losses[some], lse[some])
+    counts = int((targets != IGNORED).sum())
+    total = float(losses.double().sum())
+    assert abs(float(mean) - total / counts) <= 2.0**-23 * abs(total) / counts
+    device_status()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("t", [6, 300])
 def test_what_stands_in_rows_that_do_not_count(cuda, t, dtype):
