@@ -463,7 +463,8 @@ void run_adamw(const lb_adamw_desc* desc, const lb_tensor* params, const lb_tens
         }
         t.first[t.count] = (int)first;
         if (!first) continue;
-        launch_overlapped(bits == 8 ? adamw_kernel<8> : adamw_kernel<32>, dim3((unsigned)std::min<long long>(first, grid)), dim3(kThreads), 0, (cudaStream_t)stream, 0, t);
+        auto kernel = bits == 8 ? adamw_kernel<8> : adamw_kernel<32>;
+        launch_overlapped(kernel, dim3((unsigned)std::min<long long>(first, grid)), dim3(kThreads), 0, (cudaStream_t)stream, 0, t);
     }
 }
 
