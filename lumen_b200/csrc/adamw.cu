@@ -49,9 +49,7 @@ static_assert(sizeof(AdamwTable) <= 32000, "kernel parameters");
 
 // What every element's step needs.
 struct Step {
-    float b1, b1_rest, b2, b2_rest, eps, factor, keep, rate, root_c2;
-    float root_b2, m_share, v_share;  // of moments in 8 bits: sqrt(b2), (1 - b1) factor, sqrt(1 - b2) factor
-    // keep: 1 - lr decay; rate: lr / (1 - b1^t); root_c2: 1 / sqrt(1 - b2^t)
+    float b1, b1_rest, b2, b2_rest, eps, factor, keep, rate, root_c2;  // keep: 1 - lr decay; rate: lr / (1 - b1^t); root_c2: 1 / sqrt(1 - b2^t)
 };
 __device__ Step this_step(const AdamwTable& t, Step* shared) {
     if (threadIdx.x == 0) {
@@ -64,10 +62,9 @@ __device__ Step this_step(const AdamwTable& t, Step* shared) {
         s.root_c2 = (float)(1.0 / sqrt(-expm1(step * t.log_b2)));
         s.factor = 1.0f;
         if (t.norm_at) {
-            const double quotient = t.max_norm / ((double)*t.norm_at + 1e-6);
-            s.factor = quotient >= 1.0 ? 1.0f : (float)quotient;  // NaN stays
+            const float quotient = __frcp_rn(*t.norm_at + 1e-6f) * (float)t.max_norm;
+            s.factor = quotient >= 1.0f ? 1.0f : quotient;  // NaN stays
         }
-        s.root_b2 = sqrtf(t.b2), s.m_share = t.b1_rest * s.factor, s.v_share = sqrtf(t.b2_rest) * s.factor;
         *shared = s;
     }
     __syncthreads();
@@ -206,55 +203,58 @@ __device__ __forceinline__ float more(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float root_or_zero(float v) {
-    float r;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
 __device__ __forceinline__ float inverse(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// With one step of Newton's iteration, for what a whole block's codes are found by: near the middle of two codes a unit in the last place decides.
-__device__ __forceinline__ float inverse_refined(float x) {
-    const float r = inverse(x);
-    return fmaf(fmaf(-x, r, 1.0f), r, r);
+__device__ __forceinline__ float inverse_root(float x) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // Codes `m` and `v`, weights and gradients of a lane's eight elements after a step; the block's scales in `sm` and `sv`.
 //
-// Bound by issued instructions where each operation is rounded as in the 32-bit step and quotients and roots are exact (62 an element, 158 M of them 366 us);
-// with packed arithmetic, one fused operation for a product and a sum and the hardware's roots and reciprocals, each within a few 2^-23 of a value that is then held in
-// four bits, it is memory that bounds it. v below 2^-126 is zero.
+// What is held is found by products and sums that are rounded one by one, as the 32-bit moments are, by roots with a step of Newton's iteration, which leaves them rounded but
+// for a rare unit in the last place, and by a block's reciprocal, rounded: a code next to the middle of two is then the same whoever computes it, and one that is not
+// makes the weight's next step another by a sixteenth. The weight's own step has the hardware's reciprocal.
+//
+// Bound by issued instructions where root and quotient of each element are the exact functions (62 an element, 158 M of them 366 us).
 __device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, float& sm, float& sv, float* w, const float* g) {
     uint32_t cm[4] = {m.x & 0xffff, m.x >> 16, m.y & 0xffff, m.y >> 16}, cv[4] = {v.x & 0xffff, v.x >> 16, v.y & 0xffff, v.y >> 16};
     auto same = [](float x) { return both(x, x); };
-    const Pair scale_m = same(sm * s.b1), scale_v = same(sv * s.root_b2), share_m = same(s.m_share), share_v = same(s.v_share);
-    Pair mm[4], root[4];
+    // (a packed product in front of a packed sum may become one instruction with it, whose product is not rounded: sums are scalar)
+    auto sum = [](Pair a, Pair b) {
+        const float2 x = apart(a), y = apart(b);
+        return make_float2(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
+    };
+    Pair root[4];
+    float2 mm[4];
     float top_m = 0.0f, top_v = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const Pair gg = both(g[2 * j], g[2 * j + 1]), r = from_e4m3(cv[j]) * scale_v, gs = gg * share_v;
-        mm[j] = fma2(from_e4m3(cm[j]), scale_m, gg * share_m);
-        const float2 vv = apart(fma2(r, r, gs * gs));
-        root[j] = both(root_or_zero(vv.x), root_or_zero(vv.y));
+        const Pair gg = both(g[2 * j], g[2 * j + 1]) * same(s.factor), r = from_e4m3(cv[j]) * same(sv);
+        mm[j] = sum(from_e4m3(cm[j]) * same(sm) * same(s.b1), gg * same(s.b1_rest));
+        const float2 vv = sum(r * r * same(s.b2), gg * gg * same(s.b2_rest));
+        const Pair v2 = both(vv.x, vv.y), y = both(inverse_root(fmaxf(vv.x, 0x1p-126f)), inverse_root(fmaxf(vv.y, 0x1p-126f))), near = v2 * y;
+        root[j] = fma2(fma2(-near, near, v2), y * same(0.5f), near);
         const float2 den = apart(fma2(root[j], same(s.root_c2), same(s.eps)));
-        const float2 moved = apart(fma2(mm[j] * both(inverse(den.x), inverse(den.y)), same(-s.rate), both(w[2 * j], w[2 * j + 1]) * same(s.keep)));
+        const float2 moved = apart(fma2(both(mm[j].x, mm[j].y) * both(inverse(den.x), inverse(den.y)), same(-s.rate), both(w[2 * j], w[2 * j + 1]) * same(s.keep)));
         w[2 * j] = moved.x, w[2 * j + 1] = moved.y;
-        const float2 a = apart(mm[j]), b = apart(root[j]);
-        top_m = more(more(top_m, fabsf(a.x)), fabsf(a.y)), top_v = more(more(top_v, b.x), b.y);
+        const float2 b = apart(root[j]);
+        top_m = more(more(top_m, fabsf(mm[j].x)), fabsf(mm[j].y)), top_v = more(more(top_v, b.x), b.y);
     }
     const float most_m = warp_most(top_m), most_v = warp_most(top_v);
     const bool no_m = most_m < 0x1p-100f, no_v = most_v < 0x1p-100f;
-    const float inv_m = no_m ? 0.0f : 448.0f * inverse_refined(most_m), inv_v = no_v ? 0.0f : 448.0f * inverse_refined(most_v);
+    const float inv_m = no_m ? 0.0f : __frcp_rn(most_m) * 448.0f, inv_v = no_v ? 0.0f : __frcp_rn(most_v) * 448.0f;
     sm = no_m ? 0.0f : most_m * (1.0f / 448.0f), sv = no_v ? 0.0f : most_v * (1.0f / 448.0f);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         float2 x = apart(root[j] * same(inv_v));
-        const float2 some = apart(root[j] * same(0x1p60f));  // a root is zero or 2^-63 and more
+        const float2 some = apart(root[j] * same(0x1p100f));  // a root is zero or more than 2^-75
         x.x = fmaxf(x.x, fminf(some.x, 0x1p-9f)), x.y = fmaxf(x.y, fminf(some.y, 0x1p-9f));
-        cv[j] = to_e4m3(x), cm[j] = to_e4m3(apart(mm[j] * same(inv_m)));
+        cv[j] = to_e4m3(x), cm[j] = to_e4m3(apart(both(mm[j].x, mm[j].y) * same(inv_m)));
     }
     m = make_uint2(cm[0] | cm[1] << 16, cm[2] | cm[3] << 16), v = make_uint2(cv[0] | cv[1] << 16, cv[2] | cv[3] << 16);
 }

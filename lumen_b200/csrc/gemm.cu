@@ -58,6 +58,7 @@ struct GemmArgs {
     // float32 operands in three parts of bfloat16 each (the modes that take them): K blocks of a part, 0: none; elements from a part to the next along the
     // contiguous axis. Six of the nine products of parts are added up, the smallest first.
     int part_kb, a_part, b_part;
+    int segment_kb;  // of the same modes: K blocks that are added up in tensor memory, 0: all
 };
 // Which parts of A and B the products take, two bits each: (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0).
 constexpr int kPartProducts = 6;
@@ -161,6 +162,19 @@ __device__ __forceinline__ int k_blocks(const GemmArgs& q) {
     const int whole = (q.K + BK - 1) / BK;
     if constexpr (in_parts<Args>()) return q.part_kb ? kPartProducts * q.part_kb : whole;
     return whole;
+}
+// The tensor cores' sums drop what lies below float32's last place at each step, always towards zero: 2^-25 of a sum a step in the mean, so that one of 4096 products lacks
+// 5e-6 of itself. Where that shows (results of float32), K is cut into segments: each begins anew, and the warps of the way out add them up, rounded. The products of
+// the smaller parts are one segment; the last one's, of the parts that make up nearly all, end every second block: 5e-7.
+constexpr int kPartSegment = 2;
+template <class Args>
+__device__ __forceinline__ int segment_end(const GemmArgs& q, int kb, int kb1) {
+    if constexpr (in_parts<Args>()) {
+        const int small = (kPartProducts - 1) * q.part_kb;
+        if (q.part_kb) return min(kb1, kb < small ? small : kb + kPartSegment);
+        if (q.segment_kb) return min(kb1, kb + q.segment_kb);
+    }
+    return kb1;
 }
 // Where K block `kb` lies: along K, and how much further along each operand's contiguous axis.
 template <class Args>
@@ -594,10 +608,15 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
         tmem_ld_wait();
         if (c2 == BN / 2 / 64 - 1) release();
         if (LB_RARELY(span <= 0)) continue;
+        if (FORM == SLOPE_PARTS) {  // what is left of float32's precision here is not rounded to 16 bits
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const float2 e = apart(fma2(columns(v, j), scale, shift));
-            v[2 * j] = __float_as_uint(fast_exp2(e.x)), v[2 * j + 1] = __float_as_uint(fast_exp2(e.y));
+            for (int j = 0; j < 64; j++) v[j] = __float_as_uint(expf(__uint_as_float(v[j]) - lse));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const float2 e = apart(fma2(columns(v, j), scale, shift));
+                v[2 * j] = __float_as_uint(fast_exp2(e.x)), v[2 * j + 1] = __float_as_uint(fast_exp2(e.y));
+            }
         }
         if (LB_RARELY(__any_sync(0xffffffffu, (unsigned)at < 64u))) {
 #pragma unroll
@@ -637,6 +656,48 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
             __syncwarp();
             if (lane == 0 && row < p.M) tma_store_3d(&p.map_d, stage, col0 + part * p.d_part, row, 0), bulk_commit();  // (lane 0's is the warp's first row)
         }
+    }
+}
+
+// Adds up the segments of a unit's K: the sum is left in tensor memory where the last of them lies, `local` at its number. `base`: the warp's half of the first accumulator.
+// 128 sums a thread, in registers.
+template <class Args, bool PAIR>
+__device__ __forceinline__ bool add_segments(const GemmArgs& q, int kb, int kb1, int& local, uint32_t base, uint64_t* tmem_full, uint64_t* tmem_empty, int lane,
+                                             volatile int* abort_flag) {
+    uint32_t all[BN / 2];
+#pragma unroll
+    for (int j = 0; j < BN / 2; j++) all[j] = 0u;
+    for (;;) {
+        const int buf = local & 1;
+        if (!mbar_wait(&tmem_full[buf], (uint32_t)(local >> 1) & 1, abort_flag)) return false;
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t at = base + (uint32_t)(buf * BN);
+#pragma unroll
+        for (int c = 0; c < BN / 2; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32(at + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float2 sum = apart(columns(all + c, j) + columns(v, j));
+                all[c + 2 * j] = __float_as_uint(sum.x), all[c + 2 * j + 1] = __float_as_uint(sum.y);
+            }
+        }
+        kb = segment_end<Args>(q, kb, kb1);
+        if (kb >= kb1) {
+#pragma unroll
+            for (int c = 0; c < BN / 2; c += 32) tmem_st_32x32(at + c, all + c);
+            tmem_st_wait();
+            return true;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            if (PAIR) mbar_arrive_cluster(&tmem_empty[buf], 0);
+            else mbar_arrive(&tmem_empty[buf]);
+        }
+        local++;
     }
 }
 
@@ -806,7 +867,34 @@ gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
             uint32_t phase = 0;
             int local = 0;
             bool ok = true;
-            for (int unit = blockIdx.x; unit < num_units && ok; unit += gridDim.x, local++) {
+            for (int unit = blockIdx.x; unit < num_units && ok; unit += gridDim.x, local += in_parts<Args>() ? 0 : 1) {
+                if constexpr (in_parts<Args>()) {
+                    const int first_kb = (int)p.by_tiles.div(unit) * p.kb_per_split, num_kb = min(total_kb, first_kb + p.kb_per_split);
+                    for (int kb = first_kb; kb < num_kb && ok; local++) {
+                        const int buf = local & 1, start = kb, end = segment_end<Args>(p, kb, num_kb);
+                        const uint32_t use = (uint32_t)(local >> 1);
+                        if (!(ok = mbar_wait_warp(&tmem_empty[buf], (use & 1) ^ 1, abort_flag))) break;
+                        tc_fence_after();
+                        const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
+                        for (; kb < end; kb++) {
+                            if (!(ok = mbar_wait_warp(&full[stage], phase, abort_flag))) break;
+                            tc_fence_after();
+                            uint64_t da = desc_advance(da0, (uint32_t)(stage * kStageBytesA)), db = desc_advance(db0, (uint32_t)(stage * kStageBytesB));
+#pragma unroll
+                            for (int k = 0; k < BK / 16; k++) {
+                                mma_f16(tmem_d, da, db, idesc, (kb != start) | (k != 0), leader);
+                                da = desc_advance(da, a_step), db = desc_advance(db, b_step);
+                            }
+                            mma_commit(&empty[stage], leader);  // frees the stage once these MMAs have read it
+                            if (++stage == STAGES) {
+                                stage = 0;
+                                phase ^= 1;
+                            }
+                        }
+                        if (ok) mma_commit(&tmem_full[buf], leader);
+                    }
+                    continue;
+                }
                 const int buf = local & 1;
                 const uint32_t use = (uint32_t)(local >> 1);
                 if (!(ok = mbar_wait_warp(&tmem_empty[buf], (use & 1) ^ 1, abort_flag))) break;
@@ -869,14 +957,18 @@ gemm_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
                 else drain_tile(p, tbase, row, row_off, col_base, b, vec_ok, stage, lane, release);
             } else {
                 const LossRow at = loss_row(p, row);
-                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
+                const uint32_t base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(col_half * (BN / 2));
+                const int kb0 = split * p.kb_per_split, kb1 = min(total_kb, kb0 + p.kb_per_split);
+                if (segment_end<Args>(p, kb0, kb1) < kb1 && !(ok = add_segments<Args, false>(p, kb0, kb1, local, base, tmem_full, tmem_empty, lane, abort_flag))) break;
+                const int last = local & 1;
+                if (!(ok = mbar_wait(&tmem_full[last], (uint32_t)(local >> 1) & 1, abort_flag))) break;
                 __syncwarp();
                 tc_fence_after();
-                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
+                const uint32_t tbase = base + (uint32_t)(last * BN);
                 auto release = [&] {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&tmem_empty[buf]);
+                    if (lane == 0) mbar_arrive(&tmem_empty[last]);
                 };
                 drain_loss(p, tbase, row, n_blk, col_half, at, stage, lane, release);
             }
@@ -1046,7 +1138,38 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             uint32_t phase = 0;
             int local = 0;
             bool ok = true;
-            for (int unit = pair; unit < num_units && ok; unit += num_pairs, local++) {
+            for (int unit = pair; unit < num_units && ok; unit += num_pairs, local += in_parts<Args>() ? 0 : 1) {
+                if constexpr (in_parts<Args>()) {
+                    int at = listed(p, unit), which;
+                    if (Args::mode == PAIR_LISTED && at == kNone) break;
+                    const GemmArgs& q = product_of(p, at, which);
+                    if constexpr (many_products<Args>()) operands(q);
+                    const int kb0 = (int)q.by_tiles.div(at) * q.kb_per_split, kb1 = min(k_blocks<Args>(q), kb0 + q.kb_per_split);
+                    for (int kb = kb0; kb < kb1 && ok; local++) {
+                        const int buf = local & 1, start = kb, end = segment_end<Args>(q, kb, kb1);
+                        const uint32_t use = (uint32_t)(local >> 1);
+                        if (!(ok = mbar_wait_cluster_warp(&tmem_empty[buf], (use & 1) ^ 1, abort_flag))) break;
+                        tc_fence_after();
+                        const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
+                        for (; kb < end; kb++) {
+                            if (!(ok = mbar_wait_warp(&full[stage], phase, abort_flag))) break;
+                            tc_fence_after();
+                            uint64_t da = desc_advance(da0, (uint32_t)(stage * kPairStageBytesA)), db = desc_advance(db0, (uint32_t)(stage * kPairStageBytesB));
+#pragma unroll
+                            for (int k = 0; k < BK / 16; k++) {
+                                mma_f16_pair(tmem_d, da, db, idesc, (kb != start) | (k != 0), leader);
+                                da = desc_advance(da, a_step), db = desc_advance(db, b_step);
+                            }
+                            mma_commit_pair(&empty[stage], 3, leader);  // frees the stage in both CTAs
+                            if (++stage == STAGES_) {
+                                stage = 0;
+                                phase ^= 1;
+                            }
+                        }
+                        if (ok) mma_commit_pair(&tmem_full[buf], 3, leader);
+                    }
+                    continue;
+                }
                 const int buf = local & 1;
                 const uint32_t use = (uint32_t)(local >> 1);
                 int at = listed(p, unit), which;
@@ -1106,6 +1229,21 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(&tmem_empty[buf], 0);
             };
+            // the modes that take K in segments: the sum of all of them, once it is there, and the hand-over of where it lies
+            [[maybe_unused]] const uint32_t base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(col_half * (BN / 2));
+            [[maybe_unused]] auto whole_sum = [&] {
+                const int kb0 = split * q.kb_per_split, kb1 = min(k_blocks<Args>(q), kb0 + q.kb_per_split);
+                if (segment_end<Args>(q, kb0, kb1) < kb1 && !add_segments<Args, true>(q, kb0, kb1, local, base, tmem_full, tmem_empty, lane, abort_flag)) return false;
+                if (!mbar_wait(&tmem_full[local & 1], (uint32_t)(local >> 1) & 1, abort_flag)) return false;
+                __syncwarp();
+                tc_fence_after();
+                return true;
+            };
+            [[maybe_unused]] auto release_last = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(&tmem_empty[local & 1], 0);
+            };
             if constexpr (Args::mode == PAIR_GATED) {
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
                 __syncwarp();
@@ -1120,20 +1258,15 @@ gemm_tcgen05_pair(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 else drain_gated<ACT_RELU, true>(p, tbase, row, col0, stage, lane, release);
             } else if constexpr (Args::mode == PAIR_SPANS || Args::mode == PAIR_LOSS_SLOPES) {
                 const LossRow at_row = loss_row(p, row);
-                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
-                __syncwarp();
-                tc_fence_after();
-                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                drain_loss(p, tbase, row, n_blk, col_half, at_row, stage, lane, release);
+                if (!(ok = whole_sum())) break;
+                drain_loss(p, base + (uint32_t)((local & 1) * BN), row, n_blk, col_half, at_row, stage, lane, release_last);
             } else if constexpr (Args::mode == PAIR_SUM || Args::mode == PAIR_LISTED) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
-                if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
-                __syncwarp();
-                tc_fence_after();
-                const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + col_half * (BN / 2));
-                if (LB_RARELY(q.splits > 1)) drain_partial(q, tbase, row, col_base, 0, split, stage, lane, release);
-                else if (q.d_f16) drain_sum<true>(q, tbase, row, col_base, stage, lane, release);
-                else drain_sum<false>(q, tbase, row, col_base, stage, lane, release);
+                if (!(ok = whole_sum())) break;
+                const uint32_t tbase = base + (uint32_t)((local & 1) * BN);
+                if (LB_RARELY(q.splits > 1)) drain_partial(q, tbase, row, col_base, 0, split, stage, lane, release_last);
+                else if (q.d_f16) drain_sum<true>(q, tbase, row, col_base, stage, lane, release_last);
+                else drain_sum<false>(q, tbase, row, col_base, stage, lane, release_last);
             } else if constexpr (Args::mode == PAIR_GROUP) {
                 const int col_base = n_blk * BN + col_half * (BN / 2);
                 if (!(ok = mbar_wait(&tmem_full[buf], use & 1, abort_flag))) break;
@@ -1894,6 +2027,7 @@ static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, con
 void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, int first, SpanSum* spans, float* hit, void* stream, Parts parts) {
     SpansArgs p{};
     p.targets = targets, p.first = first, p.spans = spans, p.hit = hit;
+    p.segment_kb = x.shape[1] > 24 * BK ? 8 : 0;  // losses are float32: 1e-6 of a loss of 4096 products whole, 2e-7 in segments
     launch_loss(p, x, w, parts, stream);
 }
 void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,
