@@ -27,7 +27,8 @@ namespace {
 
 constexpr int kThreads = 256, kMost = 240;
 constexpr int kBlock = 256;  // elements that share a scale
-constexpr int chunk_elements(int bits) { return bits == 8 ? 8192 : 4096; }
+constexpr int chunk_elements(int bits) { return bits == 8 ? 6144 : 4096; }
+constexpr int blocks_per_sm(int bits) { return bits == 8 ? 3 : 2; }
 
 struct AdamwTable {
     void *p[kMost], *m[kMost], *v[kMost];
@@ -247,7 +248,10 @@ __device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, fl
     }
     const float most_m = warp_most(top_m), most_v = warp_most(top_v);
     const bool no_m = most_m < 0x1p-100f, no_v = most_v < 0x1p-100f;
-    const float inv_m = no_m ? 0.0f : __frcp_rn(most_m) * 448.0f, inv_v = no_v ? 0.0f : __frcp_rn(most_v) * 448.0f;
+    // one reciprocal for both: odd lanes have the roots'
+    const bool odd = threadIdx.x & 1;
+    const float mine = __frcp_rn(odd ? most_v : most_m) * 448.0f, other = __shfl_xor_sync(0xffffffffu, mine, 1);
+    const float inv_m = no_m ? 0.0f : odd ? other : mine, inv_v = no_v ? 0.0f : odd ? mine : other;
     sm = no_m ? 0.0f : most_m * (1.0f / 448.0f), sv = no_v ? 0.0f : most_v * (1.0f / 448.0f);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -293,7 +297,7 @@ __device__ __forceinline__ void chunk_step_8bit(const AdamwTable& t, int k, long
     float *master = MASTER ? t.master[k] + at : nullptr, *m_scale = t.m_scale[k] + at / kBlock, *v_scale = t.v_scale[k] + at / kBlock;
     using W = std::conditional_t<MASTER, float, P>;
     W* from = MASTER ? (W*)master : (W*)p;
-    constexpr int warps = kThreads / 32, U = sizeof(W) + sizeof(G) <= 4 ? 4 : 2;
+    constexpr int warps = kThreads / 32, U = sizeof(W) + sizeof(G) <= 4 ? 3 : 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, whole = t.head[k] == 0 ? n / kBlock : 0;
     struct Held {
         Some<W, 8> w;
@@ -350,7 +354,7 @@ __device__ __forceinline__ void chunk_of(const AdamwTable& t, int k, long long a
     }
 }
 template <int BITS>
-__global__ void __launch_bounds__(kThreads, 2) adamw_kernel(const __grid_constant__ AdamwTable t) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(BITS)) adamw_kernel(const __grid_constant__ AdamwTable t) {
     __shared__ Step shared;
     grid_wait();
     const Step s = this_step(t, &shared);
@@ -436,7 +440,7 @@ void run_adamw(const lb_adamw_desc* desc, const lb_tensor* params, const lb_tens
     if (meeting(places, a, b)) refuse(format("%s %d and %s %d share memory", names[a->what], (int)a->index, names[b->what], (int)b->index));
     driver();
 
-    const int grid = device_info().sms * 2;
+    const int grid = device_info().sms * blocks_per_sm(bits);
     for (int k = 0; k < n;) {
         AdamwTable t;
         t.b1 = (float)desc->beta1, t.b1_rest = (float)(1.0 - desc->beta1), t.b2 = (float)desc->beta2, t.b2_rest = (float)(1.0 - desc->beta2), t.eps = (float)desc->eps;
