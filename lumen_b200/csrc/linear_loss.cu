@@ -151,18 +151,32 @@ __device__ __forceinline__ LossSum block_sum(LossSum v, LossSum* held) {
     return v;
 }
 
-// Joins the spans of each row ([span][row]), R rows a block and 256 / R threads a row, in an order of their own: the same bits every time.
+// Joins the spans of each row ([span][row]), R rows a block and 256 / R threads a row, eight spans of a thread on their way at a time, in an order of their own: the same bits every
+// time. With `value` the block is the only one, and leaves the sum or mean itself.
 template <int R>
-__global__ void __launch_bounds__(256) rows_kernel(const SpanSum* spans, int n_spans, long long rows, const float* hit, Targets targets, float* lse, float* losses, LossSum* sums) {
+__global__ void __launch_bounds__(256) rows_kernel(const SpanSum* spans, int n_spans, long long rows, const float* hit, Targets targets, float* lse, float* losses, LossSum* sums,
+                                                   float* value, bool mean) {
     __shared__ SpanSum held[256];
     __shared__ LossSum total[8];
     grid_wait();
-    constexpr int G = 256 / R;
+    constexpr int G = 256 / R, AHEAD = 8;
     const int r = threadIdx.x % R, group = threadIdx.x / R;
     const long long row = (long long)blockIdx.x * R + r;
     SpanSum v{-INFINITY, 0.0f};
     if (row < rows)
-        for (int k = group; k < n_spans; k += G) v = join(v, spans[k * rows + row]);
+        for (int k0 = group; k0 < n_spans; k0 += G * AHEAD) {
+            SpanSum next[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) next[k] = k0 + k * G < n_spans ? spans[(long long)(k0 + k * G) * rows + row] : SpanSum{-INFINITY, 0.0f};
+            float most = v.most;
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) most = fmaxf(most, next[k].most);
+            const float base = most == -INFINITY ? 0.0f : most;
+            float sum = v.sum * exp2_approx((v.most - base) * kLog2e);
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) sum += next[k].sum * exp2_approx((next[k].most - base) * kLog2e);
+            v = {most, sum};
+        }
     held[threadIdx.x] = v;
     for (int half = G / 2; half; half /= 2) {
         __syncthreads();
@@ -178,9 +192,11 @@ __global__ void __launch_bounds__(256) rows_kernel(const SpanSum* spans, int n_s
         if (losses) losses[row] = loss;
         mine = {loss, counts};
     }
-    if (!sums) return;
+    if (!sums && !value) return;
     mine = block_sum(mine, total);
-    if (threadIdx.x == 0) sums[blockIdx.x] = mine;
+    if (threadIdx.x) return;
+    if (value) *value = (float)(mean ? mine.sum / (double)max(mine.counted, 1LL) : mine.sum);
+    else sums[blockIdx.x] = mine;
 }
 __global__ void __launch_bounds__(256) loss_kernel(const LossSum* sums, long long n, bool mean, float* loss) {
     __shared__ LossSum total[8];
@@ -509,11 +525,13 @@ struct Forward : Loss {
         const long long piece = parts ? piece_of(6, std::max(at_once, part)) : piece_of(4, at_once), pieces = (V + piece - 1) / piece, last = V - (pieces - 1) * piece;
         auto spans_of = [&](long long cols) { return parts ? (long long)gemm_spans(cols) : (cols + kSpan - 1) / kSpan; };
         const long long n_spans = few32 ? (V + kFewSpan - 1) / kFewSpan : few ? skinny_spans(V) : fused ? gemm_spans(V) : (pieces - 1) * spans_of(piece) + spans_of(last);
-        const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 ? 8 : 1;
+        // rows of a block: enough for every SM, or all of a few, whose sum is then theirs
+        const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 || (T <= 8 && reduction != LB_REDUCTION_NONE) ? 8 : 1;
         const long long blocks = (at_once + R - 1) / R, rounds = T ? (T + at_once - 1) / at_once : 0, all_blocks = rounds ? (rounds - 1) * blocks + (T - (rounds - 1) * at_once + R - 1) / R : 0;
         SpanSum* spans = take<SpanSum>(n_spans * at_once);
         float* hit = take<float>(at_once);
-        LossSum* sums = reduction == LB_REDUCTION_NONE ? nullptr : take<LossSum>(all_blocks);
+        const bool alone = all_blocks == 1, mean = reduction == LB_REDUCTION_MEAN;
+        LossSum* sums = reduction == LB_REDUCTION_NONE || alone ? nullptr : take<LossSum>(all_blocks);
         const long long ld = up(piece, 8);
         float* logits = take<float>(fused || parts ? 0 : at_once * ld);
         char *x_parts = take<char>(parts ? at_once * 6 * part : 0), *w_parts = take<char>(parts ? piece * 6 * part : 0);
@@ -543,12 +561,12 @@ struct Forward : Loss {
             }
             auto join_rows = [&](auto kernel) {
                 launch_overlapped(kernel, dim3((unsigned)((n + R - 1) / R)), dim3(256), 0, s, 0, (const SpanSum*)spans, (int)n_spans, n, (const float*)hit, classes, (float*)lse.ptr + t0,
-                                  sums ? nullptr : (float*)loss.ptr + t0, sums ? sums + round * blocks : nullptr);
+                                  reduction == LB_REDUCTION_NONE ? (float*)loss.ptr + t0 : nullptr, sums ? sums + round * blocks : nullptr,
+                                  reduction != LB_REDUCTION_NONE && alone ? (float*)loss.ptr : nullptr, mean);
             };
             R == 32 ? join_rows(rows_kernel<32>) : R == 8 ? join_rows(rows_kernel<8>) : join_rows(rows_kernel<1>);
         }
-        if (reduction != LB_REDUCTION_NONE)
-            launch_overlapped(loss_kernel, dim3(1), dim3(256), 0, s, 0, (const LossSum*)sums, all_blocks, reduction == LB_REDUCTION_MEAN, (float*)loss.ptr);
+        if (reduction != LB_REDUCTION_NONE && !alone) launch_overlapped(loss_kernel, dim3(1), dim3(256), 0, s, 0, (const LossSum*)sums, all_blocks, mean, (float*)loss.ptr);
     }
 };
 
