@@ -5,6 +5,9 @@
 // bisection in a table that travels as a kernel parameter. The products and sums of both moments are rounded one by one, as the traced program's
 // step (nn.adamw_update) rounds them; w is computed in float32 and rounded once to its type.
 //
+// Bound by memory: all of a thread's loads are on their way at once, 16 elements of it in vectors of 32 bytes. 158 M bfloat16 weights with float32 moments 536 us, 6.45 TB/s (groups of eight
+// elements in 16-byte vectors 605, two of them 613; three blocks an SM 560, four 567). 30 M values of three types with float32 gradients and copies, at odd places, 164.
+//
 // Moments in 8 bits: blocks of 256 elements share a float32 scale s = max / 448, and hold m / s and sqrt(v) / s as e4m3, to nearest. sqrt(v) needs half
 // the exponents that v does, and what is not zero does not become zero (a weight whose denominator vanished would jump). The scale is the block's
 // largest value itself, not a power of two: it moves a little in every step, and it is by that that the others' roundings do not repeat. Changes of v of a
@@ -221,7 +224,8 @@ __device__ __forceinline__ float inverse_root(float x) {
 // for a rare unit in the last place, and by a block's reciprocal, rounded: a code next to the middle of two is then the same whoever computes it, and one that is not
 // makes the weight's next step another by a sixteenth. The weight's own step has the hardware's reciprocal.
 //
-// Bound by issued instructions where root and quotient of each element are the exact functions (62 an element, 158 M of them 366 us).
+// Bound by issued instructions (66 % of the slots) and memory: 158 M bfloat16 weights 285 - 312 us, 5.5 TB/s at best; 62 instructions an element took 366, where root and quotient of each
+// are the exact functions; 278 with codes by approximate reciprocals and fused sums. (Two blocks an SM with four blocks of 256 at once 303, four with two 312.)
 __device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, float& sm, float& sv, float* w, const float* g) {
     uint32_t cm[4] = {m.x & 0xffff, m.x >> 16, m.y & 0xffff, m.y >> 16}, cv[4] = {v.x & 0xffff, v.x >> 16, v.y & 0xffff, v.y >> 16};
     auto same = [](float x) { return both(x, x); };

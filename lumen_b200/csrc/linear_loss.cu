@@ -3,6 +3,11 @@
 // dx = dz W, dW = dz^T x. Rows that do not count have loss and dz of zero. The logits are never kept: forward, each span of the vocabulary leaves
 // its largest logit and the sum of exponentials below it, and what follows joins the spans' pairs; backward, they are computed anew for one piece of
 // the vocabulary at a time, whose dz (rounded to the operands' type, as an operand of the tensor cores has to be) is what the two products read.
+//
+// The work is the products', in whose epilogues the rest is (gemm.cu, gemm_skinny.cu); kernels here prepare rows, join spans, and are the way of layouts and types that the tensor
+// cores do not take. Bound by the tensor cores and, with few rows, by the weights' bytes. us, bfloat16: 16384 x 1024 x 32768 forward 697 (1.58 PFLOP/s; 804 under the power
+// cap, where a library product of that many FLOPs takes 769), backward 2440 - 2800 there for 3.3 TFLOP of products; 4 tokens of it 12.6 in a graph (67 MB, 5.3 TB/s with both kernels), 61 x 4096 x 131072 180
+// (1.07 GB, 6.0 TB/s). Pieces of 256 MB of dz: 64 MB, which would stay in the L2, 2700 us where these take 2460, 128 MB 2470, 512 MB 2320.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -65,8 +70,9 @@ __global__ void __launch_bounds__(kRowThreads) span_kernel(const float* logits, 
 }
 
 // Few rows of float32, straight from the weights, which are read once: a warp takes four classes' rows at a time, its lanes a vector of K each, against all tokens (from
-// the L1), and the lanes' sums are added at the end. A block's 32 classes are a span; with `logits` those are stored instead. Bound by the weights' bytes up to
-// eight tokens, then by the fused multiply-adds and the loads of x, 16 and 4 a warp and vector of four classes.
+// the L1), and the lanes' sums are added at the end. A block's 32 classes are a span; with `logits` those are stored instead. Bound by the time that a warp's four vectors take to
+// arrive (weights of 134 MB: 4 tokens 40 us in a graph, 3.3 TB/s) and, with more tokens, by the loads of x and the registers: 16 tokens 72. The next vectors fetched ahead took
+// 63 us with 8 tokens instead of 43, in half the registers that ptxas then found.
 constexpr int kFewWarps = 8, kFewRows = 4, kFewSpan = kFewWarps * kFewRows, kFewTokens = 16;
 template <int TOKENS, int VEC>
 __global__ void __launch_bounds__(kFewWarps * 32) few_kernel(const float* x, long long ld_x, const float* w, long long ld_w, int T, int D, int V, Targets targets, SpanSum* spans,
