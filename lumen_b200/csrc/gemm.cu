@@ -16,7 +16,6 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
-#include <queue>
 #include <vector>
 
 #include "divide.cuh"
@@ -1917,29 +1916,35 @@ void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begin
     if (out) p.d = out->ptr, p.ldd = out->stride[0], p.d_f32 = out->dtype == LB_F32;
     launch_pairs(operand_map(a, a_cols, BM, parts.a), operand_map(w, !b_cols, BN / 2, parts.b), p, tiles, stream);
 }
-// The units of two products in the order of the longer K, each to the pair that has least to do so far: us as in pairs_us. False where the table does not hold them. Taken in turn
+// The units of two products in the order of the longer K, each to the pair that has least to do so far: us as in pairs_us, `slots` units a pair at most. False where the table
+// does not hold them. Pairs are of two kinds, those that the first product's last round reaches and the others, and within a kind all alike: what has least is a kind. Taken in turn
 // instead, a pair would have up to 1024 blocks of K of a piece of 16384 x 8192 x 1024 where the mean is 886. us of both products of 2600 x 840 x 10007, two launches -> one: 128 -> 74; of that
 // piece 188 and 193 -> 381.
-static bool list_units(const long long* tiles, const long long* blocks, int pairs, std::vector<std::vector<uint16_t>>& of, double& us) {
-    if (tiles[0] + tiles[1] >= kListed - pairs || tiles[0] + tiles[1] >= kNone) return false;
-    typedef std::pair<double, int> Load;
-    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
-    for (int k = 0; k < pairs; k++) least.push({0.0, k});
-    of.assign((size_t)pairs, {});
-    us = 0.0;
-    size_t most = 0;
+static bool share_units(const long long* tiles, const long long* blocks, int pairs, uint16_t* table, int& slots, double& us) {
+    if (tiles[0] + tiles[1] >= std::min(kListed, kNone)) return false;
+    const double cost[2] = {0.3 * (double)blocks[0] + 2.0, 0.3 * (double)blocks[1] + 2.0};
+    const int whole = (int)(tiles[0] / pairs), reached = (int)(tiles[0] % pairs);
+    struct Kind {
+        int first, size, units;
+        double load;
+    } kinds[2] = {{0, reached, whole + 1, (whole + 1) * cost[0]}, {reached, pairs - reached, whole, whole * cost[0]}};
+    us = reached ? kinds[0].load : kinds[1].load;
+    slots = reached ? whole + 1 : whole;
     int unit = 0;
-    for (int k = 0; k < 2; k++)
-        for (long long i = 0; i < tiles[k]; i++, unit++) {
-            Load l = least.top();
-            least.pop();
-            l.first += 0.3 * (double)blocks[k] + 2.0;
-            of[(size_t)l.second].push_back((uint16_t)unit);
-            most = std::max(most, of[(size_t)l.second].size()), us = std::max(us, l.first);
-            least.push(l);
-        }
+    auto put = [&](int slot, int pair) {
+        if (table && (slot + 1) * pairs <= kListed) table[slot * pairs + pair] = (uint16_t)unit;
+        unit++;
+    };
+    for (int k = 0; k < tiles[0] && table; k++) put(k / pairs, k % pairs);
+    for (long long left = tiles[1]; left > 0;) {
+        Kind& kind = kinds[reached && kinds[0].load <= kinds[1].load ? 0 : 1];
+        const int n = (int)std::min<long long>(left, kind.size);
+        for (int k = 0; k < n && table; k++) put(kind.units, kind.first + k);
+        left -= n, kind.units++, kind.load += cost[1];
+        us = std::max(us, kind.load), slots = std::max(slots, kind.units);
+    }
     us += 3.0 + 0.1 * (double)(tiles[0] * blocks[0] + tiles[1] * blocks[1]) / pairs;
-    return most * (size_t)pairs <= kListed;
+    return (long long)slots * pairs <= kListed;
 }
 static void listed_sizes(const lb_tensor* a, const lb_tensor* b, int* order, long long* tiles, long long* blocks, bool parts) {
     order[0] = a[0].shape[1] < a[1].shape[1], order[1] = 1 - order[0];
@@ -1962,16 +1967,16 @@ bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out)
         if (gemm_route(x.rows, y.cols, x.cols, 1, sms, 0, split > 1 ? gemm_scratch_bytes(x.rows, y.cols, x.cols, 1) : 0, nullptr).ranges) return false;
         alone += pairs_us(k == order[0] ? tiles[0] : tiles[1], k == order[0] ? blocks[0] : blocks[1], split, pairs, (double)(x.rows * y.cols) * 1e-6);
     }
-    std::vector<std::vector<uint16_t>> of;
-    return list_units(tiles, blocks, pairs, of, shared) && shared < alone;
+    int slots;
+    return share_units(tiles, blocks, pairs, nullptr, slots, shared) && shared < alone;
 }
 bool gemm_sums_fit(const lb_tensor* a, const lb_tensor* b) {
     int order[2];
     long long tiles[2], blocks[2];
     listed_sizes(a, b, order, tiles, blocks, true);
-    std::vector<std::vector<uint16_t>> of;
+    int slots;
     double us;
-    return list_units(tiles, blocks, sm_count_hint() / 2, of, us);
+    return share_units(tiles, blocks, sm_count_hint() / 2, nullptr, slots, us);
 }
 void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, const bool* begins, const lb_tensor* const* out, const float* undo, void* stream,
                const Parts* parts) {
@@ -1999,14 +2004,11 @@ void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, co
         LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<ListedArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(PAIR_LISTED)));
     });
     const int resident = resident_pairs(dev), pairs = (int)std::min<long long>(tiles[0] + tiles[1], resident > 0 ? resident : dev.sms / 2);
-    std::vector<std::vector<uint16_t>> of;
+    std::fill(p.unit_of, p.unit_of + kListed, (uint16_t)kNone);
+    int slots;
     double us;
-    if (!list_units(tiles, blocks, pairs, of, us)) fail(LB_ERR_UNSUPPORTED, "gemm: too many output tiles for one launch");
-    size_t most = 0;
-    for (const auto& list : of) most = std::max(most, list.size());
-    for (size_t slot = 0; slot < most; slot++)
-        for (int k = 0; k < pairs; k++) p.unit_of[slot * pairs + k] = slot < of[(size_t)k].size() ? of[(size_t)k][slot] : (uint16_t)kNone;
-    p.units = (int)most * pairs;
+    if (!share_units(tiles, blocks, pairs, p.unit_of, slots, us)) fail(LB_ERR_UNSUPPORTED, "gemm: too many output tiles for one launch");
+    p.units = slots * pairs;
     launch_overlapped(gemm_tcgen05_pair<ListedArgs>, dim3((unsigned)(2 * pairs)), dim3(kThreads), pair_smem(PAIR_LISTED), (cudaStream_t)stream, 0, p.map_a[0], p.map_b[0], p);
 }
 template <class Args>

@@ -267,6 +267,24 @@ def test_more_tensors_than_a_launch_takes(cuda):
         model.check(4)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_past_32_bits(cuda, bits):
+    """A parameter of more than 2^31 elements moves as its end does by itself."""
+    n, end = (1 << 31) + 1000, 1000 + 256 * 40
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device=cuda), torch.zeros(n, dtype=torch.bfloat16, device=cuda)
+    p[-end:] = torch.randn(end, device=cuda).to(torch.bfloat16)
+    g[-end:] = torch.randn(end, device=cuda).to(torch.bfloat16)
+    small, grad = p[-end:].clone(), g[-end:].clone()
+    for params, grads in (([p], [g]), ([small], [grad])):
+        m, v, ms, vs = adamw_state(params, bits)
+        adamw_step(params, grads, m, v, 1, exp_avg_scale=ms, exp_avg_sq_scale=vs)
+        if params[0] is p:
+            kept = m[0][-end:].clone(), v[0][-end:].clone()
+            assert not p[: 1 << 20].any()
+            del m, v, ms, vs
+    assert torch.equal(p[-end:], small) and torch.equal(kept[0], m[0]) and torch.equal(kept[1], v[0])
+
+
 def test_shapes_strides_and_what_autograd_knows(cuda):
     p = torch.randn(40, 24, device=cuda).to(torch.bfloat16).t().requires_grad_()
     g = torch.randn_like(p.detach())

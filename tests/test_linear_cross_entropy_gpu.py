@@ -86,7 +86,7 @@ SHAPES = [
     (1, 64, 256), (1, 1024, 5000), (2, 8, 1), (2, 16, 2), (3, 40, 7), (4, 256, 30011), (7, 136, 129), (8, 512, 4096), (9, 64, 1000), (16, 328, 2048), (17, 72, 5003),
     (31, 104, 127), (32, 512, 513), (33, 64, 128), (61, 1024, 4099), (100, 264, 255), (127, 40, 257), (128, 128, 256), (129, 256, 1031), (200, 8, 12000),
     (256, 128, 256), (257, 520, 385), (300, 1120, 3001), (511, 72, 129), (700, 8, 8), (1000, 320, 1160), (1531, 96, 700), (2600, 64, 520), (5000, 16, 40),
-    (20000, 8, 9), (5, 15, 9), (40, 33, 70), (130, 100, 61), (600, 24, 1), (65, 4096, 300), (1400, 520, 4001), (2600, 840, 3001), (3000, 264, 10000),
+    (20000, 8, 9), (5, 15, 9), (40, 33, 70), (130, 100, 61), (600, 24, 1), (65, 4096, 300), (1400, 520, 4001), (2600, 840, 3001), (3000, 264, 10000), (300, 101, 2003),
 ]  # fmt: skip
 
 
@@ -116,6 +116,29 @@ def test_a_vocabulary_in_several_pieces(cuda, dtype, shape):
     check_forward(x, w, targets, "mean", loss, lse)
     check_backward(x, w, targets, lse, "mean", None, *linear_cross_entropy_backward(None, x, w, targets, lse))
     device_status()
+
+
+@pytest.mark.parametrize("t", [3, 40])
+def test_offsets_past_32_bits(cuda, t):
+    """Weights and their gradient of more than 2^31 elements."""
+    d, v = 16384, 140001
+    x, w, targets = operands(cuda, t, d, v, torch.bfloat16)
+    targets[0], targets[1], targets[2] = v - 1, v - 5, IGNORED
+    loss, lse = linear_cross_entropy(x, w, targets, reduction="none")
+    z, off = (torch.cat(parts, 1) for parts in zip(*(logits_of(x, some) for some in w.split(8192))))
+    want = torch.logsumexp(z, -1)
+    within(lse, want, off.amax(-1) + (v / 128 + 64) * 2.0**-21 + 2.0**-21 * (want.abs() + z.abs().amax(-1)), "lse")
+    assert float(loss[2]) == 0 and abs(float(loss[0]) - float(want[0] - z[0, v - 1])) < 1e-3
+    d_x, d_w = linear_cross_entropy_backward(None, x, w, targets, lse, reduction="none")
+    last = slice(v - 300, v)
+    counts = (targets != IGNORED)[:, None]
+    dz = (torch.exp(z - lse.double()[:, None]) - torch.nn.functional.one_hot(targets.clamp(min=0), v)) * counts
+    for rows in (last, slice(0, 300)):  # a gradient's every term is a rounded dz times an element
+        part = dz[:, rows].t()
+        within(d_w[rows], part @ x.double(), 2 * half(torch.bfloat16) * (part.abs() @ x.double().abs()) + 1e-6, "d_weight")
+    want = sum(dz[:, k : k + 8192] @ w[k : k + 8192].double() for k in range(0, v, 8192))
+    size = sum(dz[:, k : k + 8192].abs() @ w[k : k + 8192].double().abs() for k in range(0, v, 8192))
+    within(d_x, want, 2 * half(torch.bfloat16) * size, "d_x")
 
 
 @pytest.mark.parametrize("dtype, shape", [(torch.bfloat16, (300001, 8, 16385)), (torch.float32, (70001, 8, 300)), (torch.float16, (66001, 7, 40))])
