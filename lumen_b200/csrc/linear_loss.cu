@@ -142,6 +142,15 @@ __global__ void __launch_bounds__(kFewWarps * 32) few_kernel(const float* x, lon
     }
 }
 
+// Rows of 16-bit elements, 16-byte aligned, to where they begin on 128 bytes; a warp a row.
+__global__ void __launch_bounds__(256) align_kernel(const uint4* x, long long ld_x, long long rows, int vectors, uint4* out, long long ld_out) {
+    grid_wait();
+    const int lane = threadIdx.x & 31;
+    for (long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32; row < rows; row += (long long)gridDim.x * 8)
+#pragma unroll 4
+        for (int c = lane; c < vectors; c += 32) out[row * ld_out + c] = x[row * ld_x + c];
+}
+
 // What a block of rows adds to the loss.
 struct LossSum {
     double sum;
@@ -534,6 +543,11 @@ struct Forward : Loss {
         // rows of a block: enough for every SM, or all of a few, whose sum is then theirs
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 || (T <= 8 && reduction != LB_REDUCTION_NONE) ? 8 : 1;
         const long long blocks = (at_once + R - 1) / R, rounds = T ? (T + at_once - 1) / at_once : 0, all_blocks = rounds ? (rounds - 1) * blocks + (T - (rounds - 1) * at_once + R - 1) / R : 0;
+        // Rows that begin within a sector, of both operands, slow the product down (8192 x 840 x 20000 279 us, 208 where they do in one of them only; 2600 x 840 x 10007 46.8 and 38.6): then x
+        // is copied first, which with the copy takes 215 us and 40.8; 500 x 840 x 20000 takes 36.5 instead of 44.0.
+        auto within = [](const lb_tensor& t) { return t.stride[0] % 16 != 0; };
+        const bool aligns = fused && !few && at_once > 128 && D % 8 == 0 && x.stride[1] == 1 && w.stride[1] == 1 && within(x) && within(w);
+        char* x_copy = take<char>(aligns ? at_once * part * 2 : 0);
         SpanSum* spans = take<SpanSum>(n_spans * at_once);
         float* hit = take<float>(at_once);
         const bool alone = all_blocks == 1, mean = reduction == LB_REDUCTION_MEAN;
@@ -551,7 +565,14 @@ struct Forward : Loss {
             classes.at = (const char*)targets.at + t0 * targets.step * (targets.wide ? 8 : 4);
             if (few32) run_few(rows, w, classes, spans, hit, nullptr, 0, s);
             else if (few16) skinny_loss(rows, w, classes, spans, hit, s);
-            else if (fused) gemm_loss(rows, w, classes, 0, spans, hit, s);
+            else if (fused) {
+                lb_tensor operand = rows;
+                if (aligns) {
+                    operand.ptr = x_copy, operand.stride[0] = part;
+                    launch_overlapped(align_kernel, dim3(row_blocks((n + 7) / 8)), dim3(256), 0, s, 0, (const uint4*)rows.ptr, (long long)x.stride[0] / 8, n, (int)(D / 8), (uint4*)x_copy, part / 8);
+                }
+                gemm_loss(operand, w, classes, 0, spans, hit, s);
+            }
             if (parts) split(rows, nullptr, copies, s);
             for (long long k = 0; k < pieces && !fused; k++) {
                 const long long first = k * piece, cols = std::min(piece, V - first);
