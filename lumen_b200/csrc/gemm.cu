@@ -95,6 +95,7 @@ struct alignas(64) LossSlopesArgs : GemmArgs {
     static constexpr int mode = PAIR_LOSS_SLOPES;
     CUtensorMap map_d;  // pieces of 32 rows of 64
     int d_part;         // float32 operands: dz's parts are as far apart
+    int d_rests;        // 16 bits: what dz's rounding leaves is stored too
     const float *lse, *g;
     const int* classes;
     long long lse_step;
@@ -593,13 +594,15 @@ __device__ __forceinline__ SpanSum drain_span(uint32_t tbase, int width, int tar
 // A row's 128 columns of dz: (exp(z - lse) - [class]) g, rounded once. `target`: the class's column here; a row that does not count is zero whatever
 // its logits are. 32 rows of 64 columns leave by TMA at a time, from a place of the warp's own, which the next ones' exponentials leave time to be read out.
 // A piece of 16384 x 8192 x 1024: 179 us, the tensor pipe 85 % busy; stored through registers 210 under the power cap (179 without the stores, 210 without the exponentials), 2600 x 10007 x 840 50 -> 40.
-// FORM: bfloat16, float16, or float32 in three parts of bfloat16, each what the ones before leave, rounded; columns behind the last are zero there, as K's end is of a product's operand.
-enum SlopeForm { SLOPE_BF16, SLOPE_F16, SLOPE_PARTS };
+// FORM: bfloat16, float16, either with what the rounding left, rounded (M rows below), or float32 in three parts of bfloat16, each what the ones before leave, rounded; columns behind the last
+// are zero there, as K's end is of a product's operand.
+enum SlopeForm { SLOPE_BF16, SLOPE_F16, SLOPE_BF16_RESTS, SLOPE_F16_RESTS, SLOPE_PARTS };
 template <SlopeForm FORM, class Release>
 __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t tbase, int row, int col_base, float lse, float g, bool counts, int target, uint4* stage, int lane,
                                              Release release) {
     const Pair scale = both(kLog2e, kLog2e), shift = both(lse * -kLog2e, lse * -kLog2e), weight = both(g, g);
     const uint32_t keep = counts ? 0xffffffffu : 0u, area = smem_u32(stage) + lane * 128;
+    constexpr bool F16 = FORM == SLOPE_F16 || FORM == SLOPE_F16_RESTS, RESTS = FORM == SLOPE_BF16_RESTS || FORM == SLOPE_F16_RESTS;
 #pragma unroll 1
     for (int c2 = 0; c2 < BN / 2 / 64; c2++) {
         const int col0 = col_base + c2 * 64, span = p.N - col0, at = target - c2 * 64;
@@ -624,20 +627,20 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
             for (int j = 0; j < 64; j++)
                 if (j == at) v[j] = __float_as_uint(__uint_as_float(v[j]) - 1.0f);
         }
-        if (FORM == SLOPE_PARTS) {
+        if (FORM == SLOPE_PARTS || RESTS) {
 #pragma unroll
             for (int j = 0; j < 32; j++) {
                 const float2 d = apart(columns(v, j) * weight);
                 v[2 * j] = __float_as_uint(d.x) & keep, v[2 * j + 1] = __float_as_uint(d.y) & keep;
             }
-            if (LB_RARELY(span < 64)) {
+            if (FORM == SLOPE_PARTS && LB_RARELY(span < 64)) {
 #pragma unroll
                 for (int j = 0; j < 64; j++)
                     if (j >= span) v[j] = 0u;
             }
         }
 #pragma unroll 1
-        for (int part = 0; part < (FORM == SLOPE_PARTS ? 3 : 1); part++) {
+        for (int part = 0; part < (FORM == SLOPE_PARTS ? 3 : RESTS ? 2 : 1); part++) {
             uint32_t w[32];
 #pragma unroll
             for (int j = 0; j < 32; j++) {
@@ -645,8 +648,12 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
                     w[j] = narrow<false>(columns(v, j));
                     const float2 rest = apart(columns(v, j) + -widen<false>(w[j]));
                     v[2 * j] = __float_as_uint(rest.x), v[2 * j + 1] = __float_as_uint(rest.y);
+                } else if (RESTS) {  // (infinity and NaN leave nothing)
+                    w[j] = narrow<F16>(columns(v, j));
+                    const float2 rest = apart(columns(v, j) + -widen<F16>(w[j]));
+                    v[2 * j] = fabsf(rest.x) < INFINITY ? __float_as_uint(rest.x) : 0u, v[2 * j + 1] = fabsf(rest.y) < INFINITY ? __float_as_uint(rest.y) : 0u;
                 } else {
-                    w[j] = narrow<FORM == SLOPE_F16>(columns(v, j) * weight) & keep;
+                    w[j] = narrow<F16>(columns(v, j) * weight) & keep;
                 }
             }
             if (lane == 0) bulk_wait_read();  // the place has been read out
@@ -655,7 +662,7 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
             for (int q = 0; q < 8; q++) st_shared(area + ((q ^ (lane & 7)) << 4), make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]));
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0 && row < p.M) tma_store_3d(&p.map_d, stage, col0 + part * p.d_part, row, 0), bulk_commit();  // (lane 0's is the warp's first row)
+            if (lane == 0 && row < p.M) tma_store_3d(&p.map_d, stage, RESTS ? col0 : col0 + part * p.d_part, row, RESTS ? part : 0), bulk_commit();  // (lane 0's is the warp's first row)
         }
     }
 }
@@ -725,6 +732,8 @@ __device__ __forceinline__ void drain_loss(const Args& p, uint32_t tbase, int ro
     } else {
         const bool counts = r.target >= 0;
         if (p.d_part) drain_slopes<SLOPE_PARTS>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
+        else if (p.d_rests && p.d_f16) drain_slopes<SLOPE_F16_RESTS>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
+        else if (p.d_rests) drain_slopes<SLOPE_BF16_RESTS>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
         else if (p.d_f16) drain_slopes<SLOPE_F16>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
         else drain_slopes<SLOPE_BF16>(p, tbase, row, col_base, r.lse, r.g, counts, target, stage, lane, release);
     }
@@ -2010,8 +2019,9 @@ void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, i
 void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,
                       void* stream, Parts parts, long long dz_part) {
     LossSlopesArgs p{};
-    p.lse = lse, p.lse_step = lse_step, p.g = g, p.classes = classes, p.first = first, p.d_part = (int)dz_part;
+    p.lse = lse, p.lse_step = lse_step, p.g = g, p.classes = classes, p.first = first, p.d_part = (int)dz_part, p.d_rests = dz.shape[0] == 2 * x.shape[0];
     View3 d = view3(dz, "dz");
+    if (p.d_rests) d.rows = x.shape[0], d.batch = 2, d.sb = x.shape[0] * dz.stride[0];
     if (dz_part) d.cols = 3 * dz_part;
     p.map_d = make_map(d, true, 64, 32);
     launch_loss(p, x, w, parts, stream);

@@ -92,7 +92,8 @@ void gemm_group(const lb_tensor* a, const lb_tensor* b, const lb_tensor* d, int 
 
 // The linear cross entropy's products z = x w^T with their epilogues, 16-bit operands on CTA pairs: x [M, K], w [N, K]. Forward: each row's span sums, `spans`
 // [gemm_spans(N)][M], and its target's logit; `first`: the class of w's first row. Backward: dz [M, N] = (exp(z - lse) - [class]) g, where `w` holds the classes from `first` on; a row of class -1 is
-// zero, and columns up to the next multiple of eight may be written. `_takes`: whether the operands' layouts are theirs.
+// zero, and columns up to the next multiple of eight may be written. A dz of twice the rows: what the rounding of the first M leaves, rounded, is in the others. `_takes`: whether the operands'
+// layouts are theirs.
 //
 // float32 operands come in three parts of bfloat16: tensors of that type and of the operand's size, whose other parts lie `Parts` elements further along the
 // contiguous axis each (behind the first along K: zeros up to a multiple of 64). A product is then the sum of six of parts, which lacks 2^-23 of it.

@@ -254,9 +254,9 @@ __global__ void __launch_bounds__(256) count_kernel(Targets targets, LossGrad gr
 }
 
 // Of each row: the gradient of its logits' scale g (zero where it does not count), its class, and a copy of x whose rows that do not count are zero, so that
-// what stands there (padding may hold infinities or NaN) does not get into dW. float16: g times a power of two that puts the largest near 2^13, since most
-// of dz is far below float16's smallest values; `undo` is what takes it away again.
-template <class T>
+// what stands there (padding may hold infinities or NaN) does not get into dW. 16 bits: g in units of the largest, so that of equal ones, as a mean's are, no rounding of dz is all rows' own,
+// times 2^13 for float16, since most of dz is far below its smallest values; `undo` is what takes both away again. REST: as many rows of x again, for what dz's rounding leaves.
+template <class T, bool REST>
 __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGrad grad, long long rows, const RowCount* counts, int n_counts, bool mean, const T* x, long long ld_x,
                                                         long long x_col, int D, T* x_out, long long ld_out, float* g, int* classes, float* undo) {
     __shared__ RowCount held[8];
@@ -270,22 +270,30 @@ __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGra
     }
     all = block_count(all, held);
     const float counted = mean ? (float)max(all.counted, 1LL) : 1.0f;
-    float scale = 1.0f;
-    if (sizeof(T) == 2 && undo && all.most > 0.0f && all.most < INFINITY) scale = exp2f((float)max(-120, min(120, 13 - ilogbf(all.most / counted))));
-    if (undo && blockIdx.x == 0 && threadIdx.x == 0) *undo = 1.0f / scale;
+    const float top = std::is_same_v<T, __half> ? 8192.0f : 1.0f;
+    const bool scaled = undo && all.most > 0.0f && all.most < INFINITY;
+    if (undo && blockIdx.x == 0 && threadIdx.x == 0) *undo = scaled ? all.most / counted / top : 1.0f;
     constexpr int V = 16 / sizeof(T);
     const bool vectors = x_col == 1 && D % V == 0 && ld_x % V == 0 && (uintptr_t)x % 16 == 0;
     const int lane = threadIdx.x & 31;
     for (long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32; row < rows; row += (long long)gridDim.x * 8) {  // a warp a row
         const int target = targets.of(row);
-        if (lane == 0) g[row] = target < 0 ? 0.0f : grad.of(row) / counted * scale, classes[row] = target;
+        if (lane == 0) g[row] = target < 0 ? 0.0f : scaled ? grad.of(row) / all.most * top : grad.of(row) / counted, classes[row] = target;
         const T* from = x + row * ld_x;
         T* to = x_out + row * ld_out;
         if (vectors) {
 #pragma unroll 4
-            for (int c = lane; c < D / V; c += 32) ((uint4*)to)[c] = target < 0 ? make_uint4(0u, 0u, 0u, 0u) : ((const uint4*)from)[c];
+            for (int c = lane; c < D / V; c += 32) {
+                const uint4 v = target < 0 ? make_uint4(0u, 0u, 0u, 0u) : ((const uint4*)from)[c];
+                ((uint4*)to)[c] = v;
+                if (REST) ((uint4*)(to + rows * ld_out))[c] = v;
+            }
         } else {
-            for (int c = lane; c < D; c += 32) to[c] = target < 0 ? from_float<T>(0.0f) : from[c * x_col];
+            for (int c = lane; c < D; c += 32) {
+                const T v = target < 0 ? from_float<T>(0.0f) : from[c * x_col];
+                to[c] = v;
+                if (REST) to[rows * ld_out + c] = v;
+            }
         }
     }
 }
@@ -326,16 +334,23 @@ __global__ void __launch_bounds__(256) parts_kernel(const float* from, long long
     }
 }
 
-// dz of logits that lie in memory; may take their place.
+// dz of logits that lie in memory; may take their place. `rests`: what its rounding leaves, rounded, as many rows below.
 template <class T>
 __global__ void __launch_bounds__(kRowThreads) slope_kernel(const float* logits, long long ld, long long rows, int first, int cols, const float* lse, long long lse_step,
-                                                            const float* g, const int* classes, T* out, long long ld_out) {
+                                                            const float* g, const int* classes, T* out, long long ld_out, bool rests) {
     grid_wait();
     for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
         const float all = lse[row * lse_step], scale = g[row];
         const int at = classes[row], target = at - first;
-        for (int c = blockIdx.x * kRowThreads + threadIdx.x; c < cols; c += gridDim.x * kRowThreads)
-            out[row * ld_out + c] = from_float<T>(at < 0 ? 0.0f : (expf(logits[row * ld + c] - all) - (c == target ? 1.0f : 0.0f)) * scale);
+        for (int c = blockIdx.x * kRowThreads + threadIdx.x; c < cols; c += gridDim.x * kRowThreads) {
+            const float d = at < 0 ? 0.0f : (expf(logits[row * ld + c] - all) - (c == target ? 1.0f : 0.0f)) * scale;
+            const T rounded = from_float<T>(d);
+            out[row * ld_out + c] = rounded;
+            if (rests) {
+                const float rest = d - to_float(rounded);
+                out[(rows + row) * ld_out + c] = from_float<T>(fabsf(rest) < INFINITY ? rest : 0.0f);  // (infinity and NaN leave nothing)
+            }
+        }
     }
 }
 
@@ -635,29 +650,33 @@ struct Backward : Loss {
     void run(cudaStream_t s, bool only_count) {
         held = 0;
         const int item = dtype_size(dtype);
-        const bool half = dtype == LB_F16;
+        const bool scaled = item == 2;  // `undo` is what the products' results are to be multiplied by
+        // dz of few rows is held in two parts, the second what the rounding of the first leaves, as rows of their own (of x too): with as few terms a sum's error would be that of one rounding, and
+        // the products' tiles have the room
+        const bool rests = item == 2 && T <= 64;
+        const long long R = rests ? 2 * T : T;
         const bool fused = T && gemm_loss_takes(x, w), parts = in_parts() && D % 8 == 0 && in_vectors(dx) && in_vectors(dw);
-        const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(fused ? 2 : 4, T), pieces = (V + piece - 1) / piece, ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
+        const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(fused ? 2 : 4, R), pieces = (V + piece - 1) / piece, ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
         const int n_counts = (int)std::min<long long>(64, (T + 255) / 256);
         RowCount* counts = take<RowCount>(n_counts);
         float *g = take<float>(T), *undo = take<float>(1);
         int* classes = take<int>(T);
-        char *x_kept = take<char>(parts ? T * 6 * part : T * ld_kept * item), *w_parts = take<char>(parts ? piece * 6 * part : 0);
+        char *x_kept = take<char>(parts ? T * 6 * part : R * ld_kept * item), *w_parts = take<char>(parts ? piece * 6 * part : 0);
         float* logits = take<float>(fused || parts ? 0 : T * ld);
-        char* slopes = parts ? take<char>(T * 6 * ld) : dtype == LB_F32 ? (char*)logits : take<char>(T * ld * item);
-        const lb_tensor kept = matrix(x_kept, dtype, T, D, ld_kept), dz = matrix(slopes, dtype, T, piece, ld);
-        // sums over pieces, and what takes float16's scale away: in the products' epilogue where they run on whole tiles, else behind them
+        char* slopes = parts ? take<char>(T * 6 * ld) : dtype == LB_F32 ? (char*)logits : take<char>(R * ld * item);
+        const lb_tensor kept = matrix(x_kept, dtype, T, D, ld_kept), kept_all = matrix(x_kept, dtype, R, D, ld_kept), dz = matrix(slopes, dtype, R, piece, ld);
+        // sums over pieces, and what takes the scale away: in the products' epilogue where they run on whole tiles, else behind them
         // (both in one launch where that fills the GPU better)
-        const lb_tensor sums_a[] = {transposed(dz), dz}, sums_b[] = {kept, rows_of(w, 0, piece)}, sums_out[] = {dw, dx};
-        const bool folds = pieces > 1 || half, both = !parts && T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
-                   dw_tiles = both || (half && T && gemm_sum_takes(sums_a[0], sums_b[0], dw));
+        const lb_tensor sums_a[] = {transposed(dz), dz}, sums_b[] = {kept_all, rows_of(w, 0, piece)}, sums_out[] = {dw, dx};
+        const bool folds = pieces > 1 || scaled, both = !parts && !rests && T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && !rests && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
+                   dw_tiles = both || (scaled && T && gemm_sum_takes(sums_a[0], sums_b[0], dw));
         const int ranges = dtype != LB_F32 || !T ? 1 : parts ? gemm_part_ranges(T, D, piece) : core_ranges(piece), dw_ranges = parts ? gemm_part_ranges(piece, D, T) : 1;
         float *dx_piece = ranges > 1 || (folds && !dx_tiles && !parts) ? take<float>((ranges + 1) * T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
-        float* dw_piece = (half && !dw_tiles) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
+        float* dw_piece = (scaled && !dw_tiles) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
         size_t more = 0;
-        if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept)});
+        if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept_all)});
         const GemmTuning few{T ? few_ranges(piece) : 0, 0};
-        if (few.splits > 1) more = std::max<size_t>(more, (size_t)few.splits * T * D * 4);
+        if (few.splits > 1) more = std::max<size_t>(more, (size_t)few.splits * R * D * 4);
         void* product = take<char>(more);
         if (only_count) return;
         if (T == 0) {
@@ -669,8 +688,11 @@ struct Backward : Loss {
         if (!counts_itself) launch_overlapped(count_kernel, dim3((unsigned)n_counts), dim3(256), 0, s, 0, targets, d_loss, T, counts);
         by_type(dtype, [&](auto* type) {
             using E = std::remove_pointer_t<decltype(type)>;
-            launch_overlapped(row_grads_kernel<E>, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, counts_itself ? (const RowCount*)nullptr : (const RowCount*)counts, n_counts, reduction == LB_REDUCTION_MEAN,
-                              (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], parts ? 0 : (int)D, (E*)x_kept, ld_kept, g, classes, half ? undo : nullptr);
+            auto go = [&](auto kernel) {
+                launch_overlapped(kernel, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, counts_itself ? (const RowCount*)nullptr : (const RowCount*)counts, n_counts,
+                                  reduction == LB_REDUCTION_MEAN, (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], parts ? 0 : (int)D, (E*)x_kept, ld_kept, g, classes, scaled ? undo : nullptr);
+            };
+            rests ? go(row_grads_kernel<E, true>) : go(row_grads_kernel<E, false>);
         });
         if (parts) split(x, classes, parted(x_kept, T, D, part), s);
         for (long long k = 0; k < pieces; k++) {
@@ -680,7 +702,7 @@ struct Backward : Loss {
                 by_type(dtype, [&](auto* type) {
                     using E = std::remove_pointer_t<decltype(type)>;
                     launch_overlapped(fold_kernel<E>, by_rows(to.shape[0], D, 256), dim3(256), 0, s, 0, from, ranges, (long long)to.shape[0], (int)D,
-                                      sum, begins, ends ? (E*)to.ptr : (E*)nullptr, (long long)to.stride[0], half ? (const float*)undo : (const float*)nullptr);
+                                      sum, begins, ends ? (E*)to.ptr : (E*)nullptr, (long long)to.stride[0], scaled ? (const float*)undo : (const float*)nullptr);
                 });
             };
             if (parts) {
@@ -716,7 +738,7 @@ struct Backward : Loss {
             if (!fused) by_type(dtype, [&](auto* type) {
                 using E = std::remove_pointer_t<decltype(type)>;
                 launch_overlapped(slope_kernel<E>, by_rows(T, cols, 4 * kRowThreads), dim3(kRowThreads), 0, s, 0, (const float*)logits, ld, T, (int)first, (int)cols, (const float*)lse.ptr,
-                                  (long long)lse.stride[0], (const float*)g, (const int*)classes, (E*)slopes, ld);
+                                  (long long)lse.stride[0], (const float*)g, (const int*)classes, (E*)slopes, ld, rests);
             });
             const bool begins = k == 0, ends = k == pieces - 1;
             if (both) {
@@ -724,7 +746,7 @@ struct Backward : Loss {
                 float* const sum[] = {nullptr, dx_sum};
                 const bool first_of[] = {true, begins};
                 const lb_tensor* const out[] = {&dw_rows, ends ? &dx : nullptr};
-                gemm_sums(a, b, sum, first_of, out, half ? undo : nullptr, s);
+                gemm_sums(a, b, sum, first_of, out, scaled ? undo : nullptr, s);
                 continue;
             }
             if (dtype == LB_F32) {  // what leaves SMs idle by itself shares a launch
@@ -756,18 +778,18 @@ struct Backward : Loss {
                 continue;
             }
             if (dw_tiles) {
-                gemm_sum(transposed(d), kept, nullptr, true, &dw_rows, undo, s);
+                gemm_sum(transposed(d), kept_all, nullptr, true, &dw_rows, undo, s);
             } else {
-                gemm(transposed(d), kept, half ? matrix(dw_piece, LB_F32, cols, D, D) : dw_rows, EPI_NONE, 0, s, product, more, nullptr, nullptr);
-                if (half) fold(dw_piece, 1, dw_rows, nullptr, true, true);
+                gemm(transposed(d), kept_all, matrix(dw_piece, LB_F32, cols, D, D), EPI_NONE, 0, s, product, more, nullptr, nullptr);
+                fold(dw_piece, 1, dw_rows, nullptr, true, true);
             }
             if (dx_tiles) {
-                gemm_sum(d, rows, dx_sum, begins, ends ? &dx : nullptr, half ? undo : nullptr, s);
+                gemm_sum(d, rows, dx_sum, begins, ends ? &dx : nullptr, undo, s);
             } else {
                 const GemmTuning ranges_of{few_ranges(cols), 0};
                 const bool cut = ranges_of.splits > 1;
-                gemm(d, rows, folds ? matrix(dx_piece, LB_F32, T, D, D) : dx, EPI_NONE, cut ? 3 : 0, s, product, more, nullptr, cut ? &ranges_of : nullptr);
-                if (folds) fold(dx_piece, 1, dx, dx_sum, begins, ends);
+                gemm(d, rows, matrix(dx_piece, LB_F32, R, D, D), EPI_NONE, cut ? 3 : 0, s, product, more, nullptr, cut ? &ranges_of : nullptr);
+                fold(dx_piece, rests ? 2 : 1, dx, dx_sum, begins, ends);
             }
         }
     }

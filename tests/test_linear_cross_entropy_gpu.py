@@ -56,7 +56,7 @@ def check_forward(x, w, targets, reduction, loss, lse, ignored=IGNORED):
     within(loss, losses.sum() / n, tol.sum() / n + 2.0**-23 * losses.sum().abs() / n, "loss")
 
 
-def check_backward(x, w, targets, lse, reduction, d_loss, d_x, d_w, ignored=IGNORED):
+def check_backward(x, w, targets, lse, reduction, d_loss, d_x, d_w, ignored=IGNORED, rounding=None):
     dtype, v = x.dtype, w.shape[0]
     counts = targets != ignored
     x = torch.where(counts[:, None], x, 0.0)
@@ -69,7 +69,7 @@ def check_backward(x, w, targets, lse, reduction, d_loss, d_x, d_w, ignored=IGNO
     dz = torch.where(counts[:, None], (p - hit) * g[:, None], 0.0)
     # p by its argument's error (that of the logit, of the products with log2 e) and the exponential's, g by its quotient's, dz by its rounding;
     # float16's dz is scaled so that the largest |g| is 2^12 or more, and is rounded to multiples of 2^-24 or finer
-    dz_off = p * (off + 2.0**-20 + 2.0**-22 * (z.abs() + lse.double().abs()[:, None])) * g.abs()[:, None] + dz.abs() * (2.0**-21 + (half(dtype) if dtype != torch.float32 else 0))
+    dz_off = p * (off + 2.0**-20 + 2.0**-22 * (z.abs() + lse.double().abs()[:, None])) * g.abs()[:, None] + dz.abs() * (2.0**-21 + (rounding if rounding is not None else half(dtype) if dtype != torch.float32 else 0))
     dz_off = torch.where(counts[:, None], dz_off + (2.0**-37 * g.abs().max() if dtype == torch.float16 else 1e-37), 0.0)
     tiny = 2.0**-25 if dtype == torch.float16 else 1e-37
 
@@ -274,6 +274,37 @@ def test_small_and_large_gradients_in_float16(cuda, scale):
     _, lse = linear_cross_entropy(x, w, targets)
     d_loss = torch.full((), scale, device=cuda)
     check_backward(x, w, targets, lse, "mean", d_loss, *linear_cross_entropy_backward(d_loss, x, w, targets, lse))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(65, 64, 1031), (200, 64, 1031), (100, 15, 1031), (1100, 128, 2000), (2000, 1024, 4000)], ids=lambda s: "x".join(map(str, s)))
+def test_one_gradient_of_all_rows_is_not_rounded(cuda, shape, dtype):
+    """A gradient in the middle of two values of the type: dz is (p - [class]) times it, and only the first is rounded: by half a step of values
+    below one where the class is the row's, by half a step of any value elsewhere."""
+    t, d, v = shape
+    x, w, targets = operands(cuda, t, d, v, dtype, seed=5, scale=0.1)
+    targets.copy_(torch.randperm(v, device=cuda)[:t])
+    _, lse = linear_cross_entropy(x, w, targets, reduction="sum")
+    d_loss = torch.full((), 1.0 + torch.finfo(dtype).eps / 2, device=cuda)
+    d_x, d_w = linear_cross_entropy_backward(d_loss, x, w, targets, lse, reduction="sum")
+    rounding = torch.full((t, v), half(dtype), device=cuda, dtype=torch.float64)
+    rounding[torch.arange(t, device=cuda), targets] = half(dtype) / 2 * (1 + 2.0**-8)  # of a value above 1 - 2^-8
+    check_backward(x, w, targets, lse, "sum", d_loss, d_x, d_w, rounding=rounding)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 64, 300), (2, 8, 1), (14, 328, 5003), (33, 15, 130), (40, 33, 70), (64, 1024, 4096), (60, 16, 2300001)], ids=lambda s: "x".join(map(str, s)))
+def test_few_rows_gradients_are_rounded_once(cuda, shape, dtype):
+    """dz in two parts: half a step of half a step is left."""
+    t, d, v = shape
+    x, w, targets = operands(cuda, t, d, v, dtype, ignored=0.2 * (t % 2 and t > 1), seed=t)
+    g = torch.Generator(device=cuda).manual_seed(3)
+    for reduction in ("none", "mean"):
+        _, lse = linear_cross_entropy(x, w, targets, reduction=reduction)
+        d_loss = torch.randn(t, generator=g, device=cuda) if reduction == "none" else None
+        d_x, d_w = linear_cross_entropy_backward(d_loss, x, w, targets, lse, reduction=reduction)
+        check_backward(x, w, targets, lse, reduction, d_loss, d_x, d_w, rounding=half(dtype) ** 2)
+    device_status()
 
 
 @pytest.mark.parametrize("t", [5, 70, 300])
