@@ -127,6 +127,10 @@ void skinny_gated(const lb_tensor& x, const lb_tensor& w, const lb_tensor& h, co
 // The span sums of gemm_loss for them, [skinny_spans(N)][M].
 int skinny_spans(long long N);
 void skinny_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, void* stream);
+// The same for float32 operands, rows of whole 16 bytes, [skinny_float_spans(M, N)][M]; with `logits` [M][ld] those are stored instead. `_takes`: whether they are for this, not few_kernel.
+bool skinny_float_takes(const lb_tensor& x, const lb_tensor& w);
+int skinny_float_spans(long long M, long long N);
+void skinny_float_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, float* logits, long long ld, void* stream);
 void skinny_product(const lb_tensor& x, const lb_tensor& w, const lb_tensor& out, const lb_tensor* add, void* stream);
 
 }  // namespace lb

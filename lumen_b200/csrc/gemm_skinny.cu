@@ -76,6 +76,19 @@ struct SkinnyLossArgs : SkinnyArgs {
     float* hit;
 };
 
+// The span sum of WIDTH lanes' logits.
+template <int WIDTH>
+__device__ __forceinline__ SpanSum span_of(float z, bool in) {
+    float most = in ? z : -INFINITY;
+#pragma unroll
+    for (int d = WIDTH / 2; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    const float base = most == -INFINITY ? 0.0f : most;
+    float sum = in ? exp2_approx((z - base) * kLog2e) : 0.0f;
+#pragma unroll
+    for (int d = WIDTH / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return {most, sum};
+}
+
 // PLAIN, GATED, LOSS: a product; the gated block's; the linear cross entropy's span sums, of which a block's classes are one: 4 tokens of 1024 x 32768 take 10.1 us, 6.6 TB/s.
 enum SkinnyKind : int { SKINNY_PLAIN, SKINNY_GATED, SKINNY_LOSS };
 
@@ -132,15 +145,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) skinny_kernel(const Args p)
             float z = 0.0f;
             for (int k = 0; k < p.warps; k++) z += sums[k][c][m];
             const bool in = row0 + c < p.N;
-            float most = in ? z : -INFINITY;
-#pragma unroll
-            for (int d = COLS / 2; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            const float base = most == -INFINITY ? 0.0f : most;
-            float sum = in ? exp2_approx((z - base) * kLog2e) : 0.0f;
-#pragma unroll
-            for (int d = COLS / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const SpanSum sum = span_of<COLS>(z, in);
             if (m < p.M) {
-                if (c == 0) p.spans[(long long)blockIdx.x * p.M + m] = SpanSum{most, sum};
+                if (c == 0) p.spans[(long long)blockIdx.x * p.M + m] = sum;
                 if (in && p.targets.of(m) == row0 + c) p.hit[m] = z;
             }
             continue;
@@ -193,6 +200,113 @@ void launch_skinny(Args& p, int sms, cudaStream_t s) {
     }
 }
 
+// Four float32 values in three parts of bfloat16 each: the value rounded, what that leaves rounded, and the rest. Infinities become the largest finite values (times a part that is
+// zero they would be NaN); NaN stays.
+__device__ __forceinline__ void parts_of(uint4 x, uint32_t (*part)[2]) {
+    float v[4] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
+    const float most = __uint_as_float(0x7f7f0000u);
+#pragma unroll
+    for (int j = 0; j < 4; j++) asm("{\n\t.reg .f32 c;\n\tmin.NaN.f32 c, %0, %1;\n\tmax.NaN.f32 %0, c, %2;\n\t}" : "+f"(v[j]) : "f"(most), "f"(-most));
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            const uint32_t w = *(const uint32_t*)&h;
+            part[k][j] = w;
+            if (k < 2) v[2 * j] -= __uint_as_float(w << 16), v[2 * j + 1] -= __uint_as_float(w & 0xffff0000u);
+        }
+}
+
+struct FloatLossArgs : SkinnyLossArgs {
+    float* logits;  // [M][ld_out], instead of the span sums; null: those
+};
+
+// The linear cross entropy's products of up to 32 float32 tokens, on the tensor cores: both operands go into registers as they are and become three parts of bfloat16 there, six of whose
+// products are added up; those of the first parts by themselves, and both sums to what was before after every two blocks of K, rounded, since the tensor cores drop what lies below a sum's last
+// place. A block's ROWS classes are a span. Bound by the time that loads take and, with more tokens, by parting x, which every block does anew, and the products. us in a graph for 8, 16 and 32
+// tokens (behind it what the CUDA cores and, from 17 on, the parts in memory took; the weights' bytes alone): 1024 x 32768 33, 44 and 75 (46, 71, 127; 20.5), 344 x 116036 51, 65 and 115 (64, 95,
+// 207; 24.4), 3576 x 12593 46, 60 and 103 (87, 157, 342; 27.5). With 3 blocks of K on their way 37, 51 and 85 at the first, and the same with 4 and 6: fewer warps find a place.
+constexpr int kFloatWarps = 8, kFloatAhead = 2;
+template <int ROWS, int TOKENS>
+__global__ void __launch_bounds__(kFloatWarps * 32, 2) skinny_float_kernel(const FloatLossArgs p) {
+    __shared__ float sums[kFloatWarps][ROWS][TOKENS + 1];
+    grid_wait();
+    constexpr int TILES = TOKENS / 8, EIGHTS = ROWS / 8, AHEAD = kFloatAhead, PAIR = TILES < 2 ? 1 : 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row0 = blockIdx.x * ROWS;
+    const float *w[EIGHTS], *token[TILES];
+    bool row_in[EIGHTS], token_in[TILES];
+#pragma unroll
+    for (int h = 0; h < EIGHTS; h++) row_in[h] = row0 + 8 * h + g < p.N, w[h] = (const float*)p.w + (long long)(row_in[h] ? row0 + 8 * h + g : 0) * p.ld_w + 4 * t;
+#pragma unroll
+    for (int n = 0; n < TILES; n++) token_in[n] = 8 * n + g < p.M, token[n] = (const float*)p.x + (long long)(token_in[n] ? 8 * n + g : 0) * p.ld_x + 4 * t;
+    float all[ROWS / 16][TILES][4] = {};
+    const int blocks = (p.K + 15) / 16, first = warp * p.per_warp, last = min(blocks, first + p.per_warp);
+    uint4 a[AHEAD][EIGHTS], x[AHEAD][TILES];  // in turn: a place is loaded anew as soon as it has been used
+    auto load = [&](int i, int block) {
+        const int k = block * 16;
+        const bool in = block < last && k + 4 * t < p.K;
+#pragma unroll
+        for (int h = 0; h < EIGHTS; h++) a[i][h] = load_if<true>(w[h] + k, in && row_in[h]);
+#pragma unroll
+        for (int n = 0; n < TILES; n++) x[i][n] = load_if<false>(token[n] + k, in && token_in[n]);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) load(i, first + i);
+    for (int k0 = first; k0 < last; k0 += AHEAD) {
+        float most[ROWS / 16][TILES][4] = {}, rest[ROWS / 16][TILES][4] = {};
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            uint32_t ap[EIGHTS][3][2];
+#pragma unroll
+            for (int h = 0; h < EIGHTS; h++) parts_of(a[i][h], ap[h]);
+#pragma unroll
+            for (int n0 = 0; n0 < TILES; n0 += PAIR) {  // tiles and products in an order that has none wait for the one before
+                uint32_t b[PAIR][3][2];
+#pragma unroll
+                for (int n = 0; n < PAIR; n++) parts_of(x[i][n0 + n], b[n]);
+                auto add = [&](float (*d)[TILES][4], int u, int v) {
+#pragma unroll
+                    for (int n = 0; n < PAIR; n++)
+#pragma unroll
+                        for (int m = 0; m < ROWS / 16; m++)
+                            mma_16x8<false>(d[m][n0 + n], ap[2 * m][u][0], ap[2 * m + 1][u][0], ap[2 * m][u][1], ap[2 * m + 1][u][1], b[n][v][0], b[n][v][1]);
+                };
+                add(rest, 0, 2), add(most, 0, 0), add(rest, 2, 0), add(rest, 1, 1), add(rest, 0, 1), add(rest, 1, 0);
+            }
+            load(i, k0 + AHEAD + i);
+        }
+#pragma unroll
+        for (int m = 0; m < ROWS / 16; m++)
+#pragma unroll
+            for (int n = 0; n < TILES; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) all[m][n][j] += most[m][n][j] + rest[m][n][j];
+    }
+#pragma unroll
+    for (int m = 0; m < ROWS / 16; m++)
+#pragma unroll
+        for (int n = 0; n < TILES; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) sums[warp][16 * m + 8 * (j / 2) + g][8 * n + 2 * t + j % 2] = all[m][n][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * TOKENS; i += blockDim.x) {
+        const int c = i % ROWS, m = i / ROWS;
+        float z = 0.0f;
+        for (int k = 0; k < p.warps; k++) z += sums[k][c][m];
+        const bool in = row0 + c < p.N;
+        if (p.logits) {
+            if (in && m < p.M) p.logits[m * p.ld_out + row0 + c] = z;
+            continue;
+        }
+        const SpanSum sum = span_of<ROWS>(z, in);
+        if (m < p.M) {
+            if (c == 0) p.spans[(long long)blockIdx.x * p.M + m] = sum;
+            if (in && p.targets.of(m) == row0 + c) p.hit[m] = z;
+        }
+    }
+}
+
 // The rows of an operand along K in 16-byte pieces.
 bool rows_in_pieces(const lb_tensor& t) { return (uintptr_t)t.ptr % 16 == 0 && t.stride[1] == 1 && (t.shape[0] <= 1 || t.stride[0] % 8 == 0); }
 
@@ -240,6 +354,31 @@ void skinny_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets,
     p.N = (int)w.shape[0], p.out = nullptr, p.targets = targets, p.spans = spans, p.hit = hit;
     if (x.dtype == LB_F16) launch_skinny<SKINNY_LOSS, true>(p, sm_count_hint(), (cudaStream_t)stream);
     else launch_skinny<SKINNY_LOSS, false>(p, sm_count_hint(), (cudaStream_t)stream);
+}
+
+// One token, and up to four with short rows, are faster on the CUDA cores, whose loads are a warp's whole row: 1 token 31 us there and 33 here with 1024 x 32768, 22.5 and 29 with 200 x 93558,
+// 36 and 46 with 3576 x 12593; 4 tokens 40 and 33, 24 and 29.6, 58 and 46.
+bool skinny_float_takes(const lb_tensor& x, const lb_tensor& w) {
+    if (x.shape[0] == 1 || (x.shape[0] <= 4 && x.shape[1] < 512)) return false;
+    auto in_pieces = [](const lb_tensor& t) { return (uintptr_t)t.ptr % 16 == 0 && t.stride[1] == 1 && (t.shape[0] <= 1 || t.stride[0] % 4 == 0); };
+    return x.dtype == LB_F32 && x.shape[0] <= kMaxTokens && x.shape[1] % 4 == 0 && in_pieces(x) && in_pieces(w);
+}
+// Classes of a block: 32 where that leaves every SM one and the tokens' sums leave the registers for it (32 tokens of 1024 x 32768 75 us with 16, 94 with 32; 8 of them 38 and 33).
+static int float_rows(long long M, long long N) { return M <= 16 && N >= 32LL * sm_count_hint() ? 32 : 16; }
+int skinny_float_spans(long long M, long long N) { return (int)((N + float_rows(M, N) - 1) / float_rows(M, N)); }
+void skinny_float_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, SpanSum* spans, float* hit, float* logits, long long ld, void* stream) {
+    driver();
+    FloatLossArgs p{};
+    (SkinnyArgs&)p = skinny_args(x, w, w);
+    p.N = (int)w.shape[0], p.out = nullptr, p.targets = targets, p.spans = spans, p.hit = hit, p.logits = logits, p.ld_out = ld;
+    const int rows = float_rows(p.M, p.N), tiles = (p.N + rows - 1) / rows, blocks = (p.K + 15) / 16;
+    // four warps, so that blocks start and end at different times; eight where there are too few blocks for that (8 tokens of 4096 x 2000 14.4 us with four, 12.5 with eight; 344 x 116036 51 and 68)
+    const int warps = tiles <= 2 * sm_count_hint() ? kFloatWarps : kFloatWarps / 2;
+    p.warps = std::min(warps, blocks);  // (those of K; the others share what is behind)
+    p.per_warp = (blocks + p.warps - 1) / p.warps;
+    auto go = [&](auto kernel) { launch_overlapped(kernel, dim3((unsigned)tiles), dim3((unsigned)warps * 32), 0, (cudaStream_t)stream, 0, p); };
+    if (rows == 32) p.M <= 8 ? go(skinny_float_kernel<32, 8>) : go(skinny_float_kernel<32, 16>);
+    else p.M <= 8 ? go(skinny_float_kernel<16, 8>) : p.M <= 16 ? go(skinny_float_kernel<16, 16>) : go(skinny_float_kernel<16, 32>);
 }
 
 }  // namespace lb

@@ -70,9 +70,8 @@ __global__ void __launch_bounds__(kRowThreads) span_kernel(const float* logits, 
 }
 
 // Few rows of float32, straight from the weights, which are read once: a warp takes four classes' rows at a time, its lanes a vector of K each, against all tokens (from
-// the L1), and the lanes' sums are added at the end. A block's 32 classes are a span; with `logits` those are stored instead. Bound by the time that a warp's four vectors take to
-// arrive (weights of 134 MB: 4 tokens 40 us in a graph, 3.3 TB/s) and, with more tokens, by the loads of x and the registers: 16 tokens 72. The next vectors fetched ahead took
-// 63 us with 8 tokens instead of 43, in half the registers that ptxas then found.
+// the L1), and the lanes' sums are added at the end. A block's 32 classes are a span; with `logits` those are stored instead. Up to four tokens, and layouts without vectors up to 16.
+// Bound by the time that a warp's four vectors take to arrive: weights of 1024 x 32768 1 token 31 us in a graph, 4.3 TB/s; of 200 x 93558 4 tokens 24.
 constexpr int kFewWarps = 8, kFewRows = 4, kFewSpan = kFewWarps * kFewRows, kFewTokens = 16;
 template <int TOKENS, int VEC>
 __global__ void __launch_bounds__(kFewWarps * 32) few_kernel(const float* x, long long ld_x, const float* w, long long ld_w, int T, int D, int V, Targets targets, SpanSum* spans,
@@ -476,7 +475,7 @@ struct Loss {
     // Whether float32 operands go to the tensor cores in parts of 16 bits: six products of them take less than one of float32 on the CUDA cores, but there are 16 bytes
     // an element of the weights to be moved for it, and three launches. us in a graph, CUDA cores -> parts, forward and backward: 33 x 344 x 116035 228 -> 240 and 855 -> 415, 53 of
     // it 231 -> 222 and 956 -> 402, 64 x 2048 x 32768 392 -> 321 and 1248 -> 539, 300 x 64 x 5000 (9.6e7) 20.6 -> 17.4 and 59.7 -> 49.4, 1000 x 128 x 2000 36 -> 18 and 107 -> 50,
-    // 2000 x 1024 x 8000 1300 -> 151 and 4055 -> 476. Up to 16 rows few_kernel reads the weights once.
+    // 2000 x 1024 x 8000 1300 -> 151 and 4055 -> 476. Up to 32 rows' losses, and the logits of 16 rows' gradients, come straight from the weights.
     bool in_parts() const { return dtype == LB_F32 && T > kFewTokens && (double)T * (double)V * (double)D >= 3e7; }
     // The vocabulary in pieces whose [width, piece] of `item` bytes an element takes about kPieceBytes.
     long long piece_of(int item, long long width) const {
@@ -527,8 +526,7 @@ void run_few(const lb_tensor& x, const lb_tensor& w, const Targets& targets, Spa
                           (long long)w.stride[0], T, D, V, targets, spans, hit, logits, ld);
     };
     if (T <= 4) vec ? go(few_kernel<4, 4>) : go(few_kernel<4, 1>);
-    else if (T <= 8) vec ? go(few_kernel<8, 4>) : go(few_kernel<8, 1>);
-    else vec ? go(few_kernel<16, 4>) : go(few_kernel<16, 1>);
+    else T <= 8 ? go(few_kernel<8, 1>) : go(few_kernel<16, 1>);  // (those of whole vectors are skinny_float_loss's)
 }
 
 struct Forward : Loss {
@@ -549,12 +547,12 @@ struct Forward : Loss {
     }
     void run(cudaStream_t s, bool only_count) {
         held = 0;
-        const bool few16 = T && skinny_takes(x, w), few32 = T && few_float32(x, w), few = few16 || few32, parts = in_parts(), fused = few || (T && gemm_loss_takes(x, w));
+        const bool few16 = T && skinny_takes(x, w), float_tiles = T && skinny_float_takes(x, w), few32 = T && !float_tiles && few_float32(x, w), few = few16 || few32 || float_tiles, parts = !few && in_parts(), fused = few || (T && gemm_loss_takes(x, w));
         // some rows at a time, whose spans (or copies) stay small whatever the number of rows
         const long long part = up(D, 64), at_once = few ? T : std::min(T, fused ? std::max(4096LL, kPieceBytes / 8 / gemm_spans(V) / 1024 * 1024) : 65536LL);
         const long long piece = parts ? piece_of(6, std::max(at_once, part)) : piece_of(4, at_once), pieces = (V + piece - 1) / piece, last = V - (pieces - 1) * piece;
         auto spans_of = [&](long long cols) { return parts ? (long long)gemm_spans(cols) : (cols + kSpan - 1) / kSpan; };
-        const long long n_spans = few32 ? (V + kFewSpan - 1) / kFewSpan : few ? skinny_spans(V) : fused ? gemm_spans(V) : (pieces - 1) * spans_of(piece) + spans_of(last);
+        const long long n_spans = float_tiles ? skinny_float_spans(T, V) : few32 ? (V + kFewSpan - 1) / kFewSpan : few ? skinny_spans(V) : fused ? gemm_spans(V) : (pieces - 1) * spans_of(piece) + spans_of(last);
         // rows of a block: enough for every SM, or all of a few, whose sum is then theirs
         const int R = T >= 32LL * sm_count_hint() ? 32 : T >= 512 || (T <= 8 && reduction != LB_REDUCTION_NONE) ? 8 : 1;
         const long long blocks = (at_once + R - 1) / R, rounds = T ? (T + at_once - 1) / at_once : 0, all_blocks = rounds ? (rounds - 1) * blocks + (T - (rounds - 1) * at_once + R - 1) / R : 0;
@@ -578,7 +576,8 @@ struct Forward : Loss {
             const lb_tensor rows = rows_of(x, t0, n), copies = parted(x_parts, n, D, part);
             Targets classes = targets;
             classes.at = (const char*)targets.at + t0 * targets.step * (targets.wide ? 8 : 4);
-            if (few32) run_few(rows, w, classes, spans, hit, nullptr, 0, s);
+            if (float_tiles) skinny_float_loss(rows, w, classes, spans, hit, nullptr, 0, s);
+            else if (few32) run_few(rows, w, classes, spans, hit, nullptr, 0, s);
             else if (few16) skinny_loss(rows, w, classes, spans, hit, s);
             else if (fused) {
                 lb_tensor operand = rows;
@@ -733,6 +732,7 @@ struct Backward : Loss {
             lb_tensor z = matrix(logits, LB_F32, T, cols, ld), d = dz, dw_rows = rows_of(dw, first, cols);
             d.shape[1] = cols;
             if (fused) gemm_loss_slopes(kept, rows, (const float*)lse.ptr, lse.stride[0], g, classes, (int)first, d, s);
+            else if (skinny_float_takes(x, rows)) skinny_float_loss(x, rows, targets, nullptr, nullptr, logits, ld, s);
             else if (few_float32(x, rows)) run_few(x, rows, targets, nullptr, nullptr, logits, ld, s);
             else gemm(x, transposed(rows), z, EPI_NONE, 0, s, product, more, nullptr, nullptr);
             if (!fused) by_type(dtype, [&](auto* type) {

@@ -251,7 +251,7 @@ def test_layouts(cuda, t, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("t", [3, 150])
+@pytest.mark.parametrize("t", [3, 12, 30, 150])
 def test_logits_of_any_size(cuda, t, dtype):
     x, w, targets = operands(cuda, t, 64, 400, dtype, scale=600.0)  # up to some thousands: exponentials of them are infinite
     loss, lse = linear_cross_entropy(x, w, targets, reduction="none")
