@@ -17,6 +17,7 @@
 #include "launch.cuh"
 #include "linear_loss.h"
 #include "overlap.h"
+#include "pair.cuh"
 
 namespace lb {
 bool gemm(const lb_tensor& a, const lb_tensor& b, const lb_tensor& d, int epilogue, int kernel_choice, void* stream, void* scratch, size_t scratch_bytes,
@@ -369,6 +370,122 @@ __global__ void __launch_bounds__(256) fold_kernel(const float* product, int ran
         }
 }
 
+// Both gradients of a few rows in one pass over the weights: a thread has four columns of x and of dx's sums in registers, for every class it reads the weights' four, which the class's dz takes
+// to dx, and writes dW's. A block's range of classes is a part of dx, to be added up. `rests`: dz's second parts are T rows below. Bound by the loads' way and, with more tokens, by the products. A
+// backward pass in a graph, products by themselves -> this, us: float32 4 tokens of 1024 x 32768 197 -> 89 (the floor of one reading and one writing of the weights 41), 16 of it 241 -> 121, of
+// 344 x 116036 504 -> 178; bfloat16, whose tensor cores take more tokens for the same time, 4 of 1024 x 32768 66 -> 58, but 5 67 -> 71.
+constexpr int kGradThreads = 128, kGradClasses = 64;
+constexpr int grad_tokens(int item) { return item == 4 ? 16 : 4; }
+constexpr int grad_blocks(int tokens) { return tokens == 16 ? 3 : 4; }  // on an SM
+template <class E>
+__device__ __forceinline__ void load4(const E* at, Pair* v) {
+    if constexpr (sizeof(E) == 4) {
+        const float4 f = *(const float4*)at;
+        v[0] = both(f.x, f.y), v[1] = both(f.z, f.w);
+    } else {
+        const uint2 raw = *(const uint2*)at;
+        const E* e = (const E*)&raw;
+        v[0] = both(to_float(e[0]), to_float(e[1])), v[1] = both(to_float(e[2]), to_float(e[3]));
+    }
+}
+template <class E, int TOKENS>
+__global__ void __launch_bounds__(kGradThreads, grad_blocks(TOKENS)) few_grads_kernel(const E* x, long long ld_x, const E* w, long long ld_w, const E* dz, long long ld, bool rests, int T, int D,
+                                                                                      int classes, int each, E* dw, long long ld_dw, float* dx, const float* undo) {
+    __shared__ float4 z4[kGradClasses][TOKENS / 4];
+    constexpr int AHEAD = TOKENS <= 8 ? 8 : 4;
+    grid_wait();
+    const int c = (blockIdx.x * kGradThreads + threadIdx.x) * 4, first = blockIdx.y * each, last = min(classes, first + each);
+    const bool in = c < D;
+    const float scale = undo ? *undo : 1.0f;
+    Pair xs[TOKENS][2], sums[TOKENS][2];
+#pragma unroll
+    for (int t = 0; t < TOKENS; t++) {
+        xs[t][0] = xs[t][1] = sums[t][0] = sums[t][1] = both(0.0f, 0.0f);
+        if (in && t < T) load4(x + t * ld_x + c, xs[t]);
+    }
+    for (int v0 = first; v0 < last; v0 += kGradClasses) {
+        const int n = min(kGradClasses, last - v0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < kGradClasses * TOKENS; i += kGradThreads) {
+            const int v = i % kGradClasses, t = i / kGradClasses;
+            float d = 0.0f;
+            if (t < T && v < n) {
+                d = to_float(dz[t * ld + v0 + v]);
+                if (rests) d += to_float(dz[(T + t) * ld + v0 + v]);
+            }
+            ((float*)z4[v])[t] = d;
+        }
+        __syncthreads();
+        if (!in) continue;
+        const E* from = w + (long long)v0 * ld_w + c;
+        E* to = dw + (long long)v0 * ld_dw + c;
+        for (int v1 = 0; v1 < n; v1 += AHEAD) {
+            Pair ws[AHEAD][2];
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) load4(from + (long long)min(v1 + u, n - 1) * ld_w, ws[u]);
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                if (v1 + u >= n) break;
+                Pair d[2] = {both(0.0f, 0.0f), both(0.0f, 0.0f)};
+#pragma unroll
+                for (int q = 0; q < TOKENS / 4; q++) {
+                    const float4 z = z4[v1 + u][q];
+                    const float zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const Pair zz = both(zs[j], zs[j]);
+                        const int t = 4 * q + j;
+                        d[0] = fma2(xs[t][0], zz, d[0]), d[1] = fma2(xs[t][1], zz, d[1]);
+                        sums[t][0] = fma2(ws[u][0], zz, sums[t][0]), sums[t][1] = fma2(ws[u][1], zz, sums[t][1]);
+                    }
+                }
+                const float2 lo = apart(d[0]), hi = apart(d[1]);
+                E* row = to + (long long)(v1 + u) * ld_dw;
+                if constexpr (sizeof(E) == 4) {
+                    *(float4*)row = make_float4(lo.x, lo.y, hi.x, hi.y);
+                } else {
+                    const E e[4] = {from_float<E>(lo.x * scale), from_float<E>(lo.y * scale), from_float<E>(hi.x * scale), from_float<E>(hi.y * scale)};
+                    uint2 raw;
+                    memcpy(&raw, e, 8);
+                    *(uint2*)row = raw;
+                }
+            }
+        }
+    }
+    if (!in) return;
+#pragma unroll
+    for (int t = 0; t < TOKENS; t++) {
+        const float2 lo = apart(sums[t][0]), hi = apart(sums[t][1]);
+        if (t < T) *(float4*)(dx + ((long long)blockIdx.y * T + t) * D + c) = make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+}
+
+// fold_kernel for many sums: eight threads take every eighth of a value's.
+template <class T>
+__global__ void __launch_bounds__(256) fold_many_kernel(const float* product, int ranges, long long rows, int D, float* sum, bool begins, T* out, long long ld_out, const float* undo) {
+    __shared__ float held[8][32];
+    grid_wait();
+    const float scale = undo ? *undo : 1.0f;
+    const int group = threadIdx.x / 32, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane;
+    for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
+        const long long i = row * D + c;
+        float v = 0.0f;
+        if (c < D) {
+#pragma unroll 8
+            for (int k = group; k < ranges; k += 8) v += product[(long long)k * rows * D + i];
+        }
+        __syncthreads();
+        held[group][lane] = v;
+        __syncthreads();
+        if (group || c >= D) continue;
+        v = begins ? 0.0f : sum[i];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v += held[k][lane];
+        if (out) out[row * ld_out + c] = from_float<T>(v * scale);
+        else sum[i] = v;
+    }
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------
 
 lb_tensor matrix(void* ptr, int dtype, long long rows, long long cols, long long ld) {
@@ -628,6 +745,8 @@ struct Backward : Loss {
         return (int)std::max(1LL, std::min({4LL * sm_count_hint() / tiles, K / 256, 64LL}));
     }
 
+    long long few_grad_slots() const { return (long long)sm_count_hint() * grad_blocks(T <= 8 ? 8 : 16); }
+
     void results(const lb_tensor* dx_t, const lb_tensor* dw_t) {
         dx = as_rows(dx_t, 1, "d_x"), dw = as_rows(dw_t, 1, "d_weight");
         if (dx.dtype != dtype || dx.shape[0] != T || dx.shape[1] != D) refuse("d_x must have the shape and dtype of x");
@@ -656,6 +775,9 @@ struct Backward : Loss {
         const long long R = rests ? 2 * T : T;
         const bool fused = T && gemm_loss_takes(x, w), parts = in_parts() && D % 8 == 0 && in_vectors(dx) && in_vectors(dw);
         const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(fused ? 2 : 4, R), pieces = (V + piece - 1) / piece, ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
+        auto in_fours = [&](const lb_tensor& t) { return (uintptr_t)t.ptr % (4 * item) == 0 && t.stride[1] == 1 && (t.shape[0] <= 1 || t.stride[0] % 4 == 0); };
+        const bool one_pass = T && T <= grad_tokens(item) && D % 4 == 0 && in_fours(w) && in_fours(dw);
+        const long long slices = (D / 4 + kGradThreads - 1) / kGradThreads, each = std::max(16LL, one_pass ? (piece * slices + few_grad_slots() - 1) / few_grad_slots() : 1);
         const int n_counts = (int)std::min<long long>(64, (T + 255) / 256);
         RowCount* counts = take<RowCount>(n_counts);
         float *g = take<float>(T), *undo = take<float>(1);
@@ -672,6 +794,7 @@ struct Backward : Loss {
         const int ranges = dtype != LB_F32 || !T ? 1 : parts ? gemm_part_ranges(T, D, piece) : core_ranges(piece), dw_ranges = parts ? gemm_part_ranges(piece, D, T) : 1;
         float *dx_piece = ranges > 1 || (folds && !dx_tiles && !parts) ? take<float>((ranges + 1) * T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
         float* dw_piece = (scaled && !dw_tiles) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
+        float* dx_ranges = one_pass ? take<float>((piece + each - 1) / each * T * D) : nullptr;
         size_t more = 0;
         if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept_all)});
         const GemmTuning few{T ? few_ranges(piece) : 0, 0};
@@ -741,6 +864,22 @@ struct Backward : Loss {
                                   (long long)lse.stride[0], (const float*)g, (const int*)classes, (E*)slopes, ld, rests);
             });
             const bool begins = k == 0, ends = k == pieces - 1;
+            if (one_pass) {
+                const long long n_ranges = (cols + each - 1) / each;
+                const float* times = scaled ? undo : nullptr;
+                by_type(dtype, [&](auto* type) {
+                    using E = std::remove_pointer_t<decltype(type)>;
+                    auto go = [&](auto kernel) {
+                        launch_overlapped(kernel, dim3((unsigned)slices, (unsigned)n_ranges), dim3(kGradThreads), 0, s, 0, (const E*)x_kept, ld_kept, (const E*)rows.ptr, (long long)w.stride[0],
+                                          (const E*)slopes, ld, rests, (int)T, (int)D, (int)cols, (int)each, (E*)dw_rows.ptr, (long long)dw.stride[0], dx_ranges, times);
+                    };
+                    if constexpr (grad_tokens(sizeof(E)) == 4) go(few_grads_kernel<E, 4>);
+                    else T <= 4 ? go(few_grads_kernel<E, 4>) : T <= 8 ? go(few_grads_kernel<E, 8>) : go(few_grads_kernel<E, 16>);
+                    launch_overlapped(fold_many_kernel<E>, by_rows(T, D, 32), dim3(256), 0, s, 0, (const float*)dx_ranges, (int)n_ranges, T, (int)D, dx_sum, begins,
+                                      ends ? (E*)dx.ptr : (E*)nullptr, (long long)dx.stride[0], times);
+                });
+                continue;
+            }
             if (both) {
                 const lb_tensor a[] = {transposed(d), d}, b[] = {kept, rows};
                 float* const sum[] = {nullptr, dx_sum};
