@@ -1888,6 +1888,24 @@ bool gemm_sum_takes(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor&
     const GemmRoute route = gemm_route(a.rows, b.cols, a.cols, 1, sm_count_hint(), 0, gemm_scratch_bytes(a.rows, b.cols, a.cols, 1), nullptr);
     return route.ranges == 0 && route.splits == 1;
 }
+int gemm_narrow_ranges(const lb_tensor& a_t, const lb_tensor& b_t) {
+    const View3 a = view3(a_t, "a"), b = view3(b_t, "b");
+    bool a_cols, b_cols;
+    if (!tensor_core_operands(a, b, a_cols, b_cols)) return 0;
+    const int sms = sm_count_hint(), split = gemm_splits(a.rows, b.cols, a.cols, 1, sms);
+    return gemm_small_splits(a.rows, b.cols, a.cols, 1, sms, split > 1 ? gemm_tile_splits(a.rows, b.cols, a.cols, 1, sms) : 1);
+}
+void gemm_narrow(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& out, const float* undo, void* stream) {
+    driver();
+    const View3 a = view3(a_t, "a"), b = view3(b_t, "b");
+    bool a_cols, b_cols;
+    tensor_core_operands(a, b, a_cols, b_cols);
+    SmallGemmArgs q{};
+    q.M = (int)a.rows, q.N = (int)b.cols, q.K = (int)a.cols, q.a_mn_major = !a_cols, q.b_mn_major = b_cols, q.in_bf16 = a.dtype == LB_BF16;
+    q.d = out.ptr, q.d_bf16 = out.dtype == LB_BF16, q.d_f16 = out.dtype == LB_F16, q.ldd = out.stride[0], q.undo = undo, q.status = status_word();
+    q.splits = gemm_narrow_ranges(a_t, b_t);
+    gemm_small(operand_map(a, a_cols, BM, 0), operand_map(turned(b), !b_cols, 64, 0), q, 1, device_info().sms, (cudaStream_t)stream);
+}
 int gemm_part_ranges(long long M, long long N, long long K) {
     const int pairs = sm_count_hint() / 2;
     const long long tiles = (M + 2 * BM - 1) / (2 * BM) * ((N + BN - 1) / BN), total_kb = (K + BK - 1) / BK * kPartProducts;

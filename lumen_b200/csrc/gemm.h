@@ -64,6 +64,7 @@ struct SmallGemmArgs {
     int epilogue;
     const void* aux;
     long long ld_aux, aux_batch_stride;
+    const float* undo;  // what a 16-bit result is multiplied by before it is rounded; null: nothing
     int splits;  // CTAs of a cluster: 1, 2, 4 or 8, no more than the 64-wide blocks of K
     int* status;
     int tiles_m, tiles_n, vec, aux_vec;  // set by gemm_small
@@ -108,6 +109,9 @@ void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, 
 
 // sum + a b on CTA pairs, `sum` dense float32 [M, N] (nothing where it `begins`): rounded into `out` (float32 or the operands' type), times *undo unless that is null, or, with a null `out`, into sum.
 // `_takes`: whether layouts are theirs (`out` stands for all rows of the result) and lb_gemm would take whole K on pairs.
+// A product on narrow tiles, times *undo unless that is null, 16-bit results; `_ranges`: how many ranges of K, 0 where narrow tiles are not for it.
+int gemm_narrow_ranges(const lb_tensor& a, const lb_tensor& b);
+void gemm_narrow(const lb_tensor& a, const lb_tensor& b, const lb_tensor& out, const float* undo, void* stream);
 bool gemm_sum_takes(const lb_tensor& a, const lb_tensor& b, const lb_tensor& out);
 void gemm_sum(const lb_tensor& a, const lb_tensor& b, float* sum, bool begins, const lb_tensor* out, const float* undo, void* stream, Parts parts = {});
 

@@ -310,6 +310,11 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         }
         const long long at = (long long)b * p.d_batch_stride + row * p.ldd + col;
         if (p.d_bf16 || p.d_f16) {
+            if (p.undo) {
+                const float scale = *p.undo;
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] *= scale;
+            }
             uint32_t h[4];
             if (p.d_bf16) {
 #pragma unroll

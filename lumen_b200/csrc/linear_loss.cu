@@ -786,14 +786,15 @@ struct Backward : Loss {
         float* logits = take<float>(fused || parts ? 0 : T * ld);
         char* slopes = parts ? take<char>(T * 6 * ld) : dtype == LB_F32 ? (char*)logits : take<char>(R * ld * item);
         const lb_tensor kept = matrix(x_kept, dtype, T, D, ld_kept), kept_all = matrix(x_kept, dtype, R, D, ld_kept), dz = matrix(slopes, dtype, R, piece, ld);
-        // sums over pieces, and what takes the scale away: in the products' epilogue where they run on whole tiles, else behind them
+        // sums over pieces, and what takes the scale away: in the products' epilogue where they run on whole tiles or narrow ones, else behind them
         // (both in one launch where that fills the GPU better)
         const lb_tensor sums_a[] = {transposed(dz), dz}, sums_b[] = {kept_all, rows_of(w, 0, piece)}, sums_out[] = {dw, dx};
         const bool folds = pieces > 1 || scaled, both = !parts && !rests && T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && !rests && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
-                   dw_tiles = both || (scaled && T && gemm_sum_takes(sums_a[0], sums_b[0], dw));
+                   dw_tiles = both || (scaled && T && gemm_sum_takes(sums_a[0], sums_b[0], dw)), dw_narrow = scaled && T && pieces == 1 && !dw_tiles && gemm_narrow_ranges(sums_a[0], sums_b[0]),
+                   dx_narrow = scaled && T && !rests && pieces == 1 && !dx_tiles && gemm_narrow_ranges(sums_a[1], sums_b[1]);
         const int ranges = dtype != LB_F32 || !T ? 1 : parts ? gemm_part_ranges(T, D, piece) : core_ranges(piece), dw_ranges = parts ? gemm_part_ranges(piece, D, T) : 1;
-        float *dx_piece = ranges > 1 || (folds && !dx_tiles && !parts) ? take<float>((ranges + 1) * T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
-        float* dw_piece = (scaled && !dw_tiles) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
+        float *dx_piece = ranges > 1 || (folds && !dx_tiles && !dx_narrow && !parts) ? take<float>((ranges + 1) * T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
+        float* dw_piece = (scaled && !dw_tiles && !dw_narrow) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
         float* dx_ranges = one_pass ? take<float>((piece + each - 1) / each * T * D) : nullptr;
         size_t more = 0;
         if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept_all)});
@@ -918,12 +919,16 @@ struct Backward : Loss {
             }
             if (dw_tiles) {
                 gemm_sum(transposed(d), kept_all, nullptr, true, &dw_rows, undo, s);
+            } else if (dw_narrow) {
+                gemm_narrow(transposed(d), kept_all, dw_rows, undo, s);
             } else {
                 gemm(transposed(d), kept_all, matrix(dw_piece, LB_F32, cols, D, D), EPI_NONE, 0, s, product, more, nullptr, nullptr);
                 fold(dw_piece, 1, dw_rows, nullptr, true, true);
             }
             if (dx_tiles) {
                 gemm_sum(d, rows, dx_sum, begins, ends ? &dx : nullptr, undo, s);
+            } else if (dx_narrow) {
+                gemm_narrow(d, rows, dx, undo, s);
             } else {
                 const GemmTuning ranges_of{few_ranges(cols), 0};
                 const bool cut = ranges_of.splits > 1;
