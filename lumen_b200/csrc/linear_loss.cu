@@ -815,7 +815,8 @@ struct Backward : Loss {
                 launch_overlapped(kernel, dim3(row_blocks((T + 7) / 8)), dim3(256), 0, s, 0, targets, d_loss, T, counts_itself ? (const RowCount*)nullptr : (const RowCount*)counts, n_counts,
                                   reduction == LB_REDUCTION_MEAN, (const E*)x.ptr, (long long)x.stride[0], (long long)x.stride[1], parts ? 0 : (int)D, (E*)x_kept, ld_kept, g, classes, scaled ? undo : nullptr);
             };
-            rests ? go(row_grads_kernel<E, true>) : go(row_grads_kernel<E, false>);
+            if constexpr (sizeof(E) == 2) rests ? go(row_grads_kernel<E, true>) : go(row_grads_kernel<E, false>);
+            else go(row_grads_kernel<E, false>);
         });
         if (parts) split(x, classes, parted(x_kept, T, D, part), s);
         for (long long k = 0; k < pieces; k++) {

@@ -107,7 +107,7 @@ def test_forward_and_backward(cuda, shape, dtype):
     device_status()
 
 
-@pytest.mark.parametrize("dtype, shape", [(torch.bfloat16, (600, 16, 230001)), (torch.float16, (610, 16, 230001)), (torch.float32, (600, 16, 120001)), (torch.bfloat16, (600, 15, 120001)), (torch.float32, (60, 8, 1200001)),
+@pytest.mark.parametrize("dtype, shape", [(torch.bfloat16, (600, 16, 230001)), (torch.float16, (610, 16, 230001)), (torch.float32, (600, 16, 120001)), (torch.bfloat16, (600, 15, 120001)), (torch.float32, (60, 8, 1200001)), (torch.float32, (16, 8, 4300001)),
                                           (torch.bfloat16, (8192, 1024, 20001)), (torch.float16, (8200, 1000, 20001))])  # fmt: skip
 def test_a_vocabulary_in_several_pieces(cuda, dtype, shape):
     x, w, targets = operands(cuda, *shape, dtype, ignored=0.1)
@@ -156,7 +156,7 @@ def test_rows_in_several_rounds(cuda, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("t", [6, 300])
+@pytest.mark.parametrize("t", [4, 6, 25, 300])
 def test_what_stands_in_rows_that_do_not_count(cuda, t, dtype):
     x, w, targets = operands(cuda, t, 72, 500, dtype, ignored=0.4)
     targets[:3] = IGNORED
@@ -212,7 +212,7 @@ def test_classes_outside_the_vocabulary_and_what_is_ignored(cuda, t):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("t", [6, 260])
+@pytest.mark.parametrize("t", [4, 6, 14, 30, 260])
 def test_layouts(cuda, t, dtype):
     x, w, targets = operands(cuda, t, 64, 300, dtype, ignored=0.2)
     want_loss, want_lse = linear_cross_entropy(x, w, targets, reduction="none")
