@@ -1881,6 +1881,10 @@ static void set_parts(GemmArgs& p, const Parts& parts) {
     if (!parts.a) return;
     p.part_kb = (p.K + BK - 1) / BK, p.kb_per_split = kPartProducts * p.part_kb, p.a_part = (int)parts.a, p.b_part = (int)parts.b;
 }
+// The contiguous axes of operands that a `_takes` has found fit. (A piece's last row or column by itself is as fit as all of them.)
+static void operand_axes(const View3& a, const View3& b, bool& a_cols, bool& b_cols) {
+    if (!tensor_core_operands(a, b, a_cols, b_cols)) fail(LB_ERR_UNSUPPORTED, "gemm: the tcgen05 kernels need 16-bit operands with a unit stride and 16-byte aligned rows");
+}
 bool gemm_sum_takes(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& out) {
     const View3 a = view3(a_t, "a"), b = view3(b_t, "b");
     bool a_cols, b_cols;
@@ -1899,7 +1903,7 @@ void gemm_narrow(const lb_tensor& a_t, const lb_tensor& b_t, const lb_tensor& ou
     driver();
     const View3 a = view3(a_t, "a"), b = view3(b_t, "b");
     bool a_cols, b_cols;
-    tensor_core_operands(a, b, a_cols, b_cols);
+    operand_axes(a, b, a_cols, b_cols);
     SmallGemmArgs q{};
     q.M = (int)a.rows, q.N = (int)b.cols, q.K = (int)a.cols, q.a_mn_major = !a_cols, q.b_mn_major = b_cols, q.in_bf16 = a.dtype == LB_BF16;
     q.d = out.ptr, q.d_bf16 = out.dtype == LB_BF16, q.d_f16 = out.dtype == LB_F16, q.ldd = out.stride[0], q.undo = undo, q.status = status_word();
@@ -1922,7 +1926,7 @@ void gemm_part_sums(const lb_tensor& a_t, const lb_tensor& b_t, int ranges, floa
     driver();
     const View3 a = view3(a_t, "a"), b = view3(b_t, "b"), w = turned(b);
     bool a_cols, b_cols;
-    tensor_core_operands(a, b, a_cols, b_cols);
+    operand_axes(a, b, a_cols, b_cols);
     SumArgs p{};
     long long tiles;
     pair_args(p, a, w, a_cols, !b_cols, BN, tiles);
@@ -1934,7 +1938,7 @@ void gemm_sum(const lb_tensor& a_t, const lb_tensor& b_t, float* sum, bool begin
     driver();
     const View3 a = view3(a_t, "a"), b = view3(b_t, "b"), w = turned(b);
     bool a_cols, b_cols;
-    tensor_core_operands(a, b, a_cols, b_cols);
+    operand_axes(a, b, a_cols, b_cols);
     SumArgs p{};
     long long tiles;
     pair_args(p, a, w, a_cols, !b_cols, BN, tiles);
@@ -1987,7 +1991,7 @@ void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, co
         const int i = order[k];
         const View3 a = view3(a_t[i], "a"), b = view3(b_t[i], "b"), w = turned(b);
         bool a_cols, b_cols;
-        tensor_core_operands(a, b, a_cols, b_cols);
+        operand_axes(a, b, a_cols, b_cols);
         SumArgs& q = p.product[k];
         pair_args(q, a, w, a_cols, !b_cols, BN, tiles[k]);
         const Parts part = parts ? parts[i] : Parts{};
@@ -2012,8 +2016,8 @@ template <class Args>
 static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, const Parts& parts, void* stream) {
     driver();
     const View3 x = view3(x_t, "x"), w = view3(w_t, "w");
-    bool x_cols, w_rows;
-    tensor_core_operands(x, turned(w), x_cols, w_rows);
+    // the axes that gemm_loss_takes found for all of the rows: those of a piece, of which there may be one, lie as they do
+    const bool x_cols = x.sc == 1 || x.cols == 1, w_rows = w.sr == 1;
     long long tiles;
     pair_args(p, x, w, x_cols, !w_rows, BN, tiles);
     set_parts(p, parts);
