@@ -577,7 +577,7 @@ __device__ __forceinline__ SpanSum drain_span(uint32_t tbase, int width, int tar
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int j = 0; j < 64; j++) most[j & 3] = fmaxf(most[j & 3], __uint_as_float(v[j]));
-        const float top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), all.most), base = (top == -INFINITY ? 0.0f : top) * -kLog2e;
+        const float top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), all.most), base = base_of(top) * -kLog2e;
         const Pair scale = both(kLog2e, kLog2e), shift = both(base, base);
         Pair sum[2] = {both(0.0f, 0.0f), both(0.0f, 0.0f)};
 #pragma unroll

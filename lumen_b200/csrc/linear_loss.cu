@@ -18,6 +18,7 @@
 #include "linear_loss.h"
 #include "overlap.h"
 #include "pair.cuh"
+#include "parts.cuh"
 
 namespace lb {
 bool gemm(const lb_tensor& a, const lb_tensor& b, const lb_tensor& d, int epilogue, int kernel_choice, void* stream, void* scratch, size_t scratch_bytes,
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(kRowThreads) span_kernel(const float* logits, 
             const int c = from + threadIdx.x + k * kRowThreads;
             v[k] = c < cols ? z[c] : -INFINITY, most = fmaxf(most, v[k]);
         }
-        const float base = most == -INFINITY ? 0.0f : most;
+        const float base = base_of(most);
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < kEach; k++) sum += exp2_approx((v[k] - base) * kLog2e);
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) few_kernel(const float* x, lon
         float most = in ? v : -INFINITY;
 #pragma unroll
         for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        const float base = most == -INFINITY ? 0.0f : most;
+        const float base = base_of(most);
         float sum = in ? exp2_approx((v - base) * kLog2e) : 0.0f;
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const SpanSum* spans, int n_s
             float most = v.most;
 #pragma unroll
             for (int k = 0; k < AHEAD; k++) most = fmaxf(most, next[k].most);
-            const float base = most == -INFINITY ? 0.0f : most;
+            const float base = base_of(most);
             float sum = v.sum * exp2_approx((v.most - base) * kLog2e);
 #pragma unroll
             for (int k = 0; k < AHEAD; k++) sum += next[k].sum * exp2_approx((next[k].most - base) * kLog2e);
@@ -298,12 +299,10 @@ __global__ void __launch_bounds__(256) row_grads_kernel(Targets targets, LossGra
     }
 }
 
-// float32 values in three parts of bfloat16, [rows][3][part] with zeros behind the columns: the value rounded, what that leaves rounded, and the rest, 24 bits in all.
-// Infinities become the largest finite values (a product of one with a part that is zero would be NaN); NaN stays. Rows of class -1 are zero.
+// float32 values in three parts of bfloat16, [rows][3][part] with zeros behind the columns. Rows of class -1 are zero.
 __global__ void __launch_bounds__(256) parts_kernel(const float* from, long long row_step, long long col_step, long long rows, int cols, int part, const int* classes,
                                                     __nv_bfloat16* to) {
     grid_wait();
-    constexpr float kMost = 3.3895313892515355e38f;  // bfloat16's
     const bool vectors = col_step == 1 && row_step % 4 == 0 && cols % 4 == 0 && (uintptr_t)from % 16 == 0;
     for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
         const bool there = !classes || classes[row] >= 0;
@@ -321,15 +320,10 @@ __global__ void __launch_bounds__(256) parts_kernel(const float* from, long long
                         if (c + j < cols) v[j] = x[(c + j) * col_step];
                 }
             }
+            uint32_t parts[3][2];
+            parts_of<true>(v, parts);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (!isnan(v[j])) v[j] = fminf(fmaxf(v[j], -kMost), kMost);
-#pragma unroll
-            for (int k = 0; k < 3; k++) {
-                const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-                *(uint2*)(out + (long long)k * part + c) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
-                v[0] -= __low2float(a), v[1] -= __high2float(a), v[2] -= __low2float(b), v[3] -= __high2float(b);
-            }
+            for (int k = 0; k < 3; k++) *(uint2*)(out + (long long)k * part + c) = make_uint2(parts[k][0], parts[k][1]);
         }
     }
 }

@@ -20,7 +20,7 @@ struct Targets {
 #endif
 };
 
-// One row's logits over a span of the vocabulary: their largest and the sum of exp(logit - largest).
+// One row's logits over a span of the vocabulary: their largest and the sum of exp(logit - largest), of exp(logit) where the largest is infinite.
 struct SpanSum {
     float most, sum;
 };
@@ -32,9 +32,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The sum of two spans. Where nothing is above -inf the sum stays what it is, zero.
+// What is taken away from logits whose largest is `most`, before their exponentials are. Where that is infinite they stay as they are: sums of them are then zero, or infinite,
+// as the log-sum-exp is.
+__device__ __forceinline__ float base_of(float most) { return fabsf(most) == INFINITY ? 0.0f : most; }
+// The sum of two spans.
 __device__ __forceinline__ SpanSum join(SpanSum a, SpanSum b) {
-    const float most = fmaxf(a.most, b.most), base = most == -INFINITY ? 0.0f : most;
+    const float most = fmaxf(a.most, b.most), base = base_of(most);
     return {most, a.sum * exp2_approx((a.most - base) * kLog2e) + b.sum * exp2_approx((b.most - base) * kLog2e)};
 }
 #endif
