@@ -547,6 +547,11 @@ __device__ __forceinline__ void sloped_way_out(const Args& p, uint8_t* pieces, u
 }
 
 // ---- the linear cross entropy's tiles -------------------------------------------------------------------------------
+// Exponentials of logits less a number are formed as 2^(z log2 e - n) with n its product with log2 e, rounded, which one instruction does. That rounding is common to all of a row's, and
+// of the size that the number's own has in float32; but above this number it would be a factor that matters, and far above it (10^9) one that overflows. There the number
+// is taken away first.
+constexpr float kShifted = 1048576.0f;
+
 // A row's 128 logits of the tile, not stored: their largest and the sum of exponentials, 64 columns at a time, and the target's where it is among them
 // (`target`: its column here). One pass over the logits for the largest of 64, one for the exponentials of those, packed; what was before is scaled to the larger of both.
 // Bound by the products where K is 1024 and more: 16384 x 32768 x 1024 keeps the tensor pipe busy for 95 % of 647 us, 1531 x 30011 x 1120 (float16) for 90 % of its rounds.
@@ -577,16 +582,26 @@ __device__ __forceinline__ SpanSum drain_span(uint32_t tbase, int width, int tar
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int j = 0; j < 64; j++) most[j & 3] = fmaxf(most[j & 3], __uint_as_float(v[j]));
-        const float top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), all.most), base = base_of(top) * -kLog2e;
-        const Pair scale = both(kLog2e, kLog2e), shift = both(base, base);
+        const float top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), all.most), base = base_of(top);
+        const Pair scale = both(kLog2e, kLog2e), shift = both(base * -kLog2e, base * -kLog2e);
         Pair sum[2] = {both(0.0f, 0.0f), both(0.0f, 0.0f)};
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const float2 e = apart(fma2(columns(v, j), scale, shift));
+        float before = fmaf(all.most, kLog2e, base * -kLog2e);
+        auto add = [&](int j, Pair at) {
+            const float2 e = apart(at);
             sum[j & 1] = sum[j & 1] + both(fast_exp2(e.x), fast_exp2(e.y));
+        };
+        const bool far = fabsf(base) > kShifted;
+        if (LB_RARELY(__any_sync(0xffffffffu, far))) {
+            const Pair away = both(-base, -base);
+#pragma unroll
+            for (int j = 0; j < 32; j++) add(j, far ? (columns(v, j) + away) * scale : fma2(columns(v, j), scale, shift));
+            if (far) before = (all.most - base) * kLog2e;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) add(j, fma2(columns(v, j), scale, shift));
         }
         const float2 s = apart(sum[0] + sum[1]);
-        all = {top, all.sum * fast_exp2(fmaf(all.most, kLog2e, base)) + (s.x + s.y)};
+        all = {top, all.sum * fast_exp2(before) + (s.x + s.y)};
     }
     return all;
 }
@@ -602,6 +617,7 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
                                              Release release) {
     const Pair scale = both(kLog2e, kLog2e), shift = both(lse * -kLog2e, lse * -kLog2e), weight = both(g, g);
     const uint32_t keep = counts ? 0xffffffffu : 0u, area = smem_u32(stage) + lane * 128;
+    const bool far = fabsf(lse) > kShifted, any_far = __any_sync(0xffffffffu, far);
     constexpr bool F16 = FORM == SLOPE_F16 || FORM == SLOPE_F16_RESTS, RESTS = FORM == SLOPE_BF16_RESTS || FORM == SLOPE_F16_RESTS;
 #pragma unroll 1
     for (int c2 = 0; c2 < BN / 2 / 64; c2++) {
@@ -615,6 +631,13 @@ __device__ __forceinline__ void drain_slopes(const LossSlopesArgs& p, uint32_t t
         if (FORM == SLOPE_PARTS) {  // what is left of float32's precision here is not rounded to 16 bits
 #pragma unroll
             for (int j = 0; j < 64; j++) v[j] = __float_as_uint(expf(__uint_as_float(v[j]) - lse));
+        } else if (LB_RARELY(any_far)) {
+            const Pair away = both(-lse, -lse);
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const float2 e = apart(far ? (columns(v, j) + away) * scale : fma2(columns(v, j), scale, shift));
+                v[2 * j] = __float_as_uint(fast_exp2(e.x)), v[2 * j + 1] = __float_as_uint(fast_exp2(e.y));
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 32; j++) {

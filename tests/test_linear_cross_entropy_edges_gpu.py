@@ -109,6 +109,20 @@ def test_infinities_in_the_weights(cuda, shape, dtype):
 
 
 @pytest.mark.parametrize("shape", INFINITE, ids=lambda s: "x".join(map(str, s)))
+def test_the_largest_values(cuda, shape):
+    """float32 values between bfloat16's largest and float32's."""
+    x, w, targets = operands(cuda, *shape, torch.float32, seed=9)
+    x[0, 3], x[-1, 4] = 3.402e38, -3.4e38
+    w[:, 3:5] *= 2.0**-20
+    loss, lse = linear_cross_entropy(x, w, targets, reduction="none")
+    check_forward(x, w, targets, "none", loss, lse)
+    w[3, 2], w[4, 2] = 3.4e38, -3.4e38  # logits of both signs that are as large
+    x[:, 2] *= 2.0**-20
+    loss, lse = linear_cross_entropy(x, w, targets, reduction="none")
+    check_forward(x, w, targets, "none", loss, lse)
+
+
+@pytest.mark.parametrize("shape", INFINITE, ids=lambda s: "x".join(map(str, s)))
 def test_gradients_by_the_largest_values(cuda, shape):
     """Logits without them: a float32 logit of 1e32 is 1e25 apart from the next, and its exponential nothing."""
     x, w, targets = operands(cuda, *shape, torch.float32, seed=10)
@@ -117,3 +131,22 @@ def test_gradients_by_the_largest_values(cuda, shape):
     loss, lse = linear_cross_entropy(x, w, targets, reduction="none")
     check_forward(x, w, targets, "none", loss, lse)
     check_backward(x, w, targets, lse, "none", None, *linear_cross_entropy_backward(None, x, w, targets, lse, reduction="none"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", INFINITE, ids=lambda s: "x".join(map(str, s)))
+def test_logits_far_from_zero(cuda, shape, dtype):
+    """Multiples of 2^20 and more, all exact: the largest logit is the log-sum-exp, a row's probability is its largest logit's, and every result is a sum of a few exact values."""
+    t, d, v = shape
+    g = torch.Generator(device=cuda).manual_seed(11)
+    x = (torch.randint(-8, 9, (t, d), generator=g, device=cuda) * 2.0**8).to(dtype)
+    w = (torch.randint(-8, 9, (v, d), generator=g, device=cuda) * 2.0 ** (12 if dtype == torch.float16 else 30)).to(dtype)
+    targets = torch.randint(0, v, (t,), generator=g, device=cuda)
+    z = x.double() @ w.double().t()
+    top = z.amax(-1)
+    loss, lse = linear_cross_entropy(x, w, targets, reduction="none")
+    assert torch.equal(lse.double(), top) and torch.equal(loss.double(), top - z.gather(-1, targets[:, None])[:, 0])
+    dz = (z == top[:, None]).double() - torch.nn.functional.one_hot(targets, v)
+    d_x, d_w = linear_cross_entropy_backward(None, x, w, targets, lse, reduction="none")
+    assert torch.equal(d_x, (dz @ w.double()).to(dtype)) and torch.equal(d_w, (dz.t() @ x.double()).to(dtype))
+    device_status()
