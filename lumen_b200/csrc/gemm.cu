@@ -2010,6 +2010,14 @@ void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, co
     int order[2];
     long long tiles[2], blocks[2];
     listed_sizes(a_t, b_t, order, tiles, blocks, parts != nullptr);
+    const int resident = resident_pairs(dev), pairs = (int)std::min<long long>(tiles[0] + tiles[1], resident > 0 ? resident : dev.sms / 2);
+    std::fill(p.unit_of, p.unit_of + kListed, (uint16_t)kNone);
+    int slots;
+    double us;
+    if (!share_units(tiles, blocks, pairs, p.unit_of, slots, us)) {  // fewer pairs than half the SMs, which was asked with, may need more places: the same sums, a launch each
+        for (const int i : order) gemm_sum(a_t[i], b_t[i], sum[i], begins[i], out[i], undo, stream, parts ? parts[i] : Parts{});
+        return;
+    }
     for (int k = 0; k < 2; k++) {
         const int i = order[k];
         const View3 a = view3(a_t[i], "a"), b = view3(b_t[i], "b"), w = turned(b);
@@ -2027,11 +2035,6 @@ void gemm_sums(const lb_tensor* a_t, const lb_tensor* b_t, float* const* sum, co
     first_use_on_device((const void*)gemm_tcgen05_pair<ListedArgs>, [] {
         LB_CUDA(cudaFuncSetAttribute(gemm_tcgen05_pair<ListedArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(PAIR_LISTED)));
     });
-    const int resident = resident_pairs(dev), pairs = (int)std::min<long long>(tiles[0] + tiles[1], resident > 0 ? resident : dev.sms / 2);
-    std::fill(p.unit_of, p.unit_of + kListed, (uint16_t)kNone);
-    int slots;
-    double us;
-    if (!share_units(tiles, blocks, pairs, p.unit_of, slots, us)) fail(LB_ERR_UNSUPPORTED, "gemm: too many output tiles for one launch");
     p.units = slots * pairs;
     launch_overlapped(gemm_tcgen05_pair<ListedArgs>, dim3((unsigned)(2 * pairs)), dim3(kThreads), pair_smem(PAIR_LISTED), (cudaStream_t)stream, 0, p.map_a[0], p.map_b[0], p);
 }

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from lumen_b200.runtime import device_status, linear_cross_entropy, linear_cross_entropy_backward
-from tests.test_linear_cross_entropy_gpu import IGNORED, check_backward, check_forward, operands
+from tests.test_linear_cross_entropy_gpu import IGNORED, check_backward, check_forward, half, operands, within
 
 pytestmark = pytest.mark.gpu
 
@@ -149,4 +149,23 @@ def test_logits_far_from_zero(cuda, shape, dtype):
     dz = (z == top[:, None]).double() - torch.nn.functional.one_hot(targets, v)
     d_x, d_w = linear_cross_entropy_backward(None, x, w, targets, lse, reduction="none")
     assert torch.equal(d_x, (dz @ w.double()).to(dtype)) and torch.equal(d_w, (dz.t() @ x.double()).to(dtype))
+    device_status()
+
+
+@pytest.mark.parametrize("shape", [(22199, 17072, 5915), (31585, 12424, 4715)])
+def test_a_last_piece_whose_units_the_table_does_not_hold(cuda, shape):
+    """Both products of a whole piece share a launch; of a few classes behind it, whose shares are less even, they have one each."""
+    t, d, v = shape
+    x, w, targets = operands(cuda, t, d, v, torch.bfloat16, ignored=0.1)
+    targets[0], targets[1] = v - 1, v - 2
+    _, lse = linear_cross_entropy(x, w, targets, reduction="none")
+    d_x, d_w = linear_cross_entropy_backward(None, x, w, targets, lse, reduction="none")
+    counts = (targets != IGNORED)[:, None]
+    for rows in (slice(0, 150), slice(t - 150, t)):  # a gradient's every term is a rounded dz times an element
+        dz = (torch.exp(x[rows].double() @ w.double().t() - lse[rows].double()[:, None]) - torch.nn.functional.one_hot(targets[rows].clamp(min=0), v)) * counts[rows]
+        within(d_x[rows], dz @ w.double(), 2 * half(torch.bfloat16) * (dz.abs() @ w.double().abs()) + 1e-6, "d_x")
+    for classes in (slice(0, 100), slice(v - 100, v)):
+        ids = torch.arange(v, device=cuda)[classes]
+        dz = (torch.exp(x.double() @ w[classes].double().t() - lse.double()[:, None]) - (targets[:, None] == ids).double()) * counts
+        within(d_w[classes], dz.t() @ x.double(), 2 * half(torch.bfloat16) * (dz.t().abs() @ x.double().abs()) + 1e-6, "d_weight")
     device_status()

@@ -67,3 +67,9 @@ def test_random(share):
         assert us == pytest.approx(max(loads) + 3.0 + 0.1 * sum(t * b for t, b in zip(tiles, blocks)) / pairs)
         # each to the pair with the least: the fullest has at most a unit more than the mean
         assert max(loads) <= total / pairs + max(cost(0, tiles, blocks), cost(tiles[0], tiles, blocks)) + 1e-9
+
+
+def test_fewer_units_or_pairs_may_need_more_places(share):
+    """Whether a table holds two products says nothing about fewer of their units, or about fewer pairs: a launch is asked about as it is."""
+    assert share((1541, 5829), (347, 92), 74, lists=False)[0] and not share((67, 5829), (347, 1), 74, lists=False)[0]
+    assert share((1572, 6420), (1756, 421), 74, lists=False)[0] and not share((1572, 6420), (1756, 421), 72, lists=False)[0]
