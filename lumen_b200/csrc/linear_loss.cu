@@ -762,15 +762,22 @@ struct Backward : Loss {
     void run(cudaStream_t s, bool only_count) {
         held = 0;
         const int item = dtype_size(dtype);
+        if (T == 0) {  // no scratch
+            if (!only_count) LB_CUDA(cudaMemset2DAsync(dw.ptr, (size_t)(V > 1 ? dw.stride[0] : D) * item, 0, (size_t)D * item, (size_t)V, s));
+            return;
+        }
         const bool scaled = item == 2;  // `undo` is what the products' results are to be multiplied by
         // dz of few rows is held in two parts, the second what the rounding of the first leaves, as rows of their own (of x too): with as few terms a sum's error would be that of one rounding, and
         // the products' tiles have the room
         const bool rests = item == 2 && T <= 64;
         const long long R = rests ? 2 * T : T;
-        const bool fused = T && gemm_loss_takes(x, w), parts = in_parts() && D % 8 == 0 && in_vectors(dx) && in_vectors(dw);
-        const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : piece_of(fused ? 2 : 4, R), pieces = (V + piece - 1) / piece, ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
+        const bool fused = gemm_loss_takes(x, w), parts = in_parts() && D % 8 == 0 && in_vectors(dx) && in_vectors(dw);
         auto in_fours = [&](const lb_tensor& t) { return (uintptr_t)t.ptr % (4 * item) == 0 && t.stride[1] == 1 && (t.shape[0] <= 1 || t.stride[0] % 4 == 0); };
-        const bool one_pass = T && T <= grad_tokens(item) && D % 4 == 0 && in_fours(w) && in_fours(dw);
+        const bool one_pass = T <= grad_tokens(item) && D % 4 == 0 && in_fours(w) && in_fours(dw);
+        // d_weight in 16 bits that no tiles can store is rounded from float32 sums of a piece, which are bounded as dz is
+        const bool dw_sums = scaled && !one_pass && !(D % 8 == 0 && in_vectors(dw));
+        const long long part = up(D, 64), piece = parts ? piece_of(6, std::max(T, part)) : std::min(piece_of(fused ? 2 : 4, R), dw_sums ? piece_of(4, D) : V), pieces = (V + piece - 1) / piece,
+                        ld = up(piece, 64), ld_kept = up(D, 64);  // rows of whole 128 bytes
         const long long slices = (D / 4 + kGradThreads - 1) / kGradThreads, each = std::max(16LL, one_pass ? (piece * slices + few_grad_slots() - 1) / few_grad_slots() : 1);
         const int n_counts = (int)std::min<long long>(64, (T + 255) / 256);
         RowCount* counts = take<RowCount>(n_counts);
@@ -783,23 +790,21 @@ struct Backward : Loss {
         // sums over pieces, and what takes the scale away: in the products' epilogue where they run on whole tiles or narrow ones, else behind them
         // (both in one launch where that fills the GPU better)
         const lb_tensor sums_a[] = {transposed(dz), dz}, sums_b[] = {kept_all, rows_of(w, 0, piece)}, sums_out[] = {dw, dx};
-        const bool folds = pieces > 1 || scaled, both = !parts && !rests && T && gemm_sums_pay(sums_a, sums_b, sums_out), dx_tiles = both || (folds && !rests && T && gemm_sum_takes(sums_a[1], sums_b[1], dx)),
-                   dw_tiles = both || (scaled && T && gemm_sum_takes(sums_a[0], sums_b[0], dw)), dw_narrow = scaled && T && pieces == 1 && !dw_tiles && gemm_narrow_ranges(sums_a[0], sums_b[0]),
-                   dx_narrow = scaled && T && !rests && pieces == 1 && !dx_tiles && gemm_narrow_ranges(sums_a[1], sums_b[1]);
-        const int ranges = dtype != LB_F32 || !T ? 1 : parts ? gemm_part_ranges(T, D, piece) : core_ranges(piece), dw_ranges = parts ? gemm_part_ranges(piece, D, T) : 1;
-        float *dx_piece = ranges > 1 || (folds && !dx_tiles && !dx_narrow && !parts) ? take<float>((ranges + 1) * T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
-        float* dw_piece = (scaled && !dw_tiles && !dw_narrow) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
+        const bool folds = pieces > 1 || scaled, tiles = !one_pass, both = tiles && !parts && !rests && gemm_sums_pay(sums_a, sums_b, sums_out),
+                   dx_tiles = both || (tiles && folds && !rests && gemm_sum_takes(sums_a[1], sums_b[1], dx)), dw_tiles = both || (tiles && scaled && gemm_sum_takes(sums_a[0], sums_b[0], dw)),
+                   dw_narrow = tiles && scaled && pieces == 1 && !dw_tiles && gemm_narrow_ranges(sums_a[0], sums_b[0]),
+                   dx_narrow = tiles && scaled && !rests && pieces == 1 && !dx_tiles && gemm_narrow_ranges(sums_a[1], sums_b[1]);
+        const int ranges = dtype != LB_F32 || one_pass ? 1 : parts ? gemm_part_ranges(T, D, piece) : core_ranges(piece), dw_ranges = parts ? gemm_part_ranges(piece, D, T) : 1;
+        float *dx_piece = ranges > 1 || (tiles && folds && !dx_tiles && !dx_narrow && !parts) ? take<float>((ranges + 1) * T * D) : nullptr, *dx_sum = pieces > 1 ? take<float>(T * D) : nullptr;
+        float* dw_piece = (tiles && scaled && !dw_tiles && !dw_narrow) || dw_ranges > 1 ? take<float>(dw_ranges * piece * D) : nullptr;
         float* dx_ranges = one_pass ? take<float>((piece + each - 1) / each * T * D) : nullptr;
         size_t more = 0;
-        if (T && !parts) more = std::max({fused ? 0 : product_scratch(x, transposed(rows_of(w, 0, piece))), product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept_all)});
-        const GemmTuning few{T ? few_ranges(piece) : 0, 0};
+        if (!parts && !fused) more = product_scratch(x, transposed(rows_of(w, 0, piece)));
+        if (!parts && tiles) more = std::max({more, product_scratch(dz, rows_of(w, 0, piece)), product_scratch(transposed(dz), kept_all)});
+        const GemmTuning few{tiles ? few_ranges(piece) : 0, 0};
         if (few.splits > 1) more = std::max<size_t>(more, (size_t)few.splits * R * D * 4);
         void* product = take<char>(more);
         if (only_count) return;
-        if (T == 0) {
-            LB_CUDA(cudaMemset2DAsync(dw.ptr, (size_t)(V > 1 ? dw.stride[0] : D) * item, 0, (size_t)D * item, (size_t)V, s));
-            return;
-        }
         const LossGrad d_loss{(const float*)grad.ptr, grad.stride[0]};
         const bool counts_itself = T <= 1024;  // every block: a launch (2 us) costs more than that
         if (!counts_itself) launch_overlapped(count_kernel, dim3((unsigned)n_counts), dim3(256), 0, s, 0, targets, d_loss, T, counts);

@@ -169,3 +169,14 @@ def test_a_last_piece_whose_units_the_table_does_not_hold(cuda, shape):
         dz = (torch.exp(x.double() @ w[classes].double().t() - lse.double()[:, None]) - (targets[:, None] == ids).double()) * counts
         within(d_w[classes], dz.t() @ x.double(), 2 * half(torch.bfloat16) * (dz.t().abs() @ x.double().abs()) + 1e-6, "d_weight")
     device_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(4, 516, 140001), (5, 516, 140001), (61, 514, 140001), (100, 516, 140001), (300, 524, 270001)], ids=lambda s: "x".join(map(str, s)))
+def test_a_gradient_that_no_tiles_store_in_several_pieces(cuda, shape, dtype):
+    x, w, targets = operands(cuda, *shape, dtype, ignored=0.2 * (shape[0] % 2))
+    targets[0], targets[1] = shape[2] - 1, 0
+    loss, lse = linear_cross_entropy(x, w, targets)
+    check_forward(x, w, targets, "mean", loss, lse)
+    check_backward(x, w, targets, lse, "mean", None, *linear_cross_entropy_backward(None, x, w, targets, lse))
+    device_status()
