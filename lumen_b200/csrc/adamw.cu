@@ -212,9 +212,9 @@ __device__ __forceinline__ float inverse(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float inverse_root(float x) {
+__device__ __forceinline__ float inverse_root(float x) {  // (of subnormal values too)
     float r;
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -224,8 +224,8 @@ __device__ __forceinline__ float inverse_root(float x) {
 // for a rare unit in the last place, and by a block's reciprocal, rounded: a code next to the middle of two is then the same whoever computes it, and one that is not
 // makes the weight's next step another by a sixteenth. The weight's own step has the hardware's reciprocal.
 //
-// Bound by issued instructions (66 % of the slots) and memory: 158 M bfloat16 weights 285 - 312 us, 5.5 TB/s at best; 62 instructions an element took 366, where root and quotient of each
-// are the exact functions; 278 with codes by approximate reciprocals and fused sums. (Two blocks an SM with four blocks of 256 at once 303, four with two 312.)
+// Bound by issued instructions (66 % of the slots) and memory: 158 M bfloat16 weights 303 - 317 us, 5.2 TB/s at best; 2 % less where v below 2^-126 has a wrong root; 62 instructions an
+// element took 366, where root and quotient of each are the exact functions. Two blocks an SM with four blocks of 256 at once were slower by 5 %, four with two by 3 %.
 __device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, float& sm, float& sv, float* w, const float* g) {
     uint32_t cm[4] = {m.x & 0xffff, m.x >> 16, m.y & 0xffff, m.y >> 16}, cv[4] = {v.x & 0xffff, v.x >> 16, v.y & 0xffff, v.y >> 16};
     auto same = [](float x) { return both(x, x); };
@@ -242,7 +242,7 @@ __device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, fl
         const Pair gg = both(g[2 * j], g[2 * j + 1]) * same(s.factor), r = from_e4m3(cv[j]) * same(sv);
         mm[j] = sum(from_e4m3(cm[j]) * same(sm) * same(s.b1), gg * same(s.b1_rest));
         const float2 vv = sum(r * r * same(s.b2), gg * gg * same(s.b2_rest));
-        const Pair v2 = both(vv.x, vv.y), y = both(inverse_root(fmaxf(vv.x, 0x1p-126f)), inverse_root(fmaxf(vv.y, 0x1p-126f))), near = v2 * y;
+        const Pair v2 = both(vv.x, vv.y), y = both(inverse_root(fmaxf(vv.x, 0x1p-149f)), inverse_root(fmaxf(vv.y, 0x1p-149f))), near = v2 * y;
         root[j] = fma2(fma2(-near, near, v2), y * same(0.5f), near);
         const float2 den = apart(fma2(root[j], same(s.root_c2), same(s.eps)));
         const float2 moved = apart(fma2(both(mm[j].x, mm[j].y) * both(inverse(den.x), inverse(den.y)), same(-s.rate), both(w[2 * j], w[2 * j + 1]) * same(s.keep)));
