@@ -197,10 +197,12 @@ int lb_clip_grad_norm(const lb_tensor* tensors, const lb_tensor* outputs, int n_
  * z = x W^T for hidden states `x` [.., D] and `weight` [V, D] (any strides that lb_gemm takes; float16, bfloat16 or float32), lse = log sum exp(z) of each
  * row and loss = lse - z[target], without keeping z. `targets` (int32 or int64, [..]) are clamped into the vocabulary; a row whose target is
  * `ignore_index` does not count: its loss is 0, whatever stands in its x. `loss` is float32: [..], or one value, the sum or the mean over the
- * rows that count (0 where none does). `lse` [..] float32 (of every row) is what the backward pass reads. Sums are float32 and more.
+ * rows that count (0 where none does). `lse` [..] float32 (of every row) is what the backward pass reads. Sums are float32 and more. Infinities and NaN do as the formulas
+ * say, in their own rows; a float32 operand's infinity is multiplied by zero where a gradient's smaller parts are zero, and NaN there.
  * Backward: `d_loss` is the gradient of `loss`, float32 of its shape (any even spacing of rows, 0 among them; null: ones); dz = (exp(z - lse) - [target]) g with
- * each row's share g of it, computed anew for a piece of the vocabulary at a time and rounded to the operands' dtype; d_x = dz W and d_weight = dz^T x, of the
- * operands' shapes and dtype, row-major, each with one float32 sum and one rounding; rows that do not count have a d_x of 0 and no part in d_weight. Results share
+ * each row's share g of it, computed anew for a piece of the vocabulary at a time. As an operand of the products that follow dz is rounded to 16 bits where the operands
+ * have them, once with more than 64 rows, in two parts with up to 64; in float32 it is not. d_x = dz W and d_weight = dz^T x, of the operands' shapes and dtype,
+ * row-major, each with one float32 sum and one rounding; rows that do not count have a d_x of 0 (with finite weights) and no part in d_weight. Results share
  * no memory with one another or with an operand; every call repeats bit for bit. Scratch: as many bytes as the _scratch_bytes call on the same tensors
  * says, 16-byte aligned; calls that may overlap on the GPU need scratch of their own. */
 typedef enum { LB_REDUCTION_NONE = 0, LB_REDUCTION_SUM = 1, LB_REDUCTION_MEAN = 2 } lb_reduction;
@@ -224,7 +226,7 @@ int lb_linear_cross_entropy_bwd(const lb_loss_desc* desc, const lb_tensor* d_los
  * c = min(1, max_norm / (norm + 1e-6)), as lb_clip_grad_norm says, else c = 1. Parameters of float16, bfloat16 and float32 in any mix, dense in any order of
  * their dimensions; gradients of the parameter's type or float32; moments of the parameter's shape and strides: float32, or, with `exp_avg_scale` and
  * `exp_avg_sq_scale`, uint8: e4m3 codes of m / s and sqrt(v) / s, with a float32 scale s = max / 448 for each 256 elements in the order of memory (dense
- * [ceil(elements / 256)]); codes and scales of zeros are a first step's moments. `masters` (nullable; an entry with a null ptr: none) are float32 copies of 16-bit
+ * [ceil(elements / 256)]); codes and scales of zeros are a first step's moments, and a moment that is not finite takes its block's scale and codes with it. `masters` (nullable; an entry with a null ptr: none) are float32 copies of 16-bit
  * parameters, which the step is then taken on. All but gradients, `step`, `lr` and `norm` are updated in place, and share no memory with anything else
  * of the call; a gradient may be listed twice. `step`, which counts from 1 (float32, int32 or int64), `lr` and `norm` (float32) are single values on
  * the device, read when the kernel runs; a null `step` or `lr` means the desc's. The same bits every time; the call takes no scratch. */

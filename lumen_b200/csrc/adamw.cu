@@ -224,7 +224,7 @@ __device__ __forceinline__ float inverse_root(float x) {  // (of subnormal value
 // for a rare unit in the last place, and by a block's reciprocal, rounded: a code next to the middle of two is then the same whoever computes it, and one that is not
 // makes the weight's next step another by a sixteenth. The weight's own step has the hardware's reciprocal.
 //
-// Bound by issued instructions (66 % of the slots) and memory: 158 M bfloat16 weights 303 - 317 us, 5.2 TB/s at best; 2 % less where v below 2^-126 has a wrong root; 62 instructions an
+// Bound by issued instructions (69 % of the slots) and memory: 158 M bfloat16 weights 303 - 317 us, 5.2 TB/s at best; 2 % less where v below 2^-126 has a wrong root; 62 instructions an
 // element took 366, where root and quotient of each are the exact functions. Two blocks an SM with four blocks of 256 at once were slower by 5 %, four with two by 3 %.
 __device__ __forceinline__ void eight_step(const Step& s, uint2& m, uint2& v, float& sm, float& sv, float* w, const float* g) {
     uint32_t cm[4] = {m.x & 0xffff, m.x >> 16, m.y & 0xffff, m.y >> 16}, cv[4] = {v.x & 0xffff, v.x >> 16, v.y & 0xffff, v.y >> 16};

@@ -164,7 +164,7 @@ __device__ __forceinline__ int k_blocks(const GemmArgs& q) {
     return whole;
 }
 // The tensor cores' sums drop what lies below float32's last place at each step, always towards zero: 2^-25 of a sum a step in the mean, so that one of 4096 products lacks
-// 5e-6 of itself. Where that shows (results of float32), K is cut into segments: each begins anew, and the warps of the way out add them up, rounded. The products of
+// 5e-6 of itself. Where that shows (results of float32, K above 1536 or float32 operands), K is cut into segments: each begins anew, and the warps of the way out add them up, rounded. The products of
 // the smaller parts are one segment; the last one's, of the parts that make up nearly all, end every second block: 5e-7.
 constexpr int kPartSegment = 2;
 template <class Args>
@@ -2061,7 +2061,9 @@ static void launch_loss(Args& p, const lb_tensor& x_t, const lb_tensor& w_t, con
 void gemm_loss(const lb_tensor& x, const lb_tensor& w, const Targets& targets, int first, SpanSum* spans, float* hit, void* stream, Parts parts) {
     SpansArgs p{};
     p.targets = targets, p.first = first, p.spans = spans, p.hit = hit;
-    p.segment_kb = x.shape[1] > 24 * BK ? 8 : 0;  // losses are float32: 1e-6 of a loss of 4096 products whole, 2e-7 in segments
+    // Losses are float32. Relative to 64 bits, whole -> in segments of 512: K of 640 2.0e-7 -> 1.5e-7, 1024 3.3e-7 -> 1.6e-7, 1536 5.2e-7 -> 1.6e-7, 4096 1e-6 -> 2e-7; 1024 and 1120 take 0.9 and
+    // 1.8 % longer so. Up to 1536 they are whole: at most four units in the last place of float32.
+    p.segment_kb = x.shape[1] > 24 * BK ? 8 : 0;
     launch_loss(p, x, w, parts, stream);
 }
 void gemm_loss_slopes(const lb_tensor& x, const lb_tensor& w, const float* lse, long long lse_step, const float* g, const int* classes, int first, const lb_tensor& dz,

@@ -207,9 +207,14 @@ struct FloatLossArgs : SkinnyLossArgs {
 
 // The linear cross entropy's products of up to 32 float32 tokens, on the tensor cores: both operands go into registers as they are and become three parts of bfloat16 there, six of whose
 // products are added up; those of the first parts by themselves, and both sums to what was before after every two blocks of K, rounded, since the tensor cores drop what lies below a sum's last
-// place. A block's ROWS classes are a span. Bound by the time that loads take and, with more tokens, by parting x, which every block does anew, and the products. us in a graph for 8, 16 and 32
-// tokens (behind it what the CUDA cores and, from 17 on, the parts in memory took; the weights' bytes alone): 1024 x 32768 33, 44 and 75 (46, 71, 127; 20.5), 344 x 116036 51, 65 and 115 (64, 95,
-// 207; 24.4), 3576 x 12593 46, 60 and 103 (87, 157, 342; 27.5). With 3 blocks of K on their way 37, 51 and 85 at the first, and the same with 4 and 6: fewer warps find a place.
+// place. A block's ROWS classes are a span.
+//
+// Bound by the time that loads take and, with more tokens, by parting x, which every block does anew, and the products. us in a graph for 8, 16 and 32 tokens; the weights' bytes alone; what the
+// CUDA cores and, from 17 on, the parts in memory took:
+//   1024 x 32768    32, 43, 68     20.5   46, 71, 127
+//   344 x 116036    53, 65, 110    24.4   64, 95, 207
+//   3576 x 12593    40, 54, 91     27.5   87, 157, 342
+// Two blocks of K on their way: with three 10 - 15 % more, with four and six as much, since fewer warps find a place.
 constexpr int kFloatWarps = 8, kFloatAhead = 2;
 template <int ROWS, int TOKENS>
 __global__ void __launch_bounds__(kFloatWarps * 32, 2) skinny_float_kernel(const FloatLossArgs p) {

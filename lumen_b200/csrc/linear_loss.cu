@@ -583,10 +583,12 @@ struct Loss {
         in_memory(r, what);
         return r;
     }
-    // Whether float32 operands go to the tensor cores in parts of 16 bits: six products of them take less than one of float32 on the CUDA cores, but there are 16 bytes
-    // an element of the weights to be moved for it, and three launches. us in a graph, CUDA cores -> parts, forward and backward: 33 x 344 x 116035 228 -> 240 and 855 -> 415, 53 of
-    // it 231 -> 222 and 956 -> 402, 64 x 2048 x 32768 392 -> 321 and 1248 -> 539, 300 x 64 x 5000 (9.6e7) 20.6 -> 17.4 and 59.7 -> 49.4, 1000 x 128 x 2000 36 -> 18 and 107 -> 50,
-    // 2000 x 1024 x 8000 1300 -> 151 and 4055 -> 476. Up to 32 rows' losses, and the logits of 16 rows' gradients, come straight from the weights.
+    // Whether float32 operands go to the tensor cores in parts of 16 bits: from 3e7 products on. Six products of parts take less than one of float32 on the CUDA cores; making the
+    // parts moves ten bytes an element of the weights, and each product fetches the part that it takes, which are twelve more, from memory where K is long (1024 and more: a pass over K of the
+    // tiles under way does not stay in the L2). us of the loss and of both gradients in a graph, CUDA cores -> parts: 64 x 2048 x 32768 392 -> 298 and 1248 -> 529; 300 x 64 x 5000
+    // 20.6 -> 18.6 and 59.7 -> 53.6; 1000 x 128 x 2000 36 -> 19 and 107 -> 53; 2000 x 1024 x 8000 1300 -> 156 and 4055 -> 493. Where the loss does not gain by it: 33 x 344 x 116035 248 -> 236
+    // (both eager, gradients 763 -> 445), 64 x 3296 x 84985 1382 -> 1460 (5450 -> 2510), which elementary operations do in 790 (100 rows of it 2735 -> 1484, those 1441). Up to 32 rows' losses,
+    // and the logits of 16 rows' gradients, come straight from the weights.
     bool in_parts() const { return dtype == LB_F32 && T > kFewTokens && (double)T * (double)V * (double)D >= 3e7; }
     // The vocabulary in pieces whose [width, piece] of `item` bytes an element takes about kPieceBytes.
     long long piece_of(int item, long long width) const {
@@ -726,9 +728,10 @@ struct Backward : Loss {
     using Loss::Loss;
     lb_tensor grad{}, lse, dx, dw;
 
-    // Ranges of K, the vocabulary, that d_x of up to 128 rows of 16 bits is cut into on the one-CTA tiles: an SM each, where the eight that lb_gemm's narrow tiles are cut into at
-    // most would walk 48 K blocks and there are more than twice as many here. (0: lb_gemm's own choice.) us of the backward pass in a graph, that -> these: 16 x 1024 x 32768
-    // 72.7 -> 61.2, 33 of it 75.1 -> 62.8, 128 76.0 -> 66.2; where these are not taken: 5 x 496 x 18250 38 -> 40, 16 x 512 x 8000 24.3 -> 26.3, 128 x 4096 x 32768 (nine ranges) 179 -> 182.
+    // Ranges of K, the vocabulary, that d_x of up to 128 rows of 16 bits is cut into on the one-CTA tiles: an SM each, from 384 blocks of K on and where there are more than 16
+    // (the eight that lb_gemm's narrow tiles are cut into at most would walk 48 blocks and more). 0: lb_gemm's own choice. us of the backward pass in a graph, that -> these:
+    //   16 x 1024 x 32768 72.7 -> 61.2, 33 of it 75.1 -> 62.8, 128 of it 76.0 -> 66.2
+    //   not taken: 5 x 496 x 18250 38 -> 40, 16 x 512 x 8000 24.3 -> 26.3, 128 x 4096 x 32768 (nine ranges) 179 -> 182
     int few_ranges(long long K) const {
         const long long blocks = (K + 63) / 64, tiles = (D + 255) / 256, ranges = sm_count_hint() / tiles;
         return dtype == LB_F32 || T > 128 || blocks < 384 || ranges <= 16 ? 0 : (int)std::min(ranges, blocks / 8);

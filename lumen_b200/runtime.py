@@ -507,8 +507,8 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", ignore_index=-100
     """Softmax cross entropy of the projection `x @ weight^T` through `lb_linear_cross_entropy`, without the logits ever being in memory as a whole: `x`
     `[.., D]` (hidden states), `weight` `[V, D]` (an output head), `targets` `[..]` int32 or int64. Returns `(loss, lse)`: the loss of each row, or its
     sum or mean over the rows that count (0 where none does), and each row's log-sum-exp, which the backward pass reads; both float32. A row whose target
-    is `ignore_index` does not count; other targets are clamped into the vocabulary. float16, bfloat16 or float32. Bit-identical from call to call; the
-    same rows among others may differ by a rounding."""
+    is `ignore_index` does not count; other targets are clamped into the vocabulary. float16, bfloat16 or float32. Infinities and NaN in a row that counts
+    are in its loss, as the formula has them, whatever the type. Bit-identical from call to call; the same rows among others may differ by a rounding."""
     require_cuda()
     code = _reduction(reduction)
     if _Torch.takes(x, stream) and type(targets) is _Torch.tensor:
@@ -572,7 +572,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     """One AdamW step over a list of parameters through `lb_adamw_step`, in place: with `m` and `v` the moments of the gradient and of its square,
     `w (1 - lr weight_decay) - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps)` in float32, rounded once to the parameter's type. Parameters of
     float16, bfloat16 and float32 in any mix, dense in any order of their dimensions; gradients of the same type or float32. `exp_avg` and `exp_avg_sq` are
-    float32 tensors of the parameters' layout, or, with their scales, moments in 8 bits (`adamw_state` makes both). `masters`: float32 copies of 16-bit
+    float32 tensors of the parameters' layout, or, with their scales, moments in 8 bits (`adamw_state` makes both; one that is not finite takes its block of 256
+    with it). `masters`: float32 copies of 16-bit
     parameters, on which the step is then taken (None in the place of a parameter that has none). `step` counts from 1; it and `lr` are numbers or one-element
     tensors on the device (int32, int64 or float32; float32), which a captured graph reads anew in every replay. With `norm` (what `grad_norm` gives) and
     `max_norm` the gradients are taken times `min(1, max_norm / (norm + 1e-6))`, as `clip_grad_norm` would leave them, and stay as they are. Nothing waits
