@@ -226,7 +226,7 @@ int lb_linear_cross_entropy_bwd(const lb_loss_desc* desc, const lb_tensor* d_los
  * c = min(1, max_norm / (norm + 1e-6)), as lb_clip_grad_norm says, else c = 1. Parameters of float16, bfloat16 and float32 in any mix, dense in any order of
  * their dimensions; gradients of the parameter's type or float32; moments of the parameter's shape and strides: float32, or, with `exp_avg_scale` and
  * `exp_avg_sq_scale`, uint8: e4m3 codes of m / s and sqrt(v) / s, with a float32 scale s = max / 448 for each 256 elements in the order of memory (dense
- * [ceil(elements / 256)]); codes and scales of zeros are a first step's moments, and a moment that is not finite takes its block's scale and codes with it. `masters` (nullable; an entry with a null ptr: none) are float32 copies of 16-bit
+ * [ceil(elements / 256)]); codes and scales of zeros are a first step's moments, and a moment that is not finite takes its block's scale and codes with it, and its weight. `masters` (nullable; an entry with a null ptr: none) are float32 copies of 16-bit
  * parameters, which the step is then taken on. All but gradients, `step`, `lr` and `norm` are updated in place, and share no memory with anything else
  * of the call; a gradient may be listed twice. `step`, which counts from 1 (float32, int32 or int64), `lr` and `norm` (float32) are single values on
  * the device, read when the kernel runs; a null `step` or `lr` means the desc's. The same bits every time; the call takes no scratch. */
