@@ -118,7 +118,7 @@ void gemm_sum(const lb_tensor& a, const lb_tensor& b, float* sum, bool begins, c
 // The same of operands in parts with K cut into so many ranges (1: better whole), whose sums go to `partial` [ranges][M][N].
 int gemm_part_ranges(long long M, long long N, long long K);
 void gemm_part_sums(const lb_tensor& a, const lb_tensor& b, int ranges, float* partial, void* stream, Parts parts);
-// Two of them that do not depend on one another in one launch; `_pay`: whether layouts are theirs and the model of pairs says that they gain by it.
+// Two of them that do not depend on one another in one launch, or a launch each where its table does not hold their units; `_pay`: whether layouts are theirs and the model of pairs says that they gain by it.
 bool gemm_sums_pay(const lb_tensor* a, const lb_tensor* b, const lb_tensor* out);
 // `_fit`: whether two products of parts are few enough tiles for it.
 bool gemm_sums_fit(const lb_tensor* a, const lb_tensor* b);

@@ -1,4 +1,5 @@
-"""Softmax cross entropy of a projection where its ways through the kernels end: pieces of the vocabulary with a single class, infinities and NaN in what counts."""
+"""Softmax cross entropy of a projection where its ways through the kernels end: pieces of the vocabulary with a single class or too few for a shared launch, infinities, NaN and the
+largest values in what counts, logits far from zero, widths whose gradient no tile stores."""
 
 import pytest
 import torch
